@@ -274,6 +274,95 @@ int tfm_expert_routes(const tfm_plan* plan, const void* x, int64_t tokens,
                       int32_t* inverse, void* workspace, size_t workspace_bytes,
                       void* stream);
 
+/* ---- operators around the block ---------------------------------------- */
+/* What a decoder layer runs between two blocks and behind the last one. The
+ * fused block keeps the reference's own norm (tfm_moe_forward_rmsnorm); these
+ * have no counterpart in the reference. None needs a plan; rows are dense
+ * (row t starts at t * width elements) unless a stride is given; rows may be 0
+ * (nothing is read or written), at most 2^22 - 1. Activations are
+ * TFM_DTYPE_BF16 or TFM_DTYPE_F16. Rows and pointers need no alignment beyond
+ * their elements', except the codes of the products (below); 16-byte aligned
+ * ones with widths of a multiple of 8 move faster. */
+
+#define TFM_GATE_NONE 0    /* no gate                                      */
+#define TFM_GATE_CHANNEL 1 /* gate [width] in the storage dtype             */
+#define TFM_GATE_TOKEN 2   /* gate [rows] fp32                              */
+#define TFM_GATE_FULL 3    /* gate [rows, width] in the storage dtype       */
+
+/* Post norm, gate, residual and the next pre norm in one pass:
+ *   b = y                                    (post_weight NULL), or
+ *       y * rsqrt(mean(y*y) + post_eps) * post_weight
+ *   h = residual + residual_multiplier * gate * b   (residual NULL: 0)
+ *   x = h * rsqrt(mean(h*h) + pre_eps) * pre_weight
+ * in fp32 from the unrounded h; each output is rounded once. Outputs (at
+ * least one): h [rows, width]; with pre_weight also x [rows, width] in the
+ * storage dtype and/or codes [rows, width] with scales [rows] (as
+ * tfm_quantize_rows makes them, from the unrounded x). h may be y or residual
+ * itself (same address); no other overlap. width <= 32768. */
+typedef struct tfm_norm_step {
+  const void* y;           /* [rows, width]                                */
+  const void* residual;    /* [rows, width] or NULL                        */
+  const void* post_weight; /* [width] or NULL                              */
+  const void* gate;        /* by gate_kind                                 */
+  const void* pre_weight;  /* [width] or NULL                              */
+  void* h;                 /* out or NULL                                  */
+  void* x;                 /* out or NULL; needs pre_weight                */
+  int8_t* codes;           /* out or NULL; needs pre_weight and scales     */
+  float* scales;           /* out or NULL; needs codes                     */
+  int32_t gate_kind;       /* TFM_GATE_*                                   */
+  float residual_multiplier;
+  float post_eps, pre_eps; /* non-negative                                 */
+} tfm_norm_step;
+int tfm_norm_residual(const tfm_norm_step* step, int64_t rows, int32_t width, int32_t dtype,
+                      void* stream);
+
+/* Rows to 8-bit codes with a scale each: a = max(max|x[t, :]|, 2^-100),
+ * scales[t] = a / 127, codes[t, k] = round_half_even(x[t, k] * (127 / a)) in
+ * [-127, 127], so that codes * scales is x to half a step. A row with an
+ * infinity or a NaN gets codes 0 and scale NaN. width <= 131072. Serves tokens
+ * (x [rows, width]) and weight channels (w [n_out, k_in]) alike. */
+int tfm_quantize_rows(const void* x, int64_t rows, int32_t width, int32_t dtype, int8_t* codes,
+                      float* scales, void* stream);
+
+/* Product in 8-bit integers:
+ *   out[t, n] = (sum_k x[t, k] * w[n, k]) * x_scales[t] * w_scales[n] + bias[n]
+ * with an exact 32-bit sum and the rest in fp32, rounded once to dtype (here
+ * also TFM_DTYPE_F32). x [rows, k_in] and w [n_out, k_in] int8, 16-byte aligned
+ * (any int8 value, -128 included: k_in bounds the sum); bias [n_out] in dtype
+ * or NULL; out [rows, n_out]. k_in: a multiple of 16, at most 131056. n_out is
+ * any positive number. */
+#define TFM_DTYPE_F32 2 /* output of tfm_int8_qmm, logits of tfm_token_logprobs */
+int tfm_int8_qmm(const int8_t* x, const float* x_scales, int64_t rows, const int8_t* w,
+                 const float* w_scales, const void* bias, int32_t n_out, int32_t k_in,
+                 int32_t dtype, void* out, void* stream);
+
+/* tfm_quantize_rows of x [rows, k_in] (dtype) into the workspace, then
+ * tfm_int8_qmm: a linear with 8-bit weights. The workspace keeps nothing
+ * between calls and has no status word; tfm_quantize_rows' width limit holds. */
+size_t tfm_int8_linear_workspace_bytes(int64_t rows, int32_t k_in);
+int tfm_int8_linear(const void* x, int64_t rows, const int8_t* w, const float* w_scales,
+                    const void* bias, int32_t n_out, int32_t k_in, int32_t dtype, void* out,
+                    void* workspace, size_t workspace_bytes, void* stream);
+
+/* Log probabilities under softmax(scale * logits) over each row, in one pass
+ * over logits [rows, vocab] (dtype bf16, f16 or TFM_DTYPE_F32; row t starts at
+ * t * row_stride elements, row_stride >= vocab):
+ *   logprobs [rows]            of tokens[t] (int32 or int64 by token_bits 32 or
+ *                              64); NaN where tokens[t] is outside [0, vocab)
+ *   entropy [rows]             -sum p ln p, in nats
+ *   top_ids, top_logprobs [rows, top]  the top largest logits, largest first,
+ *                              ties to the lower id, NaN last (the order of
+ *                              tfm_topk's TFM_ROUTE_OLMOE rule); top <= 64, <= vocab
+ * all fp32 / int32; tokens with logprobs may be NULL, entropy may be NULL,
+ * top may be 0. Masked logits are -inf (probability 0, log probability -inf).
+ * A row of nothing but -inf has entropy 0 and log probabilities -inf; one with
+ * +inf or NaN has NaN for all of its log probabilities and its entropy. scale:
+ * positive and finite (1 / temperature, or a model's logit scaling). */
+int tfm_token_logprobs(const void* logits, int64_t rows, int32_t vocab, int64_t row_stride,
+                       int32_t dtype, const void* tokens, int32_t token_bits, int32_t top,
+                       float scale, float* logprobs, float* entropy, int32_t* top_ids,
+                       float* top_logprobs, void* stream);
+
 /* ---- stage profiler ---------------------------------------------------- */
 /* Kernel stages of tfm_moe_forward / tfm_moe_experts. */
 #define TFM_STAGE_ROUTER 0  /* router linear                               */

@@ -21,6 +21,7 @@ TFM_E_DEVICE = 5
 
 TFM_DTYPE_BF16 = 0
 TFM_DTYPE_F16 = 1
+TFM_DTYPE_F32 = 2
 TFM_ROUTE_OLMOE = 0
 TFM_ROUTE_GRANITE = 1
 TFM_ROUTER_DENSE = 0
@@ -35,6 +36,10 @@ TFM_STAGE_GATEUP = 3
 TFM_STAGE_DOWN = 4
 TFM_STAGE_COMBINE = 5
 TFM_STAGE_NORM = 6
+TFM_GATE_NONE = 0
+TFM_GATE_CHANNEL = 1
+TFM_GATE_TOKEN = 2
+TFM_GATE_FULL = 3
 TFM_STATIC_SCRATCH_BYTES = 64 << 20
 TFM_STAGE_COUNT = 7
 
@@ -90,6 +95,24 @@ class MoeWeights(ctypes.Structure):
     ]
 
 
+class NormStep(ctypes.Structure):
+    _fields_ = [
+        ("y", c_void_p),
+        ("residual", c_void_p),
+        ("post_weight", c_void_p),
+        ("gate", c_void_p),
+        ("pre_weight", c_void_p),
+        ("h", c_void_p),
+        ("x", c_void_p),
+        ("codes", c_void_p),
+        ("scales", c_void_p),
+        ("gate_kind", c_int32),
+        ("residual_multiplier", c_float),
+        ("post_eps", c_float),
+        ("pre_eps", c_float),
+    ]
+
+
 # name -> (restype, argtypes); every function of include/trifuse_moe.h.
 SIGNATURES = {
     "tfm_plan_create": (c_int, [POINTER(Geometry), POINTER(c_void_p)]),
@@ -126,6 +149,15 @@ SIGNATURES = {
     "tfm_expert_routes": (c_int, [c_void_p, c_void_p, c_int64, c_void_p, c_void_p, c_int64, c_int32,
                                   POINTER(MoeWeights), c_void_p, c_void_p, c_void_p, c_size_t,
                                   c_void_p]),
+    "tfm_norm_residual": (c_int, [POINTER(NormStep), c_int64, c_int32, c_int32, c_void_p]),
+    "tfm_quantize_rows": (c_int, [c_void_p, c_int64, c_int32, c_int32, c_void_p, c_void_p, c_void_p]),
+    "tfm_int8_qmm": (c_int, [c_void_p, c_void_p, c_int64, c_void_p, c_void_p, c_void_p, c_int32, c_int32,
+                             c_int32, c_void_p, c_void_p]),
+    "tfm_int8_linear_workspace_bytes": (c_size_t, [c_int64, c_int32]),
+    "tfm_int8_linear": (c_int, [c_void_p, c_int64, c_void_p, c_void_p, c_void_p, c_int32, c_int32, c_int32,
+                                c_void_p, c_void_p, c_size_t, c_void_p]),
+    "tfm_token_logprobs": (c_int, [c_void_p, c_int64, c_int32, c_int64, c_int32, c_void_p, c_int32, c_int32,
+                                   c_float, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p]),
     "tfm_profiler_create": (c_int, [c_int32, POINTER(c_void_p)]),
     "tfm_profiler_destroy": (None, [c_void_p]),
     "tfm_profiler_attach": (c_int, [c_void_p]),

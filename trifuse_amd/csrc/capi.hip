@@ -84,33 +84,12 @@ struct StageScope {
 };
 
 void set_last_error(const std::string& message) { g_last_error = message; }
+void clear_last_error() { g_last_error.clear(); }
 
 [[noreturn]] void fail(int code, const std::string& message) { throw Error{code, message}; }
 
 void check_hip(hipError_t err, const char* what) {
   if (err != hipSuccess) fail(TFM_E_HIP, std::string(what) + ": " + hipGetErrorString(err));
-}
-
-template <typename F>
-static int guarded(F&& f) {
-  try {
-    f();
-    g_last_error.clear();
-    return TFM_OK;
-  } catch (const Error& e) {
-    g_last_error = e.message;
-    return e.code;
-  } catch (const std::exception& e) {
-    g_last_error = std::string("internal error: ") + e.what();
-    return TFM_E_INVALID;
-  } catch (...) {
-    g_last_error = "internal error";
-    return TFM_E_INVALID;
-  }
-}
-
-static void need(bool ok, const std::string& message) {
-  if (!ok) fail(TFM_E_INVALID, message);
 }
 
 static void check_geometry(const tfm_geometry& g) {
@@ -343,21 +322,6 @@ static GroupWs carve_group(int64_t n, int E, void* base) {
   w.hist = c.take<int32_t>((size_t)group_hist_rows(group_blocks(n, kGroupChunk)) * (E + 1));
   w.bytes = align_up(c.offset, 256);
   return w;
-}
-
-static void need_ws(void* ws, size_t have, size_t want) {
-  if (!ws) fail(TFM_E_WORKSPACE, "workspace is null");
-  if ((reinterpret_cast<uintptr_t>(ws) & 255) != 0) fail(TFM_E_WORKSPACE, "workspace must be 256-byte aligned");
-  if (have < want)
-    fail(TFM_E_WORKSPACE, "workspace too small: " + std::to_string(have) + " < " + std::to_string(want));
-}
-
-static void need_ptr(const void* p, const char* name) {
-  if (!p) fail(TFM_E_INVALID, std::string(name) + " is null");
-}
-
-static void need_align16(const void* p, const char* name) {
-  if (reinterpret_cast<uintptr_t>(p) & 15) fail(TFM_E_INVALID, std::string(name) + " must be 16-byte aligned");
 }
 
 static void check_affine(const tfm_affine& a, const char* name) {

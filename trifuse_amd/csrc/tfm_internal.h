@@ -6,6 +6,7 @@
 #include <stddef.h>
 #include <stdint.h>
 
+#include <exception>
 #include <string>
 #include <utility>
 
@@ -21,6 +22,43 @@ struct Error {
 [[noreturn]] void fail(int code, const std::string& message);
 void check_hip(hipError_t err, const char* what);
 void set_last_error(const std::string& message);
+void clear_last_error();
+
+// Runs an entry point's body: TFM_OK, or the code of the error it threw.
+template <typename F>
+int guarded(F&& f) {
+  try {
+    f();
+    clear_last_error();
+    return TFM_OK;
+  } catch (const Error& e) {
+    set_last_error(e.message);
+    return e.code;
+  } catch (const std::exception& e) {
+    set_last_error(std::string("internal error: ") + e.what());
+    return TFM_E_INVALID;
+  } catch (...) {
+    set_last_error("internal error");
+    return TFM_E_INVALID;
+  }
+}
+
+// Argument checks of the entry points.
+inline void need(bool ok, const char* message) {
+  if (!ok) fail(TFM_E_INVALID, message);
+}
+inline void need_ptr(const void* p, const char* name) {
+  if (!p) fail(TFM_E_INVALID, std::string(name) + " is null");
+}
+inline void need_align16(const void* p, const char* name) {
+  if (reinterpret_cast<uintptr_t>(p) & 15) fail(TFM_E_INVALID, std::string(name) + " must be 16-byte aligned");
+}
+inline void need_ws(void* ws, size_t have, size_t want) {
+  if (!ws) fail(TFM_E_WORKSPACE, "workspace is null");
+  if ((reinterpret_cast<uintptr_t>(ws) & 255) != 0) fail(TFM_E_WORKSPACE, "workspace must be 256-byte aligned");
+  if (have < want)
+    fail(TFM_E_WORKSPACE, "workspace too small: " + std::to_string(have) + " < " + std::to_string(want));
+}
 
 inline size_t align_up(size_t v, size_t a) { return (v + a - 1) / a * a; }
 
@@ -134,6 +172,32 @@ void launch_topk_hist(int route_kind, bool f16, const uint16_t* logits, int T, i
 // dtype (bf16, or half when f16), one wave per row, bit-defined order.
 void launch_rmsnorm(bool f16, const uint16_t* x, const uint16_t* w, float eps, int T, int H,
                     uint16_t* out, hipStream_t s);
+
+// The operators around the block (residual.hip, igemm.hip, logprobs.hip).
+// Widest row that norm_residual keeps in registers, and quantize_rows.
+constexpr int kNormMaxWidth = 32768;
+constexpr int kQuantizeMaxWidth = 131072;
+// Rows of one call: a workgroup of up to 1024 threads each, under 2^32 threads.
+constexpr int64_t kMaxRows = (1 << 22) - 1;
+void launch_norm_residual(bool f16, const tfm_norm_step& step, int rows, int width, hipStream_t s);
+void launch_quantize_rows(bool f16, const uint16_t* x, int rows, int width, int8_t* codes, float* scales,
+                          hipStream_t s);
+// out[t, n] = st((sum_k x[t, k] w[n, k]) * x_scales[t] * w_scales[n] + bias[n]); K a multiple of 16.
+void launch_int8_qmm(int dtype, const int8_t* x, const float* x_scales, int64_t rows, const int8_t* w,
+                     const float* w_scales, const void* bias, int N, int K, void* out, hipStream_t s);
+struct LogprobsArgs {
+  const void* logits;
+  int64_t row_stride;  // elements
+  int rows, vocab, top;
+  float scale;
+  const void* tokens;  // int32 or int64, or null
+  bool tokens64;
+  float* logprobs;
+  float* entropy;
+  int32_t* top_ids;
+  float* top_logprobs;
+};
+void launch_token_logprobs(int dtype, const LogprobsArgs& a, hipStream_t s);
 
 // Decode path (decode.hip), T*K <= 256 routes.
 // The decode logits on the affine router itself (bits 4 or 8), each row

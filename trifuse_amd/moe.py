@@ -342,11 +342,15 @@ class MoEBlock:
         call("tfm_plan_create", ctypes.byref(self.geometry), ctypes.byref(handle))
         self._lib = lib
         self._plan = handle
+        self._unit: Optional[ctypes.c_void_p] = None
         self._ws: Optional[torch.Tensor] = None
         self._ws_bytes: Dict[int, int] = {}
         self._wcache: Dict[Tuple[int, bool], tuple] = {}
 
     def close(self) -> None:
+        if getattr(self, "_unit", None):
+            self._lib.tfm_plan_destroy(self._unit)
+            self._unit = None
         if getattr(self, "_plan", None):
             self._lib.tfm_plan_destroy(self._plan)
             self._plan = None
@@ -515,6 +519,40 @@ class MoEBlock:
              ctypes.byref(mw), y.data_ptr(), _ptr(idx), _ptr(gates), 0, ws.data_ptr(), ws.numel(),
              _stream())
         return (y, idx, gates) if return_routes else y
+
+    def forward_norms(self, h: torch.Tensor, weights: ExpertWeights, norm_weight: torch.Tensor, eps: float,
+                      post_weight: Optional[torch.Tensor] = None, gate: Optional[torch.Tensor] = None,
+                      next_weight: Optional[torch.Tensor] = None):
+        """The block between its norms (layer.rms_norm, layer.norm_residual):
+        y = moe(rms_norm(h, norm_weight, eps)) without residual or multiplier, then
+        h' = h + rm * gate * rms_norm(y, post_weight, eps) in one pass. post_weight
+        None: y as it is; gate: as layer.norm_residual. With next_weight also returns
+        the next block's input rms_norm(h', next_weight, eps), from the unrounded h'.
+        y is rounded to the storage dtype; the norms round once, where
+        forward_rmsnorm's keeps the reference's two roundings."""
+        from . import layer
+
+        T = self._check_x(h)
+        x = layer.rms_norm(h, norm_weight, eps)
+        mw = self._weights(weights, router=True)
+        y = torch.empty_like(h)
+        ws = self.workspace(T, h.device)
+        call("tfm_moe_forward", self._unit_plan(), x.data_ptr(), T, None, ctypes.byref(mw), y.data_ptr(), None, None,
+             0, ws.data_ptr(), ws.numel(), _stream())
+        return layer.norm_residual(y, h, post_weight=post_weight, gate=gate,
+                                   residual_multiplier=self.residual_multiplier, pre_weight=next_weight, eps=eps)
+
+    def _unit_plan(self):
+        """The block's plan with residual multiplier 1 (its own where that is 1)."""
+        if self.residual_multiplier == 1.0:
+            return self._plan
+        if self._unit is None:
+            g = Geometry.from_buffer_copy(self.geometry)
+            g.residual_multiplier = 1.0
+            handle = ctypes.c_void_p()
+            call("tfm_plan_create", ctypes.byref(g), ctypes.byref(handle))
+            self._unit = handle
+        return self._unit
 
     def route(self, x: torch.Tensor, router: torch.Tensor, logit_bias: Optional[torch.Tensor] = None):
         """Router linear + routing: (idx [T,K] int32, gates [T,K], logits [T,E] bf16).
