@@ -336,9 +336,10 @@ int tfm_int8_qmm(const int8_t* x, const float* x_scales, int64_t rows, const int
                  const float* w_scales, const void* bias, int32_t n_out, int32_t k_in,
                  int32_t dtype, void* out, void* stream);
 
-/* tfm_quantize_rows of x [rows, k_in] (dtype) into the workspace, then
- * tfm_int8_qmm: a linear with 8-bit weights. The workspace keeps nothing
- * between calls and has no status word; tfm_quantize_rows' width limit holds. */
+/* tfm_quantize_rows of x [rows, k_in] (dtype), then tfm_int8_qmm: a linear with
+ * 8-bit weights, bit for bit those two calls. Few rows (where the bytes below
+ * are 0) need no workspace; else it holds the codes and scales, keeps nothing
+ * between calls and has no status word. */
 size_t tfm_int8_linear_workspace_bytes(int64_t rows, int32_t k_in);
 int tfm_int8_linear(const void* x, int64_t rows, const int8_t* w, const float* w_scales,
                     const void* bias, int32_t n_out, int32_t k_in, int32_t dtype, void* out,

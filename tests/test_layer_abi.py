@@ -91,14 +91,15 @@ def test_int8_qmm_rejects(kw, code, msg):
 
 def test_int8_linear_rejects():
     lib = _lib.load()
-    need = lib.tfm_int8_linear_workspace_bytes(5, 256)
-    assert need >= 5 * 256 + 5 * 4 and lib.tfm_int8_linear_workspace_bytes(-1, 256) == 0
-    check(lib.tfm_int8_linear(P, 5, P, P, None, 64, 256, F32, P, P, need, None), 1, "dtype")
-    check(lib.tfm_int8_linear(P, 5, P, P, None, 64, 256, BF16, P, P, need - 1, None), 3, "too small")
-    check(lib.tfm_int8_linear(P, 5, P, P, None, 64, 256, BF16, P, P + 16, need, None), 3, "aligned")
-    check(lib.tfm_int8_linear(P, 5, P, P, None, 64, 256, BF16, P, None, need, None), 3, "null")
-    check(lib.tfm_int8_linear(None, 5, P, P, None, 64, 256, BF16, P, P, need, None), 1, "x is null")
-    check(lib.tfm_int8_linear(P, 5, P, P, None, 64, 250, BF16, P, P, need, None), 2, "multiple of 16")
+    need = lib.tfm_int8_linear_workspace_bytes(500, 256)
+    assert need >= 500 * 256 + 500 * 4 and lib.tfm_int8_linear_workspace_bytes(-1, 256) == 0
+    assert lib.tfm_int8_linear_workspace_bytes(1, 256) == 0
+    check(lib.tfm_int8_linear(P, 500, P, P, None, 64, 256, F32, P, P, need, None), 1, "dtype")
+    check(lib.tfm_int8_linear(P, 500, P, P, None, 64, 256, BF16, P, P, need - 1, None), 3, "too small")
+    check(lib.tfm_int8_linear(P, 500, P, P, None, 64, 256, BF16, P, P + 16, need, None), 3, "aligned")
+    check(lib.tfm_int8_linear(P, 500, P, P, None, 64, 256, BF16, P, None, need, None), 3, "null")
+    check(lib.tfm_int8_linear(None, 500, P, P, None, 64, 256, BF16, P, P, need, None), 1, "x is null")
+    check(lib.tfm_int8_linear(P, 500, P, P, None, 64, 250, BF16, P, P, need, None), 2, "multiple of 16")
     check(lib.tfm_int8_linear(None, 0, None, None, None, 64, 256, BF16, None, None, 0, None), 0, "")
 
 

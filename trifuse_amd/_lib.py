@@ -195,7 +195,7 @@ def load() -> ctypes.CDLL:
 
 def call(name: str, *args) -> None:
     """Call an int-returning entry point and raise TfmError on failure."""
-    lib = load()
+    lib = _lib if _lib is not None else load()
     status = getattr(lib, name)(*args)
     if status != TFM_OK:
         msg = lib.tfm_last_error().decode(errors="replace")

@@ -100,7 +100,7 @@ int tfm_int8_qmm(const int8_t* x, const float* x_scales, int64_t rows, const int
 }
 
 size_t tfm_int8_linear_workspace_bytes(int64_t rows, int32_t k_in) {
-  if (rows < 0 || rows > kMaxRows || k_in <= 0) return 0;
+  if (rows < 0 || rows > kMaxRows || k_in <= 0 || int8_linear_few(rows, k_in)) return 0;
   return carve_linear(rows, k_in, nullptr).bytes;
 }
 
@@ -116,9 +116,14 @@ int tfm_int8_linear(const void* x, int64_t rows, const int8_t* w, const float* w
     need_ptr(w_scales, "w_scales");
     need_ptr(out, "out");
     need_align16(w, "w");
+    hipStream_t s = static_cast<hipStream_t>(stream);
+    if (int8_linear_few(rows, k_in)) {
+      launch_int8_linear_few(dtype == TFM_DTYPE_F16, static_cast<const uint16_t*>(x), rows, w, w_scales, bias, n_out,
+                             k_in, out, s);
+      return;
+    }
     const LinearWs ws = carve_linear(rows, k_in, workspace);
     need_ws(workspace, workspace_bytes, ws.bytes);
-    hipStream_t s = static_cast<hipStream_t>(stream);
     launch_quantize_rows(dtype == TFM_DTYPE_F16, static_cast<const uint16_t*>(x), (int)rows, k_in, ws.codes, ws.scales,
                          s);
     launch_int8_qmm(dtype, ws.codes, ws.scales, rows, w, w_scales, bias, n_out, k_in, out, s);

@@ -6,11 +6,13 @@
 // igemm_tile_kernel: BM tokens x BN channels a workgroup, 32x32x32 MFMAs. Both
 // operands go from memory straight into LDS (16 bytes a lane), 128 bytes of K a
 // stage, two stages; a row's eight 16-byte pieces are stored in the order
-// piece ^ (row % 8), so that the 8 rows a quarter-wave reads lie in different banks.
+// piece ^ (row / 2 % 8), so that the 16 rows that are read at a time (256 bytes a
+// clock) lie in different banks.
 #include <type_traits>
 
 #include "tfm_device.h"
 #include "tfm_internal.h"
+#include "rows.h"
 
 namespace tfm {
 
@@ -44,13 +46,27 @@ __device__ __forceinline__ i32x16_t mfma_i8(i32x4_t a, i32x4_t b, i32x16_t c) {
 #endif
 }
 
+__device__ __forceinline__ i32x4_t mfma_i8_16(i32x4_t a, i32x4_t b, i32x4_t c) {
+#if defined(__HIP_DEVICE_COMPILE__)
+  return __builtin_amdgcn_mfma_i32_16x16x64_i8(a, b, c, 0, 0, 0);
+#else
+  (void)a; (void)b;
+  return c;
+#endif
+}
+
 // One output in the storage type OUT (TFM_DTYPE_*).
 template <int OUT>
 struct Out {
   using type = std::conditional_t<OUT == TFM_DTYPE_F32, float, uint16_t>;
-  __device__ static __forceinline__ type make(float v) {
-    if constexpr (OUT == TFM_DTYPE_F32) return v;
-    else return f2st<OUT == TFM_DTYPE_F16>(v);
+  __device__ static __forceinline__ void pair(type* to, float a, float b) {
+    if constexpr (OUT == TFM_DTYPE_F32) {
+      to[0] = a;
+      to[1] = b;
+    } else {
+      const uint32_t p = pack_st2<OUT == TFM_DTYPE_F16>(a, b);
+      __builtin_memcpy(to, &p, 4);
+    }
   }
   __device__ static __forceinline__ float wide(type v) {
     if constexpr (OUT == TFM_DTYPE_F32) return v;
@@ -66,40 +82,73 @@ struct IgArgs {
   const void* bias;
   void* out;
   int T, N, K;
+  int mt, nt;     // tiles of the grid
+  bool vec_out;   // rows of out start at 16-byte lines
 };
 
-template <int BM, int BN, int WM, int WN, int OUT>
-__global__ __launch_bounds__(BM / WM * (BN / WN) * 64) void igemm_tile_kernel(IgArgs a) {
+// Tile of workgroup `id` of a grid of mt x nt tiles: workgroups go round robin
+// to the 8 XCDs, each of which takes a contiguous run of tiles, in bands of
+// kBand token tiles walked channel tile by channel tile, so that the tiles an
+// XCD works on at a time share rows of both operands in its L2.
+constexpr int kXcds = 8, kBand = 8;
+__device__ __forceinline__ int2 ig_tile(int id, int mt, int nt) {
+  const int tiles = mt * nt, q = tiles / kXcds, r = tiles % kXcds;
+  const int xcd = id % kXcds, at = xcd * q + (xcd < r ? xcd : r) + id / kXcds;
+  const int band = at / (kBand * nt), left = mt - band * kBand, h = left < kBand ? left : kBand;
+  const int in = at - band * kBand * nt;
+  return make_int2(band * kBand + in % h, in / h);
+}
+
+// PIECE outputs (16 bytes) at column c of a row, those below N.
+template <typename T, int PIECE>
+__device__ __forceinline__ void store_piece(T* row, int c, int N, bool vec, const T* v) {
+  if (vec && c + PIECE <= N) {
+    *reinterpret_cast<uint4*>(row + c) = *reinterpret_cast<const uint4*>(v);
+  } else {
+#pragma unroll
+    for (int j = 0; j < PIECE; ++j)
+      if (c + j < N) row[c + j] = v[j];
+  }
+}
+
+template <int BM, int BN, int WM, int WN, int MINW, int OUT>
+__global__ __launch_bounds__(BM / WM * (BN / WN) * 64, MINW) void igemm_tile_kernel(IgArgs a) {
   constexpr int WAVES_M = BM / WM, WAVES_N = BN / WN, WAVES = WAVES_M * WAVES_N;
   constexpr int MB = WM / 32, NB = WN / 32;
   constexpr int LX = BM / 8 / WAVES, LW = BN / 8 / WAVES;  // 8-row copies a wave makes per stage
+  static_assert(WAVES == 4 || WAVES == 8, "a stage array serves one or two waves in the epilogue");
   static_assert(LX * 8 * WAVES == BM && LW * 8 * WAVES == BN, "copies tile the rows");
+  // One array a stage and operand, so that reads of one stage do not wait for copies into the other.
   __shared__ __attribute__((aligned(128))) int8_t sx0[BM * kBK], sx1[BM * kBK], sw0[BN * kBK], sw1[BN * kBK];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int m0 = blockIdx.y * BM, n0 = blockIdx.x * BN;
+  const int2 tile = ig_tile(blockIdx.x, a.mt, a.nt);
+  const int m0 = tile.x * BM, n0 = tile.y * BN;
   const int K = a.K, KT = (K + kBK - 1) / kBK;
   const int mrows = a.T - m0 < BM ? a.T - m0 : BM, nrows = a.N - n0 < BN ? a.N - n0 : BN;
   const auto rx = ig_rsrc(a.x + (int64_t)m0 * K, (uint32_t)mrows * (uint32_t)K);
   const auto rw = ig_rsrc(a.w + (int64_t)n0 * K, (uint32_t)nrows * (uint32_t)K);
-  // This lane's piece of an 8-row copy; pieces past K read out of range (zeros).
-  const int crow = lane >> 3, piece = (lane & 7) ^ crow;
+  // This lane's piece of an 8-row copy. Rows past the matrix are out of the
+  // buffer's range and pieces past K are sent there: both read as zeros.
+  const int crow = lane >> 3, piece = (lane & 7) ^ ((4 * wave + (crow >> 1)) & 7);  // rows 8 apart by wave, then by 8 * WAVES
+  const uint32_t v0 = (uint32_t)((wave * 8 + crow) * K + piece * 16);
+  const uint32_t hop = (uint32_t)(WAVES * 8 * K);  // between this wave's copies
   auto load = [&](int8_t* dx, int8_t* dw, int kt) {
-    const bool past = kt * kBK + piece * 16 >= K;
+    const uint32_t soff = (uint32_t)(kt * kBK), v = (int)soff + piece * 16 >= K ? 0x80000000u : v0;
 #pragma unroll
-    for (int i = 0; i < LX; ++i) {
-      const int r = (i * WAVES + wave) * 8;
-      ig_dma16(rx, dx + r * kBK, past ? 0x80000000u : (uint32_t)((r + crow) * K + piece * 16), (uint32_t)(kt * kBK));
-    }
+    for (int i = 0; i < LX; ++i) ig_dma16(rx, dx + (i * WAVES + wave) * 8 * kBK, v + i * hop, soff);
 #pragma unroll
-    for (int i = 0; i < LW; ++i) {
-      const int r = (i * WAVES + wave) * 8;
-      ig_dma16(rw, dw + r * kBK, past ? 0x80000000u : (uint32_t)((r + crow) * K + piece * 16), (uint32_t)(kt * kBK));
-    }
+    for (int i = 0; i < LW; ++i) ig_dma16(rw, dw + (i * WAVES + wave) * 8 * kBK, v + i * hop, soff);
   };
   const int wm = wave % WAVES_M * WM, wn = wave / WAVES_M * WN;
   const int fr = lane & 31, fk = lane >> 5;  // fragment row, its 16-byte half of 32
-  auto frag = [&](const int8_t* s, int row, int ks) {
-    return *reinterpret_cast<const i32x4_t*>(s + row * kBK + (((2 * ks + fk) ^ (row & 7)) << 4));
+  i32x4_t fx[2][MB], fw[2][NB];
+  auto read = [&](auto buf, const int8_t* sx, const int8_t* sw, int ks) {
+    constexpr int B = decltype(buf)::value;
+    const int at = fr * kBK + (((2 * ks + fk) ^ ((fr >> 1) & 7)) << 4);
+#pragma unroll
+    for (int m = 0; m < MB; ++m) fx[B][m] = *reinterpret_cast<const i32x4_t*>(sx + (wm + 32 * m) * kBK + at);
+#pragma unroll
+    for (int n = 0; n < NB; ++n) fw[B][n] = *reinterpret_cast<const i32x4_t*>(sw + (wn + 32 * n) * kBK + at);
   };
   i32x16_t acc[NB][MB];
 #pragma unroll
@@ -108,65 +157,272 @@ __global__ __launch_bounds__(BM / WM * (BN / WN) * 64) void igemm_tile_kernel(Ig
     for (int m = 0; m < MB; ++m)
 #pragma unroll
       for (int i = 0; i < 16; ++i) acc[n][m][i] = 0;
-  auto compute = [&](const int8_t* sx, const int8_t* sw) {
-#pragma unroll
-    for (int ks = 0; ks < 4; ++ks) {
-      i32x4_t fx[MB], fw[NB];
-#pragma unroll
-      for (int m = 0; m < MB; ++m) fx[m] = frag(sx, wm + 32 * m + fr, ks);
-#pragma unroll
-      for (int n = 0; n < NB; ++n) fw[n] = frag(sw, wn + 32 * n + fr, ks);
-#pragma unroll
-      for (int n = 0; n < NB; ++n)
-#pragma unroll
-        for (int m = 0; m < MB; ++m) acc[n][m] = mfma_i8(fw[n], fx[m], acc[n][m]);
-    }
-  };
-  load(sx0, sw0, 0);
-  __syncthreads();
-  for (int kt = 0; kt < KT; kt += 2) {
-    if (kt + 1 < KT) load(sx1, sw1, kt + 1);
-    compute(sx0, sw0);
-    __syncthreads();
-    if (kt + 1 >= KT) break;
-    if (kt + 2 < KT) load(sx0, sw0, kt + 2);
-    compute(sx1, sw1);
-    __syncthreads();
-  }
-  // Lane l holds token l % 32 and channels 8 (i / 4) + 4 (l / 32) + i % 4 of each 32 x 32 block.
-  using O = Out<OUT>;
-  typename O::type* out = static_cast<typename O::type*>(a.out);
-  const typename O::type* bias = static_cast<const typename O::type*>(a.bias);
-#pragma unroll
-  for (int m = 0; m < MB; ++m) {
-    const int t = m0 + wm + 32 * m + fr;
-    if (t >= a.T) continue;
-    const float xs = a.xs[t];
+  auto mma = [&](auto buf, int from, int to) {
+    constexpr int B = decltype(buf)::value;
 #pragma unroll
     for (int n = 0; n < NB; ++n)
 #pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        const int c = n0 + wn + 32 * n + 8 * (i / 4) + 4 * fk + i % 4;
-        if (c < a.N) {
-          float v = (float)acc[n][m][i] * xs * a.ws[c];
-          if (bias) v += O::wide(bias[c]);
-          out[(int64_t)t * a.N + c] = O::make(v);
-        }
+      for (int m = 0; m < MB; ++m)
+        if (n * MB + m >= from && n * MB + m < to) acc[n][m] = mfma_i8(fw[B][n], fx[B][m], acc[n][m]);
+  };
+  using B0 = std::integral_constant<int, 0>;
+  using B1 = std::integral_constant<int, 1>;
+  // A step's fragment reads spread over its products.
+  auto spread = [&] {
+#pragma unroll
+    for (int i = 0; i < MB + NB; ++i) {
+      __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+      __builtin_amdgcn_sched_group_barrier(0x008, (MB * NB + MB + NB - 1) / (MB + NB), 0);
+    }
+    __builtin_amdgcn_sched_barrier(0);
+  };
+  // One stage: four steps of 32 bytes of K, each step's fragments read during
+  // the one before. The stage's last fragments are in registers before its last
+  // step's products: there all waves meet, the next stage is complete, its first
+  // fragments are read and this stage's arrays take the stage after next.
+  auto stage = [&](int8_t* cx, int8_t* cw, int8_t* nx, int8_t* nw, int kt) {
+    constexpr int ALL = MB * NB, FIRST = ALL > MB ? MB : 0;
+    read(B1{}, cx, cw, 1);
+    mma(B0{}, 0, ALL);
+    spread();
+    read(B0{}, cx, cw, 2);
+    mma(B1{}, 0, ALL);
+    spread();
+    read(B1{}, cx, cw, 3);
+    mma(B0{}, 0, ALL);
+    spread();
+    mma(B1{}, 0, FIRST);
+    __syncthreads();
+    __builtin_amdgcn_sched_barrier(0);
+    read(B0{}, nx, nw, 0);
+    load(cx, cw, kt + 2);
+    mma(B1{}, FIRST, ALL);
+#pragma unroll
+    for (int i = 0; i < ALL - FIRST; ++i) {
+      __builtin_amdgcn_sched_group_barrier(0x100, (MB + NB + ALL - FIRST - 1) / (ALL - FIRST), 0);
+      __builtin_amdgcn_sched_group_barrier(0x020, (LX + LW + ALL - FIRST - 1) / (ALL - FIRST), 0);
+      __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+    }
+    __builtin_amdgcn_sched_barrier(0);
+  };
+  load(sx0, sw0, 0);
+  __syncthreads();
+  load(sx1, sw1, 1);
+  read(B0{}, sx0, sw0, 0);
+  // Stages past the last are zeros: an odd count runs one of them.
+  for (int kt = 0; kt < KT; kt += 2) {
+    stage(sx0, sw0, sx1, sw1, kt);
+    stage(sx1, sw1, sx0, sw0, kt + 1);
+  }
+  __syncthreads();  // the copies past the end
+  // Epilogue. Lane l holds token l % 32 and channels 8 (i / 4) + 4 (l / 32) + i % 4
+  // of each 32 x 32 block: scaled and rounded, 32 tokens at a time go through the
+  // wave's own part of LDS (every wave is past its last read of it) and leave as
+  // 16-byte pieces of rows.
+  using O = Out<OUT>;
+  using T = typename O::type;
+  constexpr int PIECE = 16 / (int)sizeof(T), ROW = WN + PIECE;  // staging row, padded
+  constexpr int STAGING = (32 * ROW * (int)sizeof(T) + 8 * WN + 15) / 16 * 16;
+  static_assert(STAGING * (WAVES / 4) <= (BM < BN ? BM : BN) * kBK, "the staging fits the arrays");
+  int8_t* mine = (wave % 4 == 0 ? sx0 : wave % 4 == 1 ? sx1 : wave % 4 == 2 ? sw0 : sw1) + wave / 4 * STAGING;
+  T* st = reinterpret_cast<T*>(mine);
+  float* cs = reinterpret_cast<float*>(mine + 32 * ROW * sizeof(T));  // channel scales, then biases
+  const T* bias = static_cast<const T*>(a.bias);
+  for (int i = lane; i < WN; i += 64) {
+    const int c = n0 + wn + i < a.N ? n0 + wn + i : a.N - 1;
+    cs[i] = a.ws[c];
+    cs[WN + i] = bias ? O::wide(bias[c]) : 0.0f;
+  }
+  const bool vec = a.vec_out;
+#pragma unroll
+  for (int m = 0; m < MB; ++m) {
+    const int t0 = m0 + wm + 32 * m, t = t0 + fr;
+    const float xs = a.xs[t < a.T ? t : a.T - 1];
+#pragma unroll
+    for (int n = 0; n < NB; ++n)
+#pragma unroll
+      for (int g = 0; g < 4; ++g) {
+        T v[4];
+        const int c = 32 * n + 8 * g + 4 * fk;
+        const f32x4_t ws = *reinterpret_cast<const f32x4_t*>(cs + c);
+        f32x4_t bs = {0.0f, 0.0f, 0.0f, 0.0f};
+        if (bias) bs = *reinterpret_cast<const f32x4_t*>(cs + WN + c);
+#pragma unroll
+        for (int i = 0; i < 4; i += 2)
+          O::pair(v + i, (float)acc[n][m][4 * g + i] * xs * ws[i] + bs[i],
+                  (float)acc[n][m][4 * g + i + 1] * xs * ws[i + 1] + bs[i + 1]);
+        __builtin_memcpy(st + fr * ROW + c, v, sizeof v);
       }
+    constexpr int PIECES = WN / PIECE;  // of a row
+#pragma unroll
+    for (int i = 0; i < 32 * PIECES / 64; ++i) {
+      const int at = i * 64 + lane, r = at / PIECES, c = at % PIECES * PIECE;
+      T v[PIECE];
+      *reinterpret_cast<uint4*>(v) = *reinterpret_cast<const uint4*>(st + r * ROW + c);
+      if (t0 + r < a.T)
+        store_piece<T, PIECE>(static_cast<T*>(a.out) + (int64_t)(t0 + r) * a.N, n0 + wn + c, a.N, vec, v);
+    }
   }
 }
 
-template <int BM, int BN, int WM, int WN>
-void launch_tile(int dtype, const IgArgs& a, hipStream_t s) {
-  const int64_t mt = ((int64_t)a.T + BM - 1) / BM, nt = ((int64_t)a.N + BN - 1) / BN;
-  if (mt > 65535 || nt > (1 << 22)) fail(TFM_E_UNSUPPORTED, "int8 product: too many output tiles in one call");
-  const dim3 grid((unsigned)nt, (unsigned)mt), block(BM / WM * (BN / WN) * 64);
-  if (dtype == TFM_DTYPE_F32)
-    igemm_tile_kernel<BM, BN, WM, WN, TFM_DTYPE_F32><<<grid, block, 0, s>>>(a);
-  else if (dtype == TFM_DTYPE_F16)
-    igemm_tile_kernel<BM, BN, WM, WN, TFM_DTYPE_F16><<<grid, block, 0, s>>>(a);
+// Up to 16 tokens: each wave multiplies 16 channels, whose weights go from memory
+// to registers as MFMA operands (16x16x64: lane l holds channel l % 16, bytes
+// 16 (l / 16) .. of each 64), with all tokens, whose codes stand in LDS. KS waves
+// share 16 channels, every KS-th 64 bytes of K each, and join their sums in LDS.
+// With FUSED the codes are made here from x itself, in every workgroup; the first
+// weights are on their way meanwhile.
+constexpr int kFewRows = 16;
+constexpr int kFewLds = 64 << 10;
+constexpr int kFewStep = 64;   // bytes of K an MFMA
+constexpr int kFewAhead = 8;   // MFMAs a wave has weights in flight for
+
+__host__ __device__ inline int few_row_bytes(int K) { return (K + kFewStep - 1) / kFewStep * kFewStep + 16; }
+inline bool few_fits(int64_t rows, int K) {
+  return rows <= kFewRows && rows * (int64_t)few_row_bytes(K) + 4096 + 64 <= kFewLds;
+}
+
+template <bool FUSED, bool F16X, int KS, int OUT>
+__global__ __launch_bounds__(256) void igemm_few_kernel(IgArgs a, const uint16_t* xh) {
+  extern __shared__ __attribute__((aligned(16))) int8_t lds[];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int K = a.K, T = a.T, N = a.N;
+  const int RB = few_row_bytes(K);  // rows 16 bytes off a multiple of 64: 8 rows of one piece hit different banks
+  int8_t* const sx = lds;
+  float* const sscale = reinterpret_cast<float*>(lds + T * RB);
+  i32x4_t* const spart = reinterpret_cast<i32x4_t*>(lds + (T * RB + 64 + 15) / 16 * 16);
+  const int n0 = (blockIdx.x * (4 / KS) + wave / KS) * 16, part = wave % KS;
+  const int S = (K + kFewStep - 1) / kFewStep;
+  const int row = n0 + (lane & 15) < N ? n0 + (lane & 15) : N - 1;
+  const int kc = (lane >> 4) * 16;
+  const int8_t* const wp = a.w + (int64_t)row * K + kc;
+
+  i32x4_t w[2][kFewAhead];
+  auto load = [&](auto buf, int s0) {
+    constexpr int B = decltype(buf)::value;
+#pragma unroll
+    for (int i = 0; i < kFewAhead; ++i) {
+      const int k = (s0 + i * KS) * kFewStep;
+      w[B][i] = i32x4_t{0, 0, 0, 0};
+      if (k + kc < K) w[B][i] = *reinterpret_cast<const i32x4_t*>(wp + k);
+    }
+  };
+  using B0 = std::integral_constant<int, 0>;
+  using B1 = std::integral_constant<int, 1>;
+  load(B0{}, part);
+
+  if constexpr (FUSED) {
+    for (int t = wave; t < T; t += 4) {
+      const RowScale rs = quantize_row_wave<F16X>(xh + (int64_t)t * K, K, sx + t * RB, lane);
+      if (lane == 0) sscale[t] = rs.scale;
+    }
+  } else {
+    const int pieces = K / 16;
+    for (int i = threadIdx.x; i < T * pieces; i += 256) {
+      const int t = i / pieces, p = i % pieces;
+      *reinterpret_cast<uint4*>(sx + t * RB + 16 * p) = *reinterpret_cast<const uint4*>(a.x + (int64_t)t * K + 16 * p);
+    }
+    if (threadIdx.x < T) sscale[threadIdx.x] = a.xs[threadIdx.x];
+  }
+  __syncthreads();
+
+  // Columns past the last token repeat it; pieces past K meet zero weights.
+  const int col = lane & 15, t = col < T ? col : T - 1;
+  const int8_t* const xp = sx + t * RB + kc;
+  i32x4_t acc = {0, 0, 0, 0};
+  auto mma = [&](auto buf, int s0) {
+    constexpr int B = decltype(buf)::value;
+#pragma unroll
+    for (int i = 0; i < kFewAhead; ++i) {
+      const int s = s0 + i * KS;
+      if (s < S) acc = mfma_i8_16(w[B][i], *reinterpret_cast<const i32x4_t*>(xp + s * kFewStep), acc);
+    }
+  };
+  constexpr int HOP = kFewAhead * KS;
+  for (int s = part; s < S; s += 2 * HOP) {
+    load(B1{}, s + HOP);
+    mma(B0{}, s);
+    load(B0{}, s + 2 * HOP);
+    mma(B1{}, s + HOP);
+  }
+  if constexpr (KS > 1) {
+    if (part) spart[wave * 64 + lane] = acc;
+    __syncthreads();
+    if (part) return;
+#pragma unroll
+    for (int p = 1; p < KS; ++p) acc += spart[(wave + p) * 64 + lane];
+  }
+  if (col >= T) return;
+  using O = Out<OUT>;
+  typename O::type* out = static_cast<typename O::type*>(a.out) + (int64_t)col * N;
+  const typename O::type* bias = static_cast<const typename O::type*>(a.bias);
+  const float xs = sscale[col];
+  const int c = n0 + 4 * (lane >> 4);
+  typename O::type v[4];
+#pragma unroll
+  for (int i = 0; i < 4; i += 2) {
+    float f[2];
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      const int n = c + i + j < N ? c + i + j : N - 1;
+      f[j] = (float)acc[i + j] * xs * a.ws[n] + (bias ? O::wide(bias[n]) : 0.0f);
+    }
+    O::pair(v + i, f[0], f[1]);
+  }
+  if (a.vec_out && c + 4 <= N) {
+    __builtin_memcpy(__builtin_assume_aligned(out + c, sizeof v), v, sizeof v);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (c + i < N) out[c + i] = v[i];
+  }
+}
+
+// xh null: codes given.
+template <int KS>
+void launch_few(int dtype, const IgArgs& a, const uint16_t* xh, hipStream_t s) {
+  const unsigned groups = (unsigned)((a.N + 15) / 16), blocks = (groups + 4 / KS - 1) / (4 / KS);
+  const size_t lds = ((size_t)a.T * few_row_bytes(a.K) + 64 + 15) / 16 * 16 + (KS > 1 ? 4096 : 0);
+  const bool f16 = dtype == TFM_DTYPE_F16;
+  if (xh && f16)
+    igemm_few_kernel<true, true, KS, TFM_DTYPE_F16><<<blocks, 256, lds, s>>>(a, xh);
+  else if (xh)
+    igemm_few_kernel<true, false, KS, TFM_DTYPE_BF16><<<blocks, 256, lds, s>>>(a, xh);
+  else if (dtype == TFM_DTYPE_F32)
+    igemm_few_kernel<false, false, KS, TFM_DTYPE_F32><<<blocks, 256, lds, s>>>(a, nullptr);
+  else if (f16)
+    igemm_few_kernel<false, true, KS, TFM_DTYPE_F16><<<blocks, 256, lds, s>>>(a, nullptr);
   else
-    igemm_tile_kernel<BM, BN, WM, WN, TFM_DTYPE_BF16><<<grid, block, 0, s>>>(a);
+    igemm_few_kernel<false, false, KS, TFM_DTYPE_BF16><<<blocks, 256, lds, s>>>(a, nullptr);
+}
+
+template <int BM, int BN, int WM, int WN, int MINW>
+void launch_tile(int dtype, IgArgs a, hipStream_t s) {
+  const int64_t mt = ((int64_t)a.T + BM - 1) / BM, nt = ((int64_t)a.N + BN - 1) / BN;
+  if (mt * nt > (1 << 23)) fail(TFM_E_UNSUPPORTED, "int8 product: too many output tiles in one call");
+  a.mt = (int)mt;
+  a.nt = (int)nt;
+  const dim3 grid((unsigned)(mt * nt)), block(BM / WM * (BN / WN) * 64);
+  if (dtype == TFM_DTYPE_F32)
+    igemm_tile_kernel<BM, BN, WM, WN, MINW, TFM_DTYPE_F32><<<grid, block, 0, s>>>(a);
+  else if (dtype == TFM_DTYPE_F16)
+    igemm_tile_kernel<BM, BN, WM, WN, MINW, TFM_DTYPE_F16><<<grid, block, 0, s>>>(a);
+  else
+    igemm_tile_kernel<BM, BN, WM, WN, MINW, TFM_DTYPE_BF16><<<grid, block, 0, s>>>(a);
+}
+
+IgArgs ig_args(int dtype, const int8_t* x, const float* x_scales, int64_t rows, const int8_t* w,
+               const float* w_scales, const void* bias, int N, int K, void* out) {
+  const size_t size = dtype == TFM_DTYPE_F32 ? 4 : 2;
+  const bool vec = (size_t)N * size % 16 == 0 && reinterpret_cast<uintptr_t>(out) % 16 == 0;
+  return IgArgs{x, w, x_scales, w_scales, bias, out, (int)rows, N, K, 0, 0, vec};
+}
+
+// Waves that share 16 channels: one where the channels alone fill the chip (at least two workgroups a CU).
+void run_few(int dtype, const IgArgs& a, const uint16_t* xh, hipStream_t s) {
+  if (a.N >= 512 * 64)
+    launch_few<1>(dtype, a, xh, s);
+  else
+    launch_few<4>(dtype, a, xh, s);
 }
 
 }  // namespace
@@ -174,12 +430,37 @@ void launch_tile(int dtype, const IgArgs& a, hipStream_t s) {
 void launch_int8_qmm(int dtype, const int8_t* x, const float* x_scales, int64_t rows, const int8_t* w,
                      const float* w_scales, const void* bias, int N, int K, void* out, hipStream_t s) {
   if (rows <= 0) return;
-  const IgArgs a{x, w, x_scales, w_scales, bias, out, (int)rows, N, K};
-  if (rows > 64)
-    launch_tile<128, 128, 64, 64>(dtype, a, s);
+  const IgArgs a = ig_args(dtype, x, x_scales, rows, w, w_scales, bias, N, K, out);
+  // The largest tile that keeps the chip busy: 256 x 256 tiles (one workgroup a CU)
+  // where their last round is at least three quarters full on average, 128 x 128
+  // where each CU gets one, 64 x 64 below. us at T x K x N, 256 / 128 / 64:
+  //   8192 x 4096 x 12288 (6 full rounds of 256)   386 / 449 / 642
+  //   8192 x 2048 x 2048 (1 full round)            37.4 / 41.7 / 56.7
+  //   4096 x 2048 x 6144 (1.5 rounds)              60.3 / 59.9 / 83.4
+  //   2048 x 1536 x 2560 (320 tiles of 128)        22.0 / 15.3 / 18.1
+  //   1024 x 2048 x 2048 (128 tiles of 128)        23.4 / 10.8 / 9.3
+  //   256 x 4096 x 4096 (64 tiles of 128)          38.9 / 15.6 / 11.3
+  const int64_t big = ((rows + 255) / 256) * (((int64_t)N + 255) / 256);
+  const int64_t mid = ((rows + 127) / 128) * (((int64_t)N + 127) / 128);
+  if (few_fits(rows, K))
+    run_few(dtype, a, nullptr, s);
+  else if (big * 4 >= (big + 255) / 256 * 256 * 3)
+    launch_tile<256, 256, 128, 64, 2>(dtype, a, s);
+  else if (mid >= 256)
+    launch_tile<128, 128, 64, 32, 2>(dtype, a, s);
   else
-    launch_tile<64, 64, 32, 32>(dtype, a, s);
+    launch_tile<64, 64, 32, 32, 2>(dtype, a, s);
   check_hip(hipGetLastError(), "int8_qmm launch");
+}
+
+bool int8_linear_few(int64_t rows, int K) { return few_fits(rows, K); }
+
+void launch_int8_linear_few(bool f16, const uint16_t* x, int64_t rows, const int8_t* w, const float* w_scales,
+                            const void* bias, int N, int K, void* out, hipStream_t s) {
+  if (rows <= 0) return;
+  const int dtype = f16 ? TFM_DTYPE_F16 : TFM_DTYPE_BF16;
+  run_few(dtype, ig_args(dtype, nullptr, nullptr, rows, w, w_scales, bias, N, K, out), x, s);
+  check_hip(hipGetLastError(), "int8_linear launch");
 }
 
 }  // namespace tfm

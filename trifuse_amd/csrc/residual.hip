@@ -22,131 +22,11 @@
 
 #include "tfm_device.h"
 #include "tfm_internal.h"
+#include "rows.h"
 
 namespace tfm {
 
 namespace {
-
-// Eight storage elements, as loaded.
-struct Vec8 {
-  uint32_t w[4];
-};
-
-// Elements [0, n) of a vector of eight (n >= 8: all). UNALIGNED: rows start
-// at any element and the last vector may be partial.
-template <bool UNALIGNED>
-__device__ __forceinline__ Vec8 load8(const uint16_t* p, int n) {
-  Vec8 v{{0, 0, 0, 0}};
-  if constexpr (!UNALIGNED) {
-    if (n > 0) {
-      const uint4 u = *reinterpret_cast<const uint4*>(p);
-      v = Vec8{{u.x, u.y, u.z, u.w}};
-    }
-  } else if (n >= 8) {
-    __builtin_memcpy(v.w, p, 16);
-  } else {
-#pragma unroll
-    for (int j = 0; j < 7; ++j)
-      if (j < n) v.w[j / 2] |= (uint32_t)p[j] << (16 * (j & 1));
-  }
-  return v;
-}
-
-template <bool UNALIGNED>
-__device__ __forceinline__ void store8(uint16_t* p, const Vec8& v, int n) {
-  if constexpr (!UNALIGNED) {
-    if (n > 0) *reinterpret_cast<uint4*>(p) = make_uint4(v.w[0], v.w[1], v.w[2], v.w[3]);
-  } else if (n >= 8) {
-    __builtin_memcpy(p, v.w, 16);
-  } else {
-#pragma unroll
-    for (int j = 0; j < 7; ++j)
-      if (j < n) p[j] = (uint16_t)(v.w[j / 2] >> (16 * (j & 1)));
-  }
-}
-
-template <bool UNALIGNED>
-__device__ __forceinline__ void store_codes8(int8_t* p, uint2 v, int n) {
-  if constexpr (!UNALIGNED) {
-    if (n > 0) *reinterpret_cast<uint2*>(p) = v;
-  } else if (n >= 8) {
-    __builtin_memcpy(p, &v, 8);
-  } else {
-#pragma unroll
-    for (int j = 0; j < 7; ++j)
-      if (j < n) p[j] = (int8_t)((j < 4 ? v.x : v.y) >> (8 * (j & 3)));
-  }
-}
-
-template <bool F16>
-__device__ __forceinline__ float elem(const Vec8& v, int j) {
-  return j & 1 ? hi_st<F16>(v.w[j / 2]) : lo_st<F16>(v.w[j / 2]);
-}
-
-// Sum of one value per lane over a team of TEAM lanes; every lane gets it.
-// `part` (TEAM / 64 floats of LDS, one array per call site) joins the waves.
-template <int TEAM>
-__device__ __forceinline__ float team_sum(float v, float* part) {
-  v = wave_tree_sum64(v);
-  const float s = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v), 63));
-  if constexpr (TEAM == 64) return s;
-  if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = s;
-  __syncthreads();
-  float total = part[0];
-#pragma unroll
-  for (int w = 1; w < TEAM / 64; ++w) total += part[w];
-  return total;
-}
-
-template <int CTRL, int ROW_MASK>
-__device__ __forceinline__ uint32_t dpp_umax(uint32_t v) {
-  const uint32_t o = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, ROW_MASK, 0xf, false);
-  return v > o ? v : o;
-}
-
-template <int TEAM>
-__device__ __forceinline__ uint32_t team_umax(uint32_t v, uint32_t* part) {
-  v = dpp_umax<0xb1, 0xf>(v);
-  v = dpp_umax<0x4e, 0xf>(v);
-  v = dpp_umax<0x141, 0xf>(v);
-  v = dpp_umax<0x140, 0xf>(v);
-  v = dpp_umax<0x142, 0xa>(v);
-  v = dpp_umax<0x143, 0xc>(v);
-  const uint32_t m = (uint32_t)__builtin_amdgcn_readlane((int)v, 63);
-  if constexpr (TEAM == 64) return m;
-  if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = m;
-  __syncthreads();
-  uint32_t best = part[0];
-#pragma unroll
-  for (int w = 1; w < TEAM / 64; ++w) best = best > part[w] ? best : part[w];
-  return best;
-}
-
-// A row's scale and the factor its values take before rounding, from the
-// bits of max|x| (as integers they order like the magnitudes, NaN on top).
-struct RowScale {
-  float scale, factor;
-  bool finite;
-};
-__device__ __forceinline__ RowScale row_scale(uint32_t amax_bits) {
-  RowScale r;
-  r.finite = amax_bits < 0x7f800000u;
-  const float a = fmaxf(__uint_as_float(amax_bits), 0x1p-100f);
-  r.scale = r.finite ? a / 127.0f : __uint_as_float(0x7fc00000u);
-  r.factor = 127.0f / a;
-  return r;
-}
-
-__device__ __forceinline__ uint32_t code_of(float v, const RowScale& r) {
-  return r.finite ? (uint32_t)(int)__builtin_rintf(v * r.factor) & 0xffu : 0u;
-}
-
-__device__ __forceinline__ uint2 codes8(const float* v, const RowScale& r) {
-  uint2 c;
-  c.x = code_of(v[0], r) | code_of(v[1], r) << 8 | code_of(v[2], r) << 16 | code_of(v[3], r) << 24;
-  c.y = code_of(v[4], r) | code_of(v[5], r) << 8 | code_of(v[6], r) << 16 | code_of(v[7], r) << 24;
-  return c;
-}
 
 struct NormArgs {
   tfm_norm_step s;

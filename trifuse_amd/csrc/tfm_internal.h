@@ -185,6 +185,11 @@ void launch_quantize_rows(bool f16, const uint16_t* x, int rows, int width, int8
 // out[t, n] = st((sum_k x[t, k] w[n, k]) * x_scales[t] * w_scales[n] + bias[n]); K a multiple of 16.
 void launch_int8_qmm(int dtype, const int8_t* x, const float* x_scales, int64_t rows, const int8_t* w,
                      const float* w_scales, const void* bias, int N, int K, void* out, hipStream_t s);
+// The same from x itself, its codes made in the product's kernel: where the rows
+// are few and fit that kernel's LDS.
+bool int8_linear_few(int64_t rows, int K);
+void launch_int8_linear_few(bool f16, const uint16_t* x, int64_t rows, const int8_t* w, const float* w_scales,
+                            const void* bias, int N, int K, void* out, hipStream_t s);
 struct LogprobsArgs {
   const void* logits;
   int64_t row_stride;  // elements

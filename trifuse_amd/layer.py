@@ -33,18 +33,24 @@ from .moe import _dev, _dtype_code, _ptr
 _FLOATS = {torch.bfloat16: TFM_DTYPE_BF16, torch.float16: TFM_DTYPE_F16, torch.float32: TFM_DTYPE_F32}
 
 
+# The current stream's handle without a torch.cuda.Stream object around it
+# (0.1 against 2 to 3 us of host time a call, of 10 in all).
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
+    lambda index: torch.cuda.current_stream(index).cuda_stream)
+
+
 def _call(device: torch.device, name: str, *args) -> None:
     """An entry point on `device` and its current stream (the last argument)."""
     if device.index == torch.cuda.current_device():
-        call(name, *args, torch.cuda.current_stream().cuda_stream)
+        call(name, *args, _raw_stream(device.index))
     else:
         with torch.cuda.device(device):
-            call(name, *args, torch.cuda.current_stream().cuda_stream)
+            call(name, *args, _raw_stream(device.index))
 
 
 def _on(t: torch.Tensor, name: str, device: torch.device) -> None:
-    _dev(t, name)
-    if t.device != device:
+    if t.device != device or not t.is_contiguous():
+        _dev(t, name)
         raise ValueError(f"{name} is on {t.device}, not on {device}")
 
 
@@ -62,6 +68,11 @@ def _vector(t: Optional[torch.Tensor], name: str, n: int, dtype: torch.dtype, de
     _on(t, name, device)
     if t.dtype != dtype or t.ndim != 1 or t.shape[0] != n:
         raise ValueError(f"{name} must be {dtype} [{n}]")
+
+
+def _codes(shape: torch.Size, device: torch.device) -> Tuple[torch.Tensor, torch.Tensor]:
+    return (torch.empty(shape, dtype=torch.int8, device=device),
+            torch.empty(shape[:-1], dtype=torch.float32, device=device))
 
 
 # ---------------------------------------------------------------------------
@@ -94,13 +105,12 @@ def norm_residual(y: torch.Tensor, residual: Optional[torch.Tensor] = None, *,
     kind = TFM_GATE_NONE
     if gate is not None:
         _on(gate, "gate", dev)
-        lead = y.shape[:-1]
-        if gate.dtype == torch.float32 and (gate.shape == lead or gate.shape == (*lead, 1)):
-            kind = TFM_GATE_TOKEN
-        elif gate.dtype == y.dtype and gate.shape == (width,):
+        if gate.dtype == y.dtype and gate.shape == (width,):
             kind = TFM_GATE_CHANNEL
         elif gate.dtype == y.dtype and gate.shape == y.shape:
             kind = TFM_GATE_FULL
+        elif gate.dtype == torch.float32 and gate.shape in (y.shape[:-1], (*y.shape[:-1], 1)):
+            kind = TFM_GATE_TOKEN
         else:
             raise ValueError("gate must be [H] or y's shape in y's dtype, or fp32 with one value a row")
     if quantize and pre_weight is None:
@@ -113,8 +123,7 @@ def norm_residual(y: torch.Tensor, residual: Optional[torch.Tensor] = None, *,
             raise ValueError("out geometry/dtype differs")
     x = codes = scales = None
     if quantize:
-        codes = torch.empty(y.shape, dtype=torch.int8, device=dev)
-        scales = torch.empty(y.shape[:-1], dtype=torch.float32, device=dev)
+        codes, scales = _codes(y.shape, dev)
     elif pre_weight is not None:
         x = torch.empty_like(y)
     step = NormStep(y.data_ptr(), _ptr(residual), _ptr(post_weight), _ptr(gate), _ptr(pre_weight), out.data_ptr(),
@@ -132,12 +141,10 @@ def rms_norm(x: torch.Tensor, weight: torch.Tensor, eps: float, quantize: bool =
     dt = _dtype_code(x, "x")
     _dev(x, "x")
     rows, width = _rows(x, "x")
-    _on(weight, "weight", x.device)
     _vector(weight, "weight", width, x.dtype, x.device)
     y = codes = scales = None
     if quantize:
-        codes = torch.empty(x.shape, dtype=torch.int8, device=x.device)
-        scales = torch.empty(x.shape[:-1], dtype=torch.float32, device=x.device)
+        codes, scales = _codes(x.shape, x.device)
     else:
         y = torch.empty_like(x)
     step = NormStep(x.data_ptr(), None, None, None, weight.data_ptr(), None, _ptr(y), _ptr(codes), _ptr(scales),
@@ -156,8 +163,7 @@ def quantize_rows(x: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
     dt = _dtype_code(x, "x")
     _dev(x, "x")
     rows, width = _rows(x, "x")
-    codes = torch.empty(x.shape, dtype=torch.int8, device=x.device)
-    scales = torch.empty(x.shape[:-1], dtype=torch.float32, device=x.device)
+    codes, scales = _codes(x.shape, x.device)
     _call(x.device, "tfm_quantize_rows", x.data_ptr(), rows, width, dt, codes.data_ptr(), scales.data_ptr())
     return codes, scales
 
@@ -202,9 +208,10 @@ def int8_linear(x: torch.Tensor, w: torch.Tensor, w_scales: torch.Tensor,
     rows, width = _rows(x, "x")
     n = _int8_weight(w, w_scales, bias, width, x.dtype, x.device)
     out = torch.empty((*x.shape[:-1], n), dtype=x.dtype, device=x.device)
-    ws = torch.empty(_lib.load().tfm_int8_linear_workspace_bytes(rows, width), dtype=torch.uint8, device=x.device)
+    need = _lib.load().tfm_int8_linear_workspace_bytes(rows, width)
+    ws = torch.empty(need, dtype=torch.uint8, device=x.device) if need else None
     _call(x.device, "tfm_int8_linear", x.data_ptr(), rows, w.data_ptr(), w_scales.data_ptr(), _ptr(bias), n, width, dt,
-          out.data_ptr(), ws.data_ptr(), ws.numel())
+          out.data_ptr(), _ptr(ws), need)
     return out
 
 
