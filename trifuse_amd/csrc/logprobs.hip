@@ -7,17 +7,18 @@
 // Both terms of the entropy are non-negative: nothing cancels. Each thread keeps
 // M, S and D of what it has read and rescales S and D when M grows; differences
 // of logits are taken before the scale, so they are exact for 16-bit logits
-// near the maximum, the ones that count. The maximum's own term, 1, is kept out
-// of the running sum: ln S = log1p(R) holds its precision where one token is
-// nearly sure and R, the others' sum, is far below 1.
+// near the maximum, the ones that count. Where one token is nearly sure, S is
+// 1 + R with R far below 1: one thread alone adds the 1, its other terms are
+// summed again without it, and ln S = log1p(R) keeps its precision.
 //
 // Alternatives: logits order by a key, their value's bits made monotonic
 // (NaN below -inf) and below it the complement of their place, so that ties go
-// to the lower place and no two keys are equal. Each thread also keeps the
-// largest key among the vectors it has read (their maxima, the vector's place).
+// to the lower place and no two keys are equal. A row's items are its whole
+// vectors and then the logits left over, one by one; each thread knows the
+// largest key among the items it has read (their maxima, the item's place).
 // 64 buckets, lane l of every wave, give 64 maxima; the top-th largest of them
 // is a threshold that at least `top` logits reach. Only threads whose own
-// maximum reaches it can hold such logits: their vectors are read again
+// maximum reaches it can hold such logits: their items are read again
 // (a few in a thousand), the logits that reach the threshold go to a list in
 // LDS, and each one's rank in the list is its place among the alternatives.
 // A row made so that the list overflows takes one scan per alternative.
@@ -28,8 +29,10 @@ namespace tfm {
 
 namespace {
 
+constexpr int kAhead = 4;        // items a thread has in flight
 constexpr int kCap = 1024;       // keys the candidate list holds
 constexpr float kLow = -3.402823466e38f;
+constexpr float kSure = 0.0625f;  // R below which the sum of 1 + R would cost ln S more than 2^-20
 
 // Logits of one 16-byte vector.
 template <int DT>
@@ -66,38 +69,52 @@ __device__ __forceinline__ float value_of(uint32_t o) {
 }
 __device__ __forceinline__ uint64_t key_of(uint32_t order, uint32_t place) { return (uint64_t)order << 32 | ~place; }
 
-// Sums of the logits read so far at their maximum m: s without the maximum's own
-// term (one: 1 once there is a maximum), d the weighted differences.
+// Sums of the logits read so far at their maximum m (kLow before any).
 struct Stats {
-  float m, s, d, one;
+  float m, s, d;
 };
 
-// The same sums at a maximum m' >= m, the old maximum's term among them. The
-// difference of maxima is kept finite: an empty part (s = d = one = 0) stays empty.
-__device__ __forceinline__ Stats rescaled(Stats a, float m, float c) {
+// The same sums at a maximum m' >= m. The difference of maxima is kept finite:
+// an empty part (s = d = 0) stays empty.
+__device__ __forceinline__ Stats rescaled(const Stats& a, float m, float c) {
   const float dm = fmaxf(a.m - m, -1e30f);
   const float e = __builtin_amdgcn_exp2f(dm * c);
-  const float all = a.s + a.one;
-  return Stats{m, all * e, e * __builtin_fmaf(dm, all, a.d), 0.0f};
+  return Stats{m, a.s * e, e * __builtin_fmaf(dm, a.s, a.d)};
+}
+
+template <int CTRL, int ROW_MASK>
+__device__ __forceinline__ float dpp_fmax(float v) {
+  const int b = __float_as_int(v);
+  return fmaxf(v, __int_as_float(__builtin_amdgcn_update_dpp(b, b, CTRL, ROW_MASK, 0xf, false)));
+}
+__device__ __forceinline__ float wave_fmax(float v) {
+  v = dpp_fmax<0xb1, 0xf>(v);
+  v = dpp_fmax<0x4e, 0xf>(v);
+  v = dpp_fmax<0x141, 0xf>(v);
+  v = dpp_fmax<0x140, 0xf>(v);
+  v = dpp_fmax<0x142, 0xa>(v);
+  v = dpp_fmax<0x143, 0xc>(v);
+  return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v), 63));
 }
 
 template <int DT, int THREADS>
 __global__ __launch_bounds__(THREADS) void token_logprobs_kernel(LogprobsArgs a) {
   using L = Logits<DT>;
   constexpr int N = L::N, WAVES = THREADS / 64;
-  __shared__ float sm[WAVES], ss[WAVES], sd[WAVES];
+  __shared__ float sm[WAVES], ss[WAVES], sh[WAVES], sd[WAVES];
   __shared__ int sn[WAVES];
   __shared__ uint64_t keys[THREADS];
   __shared__ uint64_t cand[kCap];
-  __shared__ uint64_t threshold;
+  __shared__ uint8_t rank[WAVES][64];
   __shared__ int chosen[THREADS];
-  __shared__ int n_chosen, n_cand;
+  __shared__ int n_chosen, n_cand, holder;
 
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int t = blockIdx.x;
   const int V = a.vocab;
   const char* row = static_cast<const char*>(a.logits) + (int64_t)t * a.row_stride * L::SIZE;
-  const int nvec = (V + N - 1) / N;  // the last one may be partial
+  // Thread i reads items i, i + THREADS, ...
+  const int full = V / N, items = full + V % N;
   const float c = a.scale * 1.44269504f;
 
   // The given token's logit, read early.
@@ -111,101 +128,161 @@ __global__ __launch_bounds__(THREADS) void token_logprobs_kernel(LogprobsArgs a)
     }
   }
 
-  Stats st{kLow, 0.0f, 0.0f, 0.0f};
-  uint64_t best = 0;
-  auto add = [&](float* f, int n, int v) {
+  auto term = [&](float f, float m, float& s, float& d) {
+    const float x = f - m;
+    const float e = __builtin_amdgcn_exp2f(x * c);
+    s += e;
+    d = __builtin_fmaf(fmaxf(x, kLow), e, d);  // a masked logit: e = 0, not -inf * 0
+  };
+  auto max_of = [&](const float* f) {
     float m = f[0];
 #pragma unroll
-    for (int j = 1; j < N; ++j)
-      if (j < n) m = fmaxf(m, f[j]);
-    const uint64_t k = key_of(order_of(m), (uint32_t)v);
-    if (k > best) best = k;
-    if (m > st.m) {
-      st = rescaled(st, m, c);
-      st.one = 1.0f;
-      bool found = false;  // the first of the vector's maxima leaves the sum
+    for (int j = 1; j < N; ++j) m = fmaxf(m, f[j]);
+    return m;
+  };
+  Stats st{kLow, 0.0f, 0.0f};
+  int best_item = -1;  // the first item that holds st.m
+  // kAhead vectors a thread are on their way at a time; past the last one a
+  // thread reads that one again and leaves it out.
+  for (int v = tid; v < (full + THREADS - 1) / THREADS * THREADS; v += kAhead * THREADS) {
+    uint4 u[kAhead];
 #pragma unroll
-      for (int j = 0; j < N; ++j) {
-        const bool it = !found && j < n && f[j] == m;
-        f[j] = it ? -__builtin_inff() : f[j];
-        found = found || it;
-      }
+    for (int i = 0; i < kAhead; ++i) {
+      const int at = v + i * THREADS;
+      u[i] = L::load(row, at < full ? at : full - 1);
     }
 #pragma unroll
-    for (int j = 0; j < N; ++j)
-      if (j < n) {
-        const float x = f[j] - st.m;
-        const float e = __builtin_amdgcn_exp2f(x * c);
-        st.s += e;
-        st.d = __builtin_fmaf(fmaxf(x, kLow), e, st.d);  // a masked logit: e = 0, not -inf * 0
+    for (int i = 0; i < kAhead; ++i) {
+      if (v + i * THREADS >= full) break;
+      float f[N];
+#pragma unroll
+      for (int j = 0; j < N; ++j) f[j] = L::get(u[i], j);
+      const float m = max_of(f);
+      if (m > st.m) {
+        st = rescaled(st, m, c);
+        best_item = v + i * THREADS;
       }
-  };
-  const int full = V / N;
-  for (int v = tid; v < full; v += THREADS) {
-    const uint4 u = L::load(row, v);
-    float f[N];
 #pragma unroll
-    for (int j = 0; j < N; ++j) f[j] = L::get(u, j);
-    add(f, N, v);
+      for (int j = 0; j < N; ++j) term(f[j], st.m, st.s, st.d);
+    }
   }
-  if (nvec > full && tid == full % THREADS) {
-    float f[N];
-    const int n = V - full * N;
-#pragma unroll
-    for (int j = 0; j < N; ++j) f[j] = j < n ? L::one(row, (int64_t)full * N + j) : 0.0f;
-    add(f, n, full);
+  // The logits left over: item full + j to the thread whose turn it is.
+  const int turn = (tid - full % THREADS + THREADS) % THREADS;
+  if (turn < items - full) {
+    const float f = L::one(row, (int64_t)full * N + turn);
+    if (f > st.m) {
+      st = rescaled(st, f, c);
+      best_item = full + turn;
+    }
+    term(f, st.m, st.s, st.d);
   }
 
-  // The row's maximum, then its sums at that maximum.
-  float m = st.m;
+  // An item again: its logits and how many they are.
+  auto fetch = [&](int v, float* f) {
+    if (v < full) {
+      const uint4 u = L::load(row, v);
 #pragma unroll
-  for (int x = 1; x < 64; x <<= 1) m = fmaxf(m, shfl_xor_f(m, x));
-  if (lane == 0) sm[wave] = m;
-  keys[tid] = best;
+      for (int j = 0; j < N; ++j) f[j] = L::get(u, j);
+      return N;
+    }
+    f[0] = L::one(row, (int64_t)full * N + (v - full));
+#pragma unroll
+    for (int j = 1; j < N; ++j) f[j] = 0.0f;
+    return 1;
+  };
+  uint64_t best = 0;
+  if (a.top > 0) {
+    if (best_item >= 0) {
+      best = key_of(order_of(st.m), (uint32_t)best_item);
+    } else {  // nothing above the lowest number: masked logits, or none
+      for (int v = tid; v < items; v += THREADS) {
+        float f[N];
+        const int n = fetch(v, f);
+        const uint64_t k = key_of(order_of(n == N ? max_of(f) : f[0]), (uint32_t)v);
+        best = k > best ? k : best;
+      }
+    }
+    keys[tid] = best;
+  }
+
+  // The row's maximum, then its sums at that maximum; a thread that holds it
+  // adds the maximum's own 1 apart (one of them: the row's holder).
+  const float wm = wave_fmax(st.m);
+  if (lane == 0) sm[wave] = wm;
   __syncthreads();
-  m = sm[0];
+  float m = sm[0];
 #pragma unroll
   for (int w = 1; w < WAVES; ++w) m = fmaxf(m, sm[w]);
-  const float one = st.m == m ? st.one : 0.0f;
-  if (st.m != m) st = rescaled(st, m, c);
-  const float ws = wave_tree_sum64(st.s), wd = wave_tree_sum64(st.d);
-  const int wn = __popcll(__ballot(one != 0.0f));
+  const bool holds = best_item >= 0 && st.m == m;
+  if (holds) holder = tid;
+  st = rescaled(st, m, c);
+  const float ws = wave_tree_sum64(holds ? 0.0f : st.s), wh = wave_tree_sum64(holds ? st.s - 1.0f : 0.0f);
+  const float wd = wave_tree_sum64(st.d);
+  const int wn = __popcll(__ballot(holds));
   if (lane == 63) {
     ss[wave] = ws;
+    sh[wave] = wh;
     sd[wave] = wd;
     sn[wave] = wn;
   }
-  // Bucket `lane`'s largest key; the one that top - 1 others exceed.
-  if (a.top > 0 && wave == 0) {
-    uint64_t k = best;
+  // Bucket `lane`'s largest key (an empty one has a key of its own below all
+  // others); wave w counts how many of its share of the buckets exceed it.
+  uint64_t bucket = 63 - lane;
+  if (a.top > 0) {
 #pragma unroll
-    for (int w = 1; w < WAVES; ++w) {
+    for (int w = 0; w < WAVES; ++w) {
       const uint64_t o = keys[64 * w + lane];
-      k = o > k ? o : k;
+      bucket = o > bucket ? o : bucket;
     }
-    int above = 0, equal_before = 0;  // empty buckets are equal
-#pragma unroll 8
-    for (int l = 0; l < 64; ++l) {
-      const uint64_t o = (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(k >> 32), l) << 32 |
-                         (uint32_t)__builtin_amdgcn_readlane((int)k, l);
-      above += o > k;
-      equal_before += o == k && l < lane;
+    constexpr int SHARE = 64 / WAVES;
+    int above = 0;
+#pragma unroll
+    for (int i = 0; i < SHARE; ++i) {
+      const int l = wave * SHARE + i;
+      const uint64_t o = (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(bucket >> 32), l) << 32 |
+                         (uint32_t)__builtin_amdgcn_readlane((int)bucket, l);
+      above += o > bucket;
     }
-    if (above + equal_before == a.top - 1) threshold = k;
+    rank[wave][lane] = (uint8_t)above;
   }
   __syncthreads();
-  float r = ss[0], d = sd[0];
+  float r = ss[0], rh = sh[0], d = sd[0];
   int ones = sn[0];  // threads that hold the maximum
 #pragma unroll
   for (int w = 1; w < WAVES; ++w) {
     r += ss[w];
+    rh += sh[w];
     d += sd[w];
     ones += sn[w];
   }
-  // +inf among the logits: NaN, as inf - inf makes the other maxima.
-  if (m == __builtin_inff()) r = __uint_as_float(0x7fc00000u);
-  const float s = r + (float)ones;
-  const float ln_s = ones > 0 ? log1pf(r + (float)(ones - 1)) : logf(s);
+  if (ones == 1 && r + rh < kSure) {
+    // The holder's other terms, 64 of its items at a time (every wave the same sum).
+    const int h = holder;
+    float part = 0.0f;
+    int before = 0;  // maxima in items ahead of this lane's
+    for (int v0 = h; v0 < items; v0 += 64 * THREADS) {
+      const int v = v0 + lane * THREADS;
+      float f[N], unused = 0.0f;
+      const int n = v < items ? fetch(v, f) : 0;
+      bool first = false;
+#pragma unroll
+      for (int j = 0; j < N; ++j) {
+        if (j >= n) continue;
+        if (f[j] == m && !first) {
+          first = true;  // the item's first maximum: one of the row's stays out
+          continue;
+        }
+        term(f[j], m, part, unused);
+      }
+      before += __popcll(__ballot(first));
+    }
+    part = wave_tree_sum64(part);
+    rh = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(part), 63)) + (float)(before - 1);
+  }
+  r += rh;
+  // +inf among the logits: NaN, as inf - inf makes their terms.
+  const float s = m == __builtin_inff() ? __uint_as_float(0x7fc00000u) : r + (float)ones;
+  const float ln_s = ones > 0 ? log1pf(s - 1.0f < 1.0f ? r + (float)(ones - 1) : s - 1.0f) : logf(s);
   const bool empty = s == 0.0f;  // every logit is -inf
   auto logp = [&](float l) { return empty ? -__builtin_inff() : __builtin_fmaf(a.scale, l - m, -ln_s); };
   if (tid == 0) {
@@ -214,22 +291,30 @@ __global__ __launch_bounds__(THREADS) void token_logprobs_kernel(LogprobsArgs a)
   }
   if (a.top <= 0) return;
 
-  const uint64_t thr = threshold;
+  // The bucket that top - 1 others exceed is the threshold: each wave finds it.
+  int above = 0;
+#pragma unroll
+  for (int w = 0; w < WAVES; ++w) above += rank[w][lane];
+  const int at = __builtin_ctzll(__ballot(above == a.top - 1));
+  const uint64_t thr = (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(bucket >> 32), at) << 32 |
+                       (uint32_t)__builtin_amdgcn_readlane((int)bucket, at);
   if (best != 0 && best >= thr) chosen[atomicAdd(&n_chosen, 1)] = tid;
   __syncthreads();
-  const int nc = n_chosen, per = (nvec + THREADS - 1) / THREADS;
+  const int nc = n_chosen, per = (items + THREADS - 1) / THREADS;
   for (int i = tid; i < nc * per; i += THREADS) {
     const int v = chosen[i % nc] + i / nc * THREADS;
-    if (v >= nvec) continue;
-    const int n = V - v * N < N ? V - v * N : N;
+    if (v >= items) continue;
+    float f[N];
+    const int n = fetch(v, f);
+    const uint32_t first = v < full ? (uint32_t)v * N : (uint32_t)(full * N + (v - full));
+    if (key_of(order_of(n == N ? max_of(f) : f[0]), (uint32_t)v) < thr) continue;
 #pragma unroll
     for (int j = 0; j < N; ++j) {
-      if (j >= n) break;
-      const int64_t at = (int64_t)v * N + j;
-      const uint32_t o = order_of(L::one(row, at));
-      if (key_of(o, (uint32_t)v) < thr) continue;
-      const int p = atomicAdd(&n_cand, 1);
-      if (p < kCap) cand[p] = key_of(o, (uint32_t)at);
+      const uint32_t o = order_of(f[j]);
+      if (j < n && key_of(o, (uint32_t)v) >= thr) {
+        const int p = atomicAdd(&n_cand, 1);
+        if (p < kCap) cand[p] = key_of(o, first + j);
+      }
     }
   }
   __syncthreads();
@@ -239,11 +324,11 @@ __global__ __launch_bounds__(THREADS) void token_logprobs_kernel(LogprobsArgs a)
   if (n <= kCap) {
     for (int i = tid; i < n; i += THREADS) {
       const uint64_t k = cand[i];
-      int rank = 0;
-      for (int j = 0; j < n; ++j) rank += cand[j] > k;
-      if (rank < a.top) {
-        ids[rank] = (int32_t)~(uint32_t)k;
-        lps[rank] = logp(value_of((uint32_t)(k >> 32)));
+      int place = 0;
+      for (int j = 0; j < n; ++j) place += cand[j] > k;
+      if (place < a.top) {
+        ids[place] = (int32_t)~(uint32_t)k;
+        lps[place] = logp(value_of((uint32_t)(k >> 32)));
       }
     }
     return;
