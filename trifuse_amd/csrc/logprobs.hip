@@ -358,8 +358,14 @@ __global__ __launch_bounds__(THREADS) void token_logprobs_kernel(LogprobsArgs a)
 
 template <int DT>
 void launch_dt(const LogprobsArgs& a, hipStream_t s) {
-  if (a.rows < 1024 && a.vocab >= 8192)
-    token_logprobs_kernel<DT, 1024><<<a.rows, 1024, 0, s>>>(a);
+  // Few rows leave CUs to spare: wider workgroups read a long row faster, narrower
+  // ones have less to join. us of 256 / 512 threads, rows x vocabulary:
+  //   1 x 4000 5.6 / 5.6     1 x 10007 6.4 / 5.8     1 x 50304 10.4 / 8.9
+  //   256 x 10007 7.1 / 7.0  333 x 10007 8.1 / 8.5   256 x 50304 11.5 / 10.0
+  //   333 x 50304 15.9 / 14.6   768 x 50304 20.4 / 20.5   1024 x 50304 24.3 / 24.9
+  // (1024 threads: 9.5, 15.9 and 29.2 at 1, 333 and 1024 x 50304).
+  if ((a.rows <= 256 && a.vocab >= 8192) || (a.rows <= 768 && a.vocab >= 32768))
+    token_logprobs_kernel<DT, 512><<<a.rows, 512, 0, s>>>(a);
   else
     token_logprobs_kernel<DT, 256><<<a.rows, 256, 0, s>>>(a);
 }

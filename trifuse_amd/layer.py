@@ -243,15 +243,15 @@ def token_logprobs(logits: torch.Tensor, tokens: Optional[torch.Tensor] = None, 
     if type(top) is not int or not 0 <= top <= vocab:
         raise ValueError("Invalid top-k")
     dev, lead = logits.device, logits.shape[:-1]
+    entropy = torch.empty(lead, dtype=torch.float32, device=dev)
+    ids = torch.empty((*lead, top), dtype=torch.int32, device=dev)
+    best = torch.empty_like(ids, dtype=torch.float32)
     logprobs = None
     if tokens is not None:
         _on(tokens, "tokens", dev)
         if tokens.dtype not in (torch.int32, torch.int64) or tokens.shape != lead:
             raise ValueError("tokens must be int32 or int64 with one value a row of logits")
-        logprobs = torch.empty(lead, dtype=torch.float32, device=dev)
-    entropy = torch.empty(lead, dtype=torch.float32, device=dev)
-    ids = torch.empty((*lead, top), dtype=torch.int32, device=dev)
-    best = torch.empty((*lead, top), dtype=torch.float32, device=dev)
+        logprobs = torch.empty_like(entropy)
     _call(dev, "tfm_token_logprobs", logits.data_ptr(), rows, vocab, stride, code, _ptr(tokens),
           64 if tokens is not None and tokens.dtype == torch.int64 else 32, top, scale, _ptr(logprobs),
           entropy.data_ptr(), ids.data_ptr(), best.data_ptr())
