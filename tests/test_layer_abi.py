@@ -150,3 +150,21 @@ def test_host_mirror_refuses_cpu_tensors_and_other_types():
               lambda: layer.int8_linear(x.float(), w, s), lambda: layer.token_logprobs(x.double())):
         with pytest.raises(NotImplementedError):
             f()
+
+
+def test_native_host_side_refuses_what_is_no_tensor():
+    import torch
+
+    from trifuse_amd import _lib as lib
+
+    native = lib.load_layer()
+    assert lib.load_layer() is native
+    x = torch.zeros((3, 64), dtype=torch.bfloat16)
+    for f in (lambda: native.quantize_rows(0, None), lambda: native.quantize_rows(0), lambda: native.quantize_rows(0, 1.5),
+              lambda: native.rms_norm(0, [x], None, 1e-5, False)):
+        with pytest.raises(TypeError):
+            f()
+    with pytest.raises(lib.TfmUnsupported):
+        lib.raise_status(lib.TFM_E_UNSUPPORTED)
+    with pytest.raises(lib.TfmError):
+        lib.raise_status(lib.TFM_E_INVALID)

@@ -6,11 +6,14 @@ point raises: there is no CPU fallback.
 from __future__ import annotations
 
 import ctypes
+import importlib.machinery
+import importlib.util
 import threading
 from ctypes import POINTER, c_char_p, c_double, c_float, c_int, c_int32, c_int64, c_size_t, c_uint32, c_void_p
 from pathlib import Path
 
 LIB_PATH = Path(__file__).resolve().parent / "lib" / "libtrifuse_moe.so"
+LAYER_PATH = LIB_PATH.parent / "_layer.so"
 
 TFM_OK = 0
 TFM_E_INVALID = 1
@@ -193,12 +196,35 @@ def load() -> ctypes.CDLL:
     return _lib
 
 
+def raise_status(status: int) -> None:
+    """Raise the error of a status other than TFM_OK, with the calling thread's message."""
+    msg = load().tfm_last_error().decode(errors="replace")
+    if status == TFM_E_UNSUPPORTED:
+        raise TfmUnsupported(status, msg)
+    raise TfmError(status, msg)
+
+
 def call(name: str, *args) -> None:
     """Call an int-returning entry point and raise TfmError on failure."""
-    lib = _lib if _lib is not None else load()
-    status = getattr(lib, name)(*args)
+    status = getattr(load(), name)(*args)
     if status != TFM_OK:
-        msg = lib.tfm_last_error().decode(errors="replace")
-        if status == TFM_E_UNSUPPORTED:
-            raise TfmUnsupported(status, msg)
-        raise TfmError(status, msg)
+        raise_status(status)
+
+
+_layer = None
+
+
+def load_layer():
+    """The native host side of layer.py (csrc/layer_binding.cpp), bound to the library's entry points."""
+    global _layer
+    lib = load()
+    with _lock:
+        if _layer is None:
+            if not LAYER_PATH.exists():
+                raise RuntimeError(f"{LAYER_PATH} is missing: build it with `python -m trifuse_amd.build`")
+            loader = importlib.machinery.ExtensionFileLoader("_layer", str(LAYER_PATH))
+            module = importlib.util.module_from_spec(importlib.util.spec_from_loader("_layer", loader))
+            loader.exec_module(module)
+            module.bind({name: ctypes.cast(getattr(lib, name), c_void_p).value for name in SIGNATURES}, raise_status)
+            _layer = module
+    return _layer

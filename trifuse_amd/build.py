@@ -3,7 +3,9 @@
     python -m trifuse_amd.build          # compile every source, link the library
 
 The library is written to trifuse_amd/lib/libtrifuse_moe.so. Each .hip file is
-compiled to an object in trifuse_amd/lib/obj/ (in parallel), then linked.
+compiled to an object in trifuse_amd/lib/obj/ (in parallel), then linked. The
+native host side of layer.py, a Python extension over torch's C++ headers, goes
+to trifuse_amd/lib/_layer.so.
 """
 from __future__ import annotations
 
@@ -59,11 +61,35 @@ def _compile(src: str) -> Path:
     return obj
 
 
+def _build_layer() -> Path:
+    import sysconfig
+
+    import torch
+    from torch.utils.cpp_extension import include_paths, library_paths
+
+    out = LIBDIR / "_layer.so"
+    tmp = LIBDIR / "_layer.so.tmp"
+    cxx = shutil.which("g++") or "g++"
+    cmd = [cxx, "-O2", "-std=c++17", "-fPIC", "-shared", "-Wall", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+           *(f"-isystem{p}" for p in include_paths()), f"-I{sysconfig.get_paths()['include']}",
+           str(CSRC / "layer_binding.cpp"), *(f"-L{p}" for p in library_paths()), "-ltorch_python", "-ltorch_cpu",
+           "-lc10", "-o", str(tmp)]
+    res = subprocess.run(cmd, capture_output=True, text=True)
+    if res.returncode != 0:
+        raise RuntimeError(f"g++ failed for layer_binding.cpp:\n{res.stdout}\n{res.stderr}")
+    if res.stderr:
+        sys.stderr.write(res.stderr)
+    os.replace(tmp, out)
+    return out
+
+
 def build(verbose: bool = True) -> Path:
     OBJDIR.mkdir(parents=True, exist_ok=True)
     jobs = min(len(SOURCES), max(1, int(os.environ.get("MAX_JOBS", os.cpu_count() or 4))))
     with ThreadPoolExecutor(max_workers=jobs) as ex:
+        layer = ex.submit(_build_layer)
         objs = list(ex.map(_compile, SOURCES))
+        layer.result()
     out = LIBDIR / LIBNAME
     tmp = LIBDIR / (LIBNAME + ".tmp")
     cmd = [hipcc(), f"--offload-arch={ARCH}", "-shared", "-fPIC", *map(str, objs), "-o", str(tmp)]
