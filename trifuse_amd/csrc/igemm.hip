@@ -5,7 +5,7 @@
 //
 // igemm_tile_kernel: BM tokens x BN channels a workgroup, 32x32x32 MFMAs. Both
 // operands go from memory straight into LDS (16 bytes a lane), 128 bytes of K a
-// stage, two stages; a row's eight 16-byte pieces are stored in the order
+// stage, S stages; a row's eight 16-byte pieces are stored in the order
 // piece ^ (row / 2 % 8), so that the 16 rows that are read at a time (256 bytes a
 // clock) lie in different banks.
 #include <type_traits>
@@ -53,6 +53,13 @@ __device__ __forceinline__ i32x4_t mfma_i8_16(i32x4_t a, i32x4_t b, i32x4_t c) {
   (void)a; (void)b;
   return c;
 #endif
+}
+
+// All but the last OUT vector memory operations of this wave are done, and its
+// LDS reads; then a barrier.
+template <int OUT>
+__device__ __forceinline__ void stage_wait() {
+  asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(OUT) : "memory");
 }
 
 // One output in the storage type OUT (TFM_DTYPE_*).
@@ -111,7 +118,8 @@ __device__ __forceinline__ void store_piece(T* row, int c, int N, bool vec, cons
   }
 }
 
-template <int BM, int BN, int WM, int WN, int MINW, int OUT>
+// BM x BN tile, waves of WM x WN, S stages, MINW waves a SIMD at least.
+template <int BM, int BN, int WM, int WN, int S, int MINW, int OUT>
 __global__ __launch_bounds__(BM / WM * (BN / WN) * 64, MINW) void igemm_tile_kernel(IgArgs a) {
   constexpr int WAVES_M = BM / WM, WAVES_N = BN / WN, WAVES = WAVES_M * WAVES_N;
   constexpr int MB = WM / 32, NB = WN / 32;
@@ -119,7 +127,10 @@ __global__ __launch_bounds__(BM / WM * (BN / WN) * 64, MINW) void igemm_tile_ker
   static_assert(WAVES == 4 || WAVES == 8, "a stage array serves one or two waves in the epilogue");
   static_assert(LX * 8 * WAVES == BM && LW * 8 * WAVES == BN, "copies tile the rows");
   // One array a stage and operand, so that reads of one stage do not wait for copies into the other.
-  __shared__ __attribute__((aligned(128))) int8_t sx0[BM * kBK], sx1[BM * kBK], sw0[BN * kBK], sw1[BN * kBK];
+  static_assert(S == 2 || S == 4, "stages");
+  constexpr int MX = S == 4 ? BM * kBK : 16, MW = S == 4 ? BN * kBK : 16;
+  __shared__ __attribute__((aligned(128))) int8_t sx0[BM * kBK], sx1[BM * kBK], sx2[MX], sx3[MX];
+  __shared__ __attribute__((aligned(128))) int8_t sw0[BN * kBK], sw1[BN * kBK], sw2[MW], sw3[MW];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int2 tile = ig_tile(blockIdx.x, a.mt, a.nt);
   const int m0 = tile.x * BM, n0 = tile.y * BN;
@@ -179,7 +190,7 @@ __global__ __launch_bounds__(BM / WM * (BN / WN) * 64, MINW) void igemm_tile_ker
   // One stage: four steps of 32 bytes of K, each step's fragments read during
   // the one before. The stage's last fragments are in registers before its last
   // step's products: there all waves meet, the next stage is complete, its first
-  // fragments are read and this stage's arrays take the stage after next.
+  // fragments are read and this stage's arrays take the stage S later.
   auto stage = [&](int8_t* cx, int8_t* cw, int8_t* nx, int8_t* nw, int kt) {
     constexpr int ALL = MB * NB, FIRST = ALL > MB ? MB : 0;
     read(B1{}, cx, cw, 1);
@@ -192,10 +203,12 @@ __global__ __launch_bounds__(BM / WM * (BN / WN) * 64, MINW) void igemm_tile_ker
     mma(B0{}, 0, ALL);
     spread();
     mma(B1{}, 0, FIRST);
-    __syncthreads();
+    // This wave's copies of the next stage are done (later stages' may be
+    // outstanding) and so are its reads of this one; then every wave's.
+    stage_wait<(S - 2) * (LX + LW)>();
     __builtin_amdgcn_sched_barrier(0);
     read(B0{}, nx, nw, 0);
-    load(cx, cw, kt + 2);
+    load(cx, cw, kt + S);
     mma(B1{}, FIRST, ALL);
 #pragma unroll
     for (int i = 0; i < ALL - FIRST; ++i) {
@@ -206,13 +219,23 @@ __global__ __launch_bounds__(BM / WM * (BN / WN) * 64, MINW) void igemm_tile_ker
     __builtin_amdgcn_sched_barrier(0);
   };
   load(sx0, sw0, 0);
-  __syncthreads();
   load(sx1, sw1, 1);
+  if constexpr (S == 4) {
+    load(sx2, sw2, 2);
+    load(sx3, sw3, 3);
+  }
+  stage_wait<(S - 1) * (LX + LW)>();
   read(B0{}, sx0, sw0, 0);
-  // Stages past the last are zeros: an odd count runs one of them.
-  for (int kt = 0; kt < KT; kt += 2) {
+  // Stages past the last are zeros: the loop ends on a multiple of S.
+  for (int kt = 0; kt < KT; kt += S) {
     stage(sx0, sw0, sx1, sw1, kt);
-    stage(sx1, sw1, sx0, sw0, kt + 1);
+    if constexpr (S == 2) {
+      stage(sx1, sw1, sx0, sw0, kt + 1);
+    } else {
+      stage(sx1, sw1, sx2, sw2, kt + 1);
+      stage(sx2, sw2, sx3, sw3, kt + 2);
+      stage(sx3, sw3, sx0, sw0, kt + 3);
+    }
   }
   __syncthreads();  // the copies past the end
   // Epilogue. Lane l holds token l % 32 and channels 8 (i / 4) + 4 (l / 32) + i % 4
@@ -395,19 +418,22 @@ void launch_few(int dtype, const IgArgs& a, const uint16_t* xh, hipStream_t s) {
     igemm_few_kernel<false, false, KS, TFM_DTYPE_BF16><<<blocks, 256, lds, s>>>(a, nullptr);
 }
 
-template <int BM, int BN, int WM, int WN, int MINW>
+template <int BM, int BN, int WM, int WN, int S, int MINW>
 void launch_tile(int dtype, IgArgs a, hipStream_t s) {
   const int64_t mt = ((int64_t)a.T + BM - 1) / BM, nt = ((int64_t)a.N + BN - 1) / BN;
   if (mt * nt > (1 << 23)) fail(TFM_E_UNSUPPORTED, "int8 product: too many output tiles in one call");
   a.mt = (int)mt;
   a.nt = (int)nt;
   const dim3 grid((unsigned)(mt * nt)), block(BM / WM * (BN / WN) * 64);
-  if (dtype == TFM_DTYPE_F32)
-    igemm_tile_kernel<BM, BN, WM, WN, MINW, TFM_DTYPE_F32><<<grid, block, 0, s>>>(a);
-  else if (dtype == TFM_DTYPE_F16)
-    igemm_tile_kernel<BM, BN, WM, WN, MINW, TFM_DTYPE_F16><<<grid, block, 0, s>>>(a);
+  if (dtype == TFM_DTYPE_F32) {
+    if constexpr (BM == BN)  // the 256 x 192 tile has no room to stage fp32 rows
+      igemm_tile_kernel<BM, BN, WM, WN, S, MINW, TFM_DTYPE_F32><<<grid, block, 0, s>>>(a);
+    else
+      fail(TFM_E_UNSUPPORTED, "int8 product: tile without fp32 output");
+  } else if (dtype == TFM_DTYPE_F16)
+    igemm_tile_kernel<BM, BN, WM, WN, S, MINW, TFM_DTYPE_F16><<<grid, block, 0, s>>>(a);
   else
-    igemm_tile_kernel<BM, BN, WM, WN, MINW, TFM_DTYPE_BF16><<<grid, block, 0, s>>>(a);
+    igemm_tile_kernel<BM, BN, WM, WN, S, MINW, TFM_DTYPE_BF16><<<grid, block, 0, s>>>(a);
 }
 
 IgArgs ig_args(int dtype, const int8_t* x, const float* x_scales, int64_t rows, const int8_t* w,
@@ -427,29 +453,49 @@ void run_few(int dtype, const IgArgs& a, const uint16_t* xh, hipStream_t s) {
 
 }  // namespace
 
+// The tile whose rounds of the chip take least time by the measured time of a
+// round for each 128 bytes of K: 256 x 256 and 256 x 192 (one workgroup a CU)
+// 2.0 and 1.62 us, 128 x 128 (two a CU) 1.17, or 0.75 where each CU has one, 64 x 64
+// (two a CU) 0.42, or 0.36 and 0.25 in a single round of two and one. us at
+// T x K x N, in that order (* the one taken):
+//   8192 x 4096 x 12288   375* / 392 / 439 / 642
+//   4096 x 2048 x 6144    60.8 / 54.3* / 58.7 / 91
+//   8192 x 2048 x 2048    36.6* / 49.2 / 40.4 / 64
+//   4096 x 2048 x 2048    29.4 / 26.5 / 22.3* / 32.5
+//   2048 x 1536 x 2560    22.0 / 19.3 / 15.2* / 18.0
+//   1024 x 2048 x 2048    23.4 / 21.1 / 10.9 / 8.9*
+//   64 x 4096 x 12288     40.0 / 34.8 / 22.9 / 11.4*
+// The 64 x 64 tile keeps four stages of K in LDS (with two: 18.2 at the last line,
+// 9.1 above it): a CU's few workgroups there do not hide each other's loads.
+enum Tile { kTile256, kTile192, kTile128, kTile64 };
+static Tile pick_tile(int64_t T, int64_t N, bool half_out) {
+  auto tiles = [&](int bm, int bn) { return ((T + bm - 1) / bm) * ((N + bn - 1) / bn); };
+  auto rounds = [](int64_t n, int slots) { return (double)((n + slots - 1) / slots); };
+  const int64_t n128 = tiles(128, 128), n64 = tiles(64, 64);
+  const double cost[] = {2.0 * rounds(tiles(256, 256), 256),
+                         half_out ? 1.62 * rounds(tiles(256, 192), 256) : 1e30,  // fp32 rows do not fit its staging
+                         n128 <= 256 ? 0.75 : 1.17 * rounds(n128, 512),
+                         n64 <= 256 ? 0.25 : n64 <= 512 ? 0.36 : 0.42 * rounds(n64, 512)};
+  int best = 0;
+  for (int i = 1; i < 4; ++i)
+    if (cost[i] < cost[best]) best = i;
+  return (Tile)best;
+}
+
 void launch_int8_qmm(int dtype, const int8_t* x, const float* x_scales, int64_t rows, const int8_t* w,
                      const float* w_scales, const void* bias, int N, int K, void* out, hipStream_t s) {
   if (rows <= 0) return;
   const IgArgs a = ig_args(dtype, x, x_scales, rows, w, w_scales, bias, N, K, out);
-  // The largest tile that keeps the chip busy: 256 x 256 tiles (one workgroup a CU)
-  // where their last round is at least three quarters full on average, 128 x 128
-  // where each CU gets one, 64 x 64 below. us at T x K x N, 256 / 128 / 64:
-  //   8192 x 4096 x 12288 (6 full rounds of 256)   386 / 449 / 642
-  //   8192 x 2048 x 2048 (1 full round)            37.4 / 41.7 / 56.7
-  //   4096 x 2048 x 6144 (1.5 rounds)              60.3 / 59.9 / 83.4
-  //   2048 x 1536 x 2560 (320 tiles of 128)        22.0 / 15.3 / 18.1
-  //   1024 x 2048 x 2048 (128 tiles of 128)        23.4 / 10.8 / 9.3
-  //   256 x 4096 x 4096 (64 tiles of 128)          38.9 / 15.6 / 11.3
-  const int64_t big = ((rows + 255) / 256) * (((int64_t)N + 255) / 256);
-  const int64_t mid = ((rows + 127) / 128) * (((int64_t)N + 127) / 128);
-  if (few_fits(rows, K))
+  if (few_fits(rows, K)) {
     run_few(dtype, a, nullptr, s);
-  else if (big * 4 >= (big + 255) / 256 * 256 * 3)
-    launch_tile<256, 256, 128, 64, 2>(dtype, a, s);
-  else if (mid >= 256)
-    launch_tile<128, 128, 64, 32, 2>(dtype, a, s);
-  else
-    launch_tile<64, 64, 32, 32, 2>(dtype, a, s);
+  } else {
+    switch (pick_tile(rows, N, dtype != TFM_DTYPE_F32)) {
+      case kTile256: launch_tile<256, 256, 128, 64, 2, 2>(dtype, a, s); break;
+      case kTile192: launch_tile<256, 192, 64, 96, 2, 2>(dtype, a, s); break;
+      case kTile128: launch_tile<128, 128, 64, 32, 2, 2>(dtype, a, s); break;
+      case kTile64: launch_tile<64, 64, 32, 32, 4, 2>(dtype, a, s); break;
+    }
+  }
   check_hip(hipGetLastError(), "int8_qmm launch");
 }
 
