@@ -331,7 +331,9 @@ __global__ __launch_bounds__(256) void igemm_few_kernel(IgArgs a, const uint16_t
   };
   using B0 = std::integral_constant<int, 0>;
   using B1 = std::integral_constant<int, 1>;
+  constexpr int HOP = kFewAhead * KS;
   load(B0{}, part);
+  load(B1{}, part + HOP);
 
   if constexpr (FUSED) {
     for (int t = wave; t < T; t += 4) {
@@ -360,12 +362,11 @@ __global__ __launch_bounds__(256) void igemm_few_kernel(IgArgs a, const uint16_t
       if (s < S) acc = mfma_i8_16(w[B][i], *reinterpret_cast<const i32x4_t*>(xp + s * kFewStep), acc);
     }
   };
-  constexpr int HOP = kFewAhead * KS;
   for (int s = part; s < S; s += 2 * HOP) {
-    load(B1{}, s + HOP);
     mma(B0{}, s);
     load(B0{}, s + 2 * HOP);
     mma(B1{}, s + HOP);
+    load(B1{}, s + 3 * HOP);
   }
   if constexpr (KS > 1) {
     if (part) spart[wave * 64 + lane] = acc;
@@ -499,7 +500,10 @@ void launch_int8_qmm(int dtype, const int8_t* x, const float* x_scales, int64_t 
   check_hip(hipGetLastError(), "int8_qmm launch");
 }
 
-bool int8_linear_few(int64_t rows, int K) { return few_fits(rows, K); }
+// Past 8 rows making the codes in every workgroup costs more than a launch of
+// their own: 16 x 2048 x 50304 31.8 us against 26.0 and 2.5 (8 rows 27.6 against
+// 24.5 and 2.5, 8 x 2048 x 2048 6.2 against 4.9 and 2.5).
+bool int8_linear_few(int64_t rows, int K) { return rows <= 8 && few_fits(rows, K); }
 
 void launch_int8_linear_few(bool f16, const uint16_t* x, int64_t rows, const int8_t* w, const float* w_scales,
                             const void* bias, int N, int K, void* out, hipStream_t s) {

@@ -196,15 +196,10 @@ __global__ __launch_bounds__(TEAM < 256 ? 256 : TEAM) void quantize_kernel(const
     const int c = 8 * (lane + TEAM * i);
     v[i] = load8<UNALIGNED>(x + base + c, H - c);
   }
-  uint32_t big = 0;
+  u16x2_t big = {0, 0};
 #pragma unroll
-  for (int i = 0; i < NV; ++i)
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const uint32_t u = __float_as_uint(elem<F16>(v[i], j)) & 0x7fffffffu;
-      big = u > big ? u : big;
-    }
-  const RowScale rs = row_scale(team_umax<TEAM>(big, part));
+  for (int i = 0; i < NV; ++i) big = abs_max(big, v[i]);
+  const RowScale rs = row_scale(team_umax<TEAM>(abs_bits<F16>(big), part));
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
     const int c = 8 * (lane + TEAM * i);

@@ -117,15 +117,34 @@ __device__ __forceinline__ RowScale row_scale(uint32_t amax_bits) {
   return r;
 }
 
-__device__ __forceinline__ uint32_t code_of(float v, const RowScale& r) {
-  return r.finite ? (uint32_t)(int)__builtin_rintf(v * r.factor) & 0xffu : 0u;
+// Eight codes. v * factor + 1.5 * 2^23 rounds half to even at its last bit and the
+// sum's low byte is the code; the product is rounded first, as the codes are
+// defined, so the two are not contracted into one operation.
+__device__ __forceinline__ uint2 codes8(const float* v, const RowScale& r) {
+#pragma clang fp contract(off)
+  uint32_t b[8];
+#pragma unroll
+  for (int j = 0; j < 8; ++j) b[j] = __float_as_uint(v[j] * r.factor + 12582912.0f);
+  uint2 c;
+  c.x = __builtin_amdgcn_perm(__builtin_amdgcn_perm(b[3], b[2], 0x0c0c0400u), __builtin_amdgcn_perm(b[1], b[0], 0x0c0c0400u), 0x05040100u);
+  c.y = __builtin_amdgcn_perm(__builtin_amdgcn_perm(b[7], b[6], 0x0c0c0400u), __builtin_amdgcn_perm(b[5], b[4], 0x0c0c0400u), 0x05040100u);
+  return r.finite ? c : make_uint2(0, 0);
 }
 
-__device__ __forceinline__ uint2 codes8(const float* v, const RowScale& r) {
-  uint2 c;
-  c.x = code_of(v[0], r) | code_of(v[1], r) << 8 | code_of(v[2], r) << 16 | code_of(v[3], r) << 24;
-  c.y = code_of(v[4], r) | code_of(v[5], r) << 8 | code_of(v[6], r) << 16 | code_of(v[7], r) << 24;
-  return c;
+// Bits of the largest magnitude of a vector's elements, two at a time: as
+// integers the magnitudes of either storage type order like themselves, NaN on top.
+typedef uint16_t u16x2_t __attribute__((ext_vector_type(2)));
+__device__ __forceinline__ u16x2_t abs_max(u16x2_t big, const Vec8& v) {
+#pragma unroll
+  for (int k = 0; k < 4; ++k)
+    big = __builtin_elementwise_max(big, __builtin_bit_cast(u16x2_t, v.w[k] & 0x7fff7fffu));
+  return big;
+}
+// The same as the bits of a float.
+template <bool F16>
+__device__ __forceinline__ uint32_t abs_bits(u16x2_t big) {
+  const uint16_t m = big.x > big.y ? big.x : big.y;
+  return __float_as_uint(st2f<F16>(m));
 }
 
 // One wave's codes of a row of any width that is a multiple of 8, its start
@@ -133,17 +152,10 @@ __device__ __forceinline__ uint2 codes8(const float* v, const RowScale& r) {
 // to `codes` (8-byte aligned).
 template <bool F16>
 __device__ __forceinline__ RowScale quantize_row_wave(const uint16_t* x, int width, int8_t* codes, int lane) {
-  uint32_t big = 0;
+  u16x2_t big = {0, 0};
 #pragma unroll 4
-  for (int c = 8 * lane; c < width; c += 512) {
-    const Vec8 v = load8<true>(x + c, 8);
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const uint32_t u = __float_as_uint(elem<F16>(v, j)) & 0x7fffffffu;
-      big = u > big ? u : big;
-    }
-  }
-  const RowScale rs = row_scale(team_umax<64>(big, nullptr));
+  for (int c = 8 * lane; c < width; c += 512) big = abs_max(big, load8<true>(x + c, 8));
+  const RowScale rs = row_scale(team_umax<64>(abs_bits<F16>(big), nullptr));
 #pragma unroll 4
   for (int c = 8 * lane; c < width; c += 512) {
     const Vec8 v = load8<true>(x + c, 8);
