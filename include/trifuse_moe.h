@@ -329,8 +329,8 @@ int tfm_quantize_rows(const void* x, int64_t rows, int32_t width, int32_t dtype,
  * with an exact 32-bit sum and the rest in fp32, rounded once to dtype (here
  * also TFM_DTYPE_F32). x [rows, k_in] and w [n_out, k_in] int8, 16-byte aligned
  * (any int8 value, -128 included: k_in bounds the sum); bias [n_out] in dtype
- * or NULL; out [rows, n_out]. k_in: a multiple of 16, at most 131056. n_out is
- * any positive number. */
+ * or NULL; out [rows, n_out]. k_in: a multiple of 16, at most 131056. n_out: at
+ * most 2^28. */
 #define TFM_DTYPE_F32 2 /* output of tfm_int8_qmm, logits of tfm_token_logprobs */
 int tfm_int8_qmm(const int8_t* x, const float* x_scales, int64_t rows, const int8_t* w,
                  const float* w_scales, const void* bias, int32_t n_out, int32_t k_in,

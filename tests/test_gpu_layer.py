@@ -208,6 +208,16 @@ def test_int8_qmm_large(gpu, rows, n, k):
     close(out, *product64(codes, scales, w, ws, None), F32)
 
 
+@pytest.mark.parametrize("rows,n", [(2047, 8190), (2041, 6143), (2040, 2552), (1023, 2050)])
+@pytest.mark.parametrize("dtype", [BF16, F16, F32])
+def test_int8_qmm_every_tile_and_type(gpu, rows, n, dtype):
+    """Sizes that take the 256 x 256, 256 x 192 (fp32: another), 128 x 128 and 64 x 64 tiles, with ragged last ones."""
+    k = 272
+    codes, w, scales, ws, bias = codes_of((rows, k), 1), codes_of((n, k), 2), scales_of(rows, 3), scales_of(n, 4), rand((n,), 5, 1.0, dtype)
+    out = layer.int8_qmm(codes, scales, w, ws, bias=bias, dtype=dtype)
+    close(out, *product64(codes, scales, w, ws, bias), dtype)
+
+
 @pytest.mark.parametrize("rows", [1, 20, 70, 300])
 def test_int8_qmm_longest_sum(gpu, rows):
     """Every product at its largest: the sum stays below 2^31 at the longest k."""

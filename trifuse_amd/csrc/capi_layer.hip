@@ -20,7 +20,7 @@ constexpr int kProductMaxK = 131056;  // 128 * 128 * K < 2^31
 void need_product(int64_t rows, int32_t n_out, int32_t k_in) {
   need_rows(rows);
   need(n_out > 0 && k_in > 0, "n_out and k_in must be positive");
-  if (n_out > (1 << 30)) fail(TFM_E_UNSUPPORTED, "n_out past 2^30 is not built");
+  if (n_out > (1 << 28)) fail(TFM_E_UNSUPPORTED, "n_out past 2^28 is not built");
   if (k_in % 16 != 0) fail(TFM_E_UNSUPPORTED, "k_in must be a multiple of 16");
   if (k_in > kProductMaxK) fail(TFM_E_UNSUPPORTED, "k_in past 131056 could overflow the 32-bit sum");
 }

@@ -422,7 +422,7 @@ void launch_few(int dtype, const IgArgs& a, const uint16_t* xh, hipStream_t s) {
 template <int BM, int BN, int WM, int WN, int S, int MINW>
 void launch_tile(int dtype, IgArgs a, hipStream_t s) {
   const int64_t mt = ((int64_t)a.T + BM - 1) / BM, nt = ((int64_t)a.N + BN - 1) / BN;
-  if (mt * nt > (1 << 23)) fail(TFM_E_UNSUPPORTED, "int8 product: too many output tiles in one call");
+  if (mt * nt > (1 << 22)) fail(TFM_E_UNSUPPORTED, "int8 product: too many output tiles in one call");
   a.mt = (int)mt;
   a.nt = (int)nt;
   const dim3 grid((unsigned)(mt * nt)), block(BM / WM * (BN / WN) * 64);

@@ -53,6 +53,9 @@ __global__ __launch_bounds__(TEAM < 256 ? 256 : TEAM) void norm_residual_kernel(
   const uint16_t* gate = gk == TFM_GATE_FULL      ? static_cast<const uint16_t*>(a.s.gate) + base
                          : gk == TFM_GATE_CHANNEL ? static_cast<const uint16_t*>(a.s.gate)
                                                   : nullptr;
+  // Every operand is on its way before the first is used, but the weights of the
+  // widest rows, whose registers are full without them.
+  constexpr bool EARLY = TEAM < 1024;
   Vec8 yv[NV], rv[NV], gv[NV], av[NV], bv[NV];
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
@@ -73,20 +76,24 @@ __global__ __launch_bounds__(TEAM < 256 ? 256 : TEAM) void norm_residual_kernel(
       gv[i] = load8<UNALIGNED>(gate + c, H - c);
     }
   }
-  if (wpost) {
+  if (EARLY && wpost) {
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
       const int c = 8 * (lane + TEAM * i);
       av[i] = load8<UNALIGNED>(wpost + c, H - c);
     }
   }
-  if (wpre) {
+  if (EARLY && wpre) {
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
       const int c = 8 * (lane + TEAM * i);
       bv[i] = load8<UNALIGNED>(wpre + c, H - c);
     }
   }
+  auto weight = [&](const Vec8* early, const uint16_t* w, int i) {
+    const int c = 8 * (lane + TEAM * i);
+    return EARLY ? early[i] : load8<UNALIGNED>(w + c, H - c);
+  };
   const float m = gk == TFM_GATE_TOKEN ? a.s.residual_multiplier * static_cast<const float*>(a.s.gate)[t]
                                        : a.s.residual_multiplier;
 
@@ -103,9 +110,11 @@ __global__ __launch_bounds__(TEAM < 256 ? 256 : TEAM) void norm_residual_kernel(
       for (int j = 0; j < 8; ++j) s = __builtin_fmaf(h[i][j], h[i][j], s);
     const float inv = 1.0f / sqrtf(team_sum<TEAM>(s, part0) / (float)H + a.s.post_eps);
 #pragma unroll
-    for (int i = 0; i < NV; ++i)
+    for (int i = 0; i < NV; ++i) {
+      const Vec8 w = weight(av, wpost, i);
 #pragma unroll
-      for (int j = 0; j < 8; ++j) h[i][j] = h[i][j] * inv * elem<F16>(av[i], j);
+      for (int j = 0; j < 8; ++j) h[i][j] = h[i][j] * inv * elem<F16>(w, j);
+    }
   }
   if (gate) {
 #pragma unroll
@@ -145,9 +154,11 @@ __global__ __launch_bounds__(TEAM < 256 ? 256 : TEAM) void norm_residual_kernel(
     for (int j = 0; j < 8; ++j) s = __builtin_fmaf(h[i][j], h[i][j], s);
   const float inv = 1.0f / sqrtf(team_sum<TEAM>(s, part1) / (float)H + a.s.pre_eps);
 #pragma unroll
-  for (int i = 0; i < NV; ++i)
+  for (int i = 0; i < NV; ++i) {
+    const Vec8 w = weight(bv, wpre, i);
 #pragma unroll
-    for (int j = 0; j < 8; ++j) h[i][j] = h[i][j] * inv * elem<F16>(bv[i], j);
+    for (int j = 0; j < 8; ++j) h[i][j] = h[i][j] * inv * elem<F16>(w, j);
+  }
   if (a.s.x) {
     uint16_t* out = static_cast<uint16_t*>(a.s.x) + base;
 #pragma unroll
@@ -190,22 +201,29 @@ __global__ __launch_bounds__(TEAM < 256 ? 256 : TEAM) void quantize_kernel(const
   const int t = blockIdx.x * TEAMS + threadIdx.x / TEAM;
   if (t >= rows) return;  // whole waves, and no barrier with several teams
   const int64_t base = (int64_t)t * H;
+  // The widest rows do not fit their registers: read again (from the cache).
+  constexpr bool HOLD = TEAM < 1024;
   Vec8 v[NV];
-#pragma unroll
-  for (int i = 0; i < NV; ++i) {
-    const int c = 8 * (lane + TEAM * i);
-    v[i] = load8<UNALIGNED>(x + base + c, H - c);
-  }
   u16x2_t big = {0, 0};
-#pragma unroll
-  for (int i = 0; i < NV; ++i) big = abs_max(big, v[i]);
-  const RowScale rs = row_scale(team_umax<TEAM>(abs_bits<F16>(big), part));
-#pragma unroll
+#pragma unroll HOLD ? NV : 4
   for (int i = 0; i < NV; ++i) {
     const int c = 8 * (lane + TEAM * i);
+    const Vec8 u = load8<UNALIGNED>(x + base + c, H - c);
+    if constexpr (HOLD) v[i] = u;
+    big = abs_max(big, u);
+  }
+  const RowScale rs = row_scale(team_umax<TEAM>(abs_bits<F16>(big), part));
+#pragma unroll HOLD ? NV : 4
+  for (int i = 0; i < NV; ++i) {
+    const int c = 8 * (lane + TEAM * i);
+    Vec8 u;
+    if constexpr (HOLD)
+      u = v[i];
+    else
+      u = load8<UNALIGNED>(x + base + c, H - c);
     float f[8];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) f[j] = elem<F16>(v[i], j);
+    for (int j = 0; j < 8; ++j) f[j] = elem<F16>(u, j);
     store_codes8<UNALIGNED>(codes + base + c, codes8(f, rs), H - c);
   }
   if (lane == 0) scales[t] = rs.scale;
