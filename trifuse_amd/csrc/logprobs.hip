@@ -32,7 +32,7 @@ namespace {
 constexpr int kAhead = 4;        // items a thread has in flight
 constexpr int kCap = 1024;       // keys the candidate list holds
 constexpr float kLow = -3.402823466e38f;
-constexpr float kSure = 0.0625f;  // R below which the sum of 1 + R would cost ln S more than 2^-20
+constexpr float kSure = 1.0f;  // R below which the roundings of 1 + R (a few 2^-24) count beside ln S
 
 // Logits of one 16-byte vector.
 template <int DT>
