@@ -555,3 +555,42 @@ def test_forward_norms(gpu, geom_name, T, rm):
     h64, eh, _, _ = step64(y, h, None, None, rm, None)
     close(plain, h64, eh, BF16)
     assert blk.forward_norms(h[:0], w, n[0], EPS).shape == (0, geom.hidden)
+
+
+# -- sizes past 32 bits ----------------------------------------------------------------
+
+def test_offsets_past_32_bits(gpu):
+    """The last rows of calls of more than 2^32 bytes and 2^31 elements equal the same rows alone."""
+    rows, width = 70001, 32768
+    y = torch.empty((rows, width), dtype=BF16, device="cuda")
+    y[:-3] = 1.0
+    y[-3:] = rand((3, width), 1)
+    w = rand((width,), 2, 0.1, BF16, 1.0)
+    h, x = layer.norm_residual(y, y, post_weight=w, gate=y, pre_weight=w, out=y.clone())
+    h2, x2 = layer.norm_residual(y[-3:], y[-3:], post_weight=w, gate=y[-3:], pre_weight=w)
+    assert torch.equal(h[-3:], h2) and torch.equal(x[-3:], x2)
+    del h, x
+    codes, scales = layer.quantize_rows(y)
+    last = layer.quantize_rows(y[-3:])
+    assert torch.equal(codes[-3:], last[0]) and torch.equal(scales[-3:], last[1])
+    del codes, scales
+    tokens = torch.full((rows,), width - 1, device="cuda")
+    got, ref = layer.token_logprobs(y, tokens, top=4), layer.token_logprobs(y[-3:].contiguous(), tokens[-3:], top=4)
+    assert torch.equal(got[2][-3:], ref[2])
+    for a, b in zip((got[0], got[1], got[3]), (ref[0], ref[1], ref[3])):
+        assert ((a[-3:] - b).abs() <= b.abs() * 2.0 ** -20).all()  # another workgroup width: another order of the sum
+    del got, y
+    for k, n in ((32768, 16), (16, 32784)):  # the left operand, then the output, past 2^31 elements
+        codes = torch.ones((rows, k), dtype=torch.int8, device="cuda")
+        codes[-3:] = codes_of((3, k), 1)
+        one, wq, ws = scales_of(rows, 2), codes_of((n, k), 3), scales_of(n, 4)
+        out = layer.int8_qmm(codes, one, wq, ws)
+        assert torch.equal(out[-3:], layer.int8_qmm(codes[-3:], one[-3:], wq, ws))
+        del codes, out
+    w = torch.ones((140003, 16384), dtype=torch.int8, device="cuda")  # the weights past 2^31 bytes
+    w[-70:] = codes_of((70, 16384), 5)
+    ws = scales_of(140003, 6)
+    for m in (2, 40):
+        codes, one = codes_of((m, 16384), 7), scales_of(m, 8)
+        out = layer.int8_qmm(codes, one, w, ws)
+        assert torch.equal(out[:, -70:], layer.int8_qmm(codes, one, w[-70:], ws[-70:].clone()))

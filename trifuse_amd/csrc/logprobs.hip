@@ -22,6 +22,10 @@
 // (a few in a thousand), the logits that reach the threshold go to a list in
 // LDS, and each one's rank in the list is its place among the alternatives.
 // A row made so that the list overflows takes one scan per alternative.
+//
+// Bound: arithmetic beside the stream, about 12 issue slots a logit of which the
+// exponential takes four. 4096 x 50304 bf16: 79 us without alternatives (5.2 TB/s),
+// 98 with 20; one row 8.9 us, one workgroup's arithmetic.
 #include "tfm_device.h"
 #include "tfm_internal.h"
 

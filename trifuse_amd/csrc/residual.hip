@@ -16,8 +16,11 @@
 // Bound: memory (y, r in, h, x out: 8 bytes an element). A team of lanes owns
 // a row and keeps it in registers from the loads to the stores, so every
 // byte moves once; both norms' sums are a lane's own sequential sum, then
-// the pairwise tree over the wave, then the waves in order, so results do not
-// depend on the launch.
+// the pairwise tree over the wave, then the waves in order. The team follows
+// from the width alone, so that a row has the same bits in every batch (four waves
+// a row of 2048: 16 rows 3.4 against 4.2 us, 300 rows 4.0 against 4.6, 4096 rows 14.9
+// against 14.4). 16384 x 2048 with a gate for each element 59 us, 5.6 TB/s; to
+// codes 40 us; quantize_rows of the same 16.6 us, 6.0 TB/s.
 #include <type_traits>
 
 #include "tfm_device.h"
