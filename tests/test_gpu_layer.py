@@ -254,7 +254,8 @@ def test_int8_qmm_scales_bias_and_neighbours(gpu, rows):
 
 @pytest.mark.parametrize("rows,k,n,dtype", [(1, 2048, 2048, BF16), (1, 16, 1, F16), (3, 1536, 515, F16), (8, 4096, 640, BF16),
                                             (16, 2048, 1000, BF16), (17, 512, 96, F16), (64, 1040, 130, BF16),
-                                            (130, 272, 70, F16), (515, 2048, 300, BF16)])
+                                            (130, 272, 70, F16), (515, 2048, 300, BF16), (5, 272, 8200, F16),
+                                            (6, 2048, 33000, BF16), (3, 528, 32771, F16)])
 def test_int8_linear_is_quantize_then_product(gpu, rows, k, n, dtype):
     x, w, ws, bias = rand((rows, k), 1, 1.0, dtype), codes_of((n, k), 2), scales_of(n, 4), rand((n,), 5, 1.0, dtype)
     codes, scales = layer.quantize_rows(x)

@@ -296,7 +296,7 @@ __global__ __launch_bounds__(BM / WM * (BN / WN) * 64, MINW) void igemm_tile_ker
 // share 16 channels, every KS-th 64 bytes of K each, and join their sums in LDS.
 // With FUSED the codes are made here from x itself, in every workgroup; the first
 // weights are on their way meanwhile. Bound: the weights' stream where they are many
-// (8 x 2048 x 50304 24.5 us, 4.2 TB/s), else latency (1 x 2048 x 2048 4.5 us).
+// (1 x 2048 x 50304 21.5 us, 4.8 TB/s), else latency (1 x 2048 x 2048 4.4 us).
 constexpr int kFewRows = 16;
 constexpr int kFewLds = 64 << 10;
 constexpr int kFewStep = 64;   // bytes of K an MFMA
@@ -304,11 +304,11 @@ constexpr int kFewAhead = 8;   // MFMAs a wave has weights in flight for
 
 __host__ __device__ inline int few_row_bytes(int K) { return (K + kFewStep - 1) / kFewStep * kFewStep + 16; }
 inline bool few_fits(int64_t rows, int K) {
-  return rows <= kFewRows && rows * (int64_t)few_row_bytes(K) + 4096 + 64 <= kFewLds;
+  return rows <= kFewRows && rows * (int64_t)few_row_bytes(K) + 8192 + 64 <= kFewLds;
 }
 
-template <bool FUSED, bool F16X, int KS, int OUT>
-__global__ __launch_bounds__(256) void igemm_few_kernel(IgArgs a, const uint16_t* xh) {
+template <bool FUSED, bool F16X, int WV, int KS, int OUT>
+__global__ __launch_bounds__(64 * WV) void igemm_few_kernel(IgArgs a, const uint16_t* xh) {
   extern __shared__ __attribute__((aligned(16))) int8_t lds[];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int K = a.K, T = a.T, N = a.N;
@@ -316,7 +316,7 @@ __global__ __launch_bounds__(256) void igemm_few_kernel(IgArgs a, const uint16_t
   int8_t* const sx = lds;
   float* const sscale = reinterpret_cast<float*>(lds + T * RB);
   i32x4_t* const spart = reinterpret_cast<i32x4_t*>(lds + (T * RB + 64 + 15) / 16 * 16);
-  const int n0 = (blockIdx.x * (4 / KS) + wave / KS) * 16, part = wave % KS;
+  const int n0 = (blockIdx.x * (WV / KS) + wave / KS) * 16, part = wave % KS;
   const int S = (K + kFewStep - 1) / kFewStep;
   const int row = n0 + (lane & 15) < N ? n0 + (lane & 15) : N - 1;
   const int kc = (lane >> 4) * 16;
@@ -339,13 +339,13 @@ __global__ __launch_bounds__(256) void igemm_few_kernel(IgArgs a, const uint16_t
   load(B1{}, part + HOP);
 
   if constexpr (FUSED) {
-    for (int t = wave; t < T; t += 4) {
+    for (int t = wave; t < T; t += WV) {
       const RowScale rs = quantize_row_wave<F16X>(xh + (int64_t)t * K, K, sx + t * RB, lane);
       if (lane == 0) sscale[t] = rs.scale;
     }
   } else {
     const int pieces = K / 16;
-    for (int i = threadIdx.x; i < T * pieces; i += 256) {
+    for (int i = threadIdx.x; i < T * pieces; i += 64 * WV) {
       const int t = i / pieces, p = i % pieces;
       *reinterpret_cast<uint4*>(sx + t * RB + 16 * p) = *reinterpret_cast<const uint4*>(a.x + (int64_t)t * K + 16 * p);
     }
@@ -405,21 +405,23 @@ __global__ __launch_bounds__(256) void igemm_few_kernel(IgArgs a, const uint16_t
 }
 
 // xh null: codes given.
-template <int KS>
+template <int WV, int KS>
 void launch_few(int dtype, const IgArgs& a, const uint16_t* xh, hipStream_t s) {
-  const unsigned groups = (unsigned)((a.N + 15) / 16), blocks = (groups + 4 / KS - 1) / (4 / KS);
-  const size_t lds = ((size_t)a.T * few_row_bytes(a.K) + 64 + 15) / 16 * 16 + (KS > 1 ? 4096 : 0);
+  const unsigned groups = (unsigned)((a.N + 15) / 16), blocks = (groups + WV / KS - 1) / (WV / KS);
+  const size_t lds = ((size_t)a.T * few_row_bytes(a.K) + 64 + 15) / 16 * 16 + (KS > 1 ? WV * 1024 : 0);
   const bool f16 = dtype == TFM_DTYPE_F16;
   if (xh && f16)
-    igemm_few_kernel<true, true, KS, TFM_DTYPE_F16><<<blocks, 256, lds, s>>>(a, xh);
+    igemm_few_kernel<true, true, WV, KS, TFM_DTYPE_F16><<<blocks, 64 * WV, lds, s>>>(a, xh);
   else if (xh)
-    igemm_few_kernel<true, false, KS, TFM_DTYPE_BF16><<<blocks, 256, lds, s>>>(a, xh);
+    igemm_few_kernel<true, false, WV, KS, TFM_DTYPE_BF16><<<blocks, 64 * WV, lds, s>>>(a, xh);
+  else if constexpr (WV == 8)
+    fail(TFM_E_UNSUPPORTED, "int8 product: eight waves are for codes made in the kernel");
   else if (dtype == TFM_DTYPE_F32)
-    igemm_few_kernel<false, false, KS, TFM_DTYPE_F32><<<blocks, 256, lds, s>>>(a, nullptr);
+    igemm_few_kernel<false, false, WV, KS, TFM_DTYPE_F32><<<blocks, 64 * WV, lds, s>>>(a, nullptr);
   else if (f16)
-    igemm_few_kernel<false, true, KS, TFM_DTYPE_F16><<<blocks, 256, lds, s>>>(a, nullptr);
+    igemm_few_kernel<false, true, WV, KS, TFM_DTYPE_F16><<<blocks, 64 * WV, lds, s>>>(a, nullptr);
   else
-    igemm_few_kernel<false, false, KS, TFM_DTYPE_BF16><<<blocks, 256, lds, s>>>(a, nullptr);
+    igemm_few_kernel<false, false, WV, KS, TFM_DTYPE_BF16><<<blocks, 64 * WV, lds, s>>>(a, nullptr);
 }
 
 template <int BM, int BN, int WM, int WN, int S, int MINW>
@@ -447,15 +449,20 @@ IgArgs ig_args(int dtype, const int8_t* x, const float* x_scales, int64_t rows, 
   return IgArgs{x, w, x_scales, w_scales, bias, out, (int)rows, N, K, 0, 0, vec};
 }
 
-// Waves that share 16 channels: one where the channels alone fill the chip (two
-// workgroups of 64 channels a CU), else four. us with one / four: 1 x 2048 x 2048
-// 7.6 / 4.4, 8 x 4096 x 12288 18.0 / 14.9, 8 x 2048 x 50304 24.4 / 25.9, 16 x 2048 x 50304
-// 25.9 / 32.4.
+// Waves that share 16 channels: one where the channels alone fill the chip, else
+// four. us with one / four: 1 x 2048 x 2048 7.6 / 4.4, 8 x 4096 x 12288 18.0 / 14.9,
+// 8 x 2048 x 50304 24.4 / 25.9, 16 x 2048 x 50304 25.9 / 32.4.
+// Waves of a workgroup: sixteen of one each, so that few workgroups make the same
+// codes (4 / 8 / 16 waves at 8 x 2048 x 50304 27.6 / 27.2 / 26.0, at 1 row 24.1 / 23.6 /
+// 22.8); of four each four, but eight where four rows or more are made into codes
+// for many channels (5 x 4096 x 8192 13.8 / 11.8, 1 x 4096 x 12288 15.1 / 16.6).
 void run_few(int dtype, const IgArgs& a, const uint16_t* xh, hipStream_t s) {
   if (a.N >= 512 * 64)
-    launch_few<1>(dtype, a, xh, s);
+    launch_few<16, 1>(dtype, a, xh, s);
+  else if (xh && a.T >= 4 && a.N >= 8192)
+    launch_few<8, 4>(dtype, a, xh, s);
   else
-    launch_few<4>(dtype, a, xh, s);
+    launch_few<4, 4>(dtype, a, xh, s);
 }
 
 }  // namespace
