@@ -18,9 +18,12 @@
 // largest key among the items it has read (their maxima, the item's place).
 // 64 buckets, lane l of every wave, give 64 maxima; the top-th largest of them
 // is a threshold that at least `top` logits reach. Only threads whose own
-// maximum reaches it can hold such logits: their items are read again
-// (a few in a thousand), the logits that reach the threshold go to a list in
-// LDS, and each one's rank in the list is its place among the alternatives.
+// maximum reaches it can hold such logits. They read the item of their maximum
+// again; those whose second largest item may reach it too go over all of theirs
+// (no line of theirs is in the cache any more, and 25 threads' items are half the
+// row's lines: 4096 x 50304 97 us with that for every such thread). The logits that
+// reach the threshold go to a list in LDS, and each one's rank in the list is its
+// place among the alternatives.
 // A row made so that the list overflows takes one scan per alternative.
 //
 // Bound: arithmetic beside the stream, about 12 issue slots a logit of which the
@@ -146,6 +149,7 @@ __global__ __launch_bounds__(THREADS) void token_logprobs_kernel(LogprobsArgs a)
   };
   Stats st{kLow, 0.0f, 0.0f};
   int best_item = -1;  // the first item that holds st.m
+  float second = -__builtin_inff();  // no other item's maximum is larger
   // kAhead vectors a thread are on their way at a time; past the last one a
   // thread reads that one again and leaves it out.
   for (int v = tid; v < (full + THREADS - 1) / THREADS * THREADS; v += kAhead * THREADS) {
@@ -162,6 +166,7 @@ __global__ __launch_bounds__(THREADS) void token_logprobs_kernel(LogprobsArgs a)
 #pragma unroll
       for (int j = 0; j < N; ++j) f[j] = L::get(u[i], j);
       const float m = max_of(f);
+      second = __builtin_amdgcn_fmed3f(second, st.m, m);
       if (m > st.m) {
         st = rescaled(st, m, c);
         best_item = v + i * THREADS;
@@ -174,6 +179,7 @@ __global__ __launch_bounds__(THREADS) void token_logprobs_kernel(LogprobsArgs a)
   const int turn = (tid - full % THREADS + THREADS) % THREADS;
   if (turn < items - full) {
     const float f = L::one(row, (int64_t)full * N + turn);
+    second = __builtin_amdgcn_fmed3f(second, st.m, f);
     if (f > st.m) {
       st = rescaled(st, f, c);
       best_item = full + turn;
@@ -302,24 +308,32 @@ __global__ __launch_bounds__(THREADS) void token_logprobs_kernel(LogprobsArgs a)
   const int at = __builtin_ctzll(__ballot(above == a.top - 1));
   const uint64_t thr = (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(bucket >> 32), at) << 32 |
                        (uint32_t)__builtin_amdgcn_readlane((int)bucket, at);
-  if (best != 0 && best >= thr) chosen[atomicAdd(&n_chosen, 1)] = tid;
-  __syncthreads();
-  const int nc = n_chosen, per = (items + THREADS - 1) / THREADS;
-  for (int i = tid; i < nc * per; i += THREADS) {
-    const int v = chosen[i % nc] + i / nc * THREADS;
-    if (v >= items) continue;
+  const float low = value_of((uint32_t)(thr >> 32));  // NaN: no logit is below
+  auto scan = [&](int v) {
     float f[N];
     const int n = fetch(v, f);
     const uint32_t first = v < full ? (uint32_t)v * N : (uint32_t)(full * N + (v - full));
-    if (key_of(order_of(n == N ? max_of(f) : f[0]), (uint32_t)v) < thr) continue;
 #pragma unroll
     for (int j = 0; j < N; ++j) {
+      if (j >= n || f[j] < low) continue;
       const uint32_t o = order_of(f[j]);
-      if (j < n && key_of(o, (uint32_t)v) >= thr) {
-        const int p = atomicAdd(&n_cand, 1);
-        if (p < kCap) cand[p] = key_of(o, first + j);
-      }
+      if (key_of(o, (uint32_t)v) < thr) continue;
+      const int p = atomicAdd(&n_cand, 1);
+      if (p < kCap) cand[p] = key_of(o, first + j);
     }
+  };
+  if (best != 0 && best >= thr) {
+    if (best_item >= 0 && second < low)
+      scan(best_item);
+    else
+      chosen[atomicAdd(&n_chosen, 1)] = tid;
+  }
+  __syncthreads();
+  const int nc = n_chosen, per = (items + THREADS - 1) / THREADS;
+  const int bits = per > 1 ? 32 - __builtin_clz(per - 1) : 0;  // items of a thread, to a power of two
+  for (int i = tid; i < nc << bits; i += THREADS) {
+    const int v = chosen[i >> bits] + (i & ((1 << bits) - 1)) * THREADS;
+    if (v < items) scan(v);
   }
   __syncthreads();
   int32_t* ids = a.top_ids + (int64_t)t * a.top;
