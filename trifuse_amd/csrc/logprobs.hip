@@ -28,7 +28,7 @@
 //
 // Bound: arithmetic beside the stream, about 12 issue slots a logit of which the
 // exponential takes four. 4096 x 50304 bf16: 79 us without alternatives (5.2 TB/s),
-// 98 with 20; one row 8.9 us, one workgroup's arithmetic.
+// 86 to 91 with 20; one row 8.4 us, one workgroup's arithmetic.
 #include "tfm_device.h"
 #include "tfm_internal.h"
 
