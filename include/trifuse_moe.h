@@ -297,8 +297,9 @@ int tfm_expert_routes(const tfm_plan* plan, const void* x, int64_t tokens,
  * in fp32 from the unrounded h; each output is rounded once. Outputs (at
  * least one): h [rows, width]; with pre_weight also x [rows, width] in the
  * storage dtype and/or codes [rows, width] with scales [rows] (as
- * tfm_quantize_rows makes them, from the unrounded x). h may be y or residual
- * itself (same address); no other overlap. width <= 32768. */
+ * tfm_quantize_rows makes them, from the unrounded x). h may be y, residual or a full gate
+ * itself (same address); other overlaps of h or x with an input or each other
+ * are refused. width <= 32768. */
 typedef struct tfm_norm_step {
   const void* y;           /* [rows, width]                                */
   const void* residual;    /* [rows, width] or NULL                        */

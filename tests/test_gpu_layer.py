@@ -141,6 +141,9 @@ def test_norm_residual_leaves_what_is_not_its_own(gpu):
     y = rand((3, 520), 1)
     layer.norm_residual(y, out=buf[2:5])
     assert (buf[:2] == 9).all() and (buf[5:] == 9).all() and torch.equal(buf[2:5], y)
+    from trifuse_amd._lib import TfmError
+    with pytest.raises(TfmError, match="overlaps"):
+        layer.norm_residual(buf[1:4], out=buf[2:5])
     empty = layer.norm_residual(y[:0], y[:0], pre_weight=y[0])
     assert empty[0].shape == empty[1].shape == (0, 520)
 

@@ -40,6 +40,12 @@ def step(**kw):
     (dict(pre_weight=P, scales=P), 1, 64, BF16, 1, "codes and scales"),
     (dict(y=None), 1, 64, BF16, 1, "y is null"),
     (dict(pre_weight=P, x=P), 1, 64, BF16, 1, "alias"),
+    (dict(h=P + 64), 1, 64, BF16, 1, "overlaps"),
+    (dict(h=P - 2), 1, 64, BF16, 1, "overlaps"),
+    (dict(y=P + 65536, residual=P + 100), 1, 64, BF16, 1, "overlaps"),
+    (dict(y=P + 65536, gate=P + 1024, gate_kind=3), 9, 64, BF16, 1, "overlaps"),
+    (dict(pre_weight=P, h=P + 65536, x=P + 65540), 1, 64, BF16, 1, "alias h"),
+    (dict(pre_weight=P, h=P + 65536, x=P + 126), 1, 64, BF16, 1, "alias y"),
     (dict(y=None), 0, 64, BF16, 0, ""),
 ])
 def test_norm_residual_rejects(kw, rows, width, dtype, code, msg):

@@ -1,4 +1,6 @@
 // C ABI of the operators around the block: argument checks and launches.
+#include <initializer_list>
+
 #include "tfm_internal.h"
 
 using namespace tfm;
@@ -13,6 +15,12 @@ void need_storage(int32_t dtype) {
 
 void need_eps(float eps, const char* name) {
   if (!(eps >= 0.0f) || eps > 3.4e38f) fail(TFM_E_INVALID, std::string(name) + " must be a non-negative number");
+}
+
+// Two buffers of the same size that share memory without being the same.
+bool overlap(const void* a, const void* b, size_t bytes) {
+  const uintptr_t p = reinterpret_cast<uintptr_t>(a), q = reinterpret_cast<uintptr_t>(b);
+  return a && b && p != q && (p > q ? p - q : q - p) < bytes;
 }
 
 constexpr int kProductMaxK = 131056;  // 128 * 128 * K < 2^31
@@ -60,8 +68,13 @@ int tfm_norm_residual(const tfm_norm_step* step, int64_t rows, int32_t width, in
     need((step->codes == nullptr) == (step->scales == nullptr), "codes and scales go together");
     need_ptr(step->y, "y");
     if (step->gate_kind != TFM_GATE_NONE) need_ptr(step->gate, "gate");
-    need(!step->x || (step->x != step->y && step->x != step->residual && step->x != step->h),
-         "x must not alias y, residual or h");
+    const size_t bytes = (size_t)rows * (size_t)width * 2;
+    const void* full_gate = step->gate_kind == TFM_GATE_FULL ? step->gate : nullptr;
+    for (const void* in : {step->y, step->residual, full_gate}) {
+      need(!overlap(step->h, in, bytes), "h overlaps an input that it is not");
+      need(!step->x || (step->x != in && !overlap(step->x, in, bytes)), "x must not alias y, residual or gate");
+    }
+    need(!step->x || (step->x != step->h && !overlap(step->x, step->h, bytes)), "x must not alias h");
     launch_norm_residual(dtype == TFM_DTYPE_F16, *step, (int)rows, width, static_cast<hipStream_t>(stream));
   });
 }

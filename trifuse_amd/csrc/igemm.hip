@@ -239,7 +239,7 @@ __global__ __launch_bounds__(BM / WM * (BN / WN) * 64, MINW) void igemm_tile_ker
       stage(sx3, sw3, sx0, sw0, kt + 3);
     }
   }
-  __syncthreads();  // the copies past the end
+  stage_wait<0>();  // the copies past the end: the epilogue writes where they land
   // Epilogue. Lane l holds token l % 32 and channels 8 (i / 4) + 4 (l / 32) + i % 4
   // of each 32 x 32 block: scaled and rounded, 32 tokens at a time go through the
   // wave's own part of LDS (every wave is past its last read of it) and leave as
