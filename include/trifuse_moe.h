@@ -279,8 +279,10 @@ int tfm_expert_routes(const tfm_plan* plan, const void* x, int64_t tokens,
  * fused block keeps the reference's own norm (tfm_moe_forward_rmsnorm); these
  * have no counterpart in the reference. None needs a plan; rows are dense
  * (row t starts at t * width elements) unless a stride is given; rows may be 0
- * (nothing is read or written), at most 2^22 - 1. Activations are
- * TFM_DTYPE_BF16 or TFM_DTYPE_F16. Rows and pointers need no alignment beyond
+ * (nothing is read or written), at most 2^22 - 1. An output or workspace that
+ * shares memory with an input or another output is refused, but h of
+ * tfm_norm_residual as stated there. Activations are TFM_DTYPE_BF16 or
+ * TFM_DTYPE_F16. Rows and pointers need no alignment beyond
  * their elements', except the codes of the products (below); 16-byte aligned
  * ones with widths of a multiple of 8 move faster. */
 
@@ -297,9 +299,8 @@ int tfm_expert_routes(const tfm_plan* plan, const void* x, int64_t tokens,
  * in fp32 from the unrounded h; each output is rounded once. Outputs (at
  * least one): h [rows, width]; with pre_weight also x [rows, width] in the
  * storage dtype and/or codes [rows, width] with scales [rows] (as
- * tfm_quantize_rows makes them, from the unrounded x). h may be y, residual or a full gate
- * itself (same address); other overlaps of h or x with an input or each other
- * are refused. width <= 32768. */
+ * tfm_quantize_rows makes them, from the unrounded x). h may be y, residual or a
+ * full gate itself (same address). width <= 32768. */
 typedef struct tfm_norm_step {
   const void* y;           /* [rows, width]                                */
   const void* residual;    /* [rows, width] or NULL                        */
@@ -348,7 +349,8 @@ int tfm_int8_linear(const void* x, int64_t rows, const int8_t* w, const float* w
 
 /* Log probabilities under softmax(scale * logits) over each row, in one pass
  * over logits [rows, vocab] (dtype bf16, f16 or TFM_DTYPE_F32; row t starts at
- * t * row_stride elements, row_stride >= vocab):
+ * t * row_stride elements, row_stride >= vocab; what lies between rows counts
+ * as logits where outputs are kept apart from them):
  *   logprobs [rows]            of tokens[t] (int32 or int64 by token_bits 32 or
  *                              64); NaN where tokens[t] is outside [0, vocab)
  *   entropy [rows]             -sum p ln p, in nats

@@ -174,3 +174,53 @@ def test_native_host_side_refuses_what_is_no_tensor():
         lib.raise_status(lib.TFM_E_UNSUPPORTED)
     with pytest.raises(lib.TfmError):
         lib.raise_status(lib.TFM_E_INVALID)
+
+
+@pytest.mark.parametrize("kw", [
+    dict(post_weight=P), dict(post_weight=P + 64), dict(pre_weight=P + 9 * 128 - 2), dict(pre_weight=P - 126),
+    dict(gate=P + 128, gate_kind=_lib.TFM_GATE_CHANNEL), dict(gate=P, gate_kind=_lib.TFM_GATE_TOKEN),
+    dict(gate=P - 32, gate_kind=_lib.TFM_GATE_TOKEN),
+    dict(h=None, x=P, pre_weight=P + 1024), dict(h=None, x=P, pre_weight=P - 2),
+    dict(h=None, x=P, pre_weight=P + 65536, gate=P + 4, gate_kind=_lib.TFM_GATE_TOKEN),
+    dict(pre_weight=P + 65536, codes=P, scales=P + 70000), dict(pre_weight=P + 65536, codes=P + 70000, scales=P + 8),
+    dict(pre_weight=P + 65536, y=P + 20000, codes=P + 20000 + 1151, scales=P + 70000),
+    dict(pre_weight=P + 65536, codes=P + 65536 + 127, scales=P + 70000),
+    dict(pre_weight=P + 65536, codes=P + 70000, scales=P + 65536 - 35),
+    dict(pre_weight=P + 65536, codes=P + 70000, scales=P + 70575),
+    dict(pre_weight=P + 65536, gate=P + 80000, gate_kind=_lib.TFM_GATE_TOKEN, codes=P + 80035, scales=P + 70000),
+])
+def test_norm_residual_refuses_outputs_over_weights_gates_and_each_other(kw):
+    """9 rows of 64 elements: 1152 bytes, weights 128, a gate or scale for each row 36, codes 576."""
+    s = step(**{**dict(y=P + 4096 * 9, h=P), **kw})
+    check(_lib.load().tfm_norm_residual(ctypes.byref(s), 9, 64, BF16, None), 1, "overlap")
+
+
+@pytest.mark.parametrize("codes,scales", [(P, P + 8192), (P + 1151, P + 8192), (P - 575, P + 8192), (P + 8192, P + 4),
+                                          (P + 8192, P + 8192 + 572), (P + 8192, P + 8192 - 32)])
+def test_quantize_rows_refuses_overlaps(codes, scales):
+    check(_lib.load().tfm_quantize_rows(P, 9, 64, BF16, codes, scales, None), 1, "overlap")
+
+
+@pytest.mark.parametrize("out,bias", [(P, None), (P + 1024, None), (P + 4096, None), (P + 4096 + 35, None),
+                                      (P + 8192 + 640, None), (P + 12288, None), (P + 16384 - 717, P + 16384)])
+def test_products_refuse_an_output_over_an_input(out, bias):
+    """9 rows of 128 codes at P, scales at P + 4096, 20 channels of 128 at P + 8192, their scales at P + 12288."""
+    check(_lib.load().tfm_int8_qmm(P, P + 4096, 9, P + 8192, P + 12288, bias, 20, 128, F32, out, None), 1, "overlap")
+
+
+def test_int8_linear_refuses_overlaps():
+    lib, w, ws, far = _lib.load(), 1 << 24, 1 << 25, 1 << 26
+    need = lib.tfm_int8_linear_workspace_bytes(500, 256)
+    for rows, out, work in ((2, P + 512, None), (2, w + 10, None), (2, ws + 4, None), (500, P, far), (500, w, far),
+                            (500, far, P), (500, far, w - 256), (500, far, ws), (500, far + 300, far)):
+        check(lib.tfm_int8_linear(P, rows, w, ws, None, 64, 256, BF16, out, work, need if work else 0, None), 1, "overlap")
+
+
+@pytest.mark.parametrize("kw", [dict(logprobs=P), dict(entropy=P + 2 * 400 + 199), dict(ids=P + 3 * 400 - 1 - 200),
+                                dict(best=P + 5000 - 47), dict(entropy=P + 10000 + 8), dict(best=P + 30000 + 44)])
+def test_token_logprobs_refuses_overlaps(kw):
+    """3 rows of 100 logits, 200 apart, at P; 3 tokens at P + 5000."""
+    a = dict(logprobs=P + 10000, entropy=P + 20000, ids=P + 30000, best=P + 40000)
+    a.update(kw)
+    check(_lib.load().tfm_token_logprobs(P, 3, 100, 200, BF16, P + 5000, 64, 4, 1.0, a["logprobs"], a["entropy"],
+                                         a["ids"], a["best"], None), 1, "overlap")

@@ -17,11 +17,25 @@ void need_eps(float eps, const char* name) {
   if (!(eps >= 0.0f) || eps > 3.4e38f) fail(TFM_E_INVALID, std::string(name) + " must be a non-negative number");
 }
 
-// Two buffers of the same size that share memory without being the same.
-bool overlap(const void* a, const void* b, size_t bytes) {
-  const uintptr_t p = reinterpret_cast<uintptr_t>(a), q = reinterpret_cast<uintptr_t>(b);
-  return a && b && p != q && (p > q ? p - q : q - p) < bytes;
+// The bytes of one buffer; null or empty ones share memory with nothing.
+struct Span {
+  const void* at;
+  size_t bytes;
+};
+bool meet(const Span& a, const Span& b) {
+  const uintptr_t p = reinterpret_cast<uintptr_t>(a.at), q = reinterpret_cast<uintptr_t>(b.at);
+  return p && q && (p > q ? p - q < b.bytes : q - p < a.bytes) && a.bytes && b.bytes;
 }
+
+// No output shares memory with an input or another output.
+void need_apart(std::initializer_list<Span> outs, std::initializer_list<Span> ins, const char* message) {
+  for (const Span* o = outs.begin(); o != outs.end(); ++o) {
+    for (const Span& in : ins) need(!meet(*o, in), message);
+    for (const Span* other = outs.begin(); other != o; ++other) need(!meet(*o, *other), message);
+  }
+}
+
+size_t size_of(int32_t dtype) { return dtype == TFM_DTYPE_F32 ? 4 : 2; }
 
 constexpr int kProductMaxK = 131056;  // 128 * 128 * K < 2^31
 
@@ -68,13 +82,24 @@ int tfm_norm_residual(const tfm_norm_step* step, int64_t rows, int32_t width, in
     need((step->codes == nullptr) == (step->scales == nullptr), "codes and scales go together");
     need_ptr(step->y, "y");
     if (step->gate_kind != TFM_GATE_NONE) need_ptr(step->gate, "gate");
-    const size_t bytes = (size_t)rows * (size_t)width * 2;
-    const void* full_gate = step->gate_kind == TFM_GATE_FULL ? step->gate : nullptr;
-    for (const void* in : {step->y, step->residual, full_gate}) {
-      need(!overlap(step->h, in, bytes), "h overlaps an input that it is not");
-      need(!step->x || (step->x != in && !overlap(step->x, in, bytes)), "x must not alias y, residual or gate");
+    const size_t n = (size_t)rows, w = (size_t)width, bytes = n * w * 2;
+    const int32_t gk = step->gate_kind;
+    const Span y{step->y, bytes}, residual{step->residual, bytes};
+    const Span gate{gk == TFM_GATE_NONE ? nullptr : step->gate,
+                    gk == TFM_GATE_FULL ? bytes : gk == TFM_GATE_TOKEN ? n * 4 : w * 2};
+    const Span post{step->post_weight, w * 2}, pre{step->pre_weight, w * 2};
+    const Span h{step->h, bytes}, x{step->x, bytes};
+    // Each lane has read its own elements of y, residual and a full gate before it writes h; weights and
+    // the other gates are read by every row.
+    for (const Span& in : {y, residual, gk == TFM_GATE_FULL ? gate : Span{nullptr, 0}}) {
+      need(h.at == in.at || !meet(h, in), "h overlaps an input that it is not");
+      need(!meet(x, in), "x must not alias y, residual or gate");
     }
-    need(!step->x || (step->x != step->h && !overlap(step->x, step->h, bytes)), "x must not alias h");
+    need(!meet(x, h), "x must not alias h");
+    for (const Span& in : {post, pre, gk == TFM_GATE_FULL ? Span{nullptr, 0} : gate})
+      need(!meet(h, in) && !meet(x, in), "h and x must not overlap a weight or a gate that rows share");
+    need_apart({{step->codes, n * w}, {step->scales, n * 4}}, {y, residual, gate, post, pre, h, x},
+               "codes and scales must not overlap an input or another output");
     launch_norm_residual(dtype == TFM_DTYPE_F16, *step, (int)rows, width, static_cast<hipStream_t>(stream));
   });
 }
@@ -90,6 +115,8 @@ int tfm_quantize_rows(const void* x, int64_t rows, int32_t width, int32_t dtype,
     need_ptr(x, "x");
     need_ptr(codes, "codes");
     need_ptr(scales, "scales");
+    const size_t n = (size_t)rows, w = (size_t)width;
+    need_apart({{codes, n * w}, {scales, n * 4}}, {{x, n * w * 2}}, "codes and scales must not overlap x or each other");
     launch_quantize_rows(dtype == TFM_DTYPE_F16, static_cast<const uint16_t*>(x), (int)rows, width, codes, scales,
                          static_cast<hipStream_t>(stream));
   });
@@ -108,6 +135,10 @@ int tfm_int8_qmm(const int8_t* x, const float* x_scales, int64_t rows, const int
     need_ptr(out, "out");
     need_align16(x, "x");
     need_align16(w, "w");
+    const size_t m = (size_t)rows, n = (size_t)n_out, k = (size_t)k_in;
+    need_apart({{out, m * n * size_of(dtype)}},
+               {{x, m * k}, {x_scales, m * 4}, {w, n * k}, {w_scales, n * 4}, {bias, n * size_of(dtype)}},
+               "out must not overlap an input");
     launch_int8_qmm(dtype, x, x_scales, rows, w, w_scales, bias, n_out, k_in, out, static_cast<hipStream_t>(stream));
   });
 }
@@ -130,13 +161,17 @@ int tfm_int8_linear(const void* x, int64_t rows, const int8_t* w, const float* w
     need_ptr(out, "out");
     need_align16(w, "w");
     hipStream_t s = static_cast<hipStream_t>(stream);
+    const size_t m = (size_t)rows, n = (size_t)n_out, k = (size_t)k_in;
+    const Span in{x, m * k * 2}, wq{w, n * k}, wscale{w_scales, n * 4}, b{bias, n * 2}, o{out, m * n * 2};
     if (int8_linear_few(rows, k_in)) {
+      need_apart({o}, {in, wq, wscale, b}, "out must not overlap an input");
       launch_int8_linear_few(dtype == TFM_DTYPE_F16, static_cast<const uint16_t*>(x), rows, w, w_scales, bias, n_out,
                              k_in, out, s);
       return;
     }
     const LinearWs ws = carve_linear(rows, k_in, workspace);
     need_ws(workspace, workspace_bytes, ws.bytes);
+    need_apart({o, {workspace, ws.bytes}}, {in, wq, wscale, b}, "out and workspace must not overlap an input or each other");
     launch_quantize_rows(dtype == TFM_DTYPE_F16, static_cast<const uint16_t*>(x), (int)rows, k_in, ws.codes, ws.scales,
                          s);
     launch_int8_qmm(dtype, ws.codes, ws.scales, rows, w, w_scales, bias, n_out, k_in, out, s);
@@ -164,6 +199,10 @@ int tfm_token_logprobs(const void* logits, int64_t rows, int32_t vocab, int64_t 
       need_ptr(top_ids, "top_ids");
       need_ptr(top_logprobs, "top_logprobs");
     }
+    const size_t n = (size_t)rows, size = size_of(dtype), k = n * (size_t)top;
+    need_apart({{logprobs, n * 4}, {entropy, n * 4}, {top_ids, k * 4}, {top_logprobs, k * 4}},
+               {{logits, ((n - 1) * (size_t)row_stride + (size_t)vocab) * size}, {tokens, n * (size_t)(token_bits / 8)}},
+               "outputs must not overlap an input or each other");
     const LogprobsArgs a{logits, row_stride,       (int)rows, vocab,   top,     scale,
                          tokens, token_bits == 64, logprobs,  entropy, top_ids, top_logprobs};
     launch_token_logprobs(dtype, a, static_cast<hipStream_t>(stream));

@@ -156,10 +156,10 @@ PyObject* norm_residual(PyObject*, PyObject* const* v, Py_ssize_t n) {
       const at::Tensor& g = tensor(v[4], "gate");
       need_beside(g, "gate", y);
       s.gate = g.data_ptr();
-      if (g.scalar_type() == y.scalar_type() && g.dim() == 1 && g.size(0) == r.width)
-        s.gate_kind = TFM_GATE_CHANNEL;
-      else if (g.scalar_type() == y.scalar_type() && g.sizes() == y.sizes())
+      if (g.scalar_type() == y.scalar_type() && g.sizes() == y.sizes())
         s.gate_kind = TFM_GATE_FULL;
+      else if (g.scalar_type() == y.scalar_type() && g.dim() == 1 && g.size(0) == r.width)
+        s.gate_kind = TFM_GATE_CHANNEL;
       else if (g.scalar_type() == at::kFloat &&
                (g.sizes() == lead(y) || (g.dim() == y.dim() && g.size(-1) == 1 && lead(g) == lead(y))))
         s.gate_kind = TFM_GATE_TOKEN;

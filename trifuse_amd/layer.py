@@ -68,7 +68,8 @@ def norm_residual(y: torch.Tensor, residual: Optional[torch.Tensor] = None, *,
     shape, or that with a 1). Returns h without pre_weight; (h, x) with
     pre_weight [H]; (h, codes, scales) with quantize, codes int8 in y's shape
     and scales fp32 in its leading shape. x is normed from h before its
-    rounding. out receives h and may be y or residual."""
+    rounding. out receives h and may be y, residual or a gate in y's shape; it shares no
+    other memory with an input."""
     return _enqueue("norm_residual", y, residual, post_weight, gate, residual_multiplier, pre_weight, eps, post_eps,
                     quantize, out)
 
