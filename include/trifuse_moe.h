@@ -361,7 +361,7 @@ int tfm_int8_linear(const void* x, int64_t rows, const int8_t* w, const float* w
  * top may be 0. Masked logits are -inf (probability 0, log probability -inf).
  * A row of nothing but -inf has entropy 0 and log probabilities -inf; one with
  * +inf or NaN has NaN for all of its log probabilities and its entropy. scale:
- * positive and finite (1 / temperature, or a model's logit scaling). */
+ * 1e-35 to 1e30 (1 / temperature, or a model's logit scaling). */
 int tfm_token_logprobs(const void* logits, int64_t rows, int32_t vocab, int64_t row_stride,
                        int32_t dtype, const void* tokens, int32_t token_bits, int32_t top,
                        float scale, float* logprobs, float* entropy, int32_t* top_ids,

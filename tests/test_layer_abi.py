@@ -224,3 +224,9 @@ def test_token_logprobs_refuses_overlaps(kw):
     a.update(kw)
     check(_lib.load().tfm_token_logprobs(P, 3, 100, 200, BF16, P + 5000, 64, 4, 1.0, a["logprobs"], a["entropy"],
                                          a["ids"], a["best"], None), 1, "overlap")
+
+
+@pytest.mark.parametrize("scale", [9e-36, 1.1e30])
+def test_token_logprobs_refuses_scales_past_its_bounds(scale):
+    check(_lib.load().tfm_token_logprobs(P, 3, 100, 100, BF16, None, 64, 0, scale, None, P + 8192, None, None, None), 1,
+          "scale must be in")

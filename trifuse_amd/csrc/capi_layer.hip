@@ -189,7 +189,8 @@ int tfm_token_logprobs(const void* logits, int64_t rows, int32_t vocab, int64_t 
     need(dtype == TFM_DTYPE_BF16 || dtype == TFM_DTYPE_F16 || dtype == TFM_DTYPE_F32, "unknown dtype");
     need(top >= 0 && top <= vocab, "need 0 <= top <= vocab");
     if (top > 64) fail(TFM_E_UNSUPPORTED, "more than 64 alternatives are not built");
-    need(scale > 0.0f && scale <= 1e30f, "scale must be in (0, 1e30]");
+    // Below 1e-35 logits whose difference passes the largest number would still count beside each other.
+    need(scale >= 1e-35f && scale <= 1e30f, "scale must be in [1e-35, 1e30]");
     if (rows == 0) return;  // empty tensors may have null pointers
     need((tokens == nullptr) == (logprobs == nullptr), "tokens and logprobs go together");
     need(!tokens || token_bits == 32 || token_bits == 64, "token_bits must be 32 or 64");

@@ -1,13 +1,13 @@
 // Log probabilities of given tokens, entropy and the most likely alternatives
 // of softmax(scale * logits), one workgroup a row, one pass over the logits.
 //
-// With M the row's largest logit, S = sum e^(scale (l - M)) and
-// D = sum (l - M) e^(scale (l - M)):
-//   log p(l) = scale (l - M) - ln S,   entropy = ln S - scale D / S.
+// With M the row's largest logit, y = scale (l - M) / ln 2, S = sum 2^y and D = sum y 2^y:
+//   log p(l) = scale (l - M) - ln S,   entropy = ln S - ln 2 D / S.
 // Both terms of the entropy are non-negative: nothing cancels. Each thread keeps
 // M, S and D of what it has read and rescales S and D when M grows; differences
 // of logits are taken before the scale, so they are exact for 16-bit logits
-// near the maximum, the ones that count. Where one token is nearly sure, S is
+// near the maximum, the ones that count. A term of D counts while 2^y does not
+// vanish, so D stays as small as S whatever the scale. Where one token is nearly sure, S is
 // 1 + R with R far below 1: one thread alone adds the 1, its other terms are
 // summed again without it, and ln S = log1p(R) keeps its precision.
 //
@@ -81,12 +81,12 @@ struct Stats {
   float m, s, d;
 };
 
-// The same sums at a maximum m' >= m. The difference of maxima is kept finite:
-// an empty part (s = d = 0) stays empty.
+// The same sums at a maximum m' >= m. The exponent is kept finite, far below where
+// 2^y vanishes, so that nothing becomes 0 * inf.
 __device__ __forceinline__ Stats rescaled(const Stats& a, float m, float c) {
-  const float dm = fmaxf(a.m - m, -1e30f);
-  const float e = __builtin_amdgcn_exp2f(dm * c);
-  return Stats{m, a.s * e, e * __builtin_fmaf(dm, a.s, a.d)};
+  const float y = fmaxf((a.m - m) * c, -1e30f);
+  const float e = __builtin_amdgcn_exp2f(y);
+  return Stats{m, a.s * e, e * __builtin_fmaf(y, a.s, a.d)};
 }
 
 template <int CTRL, int ROW_MASK>
@@ -136,10 +136,10 @@ __global__ __launch_bounds__(THREADS) void token_logprobs_kernel(LogprobsArgs a)
   }
 
   auto term = [&](float f, float m, float& s, float& d) {
-    const float x = f - m;
-    const float e = __builtin_amdgcn_exp2f(x * c);
+    const float y = (f - m) * c;
+    const float e = __builtin_amdgcn_exp2f(y);
     s += e;
-    d = __builtin_fmaf(fmaxf(x, kLow), e, d);  // a masked logit: e = 0, not -inf * 0
+    d = __builtin_fmaf(fmaxf(y, kLow), e, d);  // a masked logit: e = 0, not -inf * 0
   };
   auto max_of = [&](const float* f) {
     float m = f[0];
@@ -294,10 +294,13 @@ __global__ __launch_bounds__(THREADS) void token_logprobs_kernel(LogprobsArgs a)
   const float s = m == __builtin_inff() ? __uint_as_float(0x7fc00000u) : r + (float)ones;
   const float ln_s = ones > 0 ? log1pf(s - 1.0f < 1.0f ? r + (float)(ones - 1) : s - 1.0f) : logf(s);
   const bool empty = s == 0.0f;  // every logit is -inf
-  auto logp = [&](float l) { return empty ? -__builtin_inff() : __builtin_fmaf(a.scale, l - m, -ln_s); };
+  // Halves: l - m may pass the largest number where scale * (l - m) does not.
+  auto logp = [&](float l) {
+    return empty ? -__builtin_inff() : __builtin_fmaf(2.0f * a.scale, 0.5f * l - 0.5f * m, -ln_s);
+  };
   if (tid == 0) {
     if (a.logprobs) a.logprobs[t] = token >= 0 && token < V ? logp(tl) : __uint_as_float(0x7fc00000u);
-    if (a.entropy) a.entropy[t] = empty ? 0.0f : ln_s - a.scale * d / s;
+    if (a.entropy) a.entropy[t] = empty ? 0.0f : ln_s - 0.693147181f * d / s;
   }
   if (a.top <= 0) return;
 

@@ -118,5 +118,5 @@ def token_logprobs(logits: torch.Tensor, tokens: Optional[torch.Tensor] = None, 
     [0, V) (None without tokens). entropy is fp32 in the leading shape, in nats.
     top_ids (int32) and top_logprobs (fp32) [..., top] are the `top` largest
     logits, largest first, ties to the lower id. Masked logits are -inf; a row
-    of nothing else has entropy 0 and log probabilities -inf."""
+    of nothing else has entropy 0 and log probabilities -inf. scale: 1e-35 to 1e30."""
     return _enqueue("token_logprobs", logits, tokens, top, scale)
