@@ -533,6 +533,9 @@ class MoEBlock:
         from . import layer
 
         T = self._check_x(h)
+        if h.get_device() != torch.cuda.current_device():  # all three calls on h's device and its stream
+            with torch.cuda.device(h.get_device()):
+                return self.forward_norms(h, weights, norm_weight, eps, post_weight, gate, next_weight)
         x = layer.rms_norm(h, norm_weight, eps)
         mw = self._weights(weights, router=True)
         y = torch.empty_like(h)
