@@ -1,5 +1,7 @@
 """The host side of the block between its norms (no GPU)."""
 import contextlib
+import threading
+import time
 
 import pytest
 import torch
@@ -41,3 +43,30 @@ def test_forward_norms_runs_on_its_tensors_device(monkeypatch, current):
     out = blk.forward_norms(h, None, torch.ones(64, dtype=torch.bfloat16), 1e-5)
     assert out.shape == h.shape and device[0] == current
     assert seen == [("norm", 101), ("tfm_moe_forward", 101), ("residual", 101)]
+
+
+def test_two_threads_make_one_second_plan(monkeypatch):
+    """Calls that need the plan without the multiplier at once share one: none is left without an owner."""
+    made, both = [], threading.Barrier(2)
+
+    def create(name, geometry, handle):
+        made.append(name)
+        if len(made) > 1:  # the block's own plan is made alone
+            time.sleep(0.2)
+        handle._obj.value = len(made)
+
+    monkeypatch.setattr(tmoe, "call", create)
+    blk = tmoe.MoEBlock(64, 64, 4, 2, residual_multiplier=0.5)
+    got = []
+
+    def use():
+        both.wait(timeout=10)
+        got.append(blk._unit_plan().value)
+
+    threads = [threading.Thread(target=use) for _ in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    blk._plan = blk._unit = None  # no plans of the library's: nothing to destroy
+    assert made == ["tfm_plan_create"] * 2 and got == [2, 2]

@@ -24,6 +24,7 @@ from __future__ import annotations
 
 import ctypes
 import dataclasses
+import threading
 from typing import Dict, Optional, Tuple
 
 import torch
@@ -343,6 +344,7 @@ class MoEBlock:
         self._lib = lib
         self._plan = handle
         self._unit: Optional[ctypes.c_void_p] = None
+        self._unit_lock = threading.Lock()
         self._ws: Optional[torch.Tensor] = None
         self._ws_bytes: Dict[int, int] = {}
         self._wcache: Dict[Tuple[int, bool], tuple] = {}
@@ -549,12 +551,13 @@ class MoEBlock:
         """The block's plan with residual multiplier 1 (its own where that is 1)."""
         if self.residual_multiplier == 1.0:
             return self._plan
-        if self._unit is None:
-            g = Geometry.from_buffer_copy(self.geometry)
-            g.residual_multiplier = 1.0
-            handle = ctypes.c_void_p()
-            call("tfm_plan_create", ctypes.byref(g), ctypes.byref(handle))
-            self._unit = handle
+        with self._unit_lock:
+            if self._unit is None:
+                g = Geometry.from_buffer_copy(self.geometry)
+                g.residual_multiplier = 1.0
+                handle = ctypes.c_void_p()
+                call("tfm_plan_create", ctypes.byref(g), ctypes.byref(handle))
+                self._unit = handle
         return self._unit
 
     def route(self, x: torch.Tensor, router: torch.Tensor, logit_bias: Optional[torch.Tensor] = None):
