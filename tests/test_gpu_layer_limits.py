@@ -90,3 +90,20 @@ def test_token_logprobs_of_the_largest_differences(gpu, dtype):
         check_logprobs(logits, tokens, 3, scale)
         assert torch.isfinite(layer.token_logprobs(logits, tokens, scale=scale)[0]).all()
     assert (layer.token_logprobs(logits, tokens)[0] == -math.inf).all()
+
+
+# -- allocation --------------------------------------------------------------------
+
+def ones(shape, dtype):
+    return torch.ones(shape, dtype=dtype, device="cuda")
+
+
+def test_an_output_that_does_not_fit_is_out_of_memory(gpu):
+    """As torch's own allocations raise it, so that a caller can retry with fewer rows; the next call works."""
+    n = 1 << 20  # an output of 2^40 elements
+    x, w, s = ones((n, 16), BF16), ones((n, 16), torch.int8), ones((n,), F32)
+    with pytest.raises(torch.OutOfMemoryError):
+        layer.int8_linear(x, w, s)
+    with pytest.raises(torch.OutOfMemoryError):
+        layer.int8_qmm(w, s, w, s)
+    assert (layer.int8_qmm(w[:5], s[:5], w[:3], s[:3], dtype=F32) == 16).all()

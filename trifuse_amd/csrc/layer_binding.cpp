@@ -10,8 +10,10 @@
 #include <ATen/ATen.h>
 #include <torch/csrc/Dtype.h>
 #include <torch/csrc/DynamicTypes.h>
+#include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/python_variable.h>
 
+#include <exception>
 #include <string>
 
 #include "../../include/trifuse_moe.h"
@@ -122,8 +124,8 @@ PyObject* guarded(F&& f) {
   try {
     return f();
   } catch (const Raised&) {
-  } catch (const std::exception& e) {
-    PyErr_SetString(PyExc_RuntimeError, e.what());
+  } catch (const std::exception&) {  // torch's own types: OutOfMemoryError among them
+    torch::translate_exception_to_python(std::current_exception());
   } catch (...) {
     PyErr_SetString(PyExc_RuntimeError, "internal error");
   }
