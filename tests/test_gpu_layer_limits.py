@@ -6,7 +6,7 @@ import torch
 
 from tests.test_gpu_layer import BF16, EPS, F32, check_logprobs, logprobs64, rand
 from trifuse_amd import layer
-from trifuse_amd._lib import TfmError
+from trifuse_amd._lib import TfmError, TfmUnsupported
 
 pytestmark = pytest.mark.gpu
 
@@ -107,3 +107,14 @@ def test_an_output_that_does_not_fit_is_out_of_memory(gpu):
     with pytest.raises(torch.OutOfMemoryError):
         layer.int8_qmm(w, s, w, s)
     assert (layer.int8_qmm(w[:5], s[:5], w[:3], s[:3], dtype=F32) == 16).all()
+
+
+def test_limits_come_before_the_output(gpu):
+    """Sizes that no product takes are refused as such, whatever their output would need."""
+    n = 1 << 20
+    for rows, k, error, message in ((n, 24, TfmUnsupported, "multiple of 16"), (1 << 22, 16, TfmError, "rows")):
+        x, w, s = ones((rows, k), BF16), ones((n, k), torch.int8), ones((max(n, rows),), F32)
+        with pytest.raises(error, match=message):
+            layer.int8_linear(x, w, s[:n])
+        with pytest.raises(error, match=message):
+            layer.int8_qmm(ones((rows, k), torch.int8), s[:rows], w, s[:n])

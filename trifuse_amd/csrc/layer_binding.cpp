@@ -105,18 +105,21 @@ at::Tensor empty(at::IntArrayRef shape, at::ScalarType type, const at::Tensor& b
 }
 at::IntArrayRef lead(const at::Tensor& t) { return t.sizes().slice(0, t.dim() - 1); }
 
+void need_ok(int status) {
+  if (status == TFM_OK) return;
+  PyObject* r = PyObject_CallFunction(raise_status, "i", status);
+  Py_XDECREF(r);
+  if (!PyErr_Occurred()) PyErr_SetString(PyExc_RuntimeError, "trifuse_moe call failed");
+  throw Raised{};
+}
+
 template <typename F>
 void enqueue(F&& f) {
   int status;
   Py_BEGIN_ALLOW_THREADS;
   status = f();
   Py_END_ALLOW_THREADS;
-  if (status != TFM_OK) {
-    PyObject* r = PyObject_CallFunction(raise_status, "i", status);
-    Py_XDECREF(r);
-    if (!PyErr_Occurred()) PyErr_SetString(PyExc_RuntimeError, "trifuse_moe call failed");
-    throw Raised{};
-  }
+  need_ok(status);
 }
 
 template <typename F>
@@ -264,6 +267,14 @@ at::Tensor product_out(const at::Tensor& x, int64_t n_out, at::ScalarType type) 
   return empty(shape, type, x);
 }
 
+// The library's limits on a product's sizes, before its output is allocated, which may be far larger than the
+// inputs: a call without rows (or with too many) checks them and does nothing.
+void need_product(const Rows& r, const at::Tensor& w, int32_t dt) {
+  constexpr int64_t kTooMany = 1 << 22;
+  need_ok(p_int8_qmm(nullptr, nullptr, r.rows < kTooMany ? 0 : r.rows, nullptr, nullptr, nullptr, (int32_t)w.size(0),
+                     r.width, dt, nullptr, nullptr));
+}
+
 const float* floats(const void* p) { return static_cast<const float*>(p); }
 
 // int8_qmm(stream, codes, scales, w, w_scales, bias, dtype)
@@ -287,6 +298,7 @@ PyObject* int8_qmm(PyObject*, PyObject* const* v, Py_ssize_t n) {
     tensor(v[4], "w_scales");
     const void* ws = vector_of(v[4], "w_scales", w.size(0), at::kFloat, codes);
     const void* bias = vector_of(v[5], "bias", w.size(0), type, codes);
+    need_product(r, w, dt);
     at::Tensor out = product_out(codes, w.size(0), type);
     void* stream = stream_of(v[0]);
     enqueue([&] {
@@ -310,6 +322,7 @@ PyObject* int8_linear(PyObject*, PyObject* const* v, Py_ssize_t n) {
     tensor(v[3], "w_scales");
     const void* ws = vector_of(v[3], "w_scales", w.size(0), at::kFloat, x);
     const void* bias = vector_of(v[4], "bias", w.size(0), x.scalar_type(), x);
+    need_product(r, w, dt);
     at::Tensor out = product_out(x, w.size(0), x.scalar_type()), space;
     const size_t need = p_int8_linear_workspace_bytes(r.rows, r.width);
     if (need) space = empty({(int64_t)need}, at::kByte, x);
