@@ -404,24 +404,31 @@ __global__ __launch_bounds__(64 * WV) void igemm_few_kernel(IgArgs a, const uint
   }
 }
 
-// xh null: codes given.
-template <int WV, int KS>
-void launch_few(int dtype, const IgArgs& a, const uint16_t* xh, hipStream_t s) {
+template <int WV, int KS, typename Kernel>
+void launch_few(Kernel kernel, const IgArgs& a, const uint16_t* xh, hipStream_t s) {
   const unsigned groups = (unsigned)((a.N + 15) / 16), blocks = (groups + WV / KS - 1) / (WV / KS);
   const size_t lds = ((size_t)a.T * few_row_bytes(a.K) + 64 + 15) / 16 * 16 + (KS > 1 ? WV * 1024 : 0);
-  const bool f16 = dtype == TFM_DTYPE_F16;
-  if (xh && f16)
-    igemm_few_kernel<true, true, WV, KS, TFM_DTYPE_F16><<<blocks, 64 * WV, lds, s>>>(a, xh);
-  else if (xh)
-    igemm_few_kernel<true, false, WV, KS, TFM_DTYPE_BF16><<<blocks, 64 * WV, lds, s>>>(a, xh);
-  else if constexpr (WV == 8)
-    fail(TFM_E_UNSUPPORTED, "int8 product: eight waves are for codes made in the kernel");
-  else if (dtype == TFM_DTYPE_F32)
-    igemm_few_kernel<false, false, WV, KS, TFM_DTYPE_F32><<<blocks, 64 * WV, lds, s>>>(a, nullptr);
-  else if (f16)
-    igemm_few_kernel<false, true, WV, KS, TFM_DTYPE_F16><<<blocks, 64 * WV, lds, s>>>(a, nullptr);
+  kernel<<<blocks, 64 * WV, lds, s>>>(a, xh);
+}
+
+// Codes made in the kernel.
+template <int WV, int KS>
+void launch_few_x(int dtype, const IgArgs& a, const uint16_t* xh, hipStream_t s) {
+  if (dtype == TFM_DTYPE_F16)
+    launch_few<WV, KS>(igemm_few_kernel<true, true, WV, KS, TFM_DTYPE_F16>, a, xh, s);
   else
-    igemm_few_kernel<false, false, WV, KS, TFM_DTYPE_BF16><<<blocks, 64 * WV, lds, s>>>(a, nullptr);
+    launch_few<WV, KS>(igemm_few_kernel<true, false, WV, KS, TFM_DTYPE_BF16>, a, xh, s);
+}
+
+// Codes given.
+template <int WV, int KS>
+void launch_few_codes(int dtype, const IgArgs& a, hipStream_t s) {
+  if (dtype == TFM_DTYPE_F32)
+    launch_few<WV, KS>(igemm_few_kernel<false, false, WV, KS, TFM_DTYPE_F32>, a, nullptr, s);
+  else if (dtype == TFM_DTYPE_F16)
+    launch_few<WV, KS>(igemm_few_kernel<false, true, WV, KS, TFM_DTYPE_F16>, a, nullptr, s);
+  else
+    launch_few<WV, KS>(igemm_few_kernel<false, false, WV, KS, TFM_DTYPE_BF16>, a, nullptr, s);
 }
 
 template <int BM, int BN, int WM, int WN, int S, int MINW>
@@ -431,12 +438,13 @@ void launch_tile(int dtype, IgArgs a, hipStream_t s) {
   a.mt = (int)mt;
   a.nt = (int)nt;
   const dim3 grid((unsigned)(mt * nt)), block(BM / WM * (BN / WN) * 64);
-  if (dtype == TFM_DTYPE_F32) {
-    if constexpr (BM == BN)  // the 256 x 192 tile has no room to stage fp32 rows
+  if constexpr (BM == BN) {  // the 256 x 192 tile has no room to stage fp32 rows and is not picked for them
+    if (dtype == TFM_DTYPE_F32) {
       igemm_tile_kernel<BM, BN, WM, WN, S, MINW, TFM_DTYPE_F32><<<grid, block, 0, s>>>(a);
-    else
-      fail(TFM_E_UNSUPPORTED, "int8 product: tile without fp32 output");
-  } else if (dtype == TFM_DTYPE_F16)
+      return;
+    }
+  }
+  if (dtype == TFM_DTYPE_F16)
     igemm_tile_kernel<BM, BN, WM, WN, S, MINW, TFM_DTYPE_F16><<<grid, block, 0, s>>>(a);
   else
     igemm_tile_kernel<BM, BN, WM, WN, S, MINW, TFM_DTYPE_BF16><<<grid, block, 0, s>>>(a);
@@ -456,13 +464,22 @@ IgArgs ig_args(int dtype, const int8_t* x, const float* x_scales, int64_t rows, 
 // codes (4 / 8 / 16 waves at 8 x 2048 x 50304 27.6 / 27.2 / 26.0, at 1 row 24.1 / 23.6 /
 // 22.8); of four each four, but eight where four rows or more are made into codes
 // for many channels (5 x 4096 x 8192 13.8 / 11.8, 1 x 4096 x 12288 15.1 / 16.6).
-void run_few(int dtype, const IgArgs& a, const uint16_t* xh, hipStream_t s) {
-  if (a.N >= 512 * 64)
-    launch_few<16, 1>(dtype, a, xh, s);
-  else if (xh && a.T >= 4 && a.N >= 8192)
-    launch_few<8, 4>(dtype, a, xh, s);
+bool few_alone(int N) { return N >= 512 * 64; }
+
+void run_few_x(int dtype, const IgArgs& a, const uint16_t* xh, hipStream_t s) {
+  if (few_alone(a.N))
+    launch_few_x<16, 1>(dtype, a, xh, s);
+  else if (a.T >= 4 && a.N >= 8192)
+    launch_few_x<8, 4>(dtype, a, xh, s);
   else
-    launch_few<4, 4>(dtype, a, xh, s);
+    launch_few_x<4, 4>(dtype, a, xh, s);
+}
+
+void run_few_codes(int dtype, const IgArgs& a, hipStream_t s) {
+  if (few_alone(a.N))
+    launch_few_codes<16, 1>(dtype, a, s);
+  else
+    launch_few_codes<4, 4>(dtype, a, s);
 }
 
 }  // namespace
@@ -501,7 +518,7 @@ void launch_int8_qmm(int dtype, const int8_t* x, const float* x_scales, int64_t 
   if (rows <= 0) return;
   const IgArgs a = ig_args(dtype, x, x_scales, rows, w, w_scales, bias, N, K, out);
   if (few_fits(rows, K)) {
-    run_few(dtype, a, nullptr, s);
+    run_few_codes(dtype, a, s);
   } else {
     switch (pick_tile(rows, N, dtype != TFM_DTYPE_F32)) {
       case kTile256: launch_tile<256, 256, 128, 64, 2, 2>(dtype, a, s); break;
@@ -522,7 +539,7 @@ void launch_int8_linear_few(bool f16, const uint16_t* x, int64_t rows, const int
                             const void* bias, int N, int K, void* out, hipStream_t s) {
   if (rows <= 0) return;
   const int dtype = f16 ? TFM_DTYPE_F16 : TFM_DTYPE_BF16;
-  run_few(dtype, ig_args(dtype, nullptr, nullptr, rows, w, w_scales, bias, N, K, out), x, s);
+  run_few_x(dtype, ig_args(dtype, nullptr, nullptr, rows, w, w_scales, bias, N, K, out), x, s);
   check_hip(hipGetLastError(), "int8_linear launch");
 }
 
