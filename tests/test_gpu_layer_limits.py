@@ -4,7 +4,8 @@ import math
 import pytest
 import torch
 
-from tests.test_gpu_layer import BF16, EPS, F32, check_logprobs, logprobs64, rand
+from tests.test_gpu_layer import (BF16, EPS, F, F16, F32, _layer_pass, _layer_state, check_logprobs, close, codes_of,
+                                  logprobs64, norm64, product64, rand, scales_of, step64)
 from trifuse_amd import layer
 from trifuse_amd._lib import TfmError, TfmUnsupported
 
@@ -118,3 +119,62 @@ def test_limits_come_before_the_output(gpu):
             layer.int8_linear(x, w, s[:n])
         with pytest.raises(error, match=message):
             layer.int8_qmm(ones((rows, k), torch.int8), s[:rows], w, s[:n])
+
+
+# -- products ----------------------------------------------------------------------
+
+@pytest.mark.parametrize("dtype", [BF16, F16, F32])
+def test_a_row_has_the_same_bits_in_every_batch(gpu, dtype):
+    """8190 channels: few rows, 64 x 64, 128 x 128, 256 x 192 (fp32: another) and 256 x 256 tiles, in this order."""
+    k, n = 272, 8190
+    codes, w, scales, ws = codes_of((2047, k), 1), codes_of((n, k), 2), scales_of(2047, 3), scales_of(n, 4)
+    bias = rand((n,), 5, 1.0, dtype)
+    whole = layer.int8_qmm(codes, scales, w, ws, bias=bias, dtype=dtype)
+    for rows in (1, 9, 16, 40, 300, 1100):
+        for at in (0, 2047 - rows):
+            part = layer.int8_qmm(codes[at:at + rows], scales[at:at + rows], w, ws, bias=bias, dtype=dtype)
+            assert torch.equal(part, whole[at:at + rows]), (rows, at)
+
+
+@pytest.mark.parametrize("rows,k,n", [(8, 7104, 640), (8, 7120, 640), (8, 8192, 640), (4, 14336, 515), (2, 32768, 96),
+                                      (1, 57216, 70), (1, 57280, 70), (16, 3520, 130), (16, 3536, 130), (3, 131056, 33)])
+@pytest.mark.parametrize("dtype", [BF16, F16])
+def test_int8_linear_of_few_long_rows(gpu, rows, k, n, dtype):
+    """Rows on both sides of what the few-row kernel's shared memory holds: quantize_rows and int8_qmm, bit for bit,
+    and int8_qmm against 64 bits."""
+    x, w, ws, bias = rand((rows, k), 1, 1.0, dtype), codes_of((n, k), 2), scales_of(n, 4), rand((n,), 5, 1.0, dtype)
+    codes, scales = layer.quantize_rows(x)
+    out = layer.int8_qmm(codes, scales, w, ws, bias=bias, dtype=dtype)
+    close(out, *product64(codes, scales, w, ws, bias), dtype)
+    assert torch.equal(layer.int8_linear(x, w, ws, bias=bias), out)
+
+
+# -- together ----------------------------------------------------------------------
+
+@pytest.mark.parametrize("rows", [1, 5, 70, 300])
+def test_each_step_of_a_pass(gpu, rows):
+    """Each step of a layer's pass against 64 bits on the step's own inputs, to one rounding of each output."""
+    s = _layer_state(rows, 512, 3001)
+
+    def codes_close(codes, scales, x64, ex):
+        step, worst = scales.double()[:, None], ex.amax(-1, keepdim=True)
+        assert ((codes.double() * step - x64).abs() <= step * (0.5 + 2.0 ** -15) + ex + worst).all()
+
+    h, codes, scales = layer.norm_residual(s["y"], s["h"], post_weight=s["w1"], gate=s["gate"], residual_multiplier=0.22,
+                                           pre_weight=s["w2"], eps=EPS, quantize=True)
+    h64, eh, x64, ex = step64(s["y"], s["h"], s["w1"], s["gate"], 0.22, s["w2"])
+    close(h, h64, eh, BF16)
+    codes_close(codes, scales, x64, ex)
+    mid = layer.int8_qmm(codes, scales, s["p"], s["ps"], dtype=BF16)
+    close(mid, *product64(codes, scales, s["p"], s["ps"], None), BF16)
+    last = layer.norm_residual(mid, h, residual_multiplier=0.22)
+    h64, eh, _, _ = step64(mid, h, None, None, 0.22, None)
+    close(last, h64, eh, BF16)
+    codes, scales = layer.rms_norm(last, s["w3"], EPS, quantize=True)
+    x64 = norm64(last.double(), s["w3"].double())
+    codes_close(codes, scales, x64, F * x64.abs())
+    logits = layer.int8_qmm(codes, scales, s["head"], s["hs"], dtype=F32)
+    close(logits, *product64(codes, scales, s["head"], s["hs"], None), F32)
+    check_logprobs(logits, s["tokens"], 5, 0.5)
+    whole = _layer_pass(s)
+    assert torch.equal(whole[0], last) and torch.equal(whole[1], logits)
