@@ -300,7 +300,8 @@ int tfm_expert_routes(const tfm_plan* plan, const void* x, int64_t tokens,
  * least one): h [rows, width]; with pre_weight also x [rows, width] in the
  * storage dtype and/or codes [rows, width] with scales [rows] (as
  * tfm_quantize_rows makes them, from the unrounded x). h may be y, residual or a
- * full gate itself (same address). width <= 32768. */
+ * full gate (or the gate [width] of a single row) itself (same address).
+ * width <= 32768. */
 typedef struct tfm_norm_step {
   const void* y;           /* [rows, width]                                */
   const void* residual;    /* [rows, width] or NULL                        */

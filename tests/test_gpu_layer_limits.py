@@ -22,6 +22,15 @@ def test_norm_residual_over_its_gate(gpu):
         assert h2.data_ptr() == into.data_ptr() and torch.equal(h2, h) and torch.equal(x2, x)
 
 
+def test_norm_residual_gated_by_its_own_row(gpu):
+    """A single row's [H] gate is the row itself, and h is written over both."""
+    for width in (512, 9000):
+        y, w = rand((1, width), 1), rand((width,), 2, 0.1, mean=1.0)
+        h, x = layer.norm_residual(y, gate=y[0].clone(), pre_weight=w, eps=EPS)
+        h2, x2 = layer.norm_residual(y, gate=y[0], pre_weight=w, eps=EPS, out=y)
+        assert torch.equal(h2, h) and torch.equal(x2, x)
+
+
 def test_norm_residual_refuses_out_over_shared_inputs(gpu):
     buf = rand((9, 64), 1)
     y, gates = rand((4, 64), 2), torch.ones(260, device="cuda")

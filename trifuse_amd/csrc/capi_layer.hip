@@ -89,14 +89,16 @@ int tfm_norm_residual(const tfm_norm_step* step, int64_t rows, int32_t width, in
                     gk == TFM_GATE_FULL ? bytes : gk == TFM_GATE_TOKEN ? n * 4 : w * 2};
     const Span post{step->post_weight, w * 2}, pre{step->pre_weight, w * 2};
     const Span h{step->h, bytes}, x{step->x, bytes};
-    // Each lane has read its own elements of y, residual and a full gate before it writes h; weights and
-    // the other gates are read by every row.
-    for (const Span& in : {y, residual, gk == TFM_GATE_FULL ? gate : Span{nullptr, 0}}) {
+    // Each lane has read its own elements of y, residual and a full gate (or a single row's) before it writes
+    // h; weights and the other gates are read by every row.
+    const bool full = gk == TFM_GATE_FULL || (gk == TFM_GATE_CHANNEL && rows == 1);
+    const Span none{nullptr, 0};
+    for (const Span& in : {y, residual, full ? gate : none}) {
       need(h.at == in.at || !meet(h, in), "h overlaps an input that it is not");
       need(!meet(x, in), "x must not alias y, residual or gate");
     }
     need(!meet(x, h), "x must not alias h");
-    for (const Span& in : {post, pre, gk == TFM_GATE_FULL ? Span{nullptr, 0} : gate})
+    for (const Span& in : {post, pre, full ? none : gate})
       need(!meet(h, in) && !meet(x, in), "h and x must not overlap a weight or a gate that rows share");
     need_apart({{step->codes, n * w}, {step->scales, n * 4}}, {y, residual, gate, post, pre, h, x},
                "codes and scales must not overlap an input or another output");
