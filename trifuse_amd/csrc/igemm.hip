@@ -7,9 +7,10 @@
 // operands go from memory straight into LDS (16 bytes a lane), 128 bytes of K a
 // stage, S stages; a row's eight 16-byte pieces are stored in the order
 // piece ^ (row / 2 % 8), so that the 16 rows that are read at a time (256 bytes a
-// clock) lie in different banks (row % 8 instead: 435 against 373 us at
-// 8192 x 4096 x 12288, half of the LDS cycles conflicts). Bound: MFMAs at the clock
-// that their power leaves, 1.9 GHz; 2.2 to 2.55 POP/s at K = 4096 to 16384.
+// clock) lie in different banks (row % 8 instead: half of the LDS cycles are
+// conflicts, 319 k against 170 k cycles a CU at 8192 x 4096 x 12288; the reads hide
+// behind the MFMAs either way, 364 us). Bound: MFMAs, busy 62 % of a CU's cycles at the
+// clock that their power leaves, about 1.8 GHz; 2.26 POP/s there, 2.43 at 8192^3 and 16384^3.
 #include <type_traits>
 
 #include "tfm_device.h"
@@ -296,7 +297,7 @@ __global__ __launch_bounds__(BM / WM * (BN / WN) * 64, MINW) void igemm_tile_ker
 // share 16 channels, every KS-th 64 bytes of K each, and join their sums in LDS.
 // With FUSED the codes are made here from x itself, in every workgroup; the first
 // weights are on their way meanwhile. Bound: the weights' stream where they are many
-// (1 x 2048 x 50304 21.5 us, 4.8 TB/s), else latency (1 x 2048 x 2048 4.4 us).
+// (8 x 2048 x 50304 22.9 us, 4.5 TB/s), else latency (1 x 2048 x 2048 4.9 us).
 constexpr int kFewRows = 16;
 constexpr int kFewLds = 64 << 10;
 constexpr int kFewStep = 64;   // bytes of K an MFMA
@@ -458,12 +459,15 @@ IgArgs ig_args(int dtype, const int8_t* x, const float* x_scales, int64_t rows, 
 }
 
 // Waves that share 16 channels: one where the channels alone fill the chip, else
-// four. us with one / four: 1 x 2048 x 2048 7.6 / 4.4, 8 x 4096 x 12288 18.0 / 14.9,
-// 8 x 2048 x 50304 24.4 / 25.9, 16 x 2048 x 50304 25.9 / 32.4.
+// four. us with one / four, codes given, four waves a workgroup: 1 x 2048 x 2048
+// 7.2 / 4.2, 8 x 4096 x 12288 15.7 / 13.8, 8 x 2048 x 50304 22.6 / 24.8, 16 x 2048 x 50304
+// 24.2 / 31.1.
 // Waves of a workgroup: sixteen of one each, so that few workgroups make the same
-// codes (4 / 8 / 16 waves at 8 x 2048 x 50304 27.6 / 27.2 / 26.0, at 1 row 24.1 / 23.6 /
-// 22.8); of four each four, but eight where four rows or more are made into codes
-// for many channels (5 x 4096 x 8192 13.8 / 11.8, 1 x 4096 x 12288 15.1 / 16.6).
+// codes (codes made, 4 / 8 / 16 waves: 8 x 2048 x 50304 25.7 / 24.8 / 23.0, 1 row 22.7 / 21.9 /
+// 21.9; right at the border of 32768 channels half of the CUs have no workgroup, codes
+// given, 4 x 2048 x 32768: 14.3 / 14.1 / 17.7); of four each four, but eight where four rows or
+// more are made into codes for many channels (5 x 4096 x 8192 13.7 / 11.7, 8 x 4096 x 12288
+// 18.6 / 16.8, 1 x 4096 x 12288 13.9 / 14.5).
 bool few_alone(int N) { return N >= 512 * 64; }
 
 void run_few_x(int dtype, const IgArgs& a, const uint16_t* xh, hipStream_t s) {
@@ -489,15 +493,15 @@ void run_few_codes(int dtype, const IgArgs& a, hipStream_t s) {
 // 2.0 and 1.62 us, 128 x 128 (two a CU) 1.17, or 0.75 where each CU has one, 64 x 64
 // (two a CU) 0.42, or 0.36 and 0.25 in a single round of two and one. us at
 // T x K x N, in that order (* the one taken):
-//   8192 x 4096 x 12288   375* / 392 / 439 / 642
-//   4096 x 2048 x 6144    60.8 / 54.3* / 58.7 / 91
-//   8192 x 2048 x 2048    36.6* / 49.2 / 40.4 / 64
-//   4096 x 2048 x 2048    29.4 / 26.5 / 22.3* / 32.5
-//   2048 x 1536 x 2560    22.0 / 19.3 / 15.2* / 18.0
-//   1024 x 2048 x 2048    23.4 / 21.1 / 10.9 / 8.9*
-//   64 x 4096 x 12288     40.0 / 34.8 / 22.9 / 11.4*
+//   8192 x 4096 x 12288   364* / 402 / 451 / 654
+//   4096 x 2048 x 6144    61.2 / 55.3* / 60.1 / 95
+//   8192 x 2048 x 2048    36.0* / 48.9 / 41.3 / 66
+//   4096 x 2048 x 2048    30.2 / 27.1 / 22.5* / 34.6
+//   2048 x 1536 x 2560    23.6 / 19.8 / 14.9* / 20.1
+//   1024 x 2048 x 2048    25.8 / 23.3 / 14.6 / 10.5*
+//   64 x 4096 x 12288     39.0 / 34.6 / 22.9 / 11.2*
 // The 64 x 64 tile keeps four stages of K in LDS (with two: 18.2 at the last line,
-// 9.1 above it): a CU's few workgroups there do not hide each other's loads.
+// 11.6 above it): a CU's few workgroups there do not hide each other's loads.
 enum Tile { kTile256, kTile192, kTile128, kTile64 };
 static Tile pick_tile(int64_t T, int64_t N, bool half_out) {
   auto tiles = [&](int bm, int bn) { return ((T + bm - 1) / bm) * ((N + bn - 1) / bn); };
@@ -530,9 +534,12 @@ void launch_int8_qmm(int dtype, const int8_t* x, const float* x_scales, int64_t 
   check_hip(hipGetLastError(), "int8_qmm launch");
 }
 
-// Past 8 rows making the codes in every workgroup costs more than a launch of
-// their own: 16 x 2048 x 50304 31.8 us against 26.0 and 2.5 (8 rows 27.6 against
-// 24.5 and 2.5, 8 x 2048 x 2048 6.2 against 4.9 and 2.5).
+// Codes made in every workgroup against a launch of their own and the product, us:
+//   1 x 2048 x 2048 4.9 / 6.5     8 x 2048 x 2048 6.2 / 7.5     8 x 2048 x 50304 23.8 / 25.4
+//   8 x 4096 x 4096 11.1 / 11.1   8 x 7104 x 4096 16.9 / 14.7
+// Past 8 rows neither side wins throughout: up to 1.4 less at 16 x 512 and 9 x 2048, as much
+// more at 9 x 1536 x 8191 (9.9 / 8.9) and 16 x 1536 x 2560 (8.7 / 8.0), far more for long rows
+// (12 x 3520 x 2560 11.7 / 10.5, 9 x 6000 x 2560 20.1 / 13.0).
 bool int8_linear_few(int64_t rows, int K) { return rows <= 8 && few_fits(rows, K); }
 
 void launch_int8_linear_few(bool f16, const uint16_t* x, int64_t rows, const int8_t* w, const float* w_scales,

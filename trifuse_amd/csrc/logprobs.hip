@@ -26,9 +26,9 @@
 // place among the alternatives.
 // A row made so that the list overflows takes one scan per alternative.
 //
-// Bound: arithmetic beside the stream, about 12 issue slots a logit of which the
-// exponential takes four. 4096 x 50304 bf16: 79 us without alternatives (5.2 TB/s),
-// 86 to 91 with 20; one row 8.4 us, one workgroup's arithmetic.
+// Bound: arithmetic beside the stream, 13 vector instructions a logit, the
+// exponential among them. 4096 x 50304 bf16: 80 us without alternatives (5.2 TB/s),
+// 86 to 88 with 20; one row 8.5 us, one workgroup's arithmetic.
 #include "tfm_device.h"
 #include "tfm_internal.h"
 
@@ -381,10 +381,10 @@ template <int DT>
 void launch_dt(const LogprobsArgs& a, hipStream_t s) {
   // Few rows leave CUs to spare: wider workgroups read a long row faster, narrower
   // ones have less to join. us of 256 / 512 threads, rows x vocabulary:
-  //   1 x 4000 5.6 / 5.6     1 x 10007 6.4 / 5.8     1 x 50304 10.4 / 8.9
-  //   256 x 10007 7.1 / 7.0  333 x 10007 8.1 / 8.5   256 x 50304 11.5 / 10.0
-  //   333 x 50304 15.9 / 14.6   768 x 50304 20.4 / 20.5   1024 x 50304 24.3 / 24.9
-  // (1024 threads: 9.5, 15.9 and 29.2 at 1, 333 and 1024 x 50304).
+  //   1 x 4000 5.2 / 5.2     1 x 10007 5.7 / 5.4     1 x 50304 10.0 / 8.5
+  //   256 x 10007 7.0 / 6.9  333 x 10007 8.0 / 8.3   256 x 50304 13.0 / 10.8
+  //   333 x 50304 15.6 / 14.6   768 x 50304 19.8 / 20.3   1024 x 50304 25.0 / 25.3
+  // (1024 threads: 9.0, 16.3 and 29.6 at 1, 333 and 1024 x 50304).
   if ((a.rows <= 256 && a.vocab >= 8192) || (a.rows <= 768 && a.vocab >= 32768))
     token_logprobs_kernel<DT, 512><<<a.rows, 512, 0, s>>>(a);
   else

@@ -18,9 +18,9 @@
 // byte moves once; both norms' sums are a lane's own sequential sum, then
 // the pairwise tree over the wave, then the waves in order. The team follows
 // from the width alone, so that a row has the same bits in every batch (four waves
-// a row of 2048: 16 rows 3.4 against 4.2 us, 300 rows 4.0 against 4.6, 4096 rows 14.9
-// against 14.4). 16384 x 2048 with a gate for each element 59 us, 5.6 TB/s; to
-// codes 40 us; quantize_rows of the same 16.6 us, 6.0 TB/s.
+// a row of 2048: 16 rows 3.2 against 4.0 us, 300 rows 3.7 against 4.3, 4096 rows 14.7
+// against 14.2). 16384 x 2048 with a gate for each element 60 us, 5.6 TB/s; without
+// one, to codes, 40 us; quantize_rows of the same 16.5 us, 6.1 TB/s.
 #include <type_traits>
 
 #include "tfm_device.h"

@@ -29,8 +29,8 @@ from . import _lib
 # A small call is bound by its host time: arguments are checked and outputs
 # allocated in native code (csrc/layer_binding.cpp), and the current device and
 # stream are asked for as numbers (0.1 us each; a torch.cuda.Stream object takes
-# 2 to 3). One row: norm_residual 5.4 us a call, int8_linear 4.4, against 8.8 and 7.8
-# with both in Python.
+# 2 to 3). One row: norm_residual about 5 us a call, int8_linear about 4 (4.7 to 5.5 and
+# 3.6 to 4.5, by the host), against 8.8 and 7.8 with both in Python.
 _current_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
     lambda index: torch.cuda.current_stream(index).cuda_stream)
