@@ -368,6 +368,107 @@ int tfm_token_logprobs(const void* logits, int64_t rows, int32_t vocab, int64_t 
                        float scale, float* logprobs, float* entropy, int32_t* top_ids,
                        float* top_logprobs, void* stream);
 
+/* ---- attention between two blocks ---------------------------------------- */
+/* Rotary positions and attention over a paged cache of 8-bit codes: what stands
+ * between a layer's fused projection and its output projection. Activations are
+ * TFM_DTYPE_BF16 or TFM_DTYPE_F16, [rows, heads, head_dim] with a stride in
+ * elements for rows and for heads (a view into the projection's output; 0 for
+ * shared ones) and head_dim elements in a row; 16-byte aligned rows move
+ * fastest, none have to be. Rows are at most 2^22 - 1 and heads 1024. */
+
+/* Angles a = position * frequencies[i] for pair i of a head's channels:
+ *   (x1, x2) -> (x1 c - x2 s, x2 c + x1 s),  c = scale cos a,  s = scale sin a
+ * with a reduced in 64 bits and the rest in fp32, rounded once. Pair i is
+ * channels (i, pairs + i), or (2i, 2i + 1) when interleaved; channels from
+ * 2 * pairs on are copied. */
+typedef struct tfm_rotation {
+  const double* frequencies; /* [pairs], radians a position (device)       */
+  int32_t pairs;
+  int32_t interleaved;
+  float scale;               /* 1, or the factor of a stretched context    */
+} tfm_rotation;
+
+/* out = x turned by its row's position (int32 or int64 by position_bits, of any
+ * sign; an angle is exact to 2^-51 of itself). out may be x itself with x's
+ * strides, and shares no other memory with an input; its rows do not overlap.
+ * head_dim <= 1024. */
+int tfm_rotary(const void* x, int64_t rows, int32_t heads, int32_t head_dim, int64_t row_stride,
+               int64_t head_stride, const void* positions, int32_t position_bits,
+               const tfm_rotation* rotation, int32_t dtype, void* out, int64_t out_row_stride,
+               int64_t out_head_stride, void* stream);
+
+/* A pool of pages, each of page_tokens tokens of every key head: int8 codes
+ * [pages, kv_heads, page_tokens, head_dim] for keys and for values (16-byte
+ * aligned), and one fp32 scale a page and head, [pages, kv_heads]: a value is
+ * code * scale. page_tokens: 16, 32, 64, 128 or 256. head_dim: 64 or 128. */
+typedef struct tfm_kv_cache {
+  int8_t* k;
+  int8_t* v;
+  float* k_scales;
+  float* v_scales;
+  int64_t pages;
+  int32_t kv_heads;
+  int32_t page_tokens;
+  int32_t head_dim;
+} tfm_kv_cache;
+
+/* The sequences of a call. Sequence b holds lengths[b] tokens with this call's
+ * own, token t in page table[b, t / page_tokens] at t % page_tokens; its rows are
+ * starts[b] .. starts[b + 1], the last of its tokens: row i of n is at position
+ * lengths[b] - n + i. starts NULL: max_rows rows each. max_rows is at least the
+ * most rows of one sequence (those past it are not seen). Rows behind the last
+ * sequence are not read, and what they would write stays as it was. All arrays
+ * are on the device and may change between replays of a captured call. A table
+ * entry that is no page is allowed where no token lies (-1, say); where one
+ * lies, that token is not written, reads as zero and is seen by no row. Lengths
+ * past the table's tokens end there. */
+typedef struct tfm_kv_batch {
+  const int32_t* table;   /* [sequences, table_width]                      */
+  const int32_t* lengths; /* [sequences]                                   */
+  const int32_t* starts;  /* [sequences + 1] or NULL                       */
+  int32_t sequences;
+  int32_t table_width;    /* table_width * page_tokens <= 2^30             */
+  int32_t max_rows;
+} tfm_kv_batch;
+
+/* Writes rows k and v [rows, kv_heads, head_dim] (own strides) to the cache, k
+ * turned by `rotation` at its position first (NULL: as it is; pairs a multiple
+ * of 8). For each page and head that gets tokens, from place p of the page on:
+ *   s' = max(s, max(max|x|, 2^-40) / 127)   with s the page's scale, or 0 at p = 0
+ *   c' = round_half_even(c * (s / s'))       the codes before place p, where s' > s
+ *   code = round_half_even(x * (1 / s'))     the new tokens
+ * all in fp32. Codes from place p on are replaced or left; a page that starts
+ * anew needs no clearing. An infinity or a NaN makes s' NaN and its page's new
+ * codes 0, so that whatever sees the page is NaN, until it starts anew. Two
+ * sequences must not get tokens in one page. Positions below 0 are not written. */
+int tfm_cache_append(const void* k, int64_t k_row_stride, int64_t k_head_stride, const void* v,
+                     int64_t v_row_stride, int64_t v_head_stride, int64_t rows,
+                     const tfm_rotation* rotation, int32_t dtype, const tfm_kv_cache* cache,
+                     const tfm_kv_batch* batch, void* stream);
+
+/* The last max_rows tokens of every sequence as values code * scale, rounded
+ * once: k and v [sequences * max_rows, kv_heads, head_dim] in dtype (also
+ * TFM_DTYPE_F32). Positions below 0 read as zero. batch->starts is NULL. */
+int tfm_cache_read(const tfm_kv_cache* cache, const tfm_kv_batch* batch, int32_t dtype, void* k,
+                   void* v, void* stream);
+
+/* out[t, h] = sum_j softmax_j(scale * q[t, h] . k_j) v_j over the tokens j that
+ * row t sees, in key head h / (heads / kv_heads): j <= its position when causal
+ * (else all of its sequence), and with window > 0 (causal only) j > position -
+ * window. A row that sees none is zero. q [rows, heads, head_dim] with strides,
+ * out [rows, heads, head_dim] dense. Products are of exact codes with halves (q
+ * after a power of two for its row, softmax weights), their sums, the softmax
+ * and its statistics fp32, one rounding at the end. Scales of a head's pages may
+ * be up to 2^100 apart. The workspace (256-byte aligned, no status word) holds
+ * the parts of sequences that several workgroups share, keeps nothing between
+ * calls, and may be 0 bytes. */
+size_t tfm_cache_attention_workspace_bytes(int64_t rows, int32_t heads, int32_t window,
+                                           const tfm_kv_cache* cache, const tfm_kv_batch* batch);
+int tfm_cache_attention(const void* q, int64_t row_stride, int64_t head_stride, int64_t rows,
+                        int32_t heads, const tfm_kv_cache* cache, const tfm_kv_batch* batch,
+                        float scale, int32_t causal, int32_t window, int32_t dtype, void* out,
+                        void* workspace, size_t workspace_bytes, void* stream);
+
 /* ---- stage profiler ---------------------------------------------------- */
 /* Kernel stages of tfm_moe_forward / tfm_moe_experts. */
 #define TFM_STAGE_ROUTER 0  /* router linear                               */

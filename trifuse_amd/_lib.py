@@ -116,6 +116,34 @@ class NormStep(ctypes.Structure):
     ]
 
 
+class Rotation(ctypes.Structure):
+    _fields_ = [("frequencies", c_void_p), ("pairs", c_int32), ("interleaved", c_int32), ("scale", c_float)]
+
+
+class KvCache(ctypes.Structure):
+    _fields_ = [
+        ("k", c_void_p),
+        ("v", c_void_p),
+        ("k_scales", c_void_p),
+        ("v_scales", c_void_p),
+        ("pages", c_int64),
+        ("kv_heads", c_int32),
+        ("page_tokens", c_int32),
+        ("head_dim", c_int32),
+    ]
+
+
+class KvBatch(ctypes.Structure):
+    _fields_ = [
+        ("table", c_void_p),
+        ("lengths", c_void_p),
+        ("starts", c_void_p),
+        ("sequences", c_int32),
+        ("table_width", c_int32),
+        ("max_rows", c_int32),
+    ]
+
+
 # name -> (restype, argtypes); every function of include/trifuse_moe.h.
 SIGNATURES = {
     "tfm_plan_create": (c_int, [POINTER(Geometry), POINTER(c_void_p)]),
@@ -161,6 +189,16 @@ SIGNATURES = {
                                 c_void_p, c_void_p, c_size_t, c_void_p]),
     "tfm_token_logprobs": (c_int, [c_void_p, c_int64, c_int32, c_int64, c_int32, c_void_p, c_int32, c_int32,
                                    c_float, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p]),
+    "tfm_rotary": (c_int, [c_void_p, c_int64, c_int32, c_int32, c_int64, c_int64, c_void_p, c_int32,
+                           POINTER(Rotation), c_int32, c_void_p, c_int64, c_int64, c_void_p]),
+    "tfm_cache_append": (c_int, [c_void_p, c_int64, c_int64, c_void_p, c_int64, c_int64, c_int64,
+                                 POINTER(Rotation), c_int32, POINTER(KvCache), POINTER(KvBatch), c_void_p]),
+    "tfm_cache_read": (c_int, [POINTER(KvCache), POINTER(KvBatch), c_int32, c_void_p, c_void_p, c_void_p]),
+    "tfm_cache_attention_workspace_bytes": (c_size_t, [c_int64, c_int32, c_int32, POINTER(KvCache),
+                                                       POINTER(KvBatch)]),
+    "tfm_cache_attention": (c_int, [c_void_p, c_int64, c_int64, c_int64, c_int32, POINTER(KvCache),
+                                    POINTER(KvBatch), c_float, c_int32, c_int32, c_int32, c_void_p, c_void_p,
+                                    c_size_t, c_void_p]),
     "tfm_profiler_create": (c_int, [c_int32, POINTER(c_void_p)]),
     "tfm_profiler_destroy": (None, [c_void_p]),
     "tfm_profiler_attach": (c_int, [c_void_p]),

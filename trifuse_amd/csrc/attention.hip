@@ -1,0 +1,805 @@
+// Attention over the paged cache of 8-bit codes.
+//
+// For a row's query q in a head, over the tokens j that it sees, with codes c and the
+// scales a (keys) and b (values) of token j's page:
+//   s_j = scale * a_j * (q . ck_j),   out = sum_j e^(s_j) b_j cv_j / sum_j e^(s_j)
+// One pass with a running maximum, over t_j = s_j log2(e) + log2(b_j):
+//   w_j = 2^(t_j - m),   out = (sum_j w_j cv_j) / (sum_j w_j / b_j)
+// so the page's value scale costs nothing an element (its logarithm rides in the
+// exponent's fused multiply-add, its inverse on the sum of 16 weights), and codes enter
+// the products as they are: a half holds every code exactly, q of bf16 exactly after a
+// power of two for its row (28 binades; what is smaller loses bits below 2^-25 of the
+// largest), and w to 2^-12 of itself. m follows the true maximum only when that has grown
+// by more than 2^8 (a half holds 2^8 as well as 1), so rescaling the sums is rare.
+//
+// "Columns" are the (row, head) pairs of one key head: they share its codes. Scores are
+// taken transposed, keys along the rows of a product and columns along its lanes: a lane
+// then owns one column's statistics, and the weights it computes are, without leaving
+// their registers, the operand of the second product, since the order of keys inside a
+// product is free as long as both operands keep it. A lane's keys of 32 are 16 (tile
+// kernel) or 8 (few kernel) consecutive ones, which lie in one page.
+//
+// Two kernels. Few columns (decoding, drafts; up to 32): memory decides. Each wave takes
+// 32 tokens at a time straight from memory into registers: key codes as 16-byte pieces of
+// a row, value codes as D/16 bytes a lane of eight rows, transposed by byte permutes into
+// the product's operand. More columns: 128 a workgroup, whose waves share tiles of 64
+// tokens, converted to halves once on their way into LDS.
+//
+// Work items are (sequence, tile of columns, part of its tokens). How many parts follows
+// on the device from the lengths, so that ragged batches spread evenly and a captured
+// call follows its lengths; parts are joined by a second kernel.
+#include "kv_cache.h"
+
+namespace tfm {
+
+namespace {
+
+constexpr float kLow = -3.402823466e38f;  // below every score; finite, so that differences are
+constexpr float kSlack = 8.0f;            // log2 of how far weights may pass 1
+
+__device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
+
+template <typename T>
+__device__ __forceinline__ T wave_sum(T v) {
+#pragma unroll
+  for (int m = 1; m < 64; m <<= 1) v += __shfl_xor(v, m, kWave);
+  return v;
+}
+
+// What one work item is.
+struct Item {
+  int b;        // sequence, -1: none
+  int tile;     // of its columns
+  int part;     // of `parts`
+  int parts;
+  int entry;    // index of part 0 of this tile
+};
+
+struct Need {
+  int tiles, tokens;  // of columns, and tokens that some row sees
+};
+__device__ __forceinline__ Need need_of(const AttentionArgs& a, int b, int columns) {
+  const KvSeq s = kv_seq(a.b, b);
+  const int lo = a.window ? max(0, s.first() - a.window + 1) : 0;
+  return Need{(s.n * a.group + columns - 1) / columns, max(s.len - lo, 0)};
+}
+
+// Tokens of a part: all of them where the tiles fill the machine by themselves, else
+// the batch's tokens (of every tile) over the items that should run.
+__device__ __forceinline__ int chunk_of(const AttentionArgs& a, int columns) {
+  if (!a.part_out) return 1 << 30;
+  long long tiles = 0, tokens = 0;
+  for (int b0 = 0; b0 < a.b.sequences; b0 += kWave) {
+    const int b = b0 + (threadIdx.x & 63);
+    if (b < a.b.sequences) {
+      const Need n = need_of(a, b, columns);
+      tiles += n.tiles;
+      tokens += (long long)n.tiles * n.tokens;
+    }
+  }
+  if (a.b.sequences > 1) {
+    tiles = wave_sum(tiles);
+    tokens = wave_sum(tokens);
+  } else {
+    tiles = __shfl(tiles, 0, kWave);
+    tokens = __shfl(tokens, 0, kWave);
+  }
+  if (tiles >= a.target) return 1 << 30;
+  const long long even = (tokens + a.target - 1) / a.target;
+  return max(a.min_chunk, (int)((even + 63) / 64 * 64));
+}
+
+// Item `index` of the batch; with by_tile, tile `index` (its part 0). Every wave finds it by itself.
+__device__ Item find_item(const AttentionArgs& a, int columns, int index, bool by_tile) {
+  const int chunk = chunk_of(a, columns);
+  int before = 0, entries = 0;  // counted items (or tiles), and items, of the sequences before
+  for (int b0 = 0; b0 < a.b.sequences; b0 += kWave) {
+    const int lane = threadIdx.x & 63, b = b0 + lane;
+    int tiles = 0, parts = 1;
+    if (b < a.b.sequences) {
+      const Need n = need_of(a, b, columns);
+      tiles = n.tiles;
+      parts = max(1, (int)(((long long)n.tokens + chunk - 1) / chunk));
+    }
+    const int mine = by_tile ? tiles : tiles * parts;
+    int upto = mine, items = tiles * parts;
+    if (a.b.sequences > 1) {
+#pragma unroll
+      for (int m = 1; m < 64; m <<= 1) {
+        const int o = __shfl_up(upto, m, kWave), p = __shfl_up(items, m, kWave);
+        if (lane >= m) {
+          upto += o;
+          items += p;
+        }
+      }
+    }
+    const uint64_t hit = __ballot(index < before + upto);
+    if (hit) {
+      const int l = __builtin_ctzll(hit);
+      const int local = index - before - (__shfl(upto, l, kWave) - __shfl(mine, l, kWave));
+      Item it;
+      it.b = b0 + l;
+      it.parts = __shfl(parts, l, kWave);
+      it.tile = by_tile ? local : local / it.parts;
+      it.part = by_tile ? 0 : local % it.parts;
+      it.entry = entries + __shfl(items, l, kWave) - __shfl(tiles, l, kWave) * it.parts + it.tile * it.parts;
+      return it;
+    }
+    before += __shfl(upto, 63, kWave);
+    entries += __shfl(items, 63, kWave);
+  }
+  return Item{-1, 0, 0, 1, 0};
+}
+
+// A column of an item: its row and head, and the tokens [lo, hi) that it sees.
+struct Column {
+  bool real;
+  int row, head, lo, hi;
+};
+__device__ __forceinline__ Column column_of(const AttentionArgs& a, const KvSeq& s, int kv_head, int c) {
+  Column o;
+  o.real = c < s.n * a.group;
+  const int i = c / a.group, position = s.first() + i;
+  o.row = s.start + i;
+  o.head = kv_head * a.group + c % a.group;
+  // A column that is none has nothing written, and does not make a tile take the masked path.
+  o.hi = a.causal && o.real ? min(s.len, position + 1) : s.len;
+  o.lo = a.window && o.real ? max(0, position - a.window + 1) : 0;
+  return o;
+}
+
+// The tokens [from, to) of an item's part, whole tiles of `step`: those that its tile's
+// columns see, cut evenly.
+__device__ __forceinline__ void part_of(const AttentionArgs& a, const KvSeq& s, const Item& it, int columns, int step,
+                                        int& from, int& to) {
+  const int c1 = min(s.n * a.group, (it.tile + 1) * columns) - 1;
+  const int first = s.first() + it.tile * columns / a.group, last = s.first() + c1 / a.group;
+  const int hi = a.causal ? min(s.len, last + 1) : s.len;
+  const int lo = a.window ? max(0, first - a.window + 1) / step * step : 0;
+  const int each = ((max(hi - lo, 0) + it.parts - 1) / it.parts + step - 1) / step * step;
+  from = min(lo + it.part * each, max(hi, 0));
+  to = min(from + each, hi);
+}
+
+// Eight elements of q as halves, times 2^e where they are bf16.
+template <bool F16>
+__device__ __forceinline__ f16x8_t q_halves(const uint4& u, float factor) {
+  if constexpr (F16) return __builtin_bit_cast(f16x8_t, u);
+  f16x8_t r;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const uint32_t w = word_of(u, j);
+    r[2 * j] = (_Float16)(lo_bf(w) * factor);
+    r[2 * j + 1] = (_Float16)(hi_bf(w) * factor);
+  }
+  return r;
+}
+__device__ __forceinline__ uint32_t abs_most(const uint4& u, uint32_t most) {  // of bf16, as fp32 bits
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const uint32_t w = word_of(u, j);
+    most = max(most, max(w << 16 & 0x7fffffffu, w & 0x7fff0000u));
+  }
+  return most;
+}
+// 2^e with the largest of a row in [2^14, 2^15), and 2^-e; both are normal numbers.
+__device__ __forceinline__ void row_factor(uint32_t most, float& factor, float& inverse) {
+  const uint32_t field = min(253u, 268u - (most >> 23));
+  factor = __uint_as_float(field << 23);
+  inverse = __uint_as_float((254u - field) << 23);
+}
+
+__device__ __forceinline__ uint4 load16(const uint16_t* p) {
+  uint4 u;
+  __builtin_memcpy(&u, p, 16);
+  return u;
+}
+
+template <bool F16>
+__device__ __forceinline__ void put_out4(uint16_t* p, const float* v) {
+  *reinterpret_cast<uint2*>(p) = make_uint2(pack_st2<F16>(v[0], v[1]), pack_st2<F16>(v[2], v[3]));
+}
+
+// ---- few columns -------------------------------------------------------------
+
+// 32 tokens of a wave, as loaded: lane (r = lane % 16, g = lane / 16) has bytes
+// D/4 * g .. of key rows 8 (r / 4) + 4 t + r % 4, and bytes D/16 * r .. of value rows 8 g + j.
+template <int D>
+struct FewTile {
+  uint4 k[2][D / 64];
+  uint32_t v[8][D / 64];
+  float ks, vs;  // of the page that tokens 8 g .. lie in
+  bool there;    // that page is one
+};
+
+template <int D>
+__device__ __forceinline__ void few_load(const AttentionArgs& a, int b, int kv_head, int token, FewTile<D>& t) {
+  const KvBatchArgs& g = a.b;
+  const int lane = threadIdx.x & 63, r = lane & 15, q = lane >> 4;
+  const int mask = (1 << g.page_shift) - 1;
+  const int kt = token + 8 * (r >> 2) + (r & 3), vt = token + 8 * q;
+  const int kp = max(kv_page(g, b, kt), 0), found = kv_page(g, b, vt), vp = max(found, 0);
+  t.there = found >= 0;
+  const int64_t kplace = (int64_t)kp * g.kv_heads + kv_head, vplace = (int64_t)vp * g.kv_heads + kv_head;
+  const int8_t* k = g.k + ((kplace << g.page_shift) + (kt & mask)) * D + (D / 4) * q;
+  const int8_t* v = g.v + ((vplace << g.page_shift) + (vt & mask)) * D + (D / 16) * r;
+#pragma unroll
+  for (int i = 0; i < 2; ++i)
+#pragma unroll
+    for (int j = 0; j < D / 64; ++j) t.k[i][j] = *reinterpret_cast<const uint4*>(k + 4 * i * D + 16 * j);
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    if constexpr (D == 128) {
+      const uint2 w = *reinterpret_cast<const uint2*>(v + i * D);
+      t.v[i][0] = w.x;
+      t.v[i][1] = w.y;
+    } else {
+      t.v[i][0] = *reinterpret_cast<const uint32_t*>(v + i * D);
+    }
+  }
+  t.ks = g.k_scales[vplace];
+  t.vs = g.v_scales[vplace];
+}
+
+// Value operand of channels D/16 * r + N: byte N of the eight rows.
+template <int N, int W>
+__device__ __forceinline__ f16x8_t few_values(const uint32_t (&x)[8][W]) {
+  f16x8_t o;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const f16x2_t h = codes_of<N % 4>(x[2 * j][N / 4], x[2 * j + 1][N / 4]);
+    o[2 * j] = h[0];
+    o[2 * j + 1] = h[1];
+  }
+  return o;
+}
+template <int N, int NV, int NC, int W>
+__device__ __forceinline__ void few_weigh(const uint32_t (&x)[8][W], const f16x8_t (&w)[NC], f32x4_t (&o)[NC][NV]) {
+  if constexpr (N < NV) {
+    const f16x8_t v = few_values<N>(x);
+#pragma unroll
+    for (int c = 0; c < NC; ++c) o[c][N] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, w[c], o[c][N], 0, 0, 0);
+    few_weigh<N + 1>(x, w, o);
+  }
+}
+
+// NC * 16 columns a workgroup of four waves, which take the part's tiles of 32 tokens in turn.
+template <bool F16, int D, int NC>
+__global__ __launch_bounds__(256) void attention_few_kernel(AttentionArgs a) {
+  constexpr int COLS = 16 * NC, NK = D / 32, NV = D / 16, PAD = D + 4;
+  __shared__ float joined[4][16][PAD];
+  __shared__ float stat_m[4][COLS], stat_l[4][COLS];
+  const int kv_head = blockIdx.x % a.b.kv_heads;
+  const Item it = find_item(a, COLS, blockIdx.x / a.b.kv_heads, false);
+  if (it.b < 0) return;
+  const KvSeq s = kv_seq(a.b, it.b);
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r = lane & 15, g = lane >> 4;
+
+  f16x8_t q[NC][NK];
+  Column col[NC];
+  float unit[NC];  // of q's halves, times scale log2(e)
+  int all_lo = 0, all_hi = s.len;
+#pragma unroll
+  for (int c = 0; c < NC; ++c) {
+    col[c] = column_of(a, s, kv_head, it.tile * COLS + 16 * c + r);
+    uint4 u[NK];
+#pragma unroll
+    for (int k = 0; k < NK; ++k)
+      u[k] = col[c].real ? load16(a.q + col[c].row * a.q_row + col[c].head * a.q_head + (D / 4) * g + 8 * k)
+                         : make_uint4(0, 0, 0, 0);
+    float factor = 1.0f;
+    unit[c] = a.scale;
+    if constexpr (!F16) {
+      uint32_t most = 0;
+#pragma unroll
+      for (int k = 0; k < NK; ++k) most = abs_most(u[k], most);
+      most = max(most, (uint32_t)__shfl_xor((int)most, 16, kWave));
+      most = max(most, (uint32_t)__shfl_xor((int)most, 32, kWave));
+      float inverse;
+      row_factor(most, factor, inverse);
+      unit[c] *= inverse;
+    }
+#pragma unroll
+    for (int k = 0; k < NK; ++k) q[c][k] = q_halves<F16>(u[k], factor);
+    all_lo = max(all_lo, col[c].lo);
+    all_hi = min(all_hi, col[c].hi);
+  }
+#pragma unroll
+  for (int m = 1; m < 16; m <<= 1) {
+    all_lo = max(all_lo, __shfl_xor(all_lo, m, kWave));
+    all_hi = min(all_hi, __shfl_xor(all_hi, m, kWave));
+  }
+
+  float m[NC], l[NC];
+  f32x4_t o[NC][NV];
+#pragma unroll
+  for (int c = 0; c < NC; ++c) {
+    m[c] = kLow;
+    l[c] = 0.0f;
+#pragma unroll
+    for (int n = 0; n < NV; ++n) o[c][n] = f32x4_t{0, 0, 0, 0};
+  }
+
+  int from, to;
+  part_of(a, s, it, COLS, 32, from, to);
+  FewTile<D> t;
+  int token = from + 32 * wave;
+  if (token < to) few_load<D>(a, it.b, kv_head, token, t);
+  for (; token < to; token += 128) {
+    FewTile<D> now = t;
+    if (token + 128 < to) few_load<D>(a, it.b, kv_head, token + 128, t);
+    // Scores: keys 8 g + 4 i + e of the tile in element e of half i.
+    f32x4_t z[NC][2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+#pragma unroll
+      for (int c = 0; c < NC; ++c) z[c][i] = f32x4_t{0, 0, 0, 0};
+#pragma unroll
+      for (int k = 0; k < NK; ++k) {
+        const uint4& u = now.k[i][k / 2];
+        const uint32_t w0 = word_of(u, 2 * (k & 1)) ^ 0x80808080u, w1 = word_of(u, 2 * (k & 1) + 1) ^ 0x80808080u;
+        const f16x2_t h[4] = {codes_lo(w0), codes_hi(w0), codes_lo(w1), codes_hi(w1)};
+        const f16x8_t key = __builtin_bit_cast(f16x8_t, h);
+#pragma unroll
+        for (int c = 0; c < NC; ++c) z[c][i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(key, q[c][k], z[c][i], 0, 0, 0);
+      }
+    }
+    const float lv = __builtin_amdgcn_logf(now.vs), inverse = 1.0f / now.vs;
+    const bool whole = token >= all_lo && token + 32 <= all_hi && !__any(!now.there);
+    f16x8_t w[NC];
+#pragma unroll
+    for (int c = 0; c < NC; ++c) {
+      const float unit_k = unit[c] * now.ks;
+      float x[8];
+      float top = kLow;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        x[e] = __builtin_fmaf(z[c][e / 4][e % 4], unit_k, lv);
+        if (!whole) {
+          const int at = token + 8 * g + e;
+          x[e] = now.there && at >= col[c].lo && at < col[c].hi ? x[e] : -__builtin_inff();
+        }
+        top = fmaxf(top, x[e]);
+      }
+      if (__any(top > m[c] + kSlack)) {
+        top = fmaxf(top, __shfl_xor(top, 16, kWave));
+        top = fmaxf(top, __shfl_xor(top, 32, kWave));
+        const float grown = fmaxf(m[c], top), less = exp2_fast(m[c] - grown);
+        m[c] = grown;
+        l[c] *= less;
+#pragma unroll
+        for (int n = 0; n < NV; ++n) o[c][n] *= less;
+      }
+      float sum = 0.0f;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const float p = exp2_fast(x[e] - m[c]);
+        sum += p;
+        w[c][e] = (_Float16)p;
+      }
+      // A page that a column sees nothing of adds nothing, whatever its scale.
+      l[c] = sum == 0.0f ? l[c] : __builtin_fmaf(sum, inverse, l[c]);
+    }
+    uint32_t x[8][D / 64];
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+#pragma unroll
+      for (int j = 0; j < D / 64; ++j) x[i][j] = now.v[i][j] ^ 0x80808080u;
+    few_weigh<0>(x, w, o);
+  }
+
+  // The waves' parts to one maximum, and together.
+#pragma unroll
+  for (int c = 0; c < NC; ++c) {
+    l[c] += __shfl_xor(l[c], 16, kWave);
+    l[c] += __shfl_xor(l[c], 32, kWave);
+    if (g == 0) {
+      stat_m[wave][16 * c + r] = m[c];
+      stat_l[wave][16 * c + r] = l[c];
+    }
+  }
+  __syncthreads();
+#pragma unroll
+  for (int c = 0; c < NC; ++c) {
+    const int mine = 16 * c + r;
+    const float most = fmaxf(fmaxf(stat_m[0][mine], stat_m[1][mine]), fmaxf(stat_m[2][mine], stat_m[3][mine]));
+    const float less = exp2_fast(m[c] - most);
+    if (c > 0) __syncthreads();
+#pragma unroll
+    for (int e = 0; e < 4; ++e)  // channels NV (4 g + e) ..
+#pragma unroll
+      for (int n = 0; n < NV; n += 4)
+        *reinterpret_cast<f32x4_t*>(&joined[wave][r][NV * (4 * g + e) + n]) =
+            f32x4_t{o[c][n][e] * less, o[c][n + 1][e] * less, o[c][n + 2][e] * less, o[c][n + 3][e] * less};
+    __syncthreads();
+    for (int i = threadIdx.x; i < 16 * (D / 4); i += 256) {
+      const int cc = i / (D / 4), d = i % (D / 4) * 4, at = 16 * c + cc;
+      const int column = it.tile * COLS + at;
+      if (column >= s.n * a.group) continue;
+      const float top = fmaxf(fmaxf(stat_m[0][at], stat_m[1][at]), fmaxf(stat_m[2][at], stat_m[3][at]));
+      float total = 0.0f, v[4] = {0, 0, 0, 0};
+#pragma unroll
+      for (int x = 0; x < 4; ++x) {
+        total = __builtin_fmaf(stat_l[x][at], exp2_fast(stat_m[x][at] - top), total);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] += joined[x][cc][d + e];
+      }
+      if (it.parts == 1) {
+        const float inverse = total == 0.0f ? 0.0f : 1.0f / total;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] *= inverse;
+        const int row = s.start + column / a.group, head = kv_head * a.group + column % a.group;
+        put_out4<F16>(a.out + ((int64_t)row * a.heads + head) * D + d, v);
+      } else {
+        const int64_t slot = ((int64_t)(it.entry + it.part) * a.b.kv_heads + kv_head) * COLS + at;
+        *reinterpret_cast<float4*>(a.part_out + slot * D + d) = make_float4(v[0], v[1], v[2], v[3]);
+        if (d == 0) a.part_ml[slot] = make_float2(top, total);
+      }
+    }
+  }
+}
+
+// ---- many columns ------------------------------------------------------------
+
+// 128 columns a workgroup of four waves; tiles of 64 tokens in two LDS stages as halves:
+// keys [64][D] and values transposed, [D][64], in 16-byte chunks whose places are XORed
+// so that the 16 lanes of one access meet all banks.
+constexpr int kTile = 64;
+
+template <int D>
+__device__ __forceinline__ int key_at(int token, int chunk) {  // in chunks
+  if constexpr (D == 128) return token * 16 + (chunk ^ ((token & 7) | (token >> 4 & 1) << 3));
+  return token * 8 + (chunk ^ ((token >> 1 & 3) | (token >> 4 & 1) << 2));
+}
+__device__ __forceinline__ int value_at(int channel, int chunk) {
+  return channel * 8 + (chunk ^ (((channel >> 1) ^ (channel >> 4)) & 7));
+}
+
+// What a thread brings of a tile: 16-byte pieces of key rows, and four channels of
+// eight value rows. With 64 channels waves 0 and 1 bring values, 2 and 3 keys.
+template <int D>
+struct Staged {
+  uint4 k[2];
+  uint32_t v[8];
+  float ks, vs;
+  bool there;
+};
+
+template <int D>
+struct Stage {
+  __device__ static bool keys() { return D == 128 || threadIdx.x >= 128; }
+  __device__ static bool values() { return D == 128 || threadIdx.x < 128; }
+  __device__ static int key_piece(int i) { return D == 128 ? threadIdx.x + 256 * i : (threadIdx.x & 127) + 128 * i; }
+  __device__ static int octet() { return threadIdx.x / (D / 4); }
+  __device__ static int quad() { return threadIdx.x % (D / 4); }
+
+  struct Pages {
+    int k[2], v, s;
+  };
+  __device__ static Pages pages(const AttentionArgs& a, int b, int token) {
+    Pages p;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) p.k[i] = keys() ? kv_page(a.b, b, token + key_piece(i) / (D / 16)) : -1;
+    p.v = values() ? kv_page(a.b, b, token + 8 * octet()) : -1;
+    p.s = threadIdx.x < 4 ? kv_page(a.b, b, token + 16 * threadIdx.x) : -1;
+    return p;
+  }
+  __device__ static void load(const AttentionArgs& a, int kv_head, int token, const Pages& p, Staged<D>& t) {
+    const KvBatchArgs& g = a.b;
+    const int mask = (1 << g.page_shift) - 1;
+    if (keys()) {
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const int piece = key_piece(i), at = token + piece / (D / 16);
+        const int64_t place = (int64_t)max(p.k[i], 0) * g.kv_heads + kv_head;
+        t.k[i] = *reinterpret_cast<const uint4*>(g.k + ((place << g.page_shift) + (at & mask)) * D + 16 * (piece % (D / 16)));
+      }
+    }
+    if (values()) {
+      const int at = token + 8 * octet();
+      const int64_t place = (int64_t)max(p.v, 0) * g.kv_heads + kv_head;
+      const int8_t* v = g.v + ((place << g.page_shift) + (at & mask)) * D + 4 * quad();
+#pragma unroll
+      for (int j = 0; j < 8; ++j) t.v[j] = *reinterpret_cast<const uint32_t*>(v + j * D);
+    }
+    if (threadIdx.x < 4) {
+      const int64_t place = (int64_t)max(p.s, 0) * g.kv_heads + kv_head;
+      t.ks = g.k_scales[place];
+      t.vs = g.v_scales[place];
+      t.there = p.s >= 0;
+    }
+  }
+  // float4 of granule (16 tokens): key scale, log2 of the value scale, its inverse, whether there is a page.
+  __device__ static void store(const Staged<D>& t, f16x8_t* keys_to, f16x8_t* values_to, float4* scales) {
+    if (keys()) {
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const int piece = key_piece(i), token = piece / (D / 16), chunk = 2 * (piece % (D / 16));
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const uint32_t w0 = word_of(t.k[i], 2 * h) ^ 0x80808080u, w1 = word_of(t.k[i], 2 * h + 1) ^ 0x80808080u;
+          const f16x2_t c[4] = {codes_lo(w0), codes_hi(w0), codes_lo(w1), codes_hi(w1)};
+          keys_to[key_at<D>(token, chunk + h)] = __builtin_bit_cast(f16x8_t, c);
+        }
+      }
+    }
+    if (values()) {
+      uint32_t x[8][1];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) x[j][0] = t.v[j] ^ 0x80808080u;
+      const int channel = 4 * quad(), chunk = octet();
+      values_to[value_at(channel, chunk)] = few_values<0>(x);
+      values_to[value_at(channel + 1, chunk)] = few_values<1>(x);
+      values_to[value_at(channel + 2, chunk)] = few_values<2>(x);
+      values_to[value_at(channel + 3, chunk)] = few_values<3>(x);
+    }
+    if (threadIdx.x < 4)
+      scales[threadIdx.x] = make_float4(t.ks, __builtin_amdgcn_logf(t.vs), 1.0f / t.vs, t.there ? 1.0f : 0.0f);
+  }
+};
+
+__device__ __forceinline__ f32x16_t zeros16() {
+  f32x16_t z;
+#pragma unroll
+  for (int i = 0; i < 16; ++i) z[i] = 0.0f;
+  return z;
+}
+
+template <bool F16, int D>
+__global__ __launch_bounds__(256, 2) void attention_tile_kernel(AttentionArgs a) {
+  constexpr int COLS = 128, NK = D / 16, NV = D / 32;
+  __shared__ f16x8_t keys[2][kTile * D / 8];
+  __shared__ f16x8_t values[2][kTile * D / 8];
+  __shared__ float4 scales[2][4];
+  const int kv_head = blockIdx.x % a.b.kv_heads;
+  Item it = find_item(a, COLS, blockIdx.x / a.b.kv_heads, false);
+  if (it.b < 0) return;
+  const KvSeq s = kv_seq(a.b, it.b);
+  if (a.causal) {  // the longest first
+    const int tiles = (s.n * a.group + COLS - 1) / COLS;
+    it.entry += (tiles - 1 - 2 * it.tile) * it.parts;
+    it.tile = tiles - 1 - it.tile;
+  }
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r = lane & 31, g = lane >> 5;
+
+  const Column col = column_of(a, s, kv_head, it.tile * COLS + 32 * wave + r);
+  f16x8_t q[NK];  // channels 16 k + 8 g ..
+  float unit = a.scale;
+  {
+    uint4 u[NK];
+#pragma unroll
+    for (int k = 0; k < NK; ++k)
+      u[k] = col.real ? load16(a.q + col.row * a.q_row + col.head * a.q_head + 16 * k + 8 * g) : make_uint4(0, 0, 0, 0);
+    float factor = 1.0f;
+    if constexpr (!F16) {
+      uint32_t most = 0;
+#pragma unroll
+      for (int k = 0; k < NK; ++k) most = abs_most(u[k], most);
+      most = max(most, (uint32_t)__shfl_xor((int)most, 32, kWave));
+      float inverse;
+      row_factor(most, factor, inverse);
+      unit *= inverse;
+    }
+#pragma unroll
+    for (int k = 0; k < NK; ++k) q[k] = q_halves<F16>(u[k], factor);
+  }
+  int all_lo = col.lo, all_hi = col.hi, any_lo = col.lo, any_hi = col.hi;
+#pragma unroll
+  for (int m = 1; m < 32; m <<= 1) {
+    all_lo = max(all_lo, __shfl_xor(all_lo, m, kWave));
+    all_hi = min(all_hi, __shfl_xor(all_hi, m, kWave));
+    any_lo = min(any_lo, __shfl_xor(any_lo, m, kWave));
+    any_hi = max(any_hi, __shfl_xor(any_hi, m, kWave));
+  }
+  // The key row that this lane's row of a product stands for: lanes of half g then hold tokens 16 g .. in order.
+  const int key_row = 16 * (r >> 2 & 1) + 4 * (r >> 3) + (r & 3);
+
+  float m = kLow, l = 0.0f;
+  f32x16_t o[NV];
+#pragma unroll
+  for (int n = 0; n < NV; ++n) o[n] = zeros16();
+
+  int from, to;
+  part_of(a, s, it, COLS, kTile, from, to);
+  using St = Stage<D>;
+  Staged<D> staged;
+  typename St::Pages next;
+  if (from < to) {
+    St::load(a, kv_head, from, St::pages(a, it.b, from), staged);
+    next = St::pages(a, it.b, from + kTile);
+    St::store(staged, keys[0], values[0], scales[0]);
+  }
+  __syncthreads();
+  int stage = 0;
+  for (int token = from; token < to; token += kTile, stage ^= 1) {
+    const bool more = token + kTile < to;
+    if (more) {
+      St::load(a, kv_head, token + kTile, next, staged);
+      next = St::pages(a, it.b, token + 2 * kTile);
+    }
+    if (token < any_hi && token + kTile > any_lo) {  // else no column of the wave sees the tile
+      f32x16_t z[2];
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        z[i] = zeros16();
+#pragma unroll
+        for (int k = 0; k < NK; ++k)
+          z[i] = __builtin_amdgcn_mfma_f32_32x32x16_f16(keys[stage][key_at<D>(32 * i + key_row, 2 * k + g)], q[k], z[i], 0, 0, 0);
+      }
+      float4 sc[2];
+      float x_unit[2], top = kLow;
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        sc[i] = scales[stage][2 * i + g];
+        x_unit[i] = unit * sc[i].x;
+      }
+      const bool whole = token >= all_lo && token + kTile <= all_hi && !__any(sc[0].w * sc[1].w == 0.0f);
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+          z[i][e] = __builtin_fmaf(z[i][e], x_unit[i], sc[i].y);
+          if (!whole) {
+            const int at = token + 32 * i + 16 * g + e;
+            z[i][e] = sc[i].w != 0.0f && at >= col.lo && at < col.hi ? z[i][e] : -__builtin_inff();
+          }
+          top = fmaxf(top, z[i][e]);
+        }
+      if (__any(top > m + kSlack)) {
+        top = fmaxf(top, __shfl_xor(top, 32, kWave));
+        const float grown = fmaxf(m, top), less = exp2_fast(m - grown);
+        m = grown;
+        l *= less;
+#pragma unroll
+        for (int n = 0; n < NV; ++n)
+#pragma unroll
+          for (int e = 0; e < 16; ++e) o[n][e] *= less;
+      }
+      f16x8_t w[2][2];
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        float sum = 0.0f;
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+          const float p = exp2_fast(z[i][e] - m);
+          sum += p;
+          w[i][e / 8][e % 8] = (_Float16)p;
+        }
+        // A page that a column sees nothing of adds nothing, whatever its scale.
+        l = sum == 0.0f ? l : __builtin_fmaf(sum, sc[i].z, l);
+      }
+#pragma unroll
+      for (int n = 0; n < NV; ++n)
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+#pragma unroll
+          for (int h = 0; h < 2; ++h)
+            o[n] = __builtin_amdgcn_mfma_f32_32x32x16_f16(values[stage][value_at(32 * n + r, 4 * i + 2 * g + h)], w[i][h], o[n], 0, 0, 0);
+    }
+    if (more) St::store(staged, keys[stage ^ 1], values[stage ^ 1], scales[stage ^ 1]);
+    __syncthreads();
+  }
+
+  l += __shfl_xor(l, 32, kWave);
+  if (!col.real) return;
+  if (it.parts == 1) {
+    const float inverse = l == 0.0f ? 0.0f : 1.0f / l;
+    uint16_t* out = a.out + ((int64_t)col.row * a.heads + col.head) * D;
+#pragma unroll
+    for (int n = 0; n < NV; ++n)
+#pragma unroll
+      for (int e = 0; e < 16; e += 4) {  // channels 32 n + 8 (e / 4) + 4 g ..
+        const float v[4] = {o[n][e] * inverse, o[n][e + 1] * inverse, o[n][e + 2] * inverse, o[n][e + 3] * inverse};
+        put_out4<F16>(out + 32 * n + 2 * e + 4 * g, v);
+      }
+  } else {
+    const int64_t slot = ((int64_t)(it.entry + it.part) * a.b.kv_heads + kv_head) * COLS + 32 * wave + r;
+    float* out = a.part_out + slot * D;
+#pragma unroll
+    for (int n = 0; n < NV; ++n)
+#pragma unroll
+      for (int e = 0; e < 16; e += 4)
+        *reinterpret_cast<float4*>(out + 32 * n + 2 * e + 4 * g) = make_float4(o[n][e], o[n][e + 1], o[n][e + 2], o[n][e + 3]);
+    if (g == 0) a.part_ml[slot] = make_float2(m, l);
+  }
+}
+
+// ---- parts together ----------------------------------------------------------
+
+// A workgroup for EACH columns of a tile that was cut into parts, `blocks` of them a tile; 256 / EACH threads a
+// column, D/4 of which read one part's sums at a time.
+template <bool F16, int D, int EACH>
+__global__ __launch_bounds__(256) void attention_join_kernel(AttentionArgs a, int columns, int blocks) {
+  constexpr int TEAM = 256 / EACH, LANES = D / 4, WAYS = TEAM / LANES;
+  __shared__ float4 sums[256];
+  __shared__ float totals[256];
+  const int kv_head = blockIdx.y;
+  const Item it = find_item(a, columns, blockIdx.x / blocks, true);
+  if (it.b < 0 || it.parts == 1) return;
+  const KvSeq s = kv_seq(a.b, it.b);
+  const int at = blockIdx.x % blocks * EACH + threadIdx.x / TEAM, column = it.tile * columns + at;
+  const int team = threadIdx.x % TEAM, way = team / LANES, d = team % LANES * 4;
+  const bool real = column < s.n * a.group;
+  float most = kLow, total = 0.0f;
+  float4 v = make_float4(0, 0, 0, 0);
+  const int64_t step = (int64_t)a.b.kv_heads * columns;
+  const int64_t slot = ((int64_t)it.entry * a.b.kv_heads + kv_head) * columns + at;
+  if (real) {
+    for (int p = 0; p < it.parts; ++p) most = fmaxf(most, a.part_ml[slot + p * step].x);
+    for (int p = way; p < it.parts; p += WAYS) {
+      const float2 ml = a.part_ml[slot + p * step];
+      const float4 x = *reinterpret_cast<const float4*>(a.part_out + (slot + p * step) * D + d);
+      const float f = exp2_fast(ml.x - most);
+      total = __builtin_fmaf(ml.y, f, total);
+      v.x = __builtin_fmaf(x.x, f, v.x);
+      v.y = __builtin_fmaf(x.y, f, v.y);
+      v.z = __builtin_fmaf(x.z, f, v.z);
+      v.w = __builtin_fmaf(x.w, f, v.w);
+    }
+  }
+  if (WAYS > 1) {
+    sums[threadIdx.x] = v;
+    totals[threadIdx.x] = total;
+    __syncthreads();
+    if (way) return;
+#pragma unroll
+    for (int w = 1; w < WAYS; ++w) {
+      const float4 o = sums[threadIdx.x + w * LANES];
+      total += totals[threadIdx.x + w * LANES];
+      v.x += o.x, v.y += o.y, v.z += o.z, v.w += o.w;
+    }
+  }
+  if (!real) return;
+  const float inverse = total == 0.0f ? 0.0f : 1.0f / total;
+  const float x[4] = {v.x * inverse, v.y * inverse, v.z * inverse, v.w * inverse};
+  const int row = s.start + column / a.group, head = kv_head * a.group + column % a.group;
+  put_out4<F16>(a.out + ((int64_t)row * a.heads + head) * D + d, x);
+}
+
+template <bool F16, int D>
+void launch_as(const AttentionPlan& p, const AttentionArgs& a, hipStream_t s) {
+  const dim3 grid((uint32_t)p.items * a.b.kv_heads);
+  auto* kernel = p.columns == 16   ? attention_few_kernel<F16, D, 1>
+                 : p.columns == 32 ? attention_few_kernel<F16, D, 2>
+                                   : attention_tile_kernel<F16, D>;
+  tfm_launch(kernel, grid, dim3(256), 0, s, a);
+  check_hip(hipGetLastError(), "cache_attention launch");
+  if (!p.split) return;
+  // Tiles of columns that can be cut: fewer than the target.
+  const int64_t tiles = (int64_t)a.b.rows * a.group / p.columns + a.b.sequences;
+  const int cut = (int)std::min<int64_t>(tiles, p.target);
+  if (p.columns == 128)
+    tfm_launch(attention_join_kernel<F16, D, 8>, dim3(cut * 16, a.b.kv_heads), dim3(256), 0, s, a, 128, 16);
+  else {
+    const int used = std::min(p.columns, a.b.max_rows * a.group);
+    tfm_launch(attention_join_kernel<F16, D, 1>, dim3(cut * used, a.b.kv_heads), dim3(256), 0, s, a, p.columns, used);
+  }
+  check_hip(hipGetLastError(), "cache_attention join launch");
+}
+
+}  // namespace
+
+AttentionPlan attention_plan(int64_t rows, int group, int kv_heads, int sequences, int max_rows, int64_t capacity) {
+  AttentionPlan p{};
+  const int64_t most = (int64_t)max_rows * group;
+  p.columns = most <= 16 ? 16 : most <= 32 ? 32 : 128;
+  const bool few = p.columns < 128;
+  // Items over all key heads that the parts aim at, and the least tokens of a part.
+  const int all = few ? 1024 : 512;
+  p.min_chunk = few ? 128 : 256;
+  p.target = std::max(1, all / kv_heads);
+  const int64_t tiles = std::min<int64_t>(rows * group / p.columns + sequences, rows * group);
+  const int64_t parts = (capacity + p.min_chunk - 1) / p.min_chunk;
+  p.split = parts > 1;
+  p.items = (int)std::max<int64_t>(1, p.split ? std::max(tiles, std::min<int64_t>(2 * p.target, tiles * parts)) : tiles);
+  return p;
+}
+
+void launch_cache_attention(bool f16, int head_dim, const AttentionPlan& p, const AttentionArgs& a, hipStream_t s) {
+  if (head_dim == 64)
+    f16 ? launch_as<true, 64>(p, a, s) : launch_as<false, 64>(p, a, s);
+  else
+    f16 ? launch_as<true, 128>(p, a, s) : launch_as<false, 128>(p, a, s);
+}
+
+}  // namespace tfm

@@ -1,41 +1,13 @@
 // C ABI of the operators around the block: argument checks and launches.
-#include <initializer_list>
-
-#include "tfm_internal.h"
+#include "capi_checks.h"
 
 using namespace tfm;
 
 namespace {
 
-void need_rows(int64_t rows) { need(rows >= 0 && rows <= kMaxRows, "rows out of range"); }
-
-void need_storage(int32_t dtype) {
-  need(dtype == TFM_DTYPE_BF16 || dtype == TFM_DTYPE_F16, "unknown dtype");
-}
-
 void need_eps(float eps, const char* name) {
   if (!(eps >= 0.0f) || eps > 3.4e38f) fail(TFM_E_INVALID, std::string(name) + " must be a non-negative number");
 }
-
-// The bytes of one buffer; null or empty ones share memory with nothing.
-struct Span {
-  const void* at;
-  size_t bytes;
-};
-bool meet(const Span& a, const Span& b) {
-  const uintptr_t p = reinterpret_cast<uintptr_t>(a.at), q = reinterpret_cast<uintptr_t>(b.at);
-  return p && q && (p > q ? p - q < b.bytes : q - p < a.bytes) && a.bytes && b.bytes;
-}
-
-// No output shares memory with an input or another output.
-void need_apart(std::initializer_list<Span> outs, std::initializer_list<Span> ins, const char* message) {
-  for (const Span* o = outs.begin(); o != outs.end(); ++o) {
-    for (const Span& in : ins) need(!meet(*o, in), message);
-    for (const Span* other = outs.begin(); other != o; ++other) need(!meet(*o, *other), message);
-  }
-}
-
-size_t size_of(int32_t dtype) { return dtype == TFM_DTYPE_F32 ? 4 : 2; }
 
 constexpr int kProductMaxK = 131056;  // 128 * 128 * K < 2^31
 

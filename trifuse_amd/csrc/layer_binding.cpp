@@ -13,6 +13,8 @@
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/python_variable.h>
 
+#include <algorithm>
+#include <cmath>
 #include <exception>
 #include <string>
 
@@ -26,6 +28,11 @@ decltype(&tfm_int8_qmm) p_int8_qmm;
 decltype(&tfm_int8_linear_workspace_bytes) p_int8_linear_workspace_bytes;
 decltype(&tfm_int8_linear) p_int8_linear;
 decltype(&tfm_token_logprobs) p_token_logprobs;
+decltype(&tfm_rotary) p_rotary;
+decltype(&tfm_cache_append) p_cache_append;
+decltype(&tfm_cache_read) p_cache_read;
+decltype(&tfm_cache_attention_workspace_bytes) p_cache_attention_workspace_bytes;
+decltype(&tfm_cache_attention) p_cache_attention;
 PyObject* raise_status;  // trifuse_amd._lib.raise_status
 
 struct Raised {};  // a Python error is set
@@ -384,6 +391,208 @@ PyObject* token_logprobs(PyObject*, PyObject* const* v, Py_ssize_t n) {
   });
 }
 
+// [rows, heads, head_dim] with any strides between rows and heads.
+struct Heads {
+  int64_t rows, row_stride, head_stride;
+  int32_t heads, dim;
+};
+Heads heads_of(const at::Tensor& t, const char* name) {
+  if (!t.is_cuda())
+    fail(PyExc_ValueError, std::string(name) + " must be a GPU tensor (the MoE path has no CPU fallback)");
+  if (t.dim() != 3 || t.size(1) <= 0 || t.size(2) <= 0 || t.size(1) > INT32_MAX || t.size(2) > INT32_MAX)
+    fail(PyExc_ValueError, std::string(name) + " must be [rows, heads, head_dim]");
+  if (t.stride(2) != 1 && t.size(2) > 1) fail(PyExc_ValueError, std::string(name) + " must have contiguous heads");
+  return Heads{t.size(0), t.stride(0), t.stride(1), (int32_t)t.size(1), (int32_t)t.size(2)};
+}
+
+void need_device(const at::Tensor& t, const char* name, const at::Tensor& x) {
+  if (t.device() != x.device())
+    fail(PyExc_ValueError, std::string(name) + " is on " + t.device().str() + ", not on " + x.device().str());
+}
+
+int truth(PyObject* o) {
+  const int v = PyObject_IsTrue(o);
+  if (v < 0) throw Raised{};
+  return v;
+}
+
+int64_t whole(PyObject* o, const char* name, int64_t least, int64_t most) {
+  const long long v = PyLong_AsLongLong(o);
+  if (v == -1 && PyErr_Occurred()) throw Raised{};
+  if (v < least || v > most) fail(PyExc_ValueError, std::string(name) + " is out of range");
+  return v;
+}
+
+// frequencies fp64 [pairs], interleaved, scale
+tfm_rotation rotation_of(PyObject* frequencies, PyObject* interleaved, PyObject* scale, const at::Tensor& x) {
+  const at::Tensor& f = tensor(frequencies, "frequencies");
+  need_beside(f, "frequencies", x);
+  if (f.scalar_type() != at::kDouble || f.dim() != 1 || f.size(0) > INT32_MAX)
+    fail(PyExc_ValueError, "frequencies must be fp64 [pairs]");
+  return tfm_rotation{static_cast<const double*>(f.data_ptr()), (int32_t)f.size(0), truth(interleaved), real(scale)};
+}
+
+// rotary(stream, x, positions, frequencies, interleaved, scale, out)
+PyObject* rotary(PyObject*, PyObject* const* v, Py_ssize_t n) {
+  return guarded([&]() -> PyObject* {
+    need_args(n, 7);
+    const at::Tensor& x = tensor(v[1], "x");
+    const int32_t dt = storage_code(x, "x");
+    const Heads h = heads_of(x, "x");
+    const at::Tensor& p = tensor(v[2], "positions");
+    need_beside(p, "positions", x);
+    if ((p.scalar_type() != at::kLong && p.scalar_type() != at::kInt) || p.dim() != 1 || p.size(0) != h.rows)
+      fail(PyExc_ValueError, "positions must be int32 or int64 [rows]");
+    const tfm_rotation r = rotation_of(v[3], v[4], v[5], x);
+    at::Tensor made;
+    if (v[6] == Py_None) made = empty(x.sizes(), x.scalar_type(), x);
+    const at::Tensor& out = v[6] == Py_None ? made : tensor(v[6], "out");
+    const Heads o = heads_of(out, "out");
+    need_device(out, "out", x);
+    if (out.scalar_type() != x.scalar_type() || out.sizes() != x.sizes())
+      fail(PyExc_ValueError, "out geometry/dtype differs");
+    void* stream = stream_of(v[0]);
+    enqueue([&] {
+      return p_rotary(x.data_ptr(), h.rows, h.heads, h.dim, h.row_stride, h.head_stride, p.data_ptr(),
+                      p.scalar_type() == at::kLong ? 64 : 32, &r, dt, out.data_ptr(), o.row_stride, o.head_stride, stream);
+    });
+    return v[6] == Py_None ? wrap(made) : Py_NewRef(v[6]);
+  });
+}
+
+// k, v, k_scales, v_scales of a KVCache
+tfm_kv_cache cache_of(PyObject* const* v, const at::Tensor* beside) {
+  const at::Tensor& k = tensor(v[0], "cache.k");
+  need_dev(k, "cache.k");
+  if (beside) need_device(k, "cache.k", *beside);
+  const at::Tensor& val = tensor(v[1], "cache.v");
+  const at::Tensor& ks = tensor(v[2], "cache.k_scales");
+  const at::Tensor& vs = tensor(v[3], "cache.v_scales");
+  need_beside(val, "cache.v", k);
+  need_beside(ks, "cache.k_scales", k);
+  need_beside(vs, "cache.v_scales", k);
+  if (k.scalar_type() != at::kChar || k.dim() != 4 || val.scalar_type() != at::kChar || val.sizes() != k.sizes())
+    fail(PyExc_ValueError, "cache.k and cache.v must be int8 [pages, kv_heads, page_tokens, head_dim]");
+  if (ks.scalar_type() != at::kFloat || vs.scalar_type() != at::kFloat || ks.sizes() != k.sizes().slice(0, 2) ||
+      vs.sizes() != ks.sizes())
+    fail(PyExc_ValueError, "cache.k_scales and cache.v_scales must be fp32 [pages, kv_heads]");
+  for (int i = 1; i < 4; ++i)
+    if (k.size(i) > INT32_MAX) fail(PyExc_ValueError, "cache.k is too large");
+  return tfm_kv_cache{static_cast<int8_t*>(k.data_ptr()),  static_cast<int8_t*>(val.data_ptr()),
+                      static_cast<float*>(ks.data_ptr()),  static_cast<float*>(vs.data_ptr()),
+                      k.size(0),                           (int32_t)k.size(1),
+                      (int32_t)k.size(2),                  (int32_t)k.size(3)};
+}
+
+// table, lengths, starts and max_rows (None: rows / sequences without starts, rows with them)
+tfm_kv_batch batch_of(PyObject* table, PyObject* lengths, PyObject* starts, PyObject* max_rows, int64_t rows,
+                      const at::Tensor& x) {
+  const at::Tensor& t = tensor(table, "table");
+  const at::Tensor& l = tensor(lengths, "lengths");
+  need_beside(t, "table", x);
+  need_beside(l, "lengths", x);
+  if (t.scalar_type() != at::kInt || t.dim() != 2 || t.size(0) > INT32_MAX || t.size(1) > INT32_MAX)
+    fail(PyExc_ValueError, "table must be int32 [sequences, pages of the longest]");
+  if (l.scalar_type() != at::kInt || l.dim() != 1 || l.size(0) != t.size(0))
+    fail(PyExc_ValueError, "lengths must be int32 [sequences]");
+  tfm_kv_batch b{static_cast<const int32_t*>(t.data_ptr()), static_cast<const int32_t*>(l.data_ptr()), nullptr,
+                 (int32_t)t.size(0), (int32_t)t.size(1), 0};
+  if (starts != Py_None) {
+    const at::Tensor& s = tensor(starts, "starts");
+    need_beside(s, "starts", x);
+    if (s.scalar_type() != at::kInt || s.dim() != 1 || s.size(0) != t.size(0) + 1)
+      fail(PyExc_ValueError, "starts must be int32 [sequences + 1]");
+    b.starts = static_cast<const int32_t*>(s.data_ptr());
+    b.max_rows = (int32_t)(max_rows == Py_None ? std::min<int64_t>(rows, INT32_MAX) : whole(max_rows, "max_rows", 0, INT32_MAX));
+  } else {
+    if (max_rows != Py_None) fail(PyExc_ValueError, "max_rows goes with starts");
+    if (b.sequences == 0 ? rows != 0 : rows % b.sequences != 0)
+      fail(PyExc_ValueError, "without starts every sequence has the same number of rows");
+    b.max_rows = b.sequences ? (int32_t)std::min<int64_t>(rows / b.sequences, INT32_MAX) : 0;
+  }
+  return b;
+}
+
+// cache_append(stream, k, v, cache.k, cache.v, cache.k_scales, cache.v_scales, table, lengths, starts, max_rows,
+//              frequencies, interleaved, rotary_scale)
+PyObject* cache_append(PyObject*, PyObject* const* v, Py_ssize_t n) {
+  return guarded([&]() -> PyObject* {
+    need_args(n, 14);
+    const at::Tensor& k = tensor(v[1], "k");
+    const at::Tensor& val = tensor(v[2], "v");
+    const int32_t dt = storage_code(k, "k");
+    const Heads h = heads_of(k, "k"), o = heads_of(val, "v");
+    need_device(val, "v", k);
+    if (val.scalar_type() != k.scalar_type() || val.sizes() != k.sizes())
+      fail(PyExc_ValueError, "v geometry/dtype differs from k's");
+    const tfm_kv_cache c = cache_of(v + 3, &k);
+    if (h.heads != c.kv_heads || h.dim != c.head_dim) fail(PyExc_ValueError, "k and v must be [rows, kv_heads, head_dim] of the cache");
+    const tfm_kv_batch b = batch_of(v[7], v[8], v[9], v[10], h.rows, k);
+    tfm_rotation r{};
+    if (v[11] != Py_None) r = rotation_of(v[11], v[12], v[13], k);
+    void* stream = stream_of(v[0]);
+    enqueue([&] {
+      return p_cache_append(k.data_ptr(), h.row_stride, h.head_stride, val.data_ptr(), o.row_stride, o.head_stride, h.rows,
+                            v[11] != Py_None ? &r : nullptr, dt, &c, &b, stream);
+    });
+    return Py_NewRef(Py_None);
+  });
+}
+
+// cache_read(stream, cache.k, cache.v, cache.k_scales, cache.v_scales, table, lengths, rows, dtype)
+PyObject* cache_read(PyObject*, PyObject* const* v, Py_ssize_t n) {
+  return guarded([&]() -> PyObject* {
+    need_args(n, 9);
+    if (!THPDtype_Check(v[8])) fail(PyExc_ValueError, "dtype must be a torch.dtype");
+    const at::ScalarType type = reinterpret_cast<THPDtype*>(v[8])->scalar_type;
+    if (type != at::kBFloat16 && type != at::kHalf && type != at::kFloat)
+      fail(PyExc_ValueError, std::string("unknown output dtype ") + c10::toString(type));
+    const int32_t dt = type == at::kBFloat16 ? TFM_DTYPE_BF16 : type == at::kHalf ? TFM_DTYPE_F16 : TFM_DTYPE_F32;
+    const tfm_kv_cache c = cache_of(v + 1, nullptr);
+    const at::Tensor& x = tensor(v[1], "cache.k");
+    const int64_t rows = whole(v[7], "rows", 0, 1 << 22);
+    const at::Tensor& t = tensor(v[5], "table");
+    const int64_t total = t.dim() > 0 ? t.size(0) * rows : 0;
+    if (total >= (1 << 22)) fail(PyExc_ValueError, "sequences * rows is out of range");
+    const tfm_kv_batch b = batch_of(v[5], v[6], Py_None, Py_None, total, x);
+    at::Tensor k = empty({total, c.kv_heads, c.head_dim}, type, x), val = empty({total, c.kv_heads, c.head_dim}, type, x);
+    void* stream = stream_of(v[0]);
+    enqueue([&] { return p_cache_read(&c, &b, dt, k.data_ptr(), val.data_ptr(), stream); });
+    return pack(wrap(k), wrap(val));
+  });
+}
+
+// cache_attention(stream, q, cache.k, cache.v, cache.k_scales, cache.v_scales, table, lengths, starts, max_rows, scale,
+//                 causal, window, out)
+PyObject* cache_attention(PyObject*, PyObject* const* v, Py_ssize_t n) {
+  return guarded([&]() -> PyObject* {
+    need_args(n, 14);
+    const at::Tensor& q = tensor(v[1], "q");
+    const int32_t dt = storage_code(q, "q");
+    const Heads h = heads_of(q, "q");
+    const tfm_kv_cache c = cache_of(v + 2, &q);
+    if (h.dim != c.head_dim) fail(PyExc_ValueError, "q must have the cache's head_dim");
+    const tfm_kv_batch b = batch_of(v[6], v[7], v[8], v[9], h.rows, q);
+    const float scale = v[10] == Py_None ? (float)(1.0 / std::sqrt((double)h.dim)) : real(v[10]);
+    const int causal = truth(v[11]);
+    const int32_t window = (int32_t)whole(v[12], "window", 0, INT32_MAX);
+    at::Tensor made, space;
+    if (v[13] == Py_None) made = empty(q.sizes(), q.scalar_type(), q);
+    const at::Tensor& out = v[13] == Py_None ? made : tensor(v[13], "out");
+    need_beside(out, "out", q);
+    if (out.scalar_type() != q.scalar_type() || out.sizes() != q.sizes())
+      fail(PyExc_ValueError, "out geometry/dtype differs");
+    const size_t need = p_cache_attention_workspace_bytes(h.rows, h.heads, window, &c, &b);
+    if (need) space = empty({(int64_t)need}, at::kByte, q);
+    void* stream = stream_of(v[0]);
+    enqueue([&] {
+      return p_cache_attention(q.data_ptr(), h.row_stride, h.head_stride, h.rows, h.heads, &c, &b, scale, causal, window, dt,
+                               out.data_ptr(), need ? space.data_ptr() : nullptr, need, stream);
+    });
+    return v[13] == Py_None ? wrap(made) : Py_NewRef(v[13]);
+  });
+}
+
 // bind({name: address}, raise_status)
 PyObject* bind(PyObject*, PyObject* const* v, Py_ssize_t n) {
   return guarded([&]() -> PyObject* {
@@ -399,6 +608,11 @@ PyObject* bind(PyObject*, PyObject* const* v, Py_ssize_t n) {
     take(p_int8_linear_workspace_bytes, "tfm_int8_linear_workspace_bytes");
     take(p_int8_linear, "tfm_int8_linear");
     take(p_token_logprobs, "tfm_token_logprobs");
+    take(p_rotary, "tfm_rotary");
+    take(p_cache_append, "tfm_cache_append");
+    take(p_cache_read, "tfm_cache_read");
+    take(p_cache_attention_workspace_bytes, "tfm_cache_attention_workspace_bytes");
+    take(p_cache_attention, "tfm_cache_attention");
     Py_XDECREF(raise_status);
     raise_status = Py_NewRef(v[1]);
     return Py_NewRef(Py_None);
@@ -408,7 +622,8 @@ PyObject* bind(PyObject*, PyObject* const* v, Py_ssize_t n) {
 #define TFM_FUNC(name) {#name, (PyCFunction)(void (*)(void))name, METH_FASTCALL, nullptr}
 PyMethodDef methods[] = {TFM_FUNC(bind),         TFM_FUNC(norm_residual), TFM_FUNC(rms_norm),
                          TFM_FUNC(quantize_rows), TFM_FUNC(int8_qmm),      TFM_FUNC(int8_linear),
-                         TFM_FUNC(token_logprobs), {nullptr, nullptr, 0, nullptr}};
+                         TFM_FUNC(token_logprobs), TFM_FUNC(rotary),        TFM_FUNC(cache_append),
+                         TFM_FUNC(cache_read),     TFM_FUNC(cache_attention), {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_layer", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 
 }  // namespace

@@ -379,4 +379,64 @@ void launch_combine_rows(bool f16, const uint16_t* Y, const int32_t* inverse, co
 void launch_rows_to_st(bool f16, const float* P, int64_t rows, int H, uint16_t* out, hipStream_t s);
 void launch_copy_i32(const int32_t* src, int32_t* dst, int64_t n, hipStream_t s);
 
+// Rotary positions and the 8-bit cache (rotary.hip, kv_cache.hip, attention.hip).
+constexpr int kMaxHeads = 1024;
+constexpr int kRotaryMaxDim = 1024;
+struct RotaryArgs {
+  const uint16_t* x;
+  uint16_t* out;
+  int64_t x_row, x_head, out_row, out_head;  // strides, elements
+  const void* positions;
+  bool positions64;
+  const double* frequencies;
+  float scale;
+  int rows, heads, pairs, rest;  // rest: channels behind the pairs that are copied (0 in place)
+  bool interleaved;
+};
+void launch_rotary(bool f16, const RotaryArgs& a, hipStream_t s);
+
+// tfm_kv_cache and tfm_kv_batch as the kernels take them.
+struct KvBatchArgs {
+  int8_t *k, *v;
+  float *k_scales, *v_scales;
+  int pages, kv_heads, page_shift;
+  const int32_t *table, *lengths, *starts;
+  int sequences, table_width, max_rows;
+  int rows;  // of the call's activations
+};
+struct KvAppendArgs {
+  KvBatchArgs b;
+  const uint16_t *k, *v;
+  int64_t k_row, k_head, v_row, v_head;
+  const double* frequencies;  // null: no rotation
+  float scale;
+  int pairs;
+  bool interleaved;
+};
+void launch_cache_append(bool f16, int head_dim, const KvAppendArgs& a, hipStream_t s);
+void launch_cache_read(int dtype, int head_dim, const KvBatchArgs& b, void* k, void* v, hipStream_t s);
+
+struct AttentionArgs {
+  KvBatchArgs b;
+  const uint16_t* q;
+  uint16_t* out;
+  int64_t q_row, q_head;
+  int heads, group;   // query heads, and those of one key head
+  float scale;        // times log2(e)
+  bool causal;
+  int window;         // 0: none
+  int min_chunk;      // least tokens of a split
+  int target;         // work items a key head that the splits aim at
+  int items;          // work items a key head in the grid
+  float* part_out;    // [items * kv_heads, columns, head_dim], null: no splits
+  float2* part_ml;    // [items * kv_heads, columns]
+};
+// How a call is cut into workgroups: `columns` (row, head) pairs of a key head each, and along the tokens.
+struct AttentionPlan {
+  int columns, min_chunk, target, items;
+  bool split;
+};
+AttentionPlan attention_plan(int64_t rows, int group, int kv_heads, int sequences, int max_rows, int64_t capacity);
+void launch_cache_attention(bool f16, int head_dim, const AttentionPlan& plan, const AttentionArgs& a, hipStream_t s);
+
 }  // namespace tfm

@@ -1,8 +1,8 @@
 """The operators of a decoder layer around its MoE block, over the HIP library.
 
 What stands between two blocks and behind the last one (tfm_norm_residual,
-tfm_quantize_rows, tfm_int8_qmm, tfm_int8_linear and tfm_token_logprobs of
-include/trifuse_moe.h, which has the exact definitions):
+tfm_quantize_rows, tfm_int8_qmm, tfm_int8_linear, tfm_token_logprobs, tfm_rotary and
+the tfm_cache_* calls of include/trifuse_moe.h, which has the exact definitions):
 
 * ``rms_norm`` and ``norm_residual``: the norm in front of a block, and in one
   pass the norm behind it, its gate, the scaled residual and the next block's
@@ -12,7 +12,10 @@ include/trifuse_moe.h, which has the exact definitions):
   scale for each token and for each channel), beside the group-wise
   ``moe.native_affine_qmm``;
 * ``token_logprobs``: log probabilities of given tokens, entropy and the most
-  likely alternatives, from the output head's logits.
+  likely alternatives, from the output head's logits;
+* ``rotary``, ``KVCache``, ``cache_append``, ``cache_read`` and ``cache_attention``:
+  from the fused projection's queries, keys and values to the output projection's
+  input, over a paged cache of 8-bit codes with a scale for each page and head.
 
 Tensors are torch tensors of one HIP device; work is enqueued on that device's
 current stream. There is no CPU fallback and no backward. Every sum, norm and
@@ -20,7 +23,8 @@ softmax is held in fp32 (products in int32) and each output is rounded once.
 """
 from __future__ import annotations
 
-from typing import Optional, Tuple
+import math
+from typing import NamedTuple, Optional, Tuple
 
 import torch
 
@@ -120,3 +124,106 @@ def token_logprobs(logits: torch.Tensor, tokens: Optional[torch.Tensor] = None, 
     logits, largest first, ties to the lower id. Masked logits are -inf; a row
     of nothing else has entropy 0 and log probabilities -inf. scale: 1e-35 to 1e30."""
     return _enqueue("token_logprobs", logits, tokens, top, scale)
+
+
+# ---------------------------------------------------------------------------
+# Rotary positions and attention over an 8-bit cache
+# ---------------------------------------------------------------------------
+
+def rotary_frequencies(pairs: int, base: float = 10000.0, *, stretch: float = 1.0, method: str = "linear",
+                       context: Optional[int] = None, slow: float = 1.0, fast: float = 32.0,
+                       device=None) -> Tuple[torch.Tensor, float]:
+    """(frequencies fp64 [pairs], scale) for ``rotary``: base ** (-i / pairs) radians a position, and for a context
+    ``stretch`` times as long as the one that a model was trained on
+
+    * "linear": every frequency divided by stretch; scale 1;
+    * "base": base multiplied by stretch ** (pairs / (pairs - 1)), which keeps the fastest pair and slows the
+      slowest to 1 / stretch; scale 1;
+    * "bands": a pair that turns at least ``fast`` times over the trained ``context`` keeps its frequency, one
+      that turns at most ``slow`` times has it divided by stretch, between them the two are mixed in proportion to
+      the turns' place; scale 0.1 ln(stretch) + 1."""
+    if pairs < 1:
+        raise ValueError("pairs must be positive")
+    if not (base > 0 and stretch >= 1 and math.isfinite(base) and math.isfinite(stretch)):
+        raise ValueError("base must be positive and stretch at least 1")
+    if method not in ("linear", "base", "bands"):
+        raise ValueError(f"unknown method {method!r}")
+    if method == "base":
+        base = base * stretch ** (pairs / max(pairs - 1, 1))
+    f = float(base) ** (-torch.arange(pairs, dtype=torch.float64) / pairs)
+    scale = 1.0
+    if method == "linear":
+        f = f / stretch
+    elif method == "bands":
+        if not context or context < 1 or not fast > slow:
+            raise ValueError("bands need the trained context and fast > slow")
+        kept = ((f * (context / (2 * math.pi)) - slow) / (fast - slow)).clamp(0, 1)
+        f = f * (kept + (1 - kept) / stretch)
+        scale = 0.1 * math.log(stretch) + 1.0
+    return f.to(device), scale
+
+
+def rotary(x: torch.Tensor, positions: torch.Tensor, frequencies: torch.Tensor, *, interleaved: bool = False,
+           scale: float = 1.0, out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Pairs of a head's channels turned by position * frequency: (x1 c - x2 s, x2 c + x1 s) with c = scale * cos and
+    s = scale * sin, angles in 64 bits, rounded once.
+
+    x [rows, heads, head_dim] bf16 or f16, any strides of rows and heads (a view into a fused projection);
+    positions int32 or int64 [rows]; frequencies fp64 [pairs] (``rotary_frequencies``), 2 * pairs <= head_dim: pair i
+    is channels (i, pairs + i), or (2i, 2i + 1) with interleaved, and channels behind the pairs are copied. out may
+    be x itself; a new one is contiguous."""
+    return _enqueue("rotary", x, positions, frequencies, interleaved, scale, out)
+
+
+class KVCache(NamedTuple):
+    """A pool of pages of keys and values: int8 codes [pages, kv_heads, page_tokens, head_dim] and fp32 scales
+    [pages, kv_heads] of each (value = code * scale). page_tokens: 16, 32, 64, 128 or 256; head_dim: 64 or 128.
+    Pages need no clearing: the first token of a page starts its scale anew."""
+    k: torch.Tensor
+    v: torch.Tensor
+    k_scales: torch.Tensor
+    v_scales: torch.Tensor
+
+    @classmethod
+    def empty(cls, pages: int, kv_heads: int, page_tokens: int, head_dim: int, device="cuda") -> "KVCache":
+        codes = (pages, kv_heads, page_tokens, head_dim)
+        return cls(*(torch.zeros(codes, dtype=torch.int8, device=device) for _ in "kv"),
+                   *(torch.zeros(codes[:2], dtype=torch.float32, device=device) for _ in "kv"))
+
+
+def cache_append(k: torch.Tensor, v: torch.Tensor, cache: KVCache, table: torch.Tensor, lengths: torch.Tensor, *,
+                 starts: Optional[torch.Tensor] = None, max_rows: Optional[int] = None,
+                 frequencies: Optional[torch.Tensor] = None, interleaved: bool = False,
+                 rotary_scale: float = 1.0) -> None:
+    """Writes a step's keys and values [rows, kv_heads, head_dim] (bf16 or f16, any strides of rows and heads) into
+    the cache, keys turned to their positions first where frequencies (as ``rotary``, pairs a multiple of 8) are given.
+
+    Sequence b has lengths[b] tokens (int32) with this step's, token t in page table[b, t // page_tokens] (int32
+    [sequences, width]). Its rows are starts[b] : starts[b + 1] (int32 [sequences + 1], max_rows at least the most of
+    one sequence; None: all rows), the last of its tokens; without starts every sequence has the same number.
+    A page and head takes the larger of its scale and max|x| / 127 of its new tokens; codes that it
+    held are rounded to a larger scale. An infinity or a NaN makes the page NaN. Pages are not shared between
+    sequences that write to them in one call."""
+    _enqueue("cache_append", k, v, *cache, table, lengths, starts, max_rows, frequencies, interleaved, rotary_scale)
+
+
+def cache_read(cache: KVCache, table: torch.Tensor, lengths: torch.Tensor, rows: int,
+               dtype: torch.dtype = torch.bfloat16) -> Tuple[torch.Tensor, torch.Tensor]:
+    """(k, v) [sequences * rows, kv_heads, head_dim] in `dtype` (bf16, f16 or fp32): the last `rows` tokens of every
+    sequence as the values that their codes stand for, to be kept elsewhere. Tokens before the first are zero."""
+    return _enqueue("cache_read", cache.k, *cache[1:], table, lengths, rows, dtype)
+
+
+def cache_attention(q: torch.Tensor, cache: KVCache, table: torch.Tensor, lengths: torch.Tensor, *,
+                    starts: Optional[torch.Tensor] = None, max_rows: Optional[int] = None,
+                    scale: Optional[float] = None, causal: bool = True, window: int = 0,
+                    out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """softmax(scale * q . k) v over the cached tokens that each row sees, in q's dtype and shape.
+
+    q [rows, heads, head_dim] bf16 or f16, any strides of rows and heads, heads a multiple of the cache's; table,
+    lengths, starts and max_rows as in ``cache_append``, behind which it goes: row i of n of sequence b is at position
+    lengths[b] - n + i, and sees tokens up to its own (causal) or all of its sequence, with window > 0 (causal) the
+    last `window` of them. A row that sees none is zero; rows behind the last sequence are not written. scale: None
+    is head_dim ** -0.5. Pass max_rows with starts where it is known: it picks the kernel (up to 32 rows times query
+    heads a key head: the one that decodes)."""
+    return _enqueue("cache_attention", q, *cache, table, lengths, starts, max_rows, scale, causal, window, out)
