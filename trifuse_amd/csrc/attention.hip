@@ -39,96 +39,108 @@ constexpr float kSlack = 8.0f;            // log2 of how far weights may pass 1
 
 __device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
 
-template <typename T>
-__device__ __forceinline__ T wave_sum(T v) {
-#pragma unroll
-  for (int m = 1; m < 64; m <<= 1) v += __shfl_xor(v, m, kWave);
-  return v;
+// Sum over the wave, and sums up to each lane, without leaving the registers.
+__device__ __forceinline__ float wave_sum(float v) {
+  return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(wave_tree_sum64(v)), 63));
+}
+template <int CTRL, int ROWS>
+__device__ __forceinline__ int dpp_add(int v) {
+  return v + __builtin_amdgcn_update_dpp(0, v, CTRL, ROWS, 0xf, false);
+}
+__device__ __forceinline__ int wave_upto(int v) {
+  v = dpp_add<0x111, 0xf>(v);  // row_shr:1, 2, 4, 8
+  v = dpp_add<0x112, 0xf>(v);
+  v = dpp_add<0x114, 0xf>(v);
+  v = dpp_add<0x118, 0xf>(v);
+  v = dpp_add<0x142, 0xa>(v);  // row_bcast:15, 31
+  return dpp_add<0x143, 0xc>(v);
 }
 
 // What one work item is.
 struct Item {
-  int b;        // sequence, -1: none
-  int tile;     // of its columns
-  int part;     // of `parts`
+  int b;      // sequence, -1: none
+  KvSeq s;
+  int tile;   // of the sequence's columns
+  int part;   // of `parts`
   int parts;
-  int entry;    // index of part 0 of this tile
+  int entry;  // index of part 0 of this tile
+  int index;  // of the tile in the batch
 };
 
-struct Need {
-  int tiles, tokens;  // of columns, and tokens that some row sees
-};
-__device__ __forceinline__ Need need_of(const AttentionArgs& a, int b, int columns) {
-  const KvSeq s = kv_seq(a.b, b);
-  const int lo = a.window ? max(0, s.first() - a.window + 1) : 0;
-  return Need{(s.n * a.group + columns - 1) / columns, max(s.len - lo, 0)};
+// A sequence's tiles of columns, and tokens that some of its rows see.
+__device__ __forceinline__ int tiles_of(const AttentionArgs& a, const KvSeq& s, int columns) {
+  return (s.n * a.group + columns - 1) / columns;
+}
+__device__ __forceinline__ int tokens_of(const AttentionArgs& a, const KvSeq& s) {
+  return max(s.len - (a.window ? max(0, s.first() - a.window + 1) : 0), 0);
 }
 
-// Tokens of a part: all of them where the tiles fill the machine by themselves, else
-// the batch's tokens (of every tile) over the items that should run.
-__device__ __forceinline__ int chunk_of(const AttentionArgs& a, int columns) {
-  if (!a.part_out) return 1 << 30;
-  long long tiles = 0, tokens = 0;
-  for (int b0 = 0; b0 < a.b.sequences; b0 += kWave) {
-    const int b = b0 + (threadIdx.x & 63);
-    if (b < a.b.sequences) {
-      const Need n = need_of(a, b, columns);
-      tiles += n.tiles;
-      tokens += (long long)n.tiles * n.tokens;
+// Item `index` of the batch. Every wave finds it by itself, a sequence a lane. A part's
+// tokens are all of them where the tiles fill the machine by themselves, else the batch's
+// tokens (of every tile) over the items that should run: at most a.target parts more than
+// there are tiles (the sum's fp32 rounding is below the allowance of 2^-18). `tiles` is the
+// batch's number of tiles where they are cut, else 0.
+__device__ Item find_item(const AttentionArgs& a, int columns, int index, int& tiles_cut) {
+  const int lane = threadIdx.x & 63;
+  auto mine = [&](int b) {
+    KvSeq s{0, 0, 0};
+    if (b < a.b.sequences) s = kv_seq(a.b, b);
+    return s;
+  };
+  KvSeq s = mine(lane);
+  int chunk = 1 << 30;
+  tiles_cut = 0;
+  if (a.part_out) {
+    float tiles = 0.0f, tokens = 0.0f;
+    for (int b0 = 0; b0 < a.b.sequences; b0 += kWave) {
+      const KvSeq o = b0 ? mine(b0 + lane) : s;
+      const float t = (float)tiles_of(a, o, columns);
+      tiles += wave_sum(t);
+      tokens += wave_sum(t * (float)tokens_of(a, o));
+    }
+    if (tiles < (float)a.target) {
+      const float even = tokens * (1.0f + 0x1p-18f) / (64.0f * (float)a.target);
+      chunk = max(a.min_chunk, 64 * ((int)fminf(even, 0x1p23f) + 1));
+      tiles_cut = (int)tiles;
     }
   }
-  if (a.b.sequences > 1) {
-    tiles = wave_sum(tiles);
-    tokens = wave_sum(tokens);
-  } else {
-    tiles = __shfl(tiles, 0, kWave);
-    tokens = __shfl(tokens, 0, kWave);
-  }
-  if (tiles >= a.target) return 1 << 30;
-  const long long even = (tokens + a.target - 1) / a.target;
-  return max(a.min_chunk, (int)((even + 63) / 64 * 64));
-}
-
-// Item `index` of the batch; with by_tile, tile `index` (its part 0). Every wave finds it by itself.
-__device__ Item find_item(const AttentionArgs& a, int columns, int index, bool by_tile) {
-  const int chunk = chunk_of(a, columns);
-  int before = 0, entries = 0;  // counted items (or tiles), and items, of the sequences before
+  int before = 0, tiles_before = 0;
   for (int b0 = 0; b0 < a.b.sequences; b0 += kWave) {
-    const int lane = threadIdx.x & 63, b = b0 + lane;
-    int tiles = 0, parts = 1;
-    if (b < a.b.sequences) {
-      const Need n = need_of(a, b, columns);
-      tiles = n.tiles;
-      parts = max(1, (int)(((long long)n.tokens + chunk - 1) / chunk));
-    }
-    const int mine = by_tile ? tiles : tiles * parts;
-    int upto = mine, items = tiles * parts;
-    if (a.b.sequences > 1) {
-#pragma unroll
-      for (int m = 1; m < 64; m <<= 1) {
-        const int o = __shfl_up(upto, m, kWave), p = __shfl_up(items, m, kWave);
-        if (lane >= m) {
-          upto += o;
-          items += p;
-        }
-      }
-    }
+    if (b0) s = mine(b0 + lane);
+    const int tiles = tiles_of(a, s, columns);
+    const int parts = max(1, (tokens_of(a, s) + chunk - 1) / chunk);
+    const int upto = wave_upto(tiles * parts), tiles_upto = wave_upto(tiles);
     const uint64_t hit = __ballot(index < before + upto);
     if (hit) {
       const int l = __builtin_ctzll(hit);
-      const int local = index - before - (__shfl(upto, l, kWave) - __shfl(mine, l, kWave));
+      auto of = [&](int v) { return __builtin_amdgcn_readlane(v, l); };
       Item it;
       it.b = b0 + l;
-      it.parts = __shfl(parts, l, kWave);
-      it.tile = by_tile ? local : local / it.parts;
-      it.part = by_tile ? 0 : local % it.parts;
-      it.entry = entries + __shfl(items, l, kWave) - __shfl(tiles, l, kWave) * it.parts + it.tile * it.parts;
+      it.s = KvSeq{of(s.start), of(s.n), of(s.len)};
+      it.parts = of(parts);
+      const int first = before + of(upto) - of(tiles) * it.parts, local = index - first;
+      it.tile = local / it.parts;
+      it.part = local - it.tile * it.parts;
+      it.entry = first + it.tile * it.parts;
+      it.index = tiles_before + of(tiles_upto) - of(tiles) + it.tile;
       return it;
     }
-    before += __shfl(upto, 63, kWave);
-    entries += __shfl(items, 63, kWave);
+    before += __builtin_amdgcn_readlane(upto, 63);
+    tiles_before += __builtin_amdgcn_readlane(tiles_upto, 63);
   }
-  return Item{-1, 0, 0, 1, 0};
+  Item none{};
+  none.b = -1;
+  return none;
+}
+
+// For the joining kernel: how many tiles are cut, and each one's first row, columns from
+// there on, first item and parts. Part 0 of each writes its own.
+__device__ __forceinline__ void tell_join(const AttentionArgs& a, const Item& it, int columns, int tiles_cut) {
+  if (!a.part_out || threadIdx.x != 0) return;
+  if (blockIdx.x == 0) a.cut[0] = make_int4(tiles_cut, 0, 0, 0);
+  if (tiles_cut && it.b >= 0 && it.part == 0)
+    a.cut[1 + it.index] = make_int4(it.s.start, it.tile * columns, it.s.n * a.group, it.parts);
+  if (tiles_cut && it.b >= 0 && it.part == 0) a.cut_entry[it.index] = it.entry;
 }
 
 // A column of an item: its row and head, and the tokens [lo, hi) that it sees.
@@ -205,28 +217,39 @@ __device__ __forceinline__ void put_out4(uint16_t* p, const float* v) {
 // 32 tokens of a wave, as loaded: lane (r = lane % 16, g = lane / 16) has bytes
 // D/4 * g .. of key rows 8 (r / 4) + 4 t + r % 4, and bytes D/16 * r .. of value rows 8 g + j.
 template <int D>
-struct FewTile {
+struct FewKeys {
   uint4 k[2][D / 64];
-  uint32_t v[8][D / 64];
-  float ks, vs;  // of the page that tokens 8 g .. lie in
-  bool there;    // that page is one
 };
-
 template <int D>
-__device__ __forceinline__ void few_load(const AttentionArgs& a, int b, int kv_head, int token, FewTile<D>& t) {
+struct FewValues {
+  uint32_t v[8][D / 64];
+};
+struct FewPages {
+  int k, v;  // of this lane's key rows and value rows; -1: none
+};
+__device__ __forceinline__ FewPages few_pages(const AttentionArgs& a, int b, int token) {
+  const int lane = threadIdx.x & 63, r = lane & 15, q = lane >> 4;
+  return FewPages{kv_page(a.b, b, token + 8 * (r >> 2)), kv_page(a.b, b, token + 8 * q)};
+}
+template <int D>
+__device__ __forceinline__ void few_load_keys(const AttentionArgs& a, int kv_head, int token, int page, FewKeys<D>& t) {
   const KvBatchArgs& g = a.b;
   const int lane = threadIdx.x & 63, r = lane & 15, q = lane >> 4;
-  const int mask = (1 << g.page_shift) - 1;
-  const int kt = token + 8 * (r >> 2) + (r & 3), vt = token + 8 * q;
-  const int kp = max(kv_page(g, b, kt), 0), found = kv_page(g, b, vt), vp = max(found, 0);
-  t.there = found >= 0;
-  const int64_t kplace = (int64_t)kp * g.kv_heads + kv_head, vplace = (int64_t)vp * g.kv_heads + kv_head;
-  const int8_t* k = g.k + ((kplace << g.page_shift) + (kt & mask)) * D + (D / 4) * q;
-  const int8_t* v = g.v + ((vplace << g.page_shift) + (vt & mask)) * D + (D / 16) * r;
+  const int at = token + 8 * (r >> 2) + (r & 3);
+  const int64_t place = (int64_t)max(page, 0) * g.kv_heads + kv_head;
+  const int8_t* k = g.k + ((place << g.page_shift) + (at & ((1 << g.page_shift) - 1))) * D + (D / 4) * q;
 #pragma unroll
   for (int i = 0; i < 2; ++i)
 #pragma unroll
     for (int j = 0; j < D / 64; ++j) t.k[i][j] = *reinterpret_cast<const uint4*>(k + 4 * i * D + 16 * j);
+}
+template <int D>
+__device__ __forceinline__ void few_load_values(const AttentionArgs& a, int kv_head, int token, int page, FewValues<D>& t) {
+  const KvBatchArgs& g = a.b;
+  const int lane = threadIdx.x & 63, r = lane & 15, q = lane >> 4;
+  const int at = token + 8 * q;
+  const int64_t place = (int64_t)max(page, 0) * g.kv_heads + kv_head;
+  const int8_t* v = g.v + ((place << g.page_shift) + (at & ((1 << g.page_shift) - 1))) * D + (D / 16) * r;
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
     if constexpr (D == 128) {
@@ -237,8 +260,11 @@ __device__ __forceinline__ void few_load(const AttentionArgs& a, int b, int kv_h
       t.v[i][0] = *reinterpret_cast<const uint32_t*>(v + i * D);
     }
   }
-  t.ks = g.k_scales[vplace];
-  t.vs = g.v_scales[vplace];
+}
+// The scales of the page that tokens 8 g .. lie in.
+__device__ __forceinline__ float2 few_load_scales(const AttentionArgs& a, int kv_head, int page) {
+  const int64_t place = (int64_t)max(page, 0) * a.b.kv_heads + kv_head;
+  return make_float2(a.b.k_scales[place], a.b.v_scales[place]);
 }
 
 // Value operand of channels D/16 * r + N: byte N of the eight rows.
@@ -265,14 +291,16 @@ __device__ __forceinline__ void few_weigh(const uint32_t (&x)[8][W], const f16x8
 
 // NC * 16 columns a workgroup of four waves, which take the part's tiles of 32 tokens in turn.
 template <bool F16, int D, int NC>
-__global__ __launch_bounds__(256) void attention_few_kernel(AttentionArgs a) {
+__global__ __launch_bounds__(256, NC == 1 ? 3 : 2) void attention_few_kernel(AttentionArgs a) {
   constexpr int COLS = 16 * NC, NK = D / 32, NV = D / 16, PAD = D + 4;
   __shared__ float joined[4][16][PAD];
   __shared__ float stat_m[4][COLS], stat_l[4][COLS];
   const int kv_head = blockIdx.x % a.b.kv_heads;
-  const Item it = find_item(a, COLS, blockIdx.x / a.b.kv_heads, false);
+  int tiles_cut;
+  const Item it = find_item(a, COLS, blockIdx.x / a.b.kv_heads, tiles_cut);
+  if (kv_head == 0) tell_join(a, it, COLS, tiles_cut);
   if (it.b < 0) return;
-  const KvSeq s = kv_seq(a.b, it.b);
+  const KvSeq& s = it.s;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r = lane & 15, g = lane >> 4;
 
   f16x8_t q[NC][NK];
@@ -282,17 +310,17 @@ __global__ __launch_bounds__(256) void attention_few_kernel(AttentionArgs a) {
 #pragma unroll
   for (int c = 0; c < NC; ++c) {
     col[c] = column_of(a, s, kv_head, it.tile * COLS + 16 * c + r);
-    uint4 u[NK];
+    uint4 raw[NK];
 #pragma unroll
     for (int k = 0; k < NK; ++k)
-      u[k] = col[c].real ? load16(a.q + col[c].row * a.q_row + col[c].head * a.q_head + (D / 4) * g + 8 * k)
+      raw[k] = col[c].real ? load16(a.q + col[c].row * a.q_row + col[c].head * a.q_head + (D / 4) * g + 8 * k)
                          : make_uint4(0, 0, 0, 0);
     float factor = 1.0f;
     unit[c] = a.scale;
     if constexpr (!F16) {
       uint32_t most = 0;
 #pragma unroll
-      for (int k = 0; k < NK; ++k) most = abs_most(u[k], most);
+      for (int k = 0; k < NK; ++k) most = abs_most(raw[k], most);
       most = max(most, (uint32_t)__shfl_xor((int)most, 16, kWave));
       most = max(most, (uint32_t)__shfl_xor((int)most, 32, kWave));
       float inverse;
@@ -300,7 +328,7 @@ __global__ __launch_bounds__(256) void attention_few_kernel(AttentionArgs a) {
       unit[c] *= inverse;
     }
 #pragma unroll
-    for (int k = 0; k < NK; ++k) q[c][k] = q_halves<F16>(u[k], factor);
+    for (int k = 0; k < NK; ++k) q[c][k] = q_halves<F16>(raw[k], factor);
     all_lo = max(all_lo, col[c].lo);
     all_hi = min(all_hi, col[c].hi);
   }
@@ -322,12 +350,22 @@ __global__ __launch_bounds__(256) void attention_few_kernel(AttentionArgs a) {
 
   int from, to;
   part_of(a, s, it, COLS, 32, from, to);
-  FewTile<D> t;
+  // Keys of the next tile are asked for when this one's scores are done, values when
+  // they are weighed; page numbers a tile earlier.
+  FewKeys<D> t;
+  FewValues<D> u;
+  FewPages page{-1, -1}, next{-1, -1};
+  float2 scale{};
   int token = from + 32 * wave;
-  if (token < to) few_load<D>(a, it.b, kv_head, token, t);
+  if (token < to) {
+    page = few_pages(a, it.b, token);
+    next = few_pages(a, it.b, token + 128);
+    few_load_keys<D>(a, kv_head, token, page.k, t);
+    few_load_values<D>(a, kv_head, token, page.v, u);
+    scale = few_load_scales(a, kv_head, page.v);
+  }
   for (; token < to; token += 128) {
-    FewTile<D> now = t;
-    if (token + 128 < to) few_load<D>(a, it.b, kv_head, token + 128, t);
+    const bool more = token + 128 < to;
     // Scores: keys 8 g + 4 i + e of the tile in element e of half i.
     f32x4_t z[NC][2];
 #pragma unroll
@@ -336,20 +374,21 @@ __global__ __launch_bounds__(256) void attention_few_kernel(AttentionArgs a) {
       for (int c = 0; c < NC; ++c) z[c][i] = f32x4_t{0, 0, 0, 0};
 #pragma unroll
       for (int k = 0; k < NK; ++k) {
-        const uint4& u = now.k[i][k / 2];
-        const uint32_t w0 = word_of(u, 2 * (k & 1)) ^ 0x80808080u, w1 = word_of(u, 2 * (k & 1) + 1) ^ 0x80808080u;
+        const uint4& raw = t.k[i][k / 2];
+        const uint32_t w0 = word_of(raw, 2 * (k & 1)) ^ 0x80808080u, w1 = word_of(raw, 2 * (k & 1) + 1) ^ 0x80808080u;
         const f16x2_t h[4] = {codes_lo(w0), codes_hi(w0), codes_lo(w1), codes_hi(w1)};
         const f16x8_t key = __builtin_bit_cast(f16x8_t, h);
 #pragma unroll
         for (int c = 0; c < NC; ++c) z[c][i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(key, q[c][k], z[c][i], 0, 0, 0);
       }
     }
-    const float lv = __builtin_amdgcn_logf(now.vs), inverse = 1.0f / now.vs;
-    const bool whole = token >= all_lo && token + 32 <= all_hi && !__any(!now.there);
+    if (more) few_load_keys<D>(a, kv_head, token + 128, next.k, t);
+    const float lv = __builtin_amdgcn_logf(scale.y), inverse = __builtin_amdgcn_rcpf(scale.y);
+    const bool there = page.v >= 0, whole = token >= all_lo && token + 32 <= all_hi && !__any(!there);
     f16x8_t w[NC];
 #pragma unroll
     for (int c = 0; c < NC; ++c) {
-      const float unit_k = unit[c] * now.ks;
+      const float unit_k = unit[c] * scale.x;
       float x[8];
       float top = kLow;
 #pragma unroll
@@ -357,7 +396,7 @@ __global__ __launch_bounds__(256) void attention_few_kernel(AttentionArgs a) {
         x[e] = __builtin_fmaf(z[c][e / 4][e % 4], unit_k, lv);
         if (!whole) {
           const int at = token + 8 * g + e;
-          x[e] = now.there && at >= col[c].lo && at < col[c].hi ? x[e] : -__builtin_inff();
+          x[e] = there && at >= col[c].lo && at < col[c].hi ? x[e] : -__builtin_inff();
         }
         top = fmaxf(top, x[e]);
       }
@@ -384,8 +423,14 @@ __global__ __launch_bounds__(256) void attention_few_kernel(AttentionArgs a) {
 #pragma unroll
     for (int i = 0; i < 8; ++i)
 #pragma unroll
-      for (int j = 0; j < D / 64; ++j) x[i][j] = now.v[i][j] ^ 0x80808080u;
+      for (int j = 0; j < D / 64; ++j) x[i][j] = u.v[i][j] ^ 0x80808080u;
     few_weigh<0>(x, w, o);
+    if (more) {
+      few_load_values<D>(a, kv_head, token + 128, next.v, u);
+      scale = few_load_scales(a, kv_head, next.v);
+      page = next;
+      next = few_pages(a, it.b, token + 256);
+    }
   }
 
   // The waves' parts to one maximum, and together.
@@ -552,11 +597,13 @@ __global__ __launch_bounds__(256, 2) void attention_tile_kernel(AttentionArgs a)
   __shared__ f16x8_t values[2][kTile * D / 8];
   __shared__ float4 scales[2][4];
   const int kv_head = blockIdx.x % a.b.kv_heads;
-  Item it = find_item(a, COLS, blockIdx.x / a.b.kv_heads, false);
+  int tiles_cut;
+  Item it = find_item(a, COLS, blockIdx.x / a.b.kv_heads, tiles_cut);
+  if (kv_head == 0) tell_join(a, it, COLS, tiles_cut);
   if (it.b < 0) return;
-  const KvSeq s = kv_seq(a.b, it.b);
+  const KvSeq& s = it.s;
   if (a.causal) {  // the longest first
-    const int tiles = (s.n * a.group + COLS - 1) / COLS;
+    const int tiles = tiles_of(a, s, COLS);
     it.entry += (tiles - 1 - 2 * it.tile) * it.parts;
     it.tile = tiles - 1 - it.tile;
   }
@@ -706,27 +753,30 @@ __global__ __launch_bounds__(256, 2) void attention_tile_kernel(AttentionArgs a)
 
 // ---- parts together ----------------------------------------------------------
 
-// A workgroup for EACH columns of a tile that was cut into parts, `blocks` of them a tile; 256 / EACH threads a
-// column, D/4 of which read one part's sums at a time.
+// A workgroup for EACH columns of a tile that was cut into parts, `blocks` of them a tile;
+// D/4 threads read a column's sums of one part at a time. With one column a workgroup the
+// others of its 256 threads take other parts.
 template <bool F16, int D, int EACH>
 __global__ __launch_bounds__(256) void attention_join_kernel(AttentionArgs a, int columns, int blocks) {
-  constexpr int TEAM = 256 / EACH, LANES = D / 4, WAYS = TEAM / LANES;
-  __shared__ float4 sums[256];
-  __shared__ float totals[256];
-  const int kv_head = blockIdx.y;
-  const Item it = find_item(a, columns, blockIdx.x / blocks, true);
-  if (it.b < 0 || it.parts == 1) return;
-  const KvSeq s = kv_seq(a.b, it.b);
-  const int at = blockIdx.x % blocks * EACH + threadIdx.x / TEAM, column = it.tile * columns + at;
-  const int team = threadIdx.x % TEAM, way = team / LANES, d = team % LANES * 4;
-  const bool real = column < s.n * a.group;
-  float most = kLow, total = 0.0f;
-  float4 v = make_float4(0, 0, 0, 0);
+  constexpr int LANES = D / 4, TEAMS = 256 / LANES, WAYS = EACH == 1 ? TEAMS : 1;
+  __shared__ float4 sums[WAYS > 1 ? 256 : 1];
+  __shared__ float totals[WAYS > 1 ? 256 : 1];
+  const int kv_head = blockIdx.y, tile = blockIdx.x / blocks;
+  const int count = a.cut[0].x;
+  const int4 info = a.cut[1 + tile];  // first row, first column, columns of the sequence, parts
+  const int entry = a.cut_entry[tile];
+  if (tile >= count || info.w == 1) return;
+  const int team = threadIdx.x / LANES, d = threadIdx.x % LANES * 4, way = WAYS > 1 ? team : 0;
   const int64_t step = (int64_t)a.b.kv_heads * columns;
-  const int64_t slot = ((int64_t)it.entry * a.b.kv_heads + kv_head) * columns + at;
-  if (real) {
-    for (int p = 0; p < it.parts; ++p) most = fmaxf(most, a.part_ml[slot + p * step].x);
-    for (int p = way; p < it.parts; p += WAYS) {
+#pragma unroll 1
+  for (int c = WAYS > 1 ? 0 : team; c < EACH; c += WAYS > 1 ? 1 : TEAMS) {
+    const int at = blockIdx.x % blocks * EACH + c, column = info.y + at;
+    if (column >= info.z) return;  // with several teams there is no barrier below
+    const int64_t slot = ((int64_t)entry * a.b.kv_heads + kv_head) * columns + at;
+    float most = kLow, total = 0.0f;
+    float4 v = make_float4(0, 0, 0, 0);
+    for (int p = 0; p < info.w; ++p) most = fmaxf(most, a.part_ml[slot + p * step].x);
+    for (int p = way; p < info.w; p += WAYS) {
       const float2 ml = a.part_ml[slot + p * step];
       const float4 x = *reinterpret_cast<const float4*>(a.part_out + (slot + p * step) * D + d);
       const float f = exp2_fast(ml.x - most);
@@ -736,24 +786,23 @@ __global__ __launch_bounds__(256) void attention_join_kernel(AttentionArgs a, in
       v.z = __builtin_fmaf(x.z, f, v.z);
       v.w = __builtin_fmaf(x.w, f, v.w);
     }
-  }
-  if (WAYS > 1) {
-    sums[threadIdx.x] = v;
-    totals[threadIdx.x] = total;
-    __syncthreads();
-    if (way) return;
+    if (WAYS > 1) {
+      sums[threadIdx.x] = v;
+      totals[threadIdx.x] = total;
+      __syncthreads();
+      if (way) return;
 #pragma unroll
-    for (int w = 1; w < WAYS; ++w) {
-      const float4 o = sums[threadIdx.x + w * LANES];
-      total += totals[threadIdx.x + w * LANES];
-      v.x += o.x, v.y += o.y, v.z += o.z, v.w += o.w;
+      for (int w = 1; w < WAYS; ++w) {
+        const float4 o = sums[threadIdx.x + w * LANES];
+        total += totals[threadIdx.x + w * LANES];
+        v.x += o.x, v.y += o.y, v.z += o.z, v.w += o.w;
+      }
     }
+    const float inverse = total == 0.0f ? 0.0f : 1.0f / total;
+    const float x[4] = {v.x * inverse, v.y * inverse, v.z * inverse, v.w * inverse};
+    const int row = info.x + column / a.group, head = kv_head * a.group + column % a.group;
+    put_out4<F16>(a.out + ((int64_t)row * a.heads + head) * D + d, x);
   }
-  if (!real) return;
-  const float inverse = total == 0.0f ? 0.0f : 1.0f / total;
-  const float x[4] = {v.x * inverse, v.y * inverse, v.z * inverse, v.w * inverse};
-  const int row = s.start + column / a.group, head = kv_head * a.group + column % a.group;
-  put_out4<F16>(a.out + ((int64_t)row * a.heads + head) * D + d, x);
 }
 
 template <bool F16, int D>
@@ -769,7 +818,7 @@ void launch_as(const AttentionPlan& p, const AttentionArgs& a, hipStream_t s) {
   const int64_t tiles = (int64_t)a.b.rows * a.group / p.columns + a.b.sequences;
   const int cut = (int)std::min<int64_t>(tiles, p.target);
   if (p.columns == 128)
-    tfm_launch(attention_join_kernel<F16, D, 8>, dim3(cut * 16, a.b.kv_heads), dim3(256), 0, s, a, 128, 16);
+    tfm_launch(attention_join_kernel<F16, D, 32>, dim3(cut * 4, a.b.kv_heads), dim3(256), 0, s, a, 128, 4);
   else {
     const int used = std::min(p.columns, a.b.max_rows * a.group);
     tfm_launch(attention_join_kernel<F16, D, 1>, dim3(cut * used, a.b.kv_heads), dim3(256), 0, s, a, p.columns, used);

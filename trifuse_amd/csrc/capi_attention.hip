@@ -84,6 +84,8 @@ AttentionPlan plan_of(int64_t rows, int32_t heads, int32_t window, const KvBatch
 struct AttentionWs {
   float* out;
   float2* ml;
+  int4* cut;
+  int* cut_entry;
   size_t bytes;
 };
 AttentionWs carve_attention(const AttentionPlan& p, int kv_heads, int head_dim, void* base) {
@@ -94,6 +96,8 @@ AttentionWs carve_attention(const AttentionPlan& p, int kv_heads, int head_dim, 
   const size_t slots = (size_t)std::min(p.items, 2 * p.target) * (size_t)kv_heads * (size_t)p.columns;
   w.out = c.take<float>(slots * (size_t)head_dim);
   w.ml = c.take<float2>(slots);
+  w.cut = c.take<int4>((size_t)p.target + 1);
+  w.cut_entry = c.take<int>((size_t)p.target);
   w.bytes = align_up(c.offset, 256);
   return w;
 }
@@ -239,6 +243,8 @@ int tfm_cache_attention(const void* q, int64_t row_stride, int64_t head_stride, 
     a.items = plan.items;
     a.part_out = ws.out;
     a.part_ml = ws.ml;
+    a.cut = ws.cut;
+    a.cut_entry = ws.cut_entry;
     launch_cache_attention(dtype == TFM_DTYPE_F16, cache->head_dim, plan, a, static_cast<hipStream_t>(stream));
   });
 }

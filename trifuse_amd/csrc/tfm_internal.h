@@ -429,7 +429,9 @@ struct AttentionArgs {
   int target;         // work items a key head that the splits aim at
   int items;          // work items a key head in the grid
   float* part_out;    // [items * kv_heads, columns, head_dim], null: no splits
-  float2* part_ml;    // [items * kv_heads, columns]
+  float2* part_ml;    // [items * kv_heads, columns]: maximum and sum
+  int4* cut;          // [1 + target]: how many tiles are cut, and what each one is
+  int* cut_entry;     // [target]: its first item
 };
 // How a call is cut into workgroups: `columns` (row, head) pairs of a key head each, and along the tokens.
 struct AttentionPlan {
