@@ -6,11 +6,14 @@
 // One pass with a running maximum, over t_j = s_j log2(e) + log2(b_j):
 //   w_j = 2^(t_j - m),   out = (sum_j w_j cv_j) / (sum_j w_j / b_j)
 // so the page's value scale costs nothing an element (its logarithm rides in the
-// exponent's fused multiply-add, its inverse on the sum of 16 weights), and codes enter
-// the products as they are: a half holds every code exactly, q of bf16 exactly after a
-// power of two for its row (28 binades; what is smaller loses bits below 2^-25 of the
-// largest), and w to 2^-12 of itself. m follows the true maximum only when that has grown
-// by more than 2^8 (a half holds 2^8 as well as 1), so rescaling the sums is rare.
+// exponent's fused multiply-add, its inverse on the sum of 8 or 16 weights). Codes enter the
+// products as they are, as halves that hold them exactly (keys plus 128, which the sum of q
+// takes out of a score again), q of bf16 exactly after a power of two for its row (28
+// binades; what is smaller loses bits below 2^-25 of the largest), and w to 2^-12 of itself,
+// in the first sum alone. m is a maximum that is taken again only when a weight has grown past
+// 2^15 (a half's relative precision is the same there), so most tiles look for none and
+// rescale nothing: what is left a score is a multiply-add, an exponential, an addition and
+// half a conversion of two.
 //
 // "Columns" are the (row, head) pairs of one key head: they share its codes. Scores are
 // taken transposed, keys along the rows of a product and columns along its lanes: a lane
@@ -35,7 +38,7 @@ namespace tfm {
 namespace {
 
 constexpr float kLow = -3.402823466e38f;  // below every score; finite, so that differences are
-constexpr float kSlack = 8.0f;            // log2 of how far weights may pass 1
+constexpr float kMost = 32768.0f;         // sum of a lane's weights of a page from which the maximum is taken again
 
 __device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
 
@@ -201,6 +204,26 @@ __device__ __forceinline__ void row_factor(uint32_t most, float& factor, float& 
   inverse = __uint_as_float((254u - field) << 23);
 }
 
+// A negative scale goes into q, so that products' units are positive.
+__device__ __forceinline__ uint4 flip_signs(uint4 u, uint32_t bits) {
+  return make_uint4(u.x ^ bits, u.y ^ bits, u.z ^ bits, u.w ^ bits);
+}
+// What a product of halves is worth, in factors that stay in range where the whole does.
+__device__ __forceinline__ float unit_of(float scale, float inverse) {
+  static_assert(kKeyUnit == 0x1p24f, "two factors of 2^12");
+  return fabsf(scale) * (inverse * 0x1p12f) * 0x1p12f;
+}
+// A unit so small that no score counts, but not zero: a hidden score, -inf, stays that.
+__device__ __forceinline__ float not_zero(float unit) { return unit < 0x1p-100f ? 0x1p-100f : unit; }
+
+// Sum of eight halves on top of `sum`.
+__device__ __forceinline__ float add_halves(const f16x8_t& h, float sum) {
+  const f16x2_t one = {(_Float16)1.0f, (_Float16)1.0f};
+#pragma unroll
+  for (int j = 0; j < 4; ++j) sum = __builtin_amdgcn_fdot2(f16x2_t{h[2 * j], h[2 * j + 1]}, one, sum, false);
+  return sum;
+}
+
 __device__ __forceinline__ uint4 load16(const uint16_t* p) {
   uint4 u;
   __builtin_memcpy(&u, p, 16);
@@ -273,7 +296,7 @@ __device__ __forceinline__ f16x8_t few_values(const uint32_t (&x)[8][W]) {
   f16x8_t o;
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
-    const f16x2_t h = codes_of<N % 4>(x[2 * j][N / 4], x[2 * j + 1][N / 4]);
+    const f16x2_t h = value_codes<N % 4>(x[2 * j][N / 4], x[2 * j + 1][N / 4]);
     o[2 * j] = h[0];
     o[2 * j + 1] = h[1];
   }
@@ -305,18 +328,20 @@ __global__ __launch_bounds__(256, NC == 1 ? 3 : 2) void attention_few_kernel(Att
 
   f16x8_t q[NC][NK];
   Column col[NC];
-  float unit[NC];  // of q's halves, times scale log2(e)
+  float unit[NC];  // of a product of halves, times scale log2(e)
+  float bias[NC];  // what the keys' 128 adds to one
   int all_lo = 0, all_hi = s.len;
+  const uint32_t flip = a.scale < 0.0f ? 0x80008000u : 0;
 #pragma unroll
   for (int c = 0; c < NC; ++c) {
     col[c] = column_of(a, s, kv_head, it.tile * COLS + 16 * c + r);
     uint4 raw[NK];
 #pragma unroll
     for (int k = 0; k < NK; ++k)
-      raw[k] = col[c].real ? load16(a.q + col[c].row * a.q_row + col[c].head * a.q_head + (D / 4) * g + 8 * k)
-                         : make_uint4(0, 0, 0, 0);
+      raw[k] = col[c].real ? flip_signs(load16(a.q + col[c].row * a.q_row + col[c].head * a.q_head + (D / 4) * g + 8 * k), flip)
+                           : make_uint4(0, 0, 0, 0);
     float factor = 1.0f;
-    unit[c] = a.scale;
+    unit[c] = unit_of(a.scale, 1.0f);
     if constexpr (!F16) {
       uint32_t most = 0;
 #pragma unroll
@@ -325,10 +350,16 @@ __global__ __launch_bounds__(256, NC == 1 ? 3 : 2) void attention_few_kernel(Att
       most = max(most, (uint32_t)__shfl_xor((int)most, 32, kWave));
       float inverse;
       row_factor(most, factor, inverse);
-      unit[c] *= inverse;
+      unit[c] = unit_of(a.scale, inverse);
     }
 #pragma unroll
     for (int k = 0; k < NK; ++k) q[c][k] = q_halves<F16>(raw[k], factor);
+    float sum = 0.0f;
+#pragma unroll
+    for (int k = 0; k < NK; ++k) sum = add_halves(q[c][k], sum);
+    sum += __shfl_xor(sum, 16, kWave);
+    sum += __shfl_xor(sum, 32, kWave);
+    bias[c] = sum * (128.0f / kKeyUnit);
     all_lo = max(all_lo, col[c].lo);
     all_hi = min(all_hi, col[c].hi);
   }
@@ -376,7 +407,7 @@ __global__ __launch_bounds__(256, NC == 1 ? 3 : 2) void attention_few_kernel(Att
       for (int k = 0; k < NK; ++k) {
         const uint4& raw = t.k[i][k / 2];
         const uint32_t w0 = word_of(raw, 2 * (k & 1)) ^ 0x80808080u, w1 = word_of(raw, 2 * (k & 1) + 1) ^ 0x80808080u;
-        const f16x2_t h[4] = {codes_lo(w0), codes_hi(w0), codes_lo(w1), codes_hi(w1)};
+        const f16x2_t h[4] = {key_codes_lo(w0), key_codes_hi(w0), key_codes_lo(w1), key_codes_hi(w1)};
         const f16x8_t key = __builtin_bit_cast(f16x8_t, h);
 #pragma unroll
         for (int c = 0; c < NC; ++c) z[c][i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(key, q[c][k], z[c][i], 0, 0, 0);
@@ -388,33 +419,40 @@ __global__ __launch_bounds__(256, NC == 1 ? 3 : 2) void attention_few_kernel(Att
     f16x8_t w[NC];
 #pragma unroll
     for (int c = 0; c < NC; ++c) {
-      const float unit_k = unit[c] * scale.x;
-      float x[8];
-      float top = kLow;
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        x[e] = __builtin_fmaf(z[c][e / 4][e % 4], unit_k, lv);
-        if (!whole) {
-          const int at = token + 8 * g + e;
-          x[e] = there && at >= col[c].lo && at < col[c].hi ? x[e] : -__builtin_inff();
+      float unit_k = not_zero(unit[c] * scale.x), shift = __builtin_fmaf(-bias[c], unit_k, lv);
+      if (!whole) {
+        const int lo = col[c].lo - token - 8 * g, hi = there ? col[c].hi - token - 8 * g : 0;
+        if (max(lo, 0) >= min(hi, 8)) {  // nothing of the page: nor of its scales, whatever they are
+          unit_k = 1.0f;
+          shift = 0.0f;
         }
-        top = fmaxf(top, x[e]);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) z[c][e / 4][e % 4] = e >= lo && e < hi ? z[c][e / 4][e % 4] : -__builtin_inff();
       }
-      if (__any(top > m[c] + kSlack)) {
+      auto score = [&](int e, float low) { return __builtin_fmaf(z[c][e / 4][e % 4], unit_k, low); };
+      auto weigh = [&] {
+        float sum = 0.0f;  // of fp32 weights: beside large value scales a small page's weights leave a half's range
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const float p = exp2_fast(score(e, shift - m[c]));
+          sum += p;
+          w[c][e] = (_Float16)p;
+        }
+        return sum;
+      };
+      float sum = weigh();
+      if (__any(sum > kMost)) {
+        float top = m[c];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) top = fmaxf(top, score(e, shift));
         top = fmaxf(top, __shfl_xor(top, 16, kWave));
         top = fmaxf(top, __shfl_xor(top, 32, kWave));
-        const float grown = fmaxf(m[c], top), less = exp2_fast(m[c] - grown);
-        m[c] = grown;
+        const float less = exp2_fast(m[c] - top);
+        m[c] = top;
         l[c] *= less;
 #pragma unroll
         for (int n = 0; n < NV; ++n) o[c][n] *= less;
-      }
-      float sum = 0.0f;
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const float p = exp2_fast(x[e] - m[c]);
-        sum += p;
-        w[c][e] = (_Float16)p;
+        sum = weigh();
       }
       // A page that a column sees nothing of adds nothing, whatever its scale.
       l[c] = sum == 0.0f ? l[c] : __builtin_fmaf(sum, inverse, l[c]);
@@ -470,7 +508,7 @@ __global__ __launch_bounds__(256, NC == 1 ? 3 : 2) void attention_few_kernel(Att
         for (int e = 0; e < 4; ++e) v[e] += joined[x][cc][d + e];
       }
       if (it.parts == 1) {
-        const float inverse = total == 0.0f ? 0.0f : 1.0f / total;
+        const float inverse = total == 0.0f ? 0.0f : kValueUnit / total;
 #pragma unroll
         for (int e = 0; e < 4; ++e) v[e] *= inverse;
         const int row = s.start + column / a.group, head = kv_head * a.group + column % a.group;
@@ -563,7 +601,7 @@ struct Stage {
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
           const uint32_t w0 = word_of(t.k[i], 2 * h) ^ 0x80808080u, w1 = word_of(t.k[i], 2 * h + 1) ^ 0x80808080u;
-          const f16x2_t c[4] = {codes_lo(w0), codes_hi(w0), codes_lo(w1), codes_hi(w1)};
+          const f16x2_t c[4] = {key_codes_lo(w0), key_codes_hi(w0), key_codes_lo(w1), key_codes_hi(w1)};
           keys_to[key_at<D>(token, chunk + h)] = __builtin_bit_cast(f16x8_t, c);
         }
       }
@@ -579,7 +617,7 @@ struct Stage {
       values_to[value_at(channel + 3, chunk)] = few_values<3>(x);
     }
     if (threadIdx.x < 4)
-      scales[threadIdx.x] = make_float4(t.ks, __builtin_amdgcn_logf(t.vs), 1.0f / t.vs, t.there ? 1.0f : 0.0f);
+      scales[threadIdx.x] = make_float4(t.ks, __builtin_amdgcn_logf(t.vs), __builtin_amdgcn_rcpf(t.vs), t.there ? 1.0f : 0.0f);
   }
 };
 
@@ -611,12 +649,14 @@ __global__ __launch_bounds__(256, 2) void attention_tile_kernel(AttentionArgs a)
 
   const Column col = column_of(a, s, kv_head, it.tile * COLS + 32 * wave + r);
   f16x8_t q[NK];  // channels 16 k + 8 g ..
-  float unit = a.scale;
+  float unit = unit_of(a.scale, 1.0f), bias = 0.0f;  // of a product of halves; what the keys' 128 adds to one
   {
+    const uint32_t flip = a.scale < 0.0f ? 0x80008000u : 0;
     uint4 u[NK];
 #pragma unroll
     for (int k = 0; k < NK; ++k)
-      u[k] = col.real ? load16(a.q + col.row * a.q_row + col.head * a.q_head + 16 * k + 8 * g) : make_uint4(0, 0, 0, 0);
+      u[k] = col.real ? flip_signs(load16(a.q + col.row * a.q_row + col.head * a.q_head + 16 * k + 8 * g), flip)
+                      : make_uint4(0, 0, 0, 0);
     float factor = 1.0f;
     if constexpr (!F16) {
       uint32_t most = 0;
@@ -625,10 +665,13 @@ __global__ __launch_bounds__(256, 2) void attention_tile_kernel(AttentionArgs a)
       most = max(most, (uint32_t)__shfl_xor((int)most, 32, kWave));
       float inverse;
       row_factor(most, factor, inverse);
-      unit *= inverse;
+      unit = unit_of(a.scale, inverse);
     }
 #pragma unroll
     for (int k = 0; k < NK; ++k) q[k] = q_halves<F16>(u[k], factor);
+#pragma unroll
+    for (int k = 0; k < NK; ++k) bias = add_halves(q[k], bias);
+    bias = (bias + __shfl_xor(bias, 32, kWave)) * (128.0f / kKeyUnit);
   }
   int all_lo = col.lo, all_hi = col.hi, any_lo = col.lo, any_hi = col.hi;
 #pragma unroll
@@ -657,6 +700,15 @@ __global__ __launch_bounds__(256, 2) void attention_tile_kernel(AttentionArgs a)
     St::store(staged, keys[0], values[0], scales[0]);
   }
   __syncthreads();
+  // Places of this lane's operands, in bytes: an XOR away from each other, and the other stage's by one more.
+  constexpr int STAGE = kTile * D * 2;
+  int key_place[NK], value_place[8];
+#pragma unroll
+  for (int k = 0; k < NK; ++k) key_place[k] = 16 * key_at<D>(key_row, 2 * k + g);
+#pragma unroll
+  for (int c = 0; c < 8; ++c) value_place[c] = 16 * value_at(r, c ^ (2 * g));
+  const char* key_base = reinterpret_cast<const char*>(keys);
+  const char* value_base = reinterpret_cast<const char*>(values);
   int stage = 0;
   for (int token = from; token < to; token += kTile, stage ^= 1) {
     const bool more = token + kTile < to;
@@ -670,67 +722,87 @@ __global__ __launch_bounds__(256, 2) void attention_tile_kernel(AttentionArgs a)
       for (int i = 0; i < 2; ++i) {
         z[i] = zeros16();
 #pragma unroll
-        for (int k = 0; k < NK; ++k)
-          z[i] = __builtin_amdgcn_mfma_f32_32x32x16_f16(keys[stage][key_at<D>(32 * i + key_row, 2 * k + g)], q[k], z[i], 0, 0, 0);
+        for (int k = 0; k < NK; ++k) {
+          const f16x8_t key = *reinterpret_cast<const f16x8_t*>(key_base + key_place[k] + 32 * i * D * 2);
+          z[i] = __builtin_amdgcn_mfma_f32_32x32x16_f16(key, q[k], z[i], 0, 0, 0);
+        }
       }
       float4 sc[2];
-      float x_unit[2], top = kLow;
+      float unit_k[2], shift[2];
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
         sc[i] = scales[stage][2 * i + g];
-        x_unit[i] = unit * sc[i].x;
+        unit_k[i] = not_zero(unit * sc[i].x);
+        shift[i] = __builtin_fmaf(-bias, unit_k[i], sc[i].y);
       }
-      const bool whole = token >= all_lo && token + kTile <= all_hi && !__any(sc[0].w * sc[1].w == 0.0f);
+      if (token < all_lo || token + kTile > all_hi || __any(sc[0].w * sc[1].w == 0.0f)) {
 #pragma unroll
-      for (int i = 0; i < 2; ++i)
-#pragma unroll
-        for (int e = 0; e < 16; ++e) {
-          z[i][e] = __builtin_fmaf(z[i][e], x_unit[i], sc[i].y);
-          if (!whole) {
-            const int at = token + 32 * i + 16 * g + e;
-            z[i][e] = sc[i].w != 0.0f && at >= col.lo && at < col.hi ? z[i][e] : -__builtin_inff();
+        for (int i = 0; i < 2; ++i) {
+          const int at = token + 32 * i + 16 * g, lo = col.lo - at, hi = sc[i].w != 0.0f ? col.hi - at : 0;
+          if (max(lo, 0) >= min(hi, 16)) {  // nothing of the page: nor of its scales, whatever they are
+            unit_k[i] = 1.0f;
+            shift[i] = 0.0f;
           }
-          top = fmaxf(top, z[i][e]);
+#pragma unroll
+          for (int e = 0; e < 16; ++e) z[i][e] = e >= lo && e < hi ? z[i][e] : -__builtin_inff();
         }
-      if (__any(top > m + kSlack)) {
+      }
+      f16x8_t w[2][2];
+      float sum[2];
+      auto weigh = [&] {
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const float low = shift[i] - m;
+#pragma unroll
+          for (int e = 0; e < 16; ++e) {
+            const float p = exp2_fast(__builtin_fmaf(z[i][e], unit_k[i], low));
+            sum[i] = e ? sum[i] + p : p;  // fp32 weights: beside large value scales a small page's leave a half's range
+            w[i][e / 8][e % 8] = (_Float16)p;
+          }
+        }
+      };
+      weigh();
+      if (__any(sum[0] > kMost || sum[1] > kMost)) {
+        float top = m;
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+#pragma unroll
+          for (int e = 0; e < 16; ++e) top = fmaxf(top, __builtin_fmaf(z[i][e], unit_k[i], shift[i]));
         top = fmaxf(top, __shfl_xor(top, 32, kWave));
-        const float grown = fmaxf(m, top), less = exp2_fast(m - grown);
-        m = grown;
+        const float less = exp2_fast(m - top);
+        m = top;
         l *= less;
 #pragma unroll
         for (int n = 0; n < NV; ++n)
 #pragma unroll
           for (int e = 0; e < 16; ++e) o[n][e] *= less;
+        weigh();
       }
-      f16x8_t w[2][2];
+      // A page that a column sees nothing of adds nothing, whatever its scale.
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        float sum = 0.0f;
-#pragma unroll
-        for (int e = 0; e < 16; ++e) {
-          const float p = exp2_fast(z[i][e] - m);
-          sum += p;
-          w[i][e / 8][e % 8] = (_Float16)p;
-        }
-        // A page that a column sees nothing of adds nothing, whatever its scale.
-        l = sum == 0.0f ? l : __builtin_fmaf(sum, sc[i].z, l);
-      }
+      for (int i = 0; i < 2; ++i) l = sum[i] == 0.0f ? l : __builtin_fmaf(sum[i], sc[i].z, l);
 #pragma unroll
       for (int n = 0; n < NV; ++n)
 #pragma unroll
         for (int i = 0; i < 2; ++i)
 #pragma unroll
-          for (int h = 0; h < 2; ++h)
-            o[n] = __builtin_amdgcn_mfma_f32_32x32x16_f16(values[stage][value_at(32 * n + r, 4 * i + 2 * g + h)], w[i][h], o[n], 0, 0, 0);
+          for (int h = 0; h < 2; ++h) {
+            const f16x8_t value = *reinterpret_cast<const f16x8_t*>(value_base + value_place[(4 * i + h) ^ (2 * n & 7)] + 32 * 128 * n);
+            o[n] = __builtin_amdgcn_mfma_f32_32x32x16_f16(value, w[i][h], o[n], 0, 0, 0);
+          }
     }
     if (more) St::store(staged, keys[stage ^ 1], values[stage ^ 1], scales[stage ^ 1]);
+#pragma unroll
+    for (int k = 0; k < NK; ++k) key_place[k] ^= STAGE;
+#pragma unroll
+    for (int c = 0; c < 8; ++c) value_place[c] ^= STAGE;
     __syncthreads();
   }
 
   l += __shfl_xor(l, 32, kWave);
   if (!col.real) return;
   if (it.parts == 1) {
-    const float inverse = l == 0.0f ? 0.0f : 1.0f / l;
+    const float inverse = l == 0.0f ? 0.0f : kValueUnit / l;
     uint16_t* out = a.out + ((int64_t)col.row * a.heads + col.head) * D;
 #pragma unroll
     for (int n = 0; n < NV; ++n)
@@ -798,7 +870,7 @@ __global__ __launch_bounds__(256) void attention_join_kernel(AttentionArgs a, in
         v.x += o.x, v.y += o.y, v.z += o.z, v.w += o.w;
       }
     }
-    const float inverse = total == 0.0f ? 0.0f : 1.0f / total;
+    const float inverse = total == 0.0f ? 0.0f : kValueUnit / total;
     const float x[4] = {v.x * inverse, v.y * inverse, v.z * inverse, v.w * inverse};
     const int row = info.x + column / a.group, head = kv_head * a.group + column % a.group;
     put_out4<F16>(a.out + ((int64_t)row * a.heads + head) * D + d, x);

@@ -44,18 +44,20 @@ __device__ __forceinline__ int kv_page(const KvBatchArgs& a, int b, int token) {
   return (uint32_t)page < (uint32_t)a.pages ? page : -1;
 }
 
-// Codes to half, exactly: with c ^ 0x80 = c + 128 as the low byte of 0x6400 a half
-// reads 1024 + (c + 128), and 1152 less is c. `w` holds four codes already XORed
-// with 0x80; two halves a call, from bytes 0 and 1 or 2 and 3.
-__device__ __forceinline__ f16x2_t minus1152(uint32_t w) {
-  return __builtin_bit_cast(f16x2_t, w) - f16x2_t{(_Float16)1152.0f, (_Float16)1152.0f};
-}
-__device__ __forceinline__ f16x2_t codes_lo(uint32_t w) { return minus1152(__builtin_amdgcn_perm(0x64646464u, w, 0x04010400u)); }
-__device__ __forceinline__ f16x2_t codes_hi(uint32_t w) { return minus1152(__builtin_amdgcn_perm(0x64646464u, w, 0x04030402u)); }
-// Byte n of two words (two keys' codes of one channel).
+// Codes as halves, in words already XORed with 0x80 a byte, where a code c reads c + 128.
+// For keys a byte becomes the subnormal half (c + 128) 2^-24 by itself: one permute for two;
+// what 128 adds to a score follows from the sum of q alone.
+constexpr float kKeyUnit = 0x1p24f;
+__device__ __forceinline__ f16x2_t key_codes_lo(uint32_t w) { return __builtin_bit_cast(f16x2_t, __builtin_amdgcn_perm(0, w, 0x0c010c00u)); }
+__device__ __forceinline__ f16x2_t key_codes_hi(uint32_t w) { return __builtin_bit_cast(f16x2_t, __builtin_amdgcn_perm(0, w, 0x0c030c02u)); }
+// For values byte N of two words (two tokens' codes of one channel), made c 2^-9 exactly by a
+// fused multiply-add; the 128 left in would cost the sums over many tokens their last bits.
+constexpr float kValueUnit = 0x1p9f;
 template <int N>
-__device__ __forceinline__ f16x2_t codes_of(uint32_t a, uint32_t b) {
-  return minus1152(__builtin_amdgcn_perm(b, a, 0x0c000c00u | N | (uint32_t)(4 + N) << 16) | 0x64006400u);
+__device__ __forceinline__ f16x2_t value_codes(uint32_t a, uint32_t b) {
+  const f16x2_t x = __builtin_bit_cast(f16x2_t, __builtin_amdgcn_perm(b, a, 0x0c000c00u | N | (uint32_t)(4 + N) << 16));
+  const f16x2_t up = {(_Float16)0x1p15f, (_Float16)0x1p15f}, down = {(_Float16)-0.25f, (_Float16)-0.25f};
+  return __builtin_elementwise_fma(x, up, down);
 }
 
 }  // namespace tfm
