@@ -326,59 +326,18 @@ __global__ __launch_bounds__(256, NC == 1 ? 3 : 2) void attention_few_kernel(Att
   const KvSeq& s = it.s;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r = lane & 15, g = lane >> 4;
 
-  f16x8_t q[NC][NK];
+  // What the first tile needs is asked for before anything is waited for.
+  uint4 raw[NC][NK];
   Column col[NC];
-  float unit[NC];  // of a product of halves, times scale log2(e)
-  float bias[NC];  // what the keys' 128 adds to one
-  int all_lo = 0, all_hi = s.len;
   const uint32_t flip = a.scale < 0.0f ? 0x80008000u : 0;
 #pragma unroll
   for (int c = 0; c < NC; ++c) {
     col[c] = column_of(a, s, kv_head, it.tile * COLS + 16 * c + r);
-    uint4 raw[NK];
 #pragma unroll
     for (int k = 0; k < NK; ++k)
-      raw[k] = col[c].real ? flip_signs(load16(a.q + col[c].row * a.q_row + col[c].head * a.q_head + (D / 4) * g + 8 * k), flip)
-                           : make_uint4(0, 0, 0, 0);
-    float factor = 1.0f;
-    unit[c] = unit_of(a.scale, 1.0f);
-    if constexpr (!F16) {
-      uint32_t most = 0;
-#pragma unroll
-      for (int k = 0; k < NK; ++k) most = abs_most(raw[k], most);
-      most = max(most, (uint32_t)__shfl_xor((int)most, 16, kWave));
-      most = max(most, (uint32_t)__shfl_xor((int)most, 32, kWave));
-      float inverse;
-      row_factor(most, factor, inverse);
-      unit[c] = unit_of(a.scale, inverse);
-    }
-#pragma unroll
-    for (int k = 0; k < NK; ++k) q[c][k] = q_halves<F16>(raw[k], factor);
-    float sum = 0.0f;
-#pragma unroll
-    for (int k = 0; k < NK; ++k) sum = add_halves(q[c][k], sum);
-    sum += __shfl_xor(sum, 16, kWave);
-    sum += __shfl_xor(sum, 32, kWave);
-    bias[c] = sum * (128.0f / kKeyUnit);
-    all_lo = max(all_lo, col[c].lo);
-    all_hi = min(all_hi, col[c].hi);
+      raw[c][k] = col[c].real ? load16(a.q + col[c].row * a.q_row + col[c].head * a.q_head + (D / 4) * g + 8 * k)
+                              : make_uint4(0, 0, 0, 0);
   }
-#pragma unroll
-  for (int m = 1; m < 16; m <<= 1) {
-    all_lo = max(all_lo, __shfl_xor(all_lo, m, kWave));
-    all_hi = min(all_hi, __shfl_xor(all_hi, m, kWave));
-  }
-
-  float m[NC], l[NC];
-  f32x4_t o[NC][NV];
-#pragma unroll
-  for (int c = 0; c < NC; ++c) {
-    m[c] = kLow;
-    l[c] = 0.0f;
-#pragma unroll
-    for (int n = 0; n < NV; ++n) o[c][n] = f32x4_t{0, 0, 0, 0};
-  }
-
   int from, to;
   part_of(a, s, it, COLS, 32, from, to);
   // Keys of the next tile are asked for when this one's scores are done, values when
@@ -395,6 +354,56 @@ __global__ __launch_bounds__(256, NC == 1 ? 3 : 2) void attention_few_kernel(Att
     few_load_values<D>(a, kv_head, token, page.v, u);
     scale = few_load_scales(a, kv_head, page.v);
   }
+
+  f16x8_t q[NC][NK];
+  float unit[NC];  // of a product of halves, times scale log2(e)
+  float bias[NC];  // what the keys' 128 adds to one
+  int all_lo = 0, all_hi = s.len;
+#pragma unroll
+  for (int c = 0; c < NC; ++c) {
+#pragma unroll
+    for (int k = 0; k < NK; ++k) raw[c][k] = flip_signs(raw[c][k], flip);
+    float factor = 1.0f;
+    unit[c] = unit_of(a.scale, 1.0f);
+    if constexpr (!F16) {
+      uint32_t most = 0;
+#pragma unroll
+      for (int k = 0; k < NK; ++k) most = abs_most(raw[c][k], most);
+      most = max(most, (uint32_t)__shfl_xor((int)most, 16, kWave));
+      most = max(most, (uint32_t)__shfl_xor((int)most, 32, kWave));
+      float inverse;
+      row_factor(most, factor, inverse);
+      unit[c] = unit_of(a.scale, inverse);
+    }
+#pragma unroll
+    for (int k = 0; k < NK; ++k) q[c][k] = q_halves<F16>(raw[c][k], factor);
+    float sum = 0.0f;
+#pragma unroll
+    for (int k = 0; k < NK; ++k) sum = add_halves(q[c][k], sum);
+    sum += __shfl_xor(sum, 16, kWave);
+    sum += __shfl_xor(sum, 32, kWave);
+    bias[c] = sum * (128.0f / kKeyUnit);
+    all_lo = max(all_lo, col[c].lo);
+    all_hi = min(all_hi, col[c].hi);
+  }
+#pragma unroll
+  for (int m = 1; m < 16; m <<= 1) {
+    all_lo = max(all_lo, __shfl_xor(all_lo, m, kWave));
+    all_hi = min(all_hi, __shfl_xor(all_hi, m, kWave));
+  }
+  all_lo = __builtin_amdgcn_readfirstlane(all_lo);
+  all_hi = __builtin_amdgcn_readfirstlane(all_hi);
+
+  float m[NC], l[NC];
+  f32x4_t o[NC][NV];
+#pragma unroll
+  for (int c = 0; c < NC; ++c) {
+    m[c] = kLow;
+    l[c] = 0.0f;
+#pragma unroll
+    for (int n = 0; n < NV; ++n) o[c][n] = f32x4_t{0, 0, 0, 0};
+  }
+
   for (; token < to; token += 128) {
     const bool more = token + 128 < to;
     // Scores: keys 8 g + 4 i + e of the tile in element e of half i.
@@ -421,6 +430,7 @@ __global__ __launch_bounds__(256, NC == 1 ? 3 : 2) void attention_few_kernel(Att
     for (int c = 0; c < NC; ++c) {
       float unit_k = not_zero(unit[c] * scale.x), shift = __builtin_fmaf(-bias[c], unit_k, lv);
       if (!whole) {
+        asm volatile("");  // a branch, not selects
         const int lo = col[c].lo - token - 8 * g, hi = there ? col[c].hi - token - 8 * g : 0;
         if (max(lo, 0) >= min(hi, 8)) {  // nothing of the page: nor of its scales, whatever they are
           unit_k = 1.0f;
@@ -648,15 +658,27 @@ __global__ __launch_bounds__(256, 2) void attention_tile_kernel(AttentionArgs a)
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r = lane & 31, g = lane >> 5;
 
   const Column col = column_of(a, s, kv_head, it.tile * COLS + 32 * wave + r);
-  f16x8_t q[NK];  // channels 16 k + 8 g ..
+  // What the first tile needs is asked for before anything is waited for.
+  uint4 u[NK];  // channels 16 k + 8 g ..
+#pragma unroll
+  for (int k = 0; k < NK; ++k)
+    u[k] = col.real ? load16(a.q + col.row * a.q_row + col.head * a.q_head + 16 * k + 8 * g) : make_uint4(0, 0, 0, 0);
+  int from, to;
+  part_of(a, s, it, COLS, kTile, from, to);
+  using St = Stage<D>;
+  Staged<D> staged;
+  typename St::Pages next;
+  if (from < to) {
+    const typename St::Pages pages = St::pages(a, it.b, from);
+    next = St::pages(a, it.b, from + kTile);
+    St::load(a, kv_head, from, pages, staged);
+  }
+  f16x8_t q[NK];
   float unit = unit_of(a.scale, 1.0f), bias = 0.0f;  // of a product of halves; what the keys' 128 adds to one
   {
     const uint32_t flip = a.scale < 0.0f ? 0x80008000u : 0;
-    uint4 u[NK];
 #pragma unroll
-    for (int k = 0; k < NK; ++k)
-      u[k] = col.real ? flip_signs(load16(a.q + col.row * a.q_row + col.head * a.q_head + 16 * k + 8 * g), flip)
-                      : make_uint4(0, 0, 0, 0);
+    for (int k = 0; k < NK; ++k) u[k] = flip_signs(u[k], flip);
     float factor = 1.0f;
     if constexpr (!F16) {
       uint32_t most = 0;
@@ -681,6 +703,10 @@ __global__ __launch_bounds__(256, 2) void attention_tile_kernel(AttentionArgs a)
     any_lo = min(any_lo, __shfl_xor(any_lo, m, kWave));
     any_hi = max(any_hi, __shfl_xor(any_hi, m, kWave));
   }
+  all_lo = __builtin_amdgcn_readfirstlane(all_lo);
+  all_hi = __builtin_amdgcn_readfirstlane(all_hi);
+  any_lo = __builtin_amdgcn_readfirstlane(any_lo);
+  any_hi = __builtin_amdgcn_readfirstlane(any_hi);
   // The key row that this lane's row of a product stands for: lanes of half g then hold tokens 16 g .. in order.
   const int key_row = 16 * (r >> 2 & 1) + 4 * (r >> 3) + (r & 3);
 
@@ -689,16 +715,7 @@ __global__ __launch_bounds__(256, 2) void attention_tile_kernel(AttentionArgs a)
 #pragma unroll
   for (int n = 0; n < NV; ++n) o[n] = zeros16();
 
-  int from, to;
-  part_of(a, s, it, COLS, kTile, from, to);
-  using St = Stage<D>;
-  Staged<D> staged;
-  typename St::Pages next;
-  if (from < to) {
-    St::load(a, kv_head, from, St::pages(a, it.b, from), staged);
-    next = St::pages(a, it.b, from + kTile);
-    St::store(staged, keys[0], values[0], scales[0]);
-  }
+  if (from < to) St::store(staged, keys[0], values[0], scales[0]);
   __syncthreads();
   // Places of this lane's operands, in bytes: an XOR away from each other, and the other stage's by one more.
   constexpr int STAGE = kTile * D * 2;
@@ -736,6 +753,7 @@ __global__ __launch_bounds__(256, 2) void attention_tile_kernel(AttentionArgs a)
         shift[i] = __builtin_fmaf(-bias, unit_k[i], sc[i].y);
       }
       if (token < all_lo || token + kTile > all_hi || __any(sc[0].w * sc[1].w == 0.0f)) {
+        asm volatile("");  // a branch: as selects this would be most of the tile's instructions
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
           const int at = token + 32 * i + 16 * g, lo = col.lo - at, hi = sc[i].w != 0.0f ? col.hi - at : 0;
