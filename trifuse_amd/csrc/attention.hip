@@ -235,6 +235,17 @@ __device__ __forceinline__ void put_out4(uint16_t* p, const float* v) {
   *reinterpret_cast<uint2*>(p) = make_uint2(pack_st2<F16>(v[0], v[1]), pack_st2<F16>(v[2], v[3]));
 }
 
+// The table's entry for a token of the sequence whose row it is; past the table's end, the
+// last (no row sees such a token). It is looked at only where it is used: with a check here
+// each load would be waited for on the spot, and all loads before it.
+__device__ __forceinline__ int entry_of(const KvBatchArgs& g, const int32_t* row, int token) {
+  return row[min(token >> g.page_shift, g.table_width - 1)];
+}
+__device__ __forceinline__ bool is_page(const KvBatchArgs& g, int id) { return (uint32_t)id < (uint32_t)g.pages; }
+__device__ __forceinline__ int64_t place_of(const KvBatchArgs& g, int id, int kv_head) {
+  return (int64_t)(is_page(g, id) ? id : 0) * g.kv_heads + kv_head;
+}
+
 // ---- few columns -------------------------------------------------------------
 
 // 32 tokens of a wave, as loaded: lane (r = lane % 16, g = lane / 16) has bytes
@@ -248,18 +259,18 @@ struct FewValues {
   uint32_t v[8][D / 64];
 };
 struct FewPages {
-  int k, v;  // of this lane's key rows and value rows; -1: none
+  int k, v;  // table entries of this lane's key rows and value rows
 };
-__device__ __forceinline__ FewPages few_pages(const AttentionArgs& a, int b, int token) {
+__device__ __forceinline__ FewPages few_pages(const AttentionArgs& a, const int32_t* table, int token) {
   const int lane = threadIdx.x & 63, r = lane & 15, q = lane >> 4;
-  return FewPages{kv_page(a.b, b, token + 8 * (r >> 2)), kv_page(a.b, b, token + 8 * q)};
+  return FewPages{entry_of(a.b, table, token + 8 * (r >> 2)), entry_of(a.b, table, token + 8 * q)};
 }
 template <int D>
 __device__ __forceinline__ void few_load_keys(const AttentionArgs& a, int kv_head, int token, int page, FewKeys<D>& t) {
   const KvBatchArgs& g = a.b;
   const int lane = threadIdx.x & 63, r = lane & 15, q = lane >> 4;
   const int at = token + 8 * (r >> 2) + (r & 3);
-  const int64_t place = (int64_t)max(page, 0) * g.kv_heads + kv_head;
+  const int64_t place = place_of(g, page, kv_head);
   const int8_t* k = g.k + ((place << g.page_shift) + (at & ((1 << g.page_shift) - 1))) * D + (D / 4) * q;
 #pragma unroll
   for (int i = 0; i < 2; ++i)
@@ -271,7 +282,7 @@ __device__ __forceinline__ void few_load_values(const AttentionArgs& a, int kv_h
   const KvBatchArgs& g = a.b;
   const int lane = threadIdx.x & 63, r = lane & 15, q = lane >> 4;
   const int at = token + 8 * q;
-  const int64_t place = (int64_t)max(page, 0) * g.kv_heads + kv_head;
+  const int64_t place = place_of(g, page, kv_head);
   const int8_t* v = g.v + ((place << g.page_shift) + (at & ((1 << g.page_shift) - 1))) * D + (D / 16) * r;
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
@@ -286,7 +297,7 @@ __device__ __forceinline__ void few_load_values(const AttentionArgs& a, int kv_h
 }
 // The scales of the page that tokens 8 g .. lie in.
 __device__ __forceinline__ float2 few_load_scales(const AttentionArgs& a, int kv_head, int page) {
-  const int64_t place = (int64_t)max(page, 0) * a.b.kv_heads + kv_head;
+  const int64_t place = place_of(a.b, page, kv_head);
   return make_float2(a.b.k_scales[place], a.b.v_scales[place]);
 }
 
@@ -342,14 +353,15 @@ __global__ __launch_bounds__(256, NC == 1 ? 3 : 2) void attention_few_kernel(Att
   part_of(a, s, it, COLS, 32, from, to);
   // Keys of the next tile are asked for when this one's scores are done, values when
   // they are weighed; page numbers a tile earlier.
+  const int32_t* table = a.b.table + (int64_t)it.b * a.b.table_width;
   FewKeys<D> t;
   FewValues<D> u;
   FewPages page{-1, -1}, next{-1, -1};
   float2 scale{};
   int token = from + 32 * wave;
   if (token < to) {
-    page = few_pages(a, it.b, token);
-    next = few_pages(a, it.b, token + 128);
+    page = few_pages(a, table, token);
+    next = few_pages(a, table, token + 128);
     few_load_keys<D>(a, kv_head, token, page.k, t);
     few_load_values<D>(a, kv_head, token, page.v, u);
     scale = few_load_scales(a, kv_head, page.v);
@@ -424,7 +436,7 @@ __global__ __launch_bounds__(256, NC == 1 ? 3 : 2) void attention_few_kernel(Att
     }
     if (more) few_load_keys<D>(a, kv_head, token + 128, next.k, t);
     const float lv = __builtin_amdgcn_logf(scale.y), inverse = __builtin_amdgcn_rcpf(scale.y);
-    const bool there = page.v >= 0, whole = token >= all_lo && token + 32 <= all_hi && !__any(!there);
+    const bool there = is_page(a.b, page.v), whole = token >= all_lo && token + 32 <= all_hi && !__any(!there);
     f16x8_t w[NC];
 #pragma unroll
     for (int c = 0; c < NC; ++c) {
@@ -477,7 +489,7 @@ __global__ __launch_bounds__(256, NC == 1 ? 3 : 2) void attention_few_kernel(Att
       few_load_values<D>(a, kv_head, token + 128, next.v, u);
       scale = few_load_scales(a, kv_head, next.v);
       page = next;
-      next = few_pages(a, it.b, token + 256);
+      next = few_pages(a, table, token + 256);
     }
   }
 
@@ -548,86 +560,83 @@ __device__ __forceinline__ int value_at(int channel, int chunk) {
   return channel * 8 + (chunk ^ (((channel >> 1) ^ (channel >> 4)) & 7));
 }
 
-// What a thread brings of a tile: 16-byte pieces of key rows, and four channels of
-// eight value rows. With 64 channels waves 0 and 1 bring values, 2 and 3 keys.
+// What a wave brings of a tile: 16 of its tokens, which lie in one page, behind each other.
+// Lanes take 16-byte pieces of key rows, and eight channels of D/32 value rows each: few and
+// wide loads, since a compute unit takes about 12 cycles for each.
 template <int D>
 struct Staged {
-  uint4 k[2];
-  uint32_t v[8];
+  uint4 k[D / 64];
+  uint2 v[D / 32];
   float ks, vs;
   bool there;
 };
 
 template <int D>
 struct Stage {
-  __device__ static bool keys() { return D == 128 || threadIdx.x >= 128; }
-  __device__ static bool values() { return D == 128 || threadIdx.x < 128; }
-  __device__ static int key_piece(int i) { return D == 128 ? threadIdx.x + 256 * i : (threadIdx.x & 127) + 128 * i; }
-  __device__ static int octet() { return threadIdx.x / (D / 4); }
-  __device__ static int quad() { return threadIdx.x % (D / 4); }
+  static constexpr int ROWS = D / 32;     // value rows a lane
+  static constexpr int LOADS = D / 64 + ROWS;
+  static constexpr int KEY_UNITS = D / 32;  // 16-byte chunks of halves a lane
+  __device__ static int lane() { return threadIdx.x & 63; }
+  __device__ static int wave() { return __builtin_amdgcn_readfirstlane(threadIdx.x >> 6); }
 
-  struct Pages {
-    int k[2], v, s;
-  };
-  __device__ static Pages pages(const AttentionArgs& a, int b, int token) {
-    Pages p;
-#pragma unroll
-    for (int i = 0; i < 2; ++i) p.k[i] = keys() ? kv_page(a.b, b, token + key_piece(i) / (D / 16)) : -1;
-    p.v = values() ? kv_page(a.b, b, token + 8 * octet()) : -1;
-    p.s = threadIdx.x < 4 ? kv_page(a.b, b, token + 16 * threadIdx.x) : -1;
-    return p;
+  // Where the 16 tokens from `token` on start in a page whose table entry is `id`, in bytes of either array.
+  __device__ static int64_t start(const AttentionArgs& a, int kv_head, int token, int id) {
+    return ((place_of(a.b, id, kv_head) << a.b.page_shift) + (token & ((1 << a.b.page_shift) - 1))) * D;
   }
-  __device__ static void load(const AttentionArgs& a, int kv_head, int token, const Pages& p, Staged<D>& t) {
-    const KvBatchArgs& g = a.b;
-    const int mask = (1 << g.page_shift) - 1;
-    if (keys()) {
-#pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        const int piece = key_piece(i), at = token + piece / (D / 16);
-        const int64_t place = (int64_t)max(p.k[i], 0) * g.kv_heads + kv_head;
-        t.k[i] = *reinterpret_cast<const uint4*>(g.k + ((place << g.page_shift) + (at & mask)) * D + 16 * (piece % (D / 16)));
-      }
-    }
-    if (values()) {
-      const int at = token + 8 * octet();
-      const int64_t place = (int64_t)max(p.v, 0) * g.kv_heads + kv_head;
-      const int8_t* v = g.v + ((place << g.page_shift) + (at & mask)) * D + 4 * quad();
-#pragma unroll
-      for (int j = 0; j < 8; ++j) t.v[j] = *reinterpret_cast<const uint32_t*>(v + j * D);
-    }
-    if (threadIdx.x < 4) {
-      const int64_t place = (int64_t)max(p.s, 0) * g.kv_heads + kv_head;
-      t.ks = g.k_scales[place];
-      t.vs = g.v_scales[place];
-      t.there = p.s >= 0;
-    }
+  __device__ static void load(const AttentionArgs& a, int64_t at, int piece, Staged<D>& t) {
+    if (piece < D / 64)
+      t.k[piece] = *reinterpret_cast<const uint4*>(a.b.k + at + 1024 * piece + 16 * lane());
+    else if (piece < LOADS)
+      t.v[piece - D / 64] = *reinterpret_cast<const uint2*>(a.b.v + at + (lane() / (D / 8) * ROWS + piece - D / 64) * D +
+                                                            8 * (lane() % (D / 8)));
   }
-  // float4 of granule (16 tokens): key scale, log2 of the value scale, its inverse, whether there is a page.
+  __device__ static void load_scales(const AttentionArgs& a, int kv_head, int id, Staged<D>& t) {
+    const int64_t place = place_of(a.b, id, kv_head);
+    t.ks = a.b.k_scales[place];
+    t.vs = a.b.v_scales[place];
+    t.there = is_page(a.b, id);
+  }
+  // Pieces on their way to a stage: unit of KEY_UNITS of keys, channel of 8 of values.
+  __device__ static void store_keys(const Staged<D>& t, int unit, f16x8_t* to) {
+    constexpr int lanes = D / 16;  // of a row
+    const int h = unit % 2, token = 16 * wave() + unit / 2 * (64 / lanes) + lane() / lanes, chunk = 2 * (lane() % lanes) + h;
+    const uint32_t w0 = word_of(t.k[unit / 2], 2 * h) ^ 0x80808080u, w1 = word_of(t.k[unit / 2], 2 * h + 1) ^ 0x80808080u;
+    const f16x2_t c[4] = {key_codes_lo(w0), key_codes_hi(w0), key_codes_lo(w1), key_codes_hi(w1)};
+    to[key_at<D>(token, chunk)] = __builtin_bit_cast(f16x8_t, c);
+  }
+  template <int N>
+  __device__ static void store_value(const Staged<D>& t, f16x8_t* to) {
+    const int channel = 8 * (lane() % (D / 8)) + N, token = ROWS * (lane() / (D / 8));  // of the wave's 16
+    f16x2_t c[ROWS / 2];
+#pragma unroll
+    for (int j = 0; j < ROWS / 2; ++j) {
+      const uint32_t x = N < 4 ? t.v[2 * j].x : t.v[2 * j].y, y = N < 4 ? t.v[2 * j + 1].x : t.v[2 * j + 1].y;
+      c[j] = value_codes<N % 4>(x ^ 0x80808080u, y ^ 0x80808080u);
+    }
+    f16x8_t* chunk = to + value_at(channel, 2 * wave() + token / 8);
+    __builtin_memcpy(reinterpret_cast<char*>(chunk) + token % 8 * 2, c, sizeof c);
+  }
+  __device__ static void store_values(const Staged<D>& t, int channel, f16x8_t* to) {
+    if (channel == 0) store_value<0>(t, to);
+    if (channel == 1) store_value<1>(t, to);
+    if (channel == 2) store_value<2>(t, to);
+    if (channel == 3) store_value<3>(t, to);
+    if (channel == 4) store_value<4>(t, to);
+    if (channel == 5) store_value<5>(t, to);
+    if (channel == 6) store_value<6>(t, to);
+    if (channel == 7) store_value<7>(t, to);
+  }
+  // float4 of the wave's 16 tokens: key scale, log2 of the value scale, its inverse, whether there is a page.
+  __device__ static void store_scales(const Staged<D>& t, float4* to) {
+    if (lane() == 0)
+      to[wave()] = make_float4(t.ks, __builtin_amdgcn_logf(t.vs), __builtin_amdgcn_rcpf(t.vs), t.there ? 1.0f : 0.0f);
+  }
   __device__ static void store(const Staged<D>& t, f16x8_t* keys_to, f16x8_t* values_to, float4* scales) {
-    if (keys()) {
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        const int piece = key_piece(i), token = piece / (D / 16), chunk = 2 * (piece % (D / 16));
+    for (int unit = 0; unit < KEY_UNITS; ++unit) store_keys(t, unit, keys_to);
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          const uint32_t w0 = word_of(t.k[i], 2 * h) ^ 0x80808080u, w1 = word_of(t.k[i], 2 * h + 1) ^ 0x80808080u;
-          const f16x2_t c[4] = {key_codes_lo(w0), key_codes_hi(w0), key_codes_lo(w1), key_codes_hi(w1)};
-          keys_to[key_at<D>(token, chunk + h)] = __builtin_bit_cast(f16x8_t, c);
-        }
-      }
-    }
-    if (values()) {
-      uint32_t x[8][1];
-#pragma unroll
-      for (int j = 0; j < 8; ++j) x[j][0] = t.v[j] ^ 0x80808080u;
-      const int channel = 4 * quad(), chunk = octet();
-      values_to[value_at(channel, chunk)] = few_values<0>(x);
-      values_to[value_at(channel + 1, chunk)] = few_values<1>(x);
-      values_to[value_at(channel + 2, chunk)] = few_values<2>(x);
-      values_to[value_at(channel + 3, chunk)] = few_values<3>(x);
-    }
-    if (threadIdx.x < 4)
-      scales[threadIdx.x] = make_float4(t.ks, __builtin_amdgcn_logf(t.vs), __builtin_amdgcn_rcpf(t.vs), t.there ? 1.0f : 0.0f);
+    for (int channel = 0; channel < 8; ++channel) store_values(t, channel, values_to);
+    store_scales(t, scales);
   }
 };
 
@@ -665,13 +674,21 @@ __global__ __launch_bounds__(256, 2) void attention_tile_kernel(AttentionArgs a)
     u[k] = col.real ? load16(a.q + col.row * a.q_row + col.head * a.q_head + 16 * k + 8 * g) : make_uint4(0, 0, 0, 0);
   int from, to;
   part_of(a, s, it, COLS, kTile, from, to);
+  const int32_t* table = a.b.table + (int64_t)it.b * a.b.table_width;
   using St = Stage<D>;
   Staged<D> staged;
-  typename St::Pages next;
+  const int mine = 16 * St::wave();  // of a tile's tokens, those that this wave brings
+  // Table entry of the next tile's, one for the wave, but in a vector register: as a scalar
+  // it would be waited for where it is loaded.
+  int next = 0, mine_v = mine;
+  asm("" : "+v"(mine_v));
   if (from < to) {
-    const typename St::Pages pages = St::pages(a, it.b, from);
-    next = St::pages(a, it.b, from + kTile);
-    St::load(a, kv_head, from, pages, staged);
+    const int id = entry_of(a.b, table, from + mine);
+    next = entry_of(a.b, table, from + kTile + mine_v);
+    const int64_t at = St::start(a, kv_head, from + mine, id);
+#pragma unroll
+    for (int i = 0; i < St::LOADS; ++i) St::load(a, at, i, staged);
+    St::load_scales(a, kv_head, id, staged);
   }
   f16x8_t q[NK];
   float unit = unit_of(a.scale, 1.0f), bias = 0.0f;  // of a product of halves; what the keys' 128 adds to one
@@ -728,88 +745,127 @@ __global__ __launch_bounds__(256, 2) void attention_tile_kernel(AttentionArgs a)
   const char* value_base = reinterpret_cast<const char*>(values);
   int stage = 0;
   for (int token = from; token < to; token += kTile, stage ^= 1) {
-    const bool more = token + kTile < to;
-    if (more) {
-      St::load(a, kv_head, token + kTile, next, staged);
-      next = St::pages(a, it.b, token + 2 * kTile);
-    }
+    // The next tile's loads (behind the last one's, its own again, which nobody uses).
+    const int ahead = token + kTile < to ? token + kTile : token;
+    const int id = __builtin_amdgcn_readfirstlane(next);
+    const int64_t at = St::start(a, kv_head, ahead + mine, id);
+    St::load_scales(a, kv_head, id, staged);
+    next = entry_of(a.b, table, ahead + kTile + mine_v);
+    f16x8_t* keys_to = keys[stage ^ 1];
+    f16x8_t* values_to = values[stage ^ 1];
     if (token < any_hi && token + kTile > any_lo) {  // else no column of the wave sees the tile
-      f32x16_t z[2];
-#pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        z[i] = zeros16();
-#pragma unroll
-        for (int k = 0; k < NK; ++k) {
-          const f16x8_t key = *reinterpret_cast<const f16x8_t*>(key_base + key_place[k] + 32 * i * D * 2);
-          z[i] = __builtin_amdgcn_mfma_f32_32x32x16_f16(key, q[k], z[i], 0, 0, 0);
+      // Matrix instructions and the rest go side by side, in steps that the scheduler keeps:
+      // the scores of the second 32 tokens beside the weights of the first, those weighed
+      // beside the second weights, those weighed beside the next tile's way into LDS.
+      // Operands are read from LDS four steps ahead.
+      f16x8_t ring[4];
+      auto fetch = [&](int j) {
+        if (j < 2 * NK) {
+          ring[j % 4] = *reinterpret_cast<const f16x8_t*>(key_base + key_place[j % NK] + 32 * (j / NK) * D * 2);
+        } else if (j < 2 * NK + 4 * NV) {
+          const int v = j - 2 * NK, n = v % NV, c = v / NV;  // chunk c = 4 i + h for i, h = v / (2 NV), v / NV % 2
+          ring[j % 4] = *reinterpret_cast<const f16x8_t*>(
+              value_base + value_place[(4 * (c / 2) + c % 2) ^ (2 * n & 7)] + 32 * 128 * n);
         }
-      }
+      };
       float4 sc[2];
-      float unit_k[2], shift[2];
+#pragma unroll
+      for (int i = 0; i < 2; ++i) sc[i] = scales[stage][2 * i + g];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) fetch(j);
+      f32x16_t z[2] = {zeros16(), zeros16()};
+      f16x8_t w[2][2];
+      float unit_k[2], shift[2], sum[2];
+      auto scores = [&](int i, int k) {
+        const int j = i * NK + k;
+        z[i] = __builtin_amdgcn_mfma_f32_32x32x16_f16(ring[j % 4], q[k], z[i], 0, 0, 0);
+        fetch(j + 4);
+      };
+      auto weighed = [&](int i, int v) {
+        const int j = 2 * NK + 2 * NV * i + v;
+        o[v % NV] = __builtin_amdgcn_mfma_f32_32x32x16_f16(ring[j % 4], w[i][v / NV], o[v % NV], 0, 0, 0);
+        fetch(j + 4);
+      };
+      auto weigh = [&](int i, int from_e, int to_e) {
+        const float low = shift[i] - m;
+#pragma unroll
+        for (int e = from_e; e < to_e; ++e) {
+          const float p = exp2_fast(__builtin_fmaf(z[i][e], unit_k[i], low));
+          sum[i] = e ? sum[i] + p : p;  // fp32 weights: beside large value scales a small page's leave a half's range
+          w[i][e / 8][e % 8] = (_Float16)p;
+        }
+      };
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
-        sc[i] = scales[stage][2 * i + g];
         unit_k[i] = not_zero(unit * sc[i].x);
         shift[i] = __builtin_fmaf(-bias, unit_k[i], sc[i].y);
       }
-      if (token < all_lo || token + kTile > all_hi || __any(sc[0].w * sc[1].w == 0.0f)) {
+      const bool partly = token < all_lo || token + kTile > all_hi || __any(sc[0].w * sc[1].w == 0.0f);
+      auto hide = [&](int i) {
+        if (!partly) return;
         asm volatile("");  // a branch: as selects this would be most of the tile's instructions
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          const int at = token + 32 * i + 16 * g, lo = col.lo - at, hi = sc[i].w != 0.0f ? col.hi - at : 0;
-          if (max(lo, 0) >= min(hi, 16)) {  // nothing of the page: nor of its scales, whatever they are
-            unit_k[i] = 1.0f;
-            shift[i] = 0.0f;
-          }
-#pragma unroll
-          for (int e = 0; e < 16; ++e) z[i][e] = e >= lo && e < hi ? z[i][e] : -__builtin_inff();
+        const int at = token + 32 * i + 16 * g, lo = col.lo - at, hi = sc[i].w != 0.0f ? col.hi - at : 0;
+        if (max(lo, 0) >= min(hi, 16)) {  // nothing of the page: nor of its scales, whatever they are
+          unit_k[i] = 1.0f;
+          shift[i] = 0.0f;
         }
-      }
-      f16x8_t w[2][2];
-      float sum[2];
-      auto weigh = [&] {
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          const float low = shift[i] - m;
-#pragma unroll
-          for (int e = 0; e < 16; ++e) {
-            const float p = exp2_fast(__builtin_fmaf(z[i][e], unit_k[i], low));
-            sum[i] = e ? sum[i] + p : p;  // fp32 weights: beside large value scales a small page's leave a half's range
-            w[i][e / 8][e % 8] = (_Float16)p;
-          }
-        }
+        for (int e = 0; e < 16; ++e) z[i][e] = e >= lo && e < hi ? z[i][e] : -__builtin_inff();
       };
-      weigh();
-      if (__any(sum[0] > kMost || sum[1] > kMost)) {
-        float top = m;
-#pragma unroll
-        for (int i = 0; i < 2; ++i)
+      auto settle = [&](int i) {
+        if (__any(sum[i] > kMost)) {
+          float top = m;
 #pragma unroll
           for (int e = 0; e < 16; ++e) top = fmaxf(top, __builtin_fmaf(z[i][e], unit_k[i], shift[i]));
-        top = fmaxf(top, __shfl_xor(top, 32, kWave));
-        const float less = exp2_fast(m - top);
-        m = top;
-        l *= less;
+          top = fmaxf(top, __shfl_xor(top, 32, kWave));
+          const float less = exp2_fast(m - top);
+          m = top;
+          l *= less;
 #pragma unroll
-        for (int n = 0; n < NV; ++n)
+          for (int n = 0; n < NV; ++n)
 #pragma unroll
-          for (int e = 0; e < 16; ++e) o[n][e] *= less;
-        weigh();
+            for (int e = 0; e < 16; ++e) o[n][e] *= less;
+          weigh(i, 0, 16);
+        }
+        // A page that a column sees nothing of adds nothing, whatever its scale.
+        l = sum[i] == 0.0f ? l : __builtin_fmaf(sum[i], sc[i].z, l);
+      };
+#pragma unroll
+      for (int k = 0; k < NK; ++k) {
+        scores(0, k);
+        if (k < St::LOADS) St::load(a, at, k, staged);
+        __builtin_amdgcn_sched_barrier(0);
       }
-      // A page that a column sees nothing of adds nothing, whatever its scale.
+      hide(0);
 #pragma unroll
-      for (int i = 0; i < 2; ++i) l = sum[i] == 0.0f ? l : __builtin_fmaf(sum[i], sc[i].z, l);
+      for (int k = 0; k < NK; ++k) {
+        scores(1, k);
+        weigh(0, 16 / NK * k, 16 / NK * (k + 1));
+        __builtin_amdgcn_sched_barrier(0);
+      }
+      settle(0);
+      hide(1);
 #pragma unroll
-      for (int n = 0; n < NV; ++n)
+      for (int v = 0; v < 2 * NV; ++v) {
+        weighed(0, v);
+        weigh(1, 8 / NV * v, 8 / NV * (v + 1));
+        __builtin_amdgcn_sched_barrier(0);
+      }
+      settle(1);
 #pragma unroll
-        for (int i = 0; i < 2; ++i)
+      for (int v = 0; v < 2 * NV; ++v) {
+        weighed(1, v);
+        if (v < St::KEY_UNITS) St::store_keys(staged, v, keys_to);
 #pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            const f16x8_t value = *reinterpret_cast<const f16x8_t*>(value_base + value_place[(4 * i + h) ^ (2 * n & 7)] + 32 * 128 * n);
-            o[n] = __builtin_amdgcn_mfma_f32_32x32x16_f16(value, w[i][h], o[n], 0, 0, 0);
-          }
+        for (int channel = 4 / NV * v; channel < 4 / NV * (v + 1); ++channel) St::store_values(staged, channel, values_to);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+      St::store_scales(staged, scales[stage ^ 1]);
+    } else {
+#pragma unroll
+      for (int i = 0; i < St::LOADS; ++i) St::load(a, at, i, staged);
+      St::store(staged, keys_to, values_to, scales[stage ^ 1]);
     }
-    if (more) St::store(staged, keys[stage ^ 1], values[stage ^ 1], scales[stage ^ 1]);
 #pragma unroll
     for (int k = 0; k < NK; ++k) key_place[k] ^= STAGE;
 #pragma unroll
