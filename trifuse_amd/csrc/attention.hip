@@ -79,10 +79,11 @@ __device__ __forceinline__ int tokens_of(const AttentionArgs& a, const KvSeq& s)
 }
 
 // Item `index` of the batch. Every wave finds it by itself, a sequence a lane. A part's
-// tokens are all of them where the tiles fill the machine by themselves, else the batch's
-// tokens (of every tile) over the items that should run: at most a.target parts more than
-// there are tiles (the sum's fp32 rounding is below the allowance of 2^-18). `tiles` is the
-// batch's number of tiles where they are cut, else 0.
+// tokens are all of them where the tiles fill the card by themselves, else such that there
+// are at most a.target items: the batch's tokens (of every tile) over a.target where that
+// comes out, else over a.target less one a tile, which always does (the sums' fp32 rounding is
+// below the allowance of 2^-18). `tiles_cut` is the batch's number of tiles where they are
+// cut, else 0.
 __device__ Item find_item(const AttentionArgs& a, int columns, int index, int& tiles_cut) {
   const int lane = threadIdx.x & 63;
   auto mine = [&](int b) {
@@ -94,16 +95,22 @@ __device__ Item find_item(const AttentionArgs& a, int columns, int index, int& t
   int chunk = 1 << 30;
   tiles_cut = 0;
   if (a.part_out) {
-    float tiles = 0.0f, tokens = 0.0f;
-    for (int b0 = 0; b0 < a.b.sequences; b0 += kWave) {
-      const KvSeq o = b0 ? mine(b0 + lane) : s;
-      const float t = (float)tiles_of(a, o, columns);
-      tiles += wave_sum(t);
-      tokens += wave_sum(t * (float)tokens_of(a, o));
-    }
+    // Sum over the batch of what f says of a sequence's tiles and tokens.
+    auto over_batch = [&](auto&& f) {
+      float sum = 0.0f;
+      for (int b0 = 0; b0 < a.b.sequences; b0 += kWave) {
+        const KvSeq o = b0 ? mine(b0 + lane) : s;
+        sum += wave_sum(f((float)tiles_of(a, o, columns), tokens_of(a, o)));
+      }
+      return sum;
+    };
+    const float tiles = over_batch([](float t, int) { return t; });
     if (tiles < (float)a.target) {
-      const float even = tokens * (1.0f + 0x1p-18f) / (64.0f * (float)a.target);
-      chunk = max(a.min_chunk, 64 * ((int)fminf(even, 0x1p23f) + 1));
+      const float tokens = over_batch([](float t, int n) { return t * (float)n; }) * (1.0f + 0x1p-18f);
+      auto chunk_for = [&](float parts) { return max(a.min_chunk, 64 * ((int)fminf(tokens / (64.0f * parts), 0x1p23f) + 1)); };
+      chunk = chunk_for((float)a.target);
+      const float items = over_batch([&](float t, int n) { return t * (float)max(1, (n + chunk - 1) / chunk); });
+      if (items > (float)a.target) chunk = chunk_for((float)a.target - tiles);
       tiles_cut = (int)tiles;
     }
   }
@@ -546,17 +553,17 @@ __global__ __launch_bounds__(256, NC == 1 ? 3 : 2) void attention_few_kernel(Att
 
 // ---- many columns ------------------------------------------------------------
 
-// 128 columns a workgroup of four waves; tiles of 64 tokens in two LDS stages as halves:
-// keys [64][D] and values transposed, [D][64], in 16-byte chunks whose places are XORed
-// so that the 16 lanes of one access meet all banks.
-constexpr int kTile = 64;
-
+// 32 columns a wave, WAVES (4 or 8) a workgroup; tiles of 16 tokens a wave in two LDS
+// stages as halves: keys [tokens][D] and values transposed, [D][tokens], in 16-byte chunks
+// whose places are XORed so that the 16 lanes of one access meet all banks.
 template <int D>
 __device__ __forceinline__ int key_at(int token, int chunk) {  // in chunks
   if constexpr (D == 128) return token * 16 + (chunk ^ ((token & 7) | (token >> 4 & 1) << 3));
   return token * 8 + (chunk ^ ((token >> 1 & 3) | (token >> 4 & 1) << 2));
 }
+template <int WAVES>
 __device__ __forceinline__ int value_at(int channel, int chunk) {
+  if constexpr (WAVES == 8) return channel * 16 + (chunk ^ ((channel ^ (channel >> 3)) & 15));
   return channel * 8 + (chunk ^ (((channel >> 1) ^ (channel >> 4)) & 7));
 }
 
@@ -571,7 +578,7 @@ struct Staged {
   bool there;
 };
 
-template <int D>
+template <int D, int WAVES>
 struct Stage {
   static constexpr int ROWS = D / 32;     // value rows a lane
   static constexpr int LOADS = D / 64 + ROWS;
@@ -613,7 +620,7 @@ struct Stage {
       const uint32_t x = N < 4 ? t.v[2 * j].x : t.v[2 * j].y, y = N < 4 ? t.v[2 * j + 1].x : t.v[2 * j + 1].y;
       c[j] = value_codes<N % 4>(x ^ 0x80808080u, y ^ 0x80808080u);
     }
-    f16x8_t* chunk = to + value_at(channel, 2 * wave() + token / 8);
+    f16x8_t* chunk = to + value_at<WAVES>(channel, 2 * wave() + token / 8);
     __builtin_memcpy(reinterpret_cast<char*>(chunk) + token % 8 * 2, c, sizeof c);
   }
   __device__ static void store_values(const Staged<D>& t, int channel, f16x8_t* to) {
@@ -628,8 +635,8 @@ struct Stage {
   }
   // float4 of the wave's 16 tokens: key scale, log2 of the value scale, its inverse, whether there is a page.
   __device__ static void store_scales(const Staged<D>& t, float4* to) {
-    if (lane() == 0)
-      to[wave()] = make_float4(t.ks, __builtin_amdgcn_logf(t.vs), __builtin_amdgcn_rcpf(t.vs), t.there ? 1.0f : 0.0f);
+    // The same from every lane: no branch among the matrix instructions.
+    to[wave()] = make_float4(t.ks, __builtin_amdgcn_logf(t.vs), __builtin_amdgcn_rcpf(t.vs), t.there ? 1.0f : 0.0f);
   }
   __device__ static void store(const Staged<D>& t, f16x8_t* keys_to, f16x8_t* values_to, float4* scales) {
 #pragma unroll
@@ -647,12 +654,13 @@ __device__ __forceinline__ f32x16_t zeros16() {
   return z;
 }
 
-template <bool F16, int D>
-__global__ __launch_bounds__(256, 2) void attention_tile_kernel(AttentionArgs a) {
-  constexpr int COLS = 128, NK = D / 16, NV = D / 32;
-  __shared__ f16x8_t keys[2][kTile * D / 8];
-  __shared__ f16x8_t values[2][kTile * D / 8];
-  __shared__ float4 scales[2][4];
+template <bool F16, int D, int WAVES>
+__global__ __launch_bounds__(64 * WAVES, 2) void attention_tile_kernel(AttentionArgs a) {
+  constexpr int COLS = 32 * WAVES, NK = D / 16, NV = D / 32;
+  constexpr int TILE = 16 * WAVES, SUBS = TILE / 64;  // tokens, worked on 64 at a time
+  __shared__ f16x8_t keys[2][TILE * D / 8];
+  __shared__ f16x8_t values[2][TILE * D / 8];
+  __shared__ float4 scales[2][WAVES];
   const int kv_head = blockIdx.x % a.b.kv_heads;
   int tiles_cut;
   Item it = find_item(a, COLS, blockIdx.x / a.b.kv_heads, tiles_cut);
@@ -673,9 +681,9 @@ __global__ __launch_bounds__(256, 2) void attention_tile_kernel(AttentionArgs a)
   for (int k = 0; k < NK; ++k)
     u[k] = col.real ? load16(a.q + col.row * a.q_row + col.head * a.q_head + 16 * k + 8 * g) : make_uint4(0, 0, 0, 0);
   int from, to;
-  part_of(a, s, it, COLS, kTile, from, to);
+  part_of(a, s, it, COLS, TILE, from, to);
   const int32_t* table = a.b.table + (int64_t)it.b * a.b.table_width;
-  using St = Stage<D>;
+  using St = Stage<D, WAVES>;
   Staged<D> staged;
   const int mine = 16 * St::wave();  // of a tile's tokens, those that this wave brings
   // Table entry of the next tile's, one for the wave, but in a vector register: as a scalar
@@ -684,7 +692,7 @@ __global__ __launch_bounds__(256, 2) void attention_tile_kernel(AttentionArgs a)
   asm("" : "+v"(mine_v));
   if (from < to) {
     const int id = entry_of(a.b, table, from + mine);
-    next = entry_of(a.b, table, from + kTile + mine_v);
+    next = entry_of(a.b, table, from + TILE + mine_v);
     const int64_t at = St::start(a, kv_head, from + mine, id);
 #pragma unroll
     for (int i = 0; i < St::LOADS; ++i) St::load(a, at, i, staged);
@@ -735,25 +743,45 @@ __global__ __launch_bounds__(256, 2) void attention_tile_kernel(AttentionArgs a)
   if (from < to) St::store(staged, keys[0], values[0], scales[0]);
   __syncthreads();
   // Places of this lane's operands, in bytes: an XOR away from each other, and the other stage's by one more.
-  constexpr int STAGE = kTile * D * 2;
+  constexpr int STAGE = TILE * D * 2;
   int key_place[NK], value_place[8];
 #pragma unroll
   for (int k = 0; k < NK; ++k) key_place[k] = 16 * key_at<D>(key_row, 2 * k + g);
 #pragma unroll
-  for (int c = 0; c < 8; ++c) value_place[c] = 16 * value_at(r, c ^ (2 * g));
+  for (int c = 0; c < 8; ++c) value_place[c] = 16 * value_at<WAVES>(r, (WAVES == 8 ? c / 2 * 4 + c % 2 : c) ^ (2 * g));
   const char* key_base = reinterpret_cast<const char*>(keys);
   const char* value_base = reinterpret_cast<const char*>(values);
   int stage = 0;
-  for (int token = from; token < to; token += kTile, stage ^= 1) {
+  for (int token = from; token < to; token += TILE, stage ^= 1) {
     // The next tile's loads (behind the last one's, its own again, which nobody uses).
-    const int ahead = token + kTile < to ? token + kTile : token;
+    const int ahead = token + TILE < to ? token + TILE : token;
     const int id = __builtin_amdgcn_readfirstlane(next);
     const int64_t at = St::start(a, kv_head, ahead + mine, id);
     St::load_scales(a, kv_head, id, staged);
-    next = entry_of(a.b, table, ahead + kTile + mine_v);
+    next = entry_of(a.b, table, ahead + TILE + mine_v);
     f16x8_t* keys_to = keys[stage ^ 1];
     f16x8_t* values_to = values[stage ^ 1];
-    if (token < any_hi && token + kTile > any_lo) {  // else no column of the wave sees the tile
+#pragma unroll
+    for (int t = 0; t < SUBS; ++t) {
+      const int base = token + 64 * t;
+      // Of the next tile's way into LDS, a unit of keys and a channel of values for each step
+      // (with two halves of a tile keys in the first, values in the second).
+      auto store_step = [&](int v) {
+        if (t == 0 && v < St::KEY_UNITS) St::store_keys(staged, v, keys_to);
+        if (t == SUBS - 1) {
+#pragma unroll
+          for (int channel = 4 / NV * v; channel < 4 / NV * (v + 1); ++channel) St::store_values(staged, channel, values_to);
+          if (v == 2 * NV - 1) St::store_scales(staged, scales[stage ^ 1]);
+        }
+      };
+      if (base >= any_hi || base + 64 <= any_lo) {  // no column of the wave sees them
+        if (t == 0)
+#pragma unroll
+          for (int i = 0; i < St::LOADS; ++i) St::load(a, at, i, staged);
+#pragma unroll
+        for (int v = 0; v < 2 * NV; ++v) store_step(v);
+        continue;
+      }
       // Matrix instructions and the rest go side by side, in steps that the scheduler keeps:
       // the scores of the second 32 tokens beside the weights of the first, those weighed
       // beside the second weights, those weighed beside the next tile's way into LDS.
@@ -761,16 +789,17 @@ __global__ __launch_bounds__(256, 2) void attention_tile_kernel(AttentionArgs a)
       f16x8_t ring[4];
       auto fetch = [&](int j) {
         if (j < 2 * NK) {
-          ring[j % 4] = *reinterpret_cast<const f16x8_t*>(key_base + key_place[j % NK] + 32 * (j / NK) * D * 2);
+          ring[j % 4] = *reinterpret_cast<const f16x8_t*>(key_base + key_place[j % NK] + (64 * t + 32 * (j / NK)) * D * 2);
         } else if (j < 2 * NK + 4 * NV) {
-          const int v = j - 2 * NK, n = v % NV, c = v / NV;  // chunk c = 4 i + h for i, h = v / (2 NV), v / NV % 2
-          ring[j % 4] = *reinterpret_cast<const f16x8_t*>(
-              value_base + value_place[(4 * (c / 2) + c % 2) ^ (2 * n & 7)] + 32 * 128 * n);
+          // Chunk 8 t + 4 i + 2 g + h of channel 32 n + r, for i, h = c / 2, c % 2.
+          const int v = j - 2 * NK, n = v % NV, c = v / NV;
+          const int chunk = (8 * t + 4 * (c / 2) + c % 2) ^ (WAVES == 8 ? 4 * n : 2 * n & 7);
+          ring[j % 4] = *reinterpret_cast<const f16x8_t*>(value_base + value_place[WAVES == 8 ? chunk / 4 * 2 + chunk % 2 : chunk] + 32 * TILE * 2 * n);
         }
       };
       float4 sc[2];
 #pragma unroll
-      for (int i = 0; i < 2; ++i) sc[i] = scales[stage][2 * i + g];
+      for (int i = 0; i < 2; ++i) sc[i] = scales[stage][4 * t + 2 * i + g];
 #pragma unroll
       for (int j = 0; j < 4; ++j) fetch(j);
       f32x16_t z[2] = {zeros16(), zeros16()};
@@ -800,11 +829,11 @@ __global__ __launch_bounds__(256, 2) void attention_tile_kernel(AttentionArgs a)
         unit_k[i] = not_zero(unit * sc[i].x);
         shift[i] = __builtin_fmaf(-bias, unit_k[i], sc[i].y);
       }
-      const bool partly = token < all_lo || token + kTile > all_hi || __any(sc[0].w * sc[1].w == 0.0f);
+      const bool partly = base < all_lo || base + 64 > all_hi || __any(sc[0].w * sc[1].w == 0.0f);
       auto hide = [&](int i) {
         if (!partly) return;
         asm volatile("");  // a branch: as selects this would be most of the tile's instructions
-        const int at = token + 32 * i + 16 * g, lo = col.lo - at, hi = sc[i].w != 0.0f ? col.hi - at : 0;
+        const int at = base + 32 * i + 16 * g, lo = col.lo - at, hi = sc[i].w != 0.0f ? col.hi - at : 0;
         if (max(lo, 0) >= min(hi, 16)) {  // nothing of the page: nor of its scales, whatever they are
           unit_k[i] = 1.0f;
           shift[i] = 0.0f;
@@ -833,7 +862,7 @@ __global__ __launch_bounds__(256, 2) void attention_tile_kernel(AttentionArgs a)
 #pragma unroll
       for (int k = 0; k < NK; ++k) {
         scores(0, k);
-        if (k < St::LOADS) St::load(a, at, k, staged);
+        if (t == 0 && k < St::LOADS) St::load(a, at, k, staged);
         __builtin_amdgcn_sched_barrier(0);
       }
       hide(0);
@@ -855,16 +884,9 @@ __global__ __launch_bounds__(256, 2) void attention_tile_kernel(AttentionArgs a)
 #pragma unroll
       for (int v = 0; v < 2 * NV; ++v) {
         weighed(1, v);
-        if (v < St::KEY_UNITS) St::store_keys(staged, v, keys_to);
-#pragma unroll
-        for (int channel = 4 / NV * v; channel < 4 / NV * (v + 1); ++channel) St::store_values(staged, channel, values_to);
+        store_step(v);
         __builtin_amdgcn_sched_barrier(0);
       }
-      St::store_scales(staged, scales[stage ^ 1]);
-    } else {
-#pragma unroll
-      for (int i = 0; i < St::LOADS; ++i) St::load(a, at, i, staged);
-      St::store(staged, keys_to, values_to, scales[stage ^ 1]);
     }
 #pragma unroll
     for (int k = 0; k < NK; ++k) key_place[k] ^= STAGE;
@@ -899,94 +921,143 @@ __global__ __launch_bounds__(256, 2) void attention_tile_kernel(AttentionArgs a)
 
 // ---- parts together ----------------------------------------------------------
 
-// A workgroup for EACH columns of a tile that was cut into parts, `blocks` of them a tile;
-// D/4 threads read a column's sums of one part at a time. With one column a workgroup the
-// others of its 256 threads take other parts.
+// Of one value a thread over aligned groups of GROUP threads (32, or all 256 by way of `part`).
+template <int GROUP, typename F>
+__device__ __forceinline__ float group_reduce(float v, float* part, F&& f) {
+#pragma unroll
+  for (int m = 1; m < (GROUP < 64 ? GROUP : 64); m <<= 1) v = f(v, __shfl_xor(v, m, kWave));
+  if constexpr (GROUP > 64) {
+    if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = v;
+    __syncthreads();
+    v = f(f(part[0], part[1]), f(part[2], part[3]));
+  }
+  return v;
+}
+
+// A workgroup for EACH columns (1 or 8) of a tile that was cut into parts, `blocks` of them a
+// tile: a column's threads first look at a part's maximum and sum each, then teams of D/4
+// threads read the parts' sums.
+constexpr int kJoinParts = 256;  // parts whose factors are held at once
 template <bool F16, int D, int EACH>
 __global__ __launch_bounds__(256) void attention_join_kernel(AttentionArgs a, int columns, int blocks) {
-  constexpr int LANES = D / 4, TEAMS = 256 / LANES, WAYS = EACH == 1 ? TEAMS : 1;
-  __shared__ float4 sums[WAYS > 1 ? 256 : 1];
-  __shared__ float totals[WAYS > 1 ? 256 : 1];
+  constexpr int GROUP = 256 / EACH, LANES = D / 4, WAYS = GROUP / LANES;
+  __shared__ float factors[EACH][kJoinParts];
+  __shared__ float4 sums[256];
+  __shared__ float part0[4], part1[4];
   const int kv_head = blockIdx.y, tile = blockIdx.x / blocks;
   const int count = a.cut[0].x;
   const int4 info = a.cut[1 + tile];  // first row, first column, columns of the sequence, parts
   const int entry = a.cut_entry[tile];
   if (tile >= count || info.w == 1) return;
-  const int team = threadIdx.x / LANES, d = threadIdx.x % LANES * 4, way = WAYS > 1 ? team : 0;
+  const int of = threadIdx.x / GROUP, t = threadIdx.x % GROUP, way = t / LANES, d = t % LANES * 4;
   const int64_t step = (int64_t)a.b.kv_heads * columns;
-#pragma unroll 1
-  for (int c = WAYS > 1 ? 0 : team; c < EACH; c += WAYS > 1 ? 1 : TEAMS) {
-    const int at = blockIdx.x % blocks * EACH + c, column = info.y + at;
-    if (column >= info.z) return;  // with several teams there is no barrier below
-    const int64_t slot = ((int64_t)entry * a.b.kv_heads + kv_head) * columns + at;
-    float most = kLow, total = 0.0f;
-    float4 v = make_float4(0, 0, 0, 0);
-    for (int p = 0; p < info.w; ++p) most = fmaxf(most, a.part_ml[slot + p * step].x);
-    for (int p = way; p < info.w; p += WAYS) {
-      const float2 ml = a.part_ml[slot + p * step];
-      const float4 x = *reinterpret_cast<const float4*>(a.part_out + (slot + p * step) * D + d);
+  const int at = blockIdx.x % blocks * EACH + of, column = info.y + at;
+  const int parts = column < info.z ? info.w : 0;  // none where there is no column
+  const int64_t slot = ((int64_t)entry * a.b.kv_heads + kv_head) * columns + at;
+  float most = kLow;
+  for (int p = t; p < parts; p += GROUP) most = fmaxf(most, a.part_ml[slot + p * step].x);
+  most = group_reduce<GROUP>(most, part0, [](float x, float y) { return fmaxf(x, y); });
+  float total = 0.0f;
+  float4 v = make_float4(0, 0, 0, 0);
+  for (int p0 = 0; p0 < info.w; p0 += kJoinParts) {
+    const int n = min(kJoinParts, parts - p0);
+    for (int p = t; p < n; p += GROUP) {
+      const float2 ml = a.part_ml[slot + (p0 + p) * step];
       const float f = exp2_fast(ml.x - most);
+      factors[of][p] = f;
       total = __builtin_fmaf(ml.y, f, total);
+    }
+    __syncthreads();
+#pragma unroll 4
+    for (int p = way; p < n; p += WAYS) {
+      const float4 x = *reinterpret_cast<const float4*>(a.part_out + (slot + (p0 + p) * step) * D + d);
+      const float f = factors[of][p];
       v.x = __builtin_fmaf(x.x, f, v.x);
       v.y = __builtin_fmaf(x.y, f, v.y);
       v.z = __builtin_fmaf(x.z, f, v.z);
       v.w = __builtin_fmaf(x.w, f, v.w);
     }
-    if (WAYS > 1) {
-      sums[threadIdx.x] = v;
-      totals[threadIdx.x] = total;
-      __syncthreads();
-      if (way) return;
-#pragma unroll
-      for (int w = 1; w < WAYS; ++w) {
-        const float4 o = sums[threadIdx.x + w * LANES];
-        total += totals[threadIdx.x + w * LANES];
-        v.x += o.x, v.y += o.y, v.z += o.z, v.w += o.w;
-      }
-    }
-    const float inverse = total == 0.0f ? 0.0f : kValueUnit / total;
-    const float x[4] = {v.x * inverse, v.y * inverse, v.z * inverse, v.w * inverse};
-    const int row = info.x + column / a.group, head = kv_head * a.group + column % a.group;
-    put_out4<F16>(a.out + ((int64_t)row * a.heads + head) * D + d, x);
+    __syncthreads();
   }
+  total = group_reduce<GROUP>(total, part1, [](float x, float y) { return x + y; });
+  if (WAYS > 1) {
+    sums[threadIdx.x] = v;
+    __syncthreads();
+  }
+  if (way || !parts) return;
+#pragma unroll
+  for (int w = 1; w < WAYS; ++w) {
+    const float4 o = sums[threadIdx.x + w * LANES];
+    v.x += o.x, v.y += o.y, v.z += o.z, v.w += o.w;
+  }
+  const float inverse = total == 0.0f ? 0.0f : kValueUnit / total;
+  const float x[4] = {v.x * inverse, v.y * inverse, v.z * inverse, v.w * inverse};
+  const int row = info.x + column / a.group, head = kv_head * a.group + column % a.group;
+  put_out4<F16>(a.out + ((int64_t)row * a.heads + head) * D + d, x);
 }
 
 template <bool F16, int D>
 void launch_as(const AttentionPlan& p, const AttentionArgs& a, hipStream_t s) {
   const dim3 grid((uint32_t)p.items * a.b.kv_heads);
-  auto* kernel = p.columns == 16   ? attention_few_kernel<F16, D, 1>
-                 : p.columns == 32 ? attention_few_kernel<F16, D, 2>
-                                   : attention_tile_kernel<F16, D>;
-  tfm_launch(kernel, grid, dim3(256), 0, s, a);
+  auto* kernel = p.columns == 16    ? attention_few_kernel<F16, D, 1>
+                 : p.columns == 32  ? attention_few_kernel<F16, D, 2>
+                 : p.columns == 128 ? attention_tile_kernel<F16, D, 4>
+                                    : attention_tile_kernel<F16, D, 8>;
+  tfm_launch(kernel, grid, dim3(p.columns == 256 ? 512 : 256), 0, s, a);
   check_hip(hipGetLastError(), "cache_attention launch");
   if (!p.split) return;
   // Tiles of columns that can be cut: fewer than the target.
   const int64_t tiles = (int64_t)a.b.rows * a.group / p.columns + a.b.sequences;
   const int cut = (int)std::min<int64_t>(tiles, p.target);
-  if (p.columns == 128)
-    tfm_launch(attention_join_kernel<F16, D, 32>, dim3(cut * 4, a.b.kv_heads), dim3(256), 0, s, a, 128, 4);
-  else {
-    const int used = std::min(p.columns, a.b.max_rows * a.group);
-    tfm_launch(attention_join_kernel<F16, D, 1>, dim3(cut * used, a.b.kv_heads), dim3(256), 0, s, a, p.columns, used);
-  }
+  const int used = std::min(p.columns, a.b.max_rows * a.group);
+  auto join = [&](auto* kernel, int each) {
+    const int blocks = (used + each - 1) / each;
+    tfm_launch(kernel, dim3(cut * blocks, a.b.kv_heads), dim3(256), 0, s, a, p.columns, blocks);
+  };
+  // Few columns in all: a workgroup each; many: several share one (1280 x 8 columns of 5 drafted rows 9.5 to 4.6 us).
+  if ((int64_t)cut * used * a.b.kv_heads <= 1024)
+    join(attention_join_kernel<F16, D, 1>, 1);
+  else
+    join(attention_join_kernel<F16, D, 8>, 8);
   check_hip(hipGetLastError(), "cache_attention join launch");
 }
 
 }  // namespace
 
-AttentionPlan attention_plan(int64_t rows, int group, int kv_heads, int sequences, int max_rows, int64_t capacity) {
+// How a call is cut. Measured on one card, us:
+// - few columns, least tokens of a part: 1 x 1407 tokens of 16 heads 9.8 with 128, 10.5 with 256,
+//   13.5 with 512 (one part 16.1).
+// - many columns: four waves (two workgroups a compute unit) or eight (one, which brings and
+//   converts a tile for twice the columns, at 1.15 of the rate: 8192 rows of 16 heads 335 against
+//   289). Eight where a sequence's columns do not leave 1 / 1.15 of its tiles empty, and either
+//   there are two rounds of them, or less than the rounds of four come to (7 chunks of 129 to 815
+//   rows 45 against 63), or tiles are cut along many tokens (800 rows behind 30000 tokens, 32
+//   heads: 438 against 507; behind 500: 43 against 42).
+// - many columns, least tokens of a part: 48 rows behind 4000 tokens 25 with 512, 36 with 1024;
+//   512 rows of a prompt 19.8 in one part, 22.5 in two.
+AttentionPlan attention_plan(int64_t rows, int group, int kv_heads, int head_dim, int sequences, int max_rows,
+                             int64_t capacity) {
   AttentionPlan p{};
-  const int64_t most = (int64_t)max_rows * group;
-  p.columns = most <= 16 ? 16 : most <= 32 ? 32 : 128;
-  const bool few = p.columns < 128;
-  // Items over all key heads that the parts aim at, and the least tokens of a part.
-  const int all = few ? 1024 : 512;
-  p.min_chunk = few ? 128 : 256;
-  p.target = std::max(1, all / kv_heads);
-  const int64_t tiles = std::min<int64_t>(rows * group / p.columns + sequences, rows * group);
-  const int64_t parts = (capacity + p.min_chunk - 1) / p.min_chunk;
-  p.split = parts > 1;
-  p.items = (int)std::max<int64_t>(1, p.split ? std::max(tiles, std::min<int64_t>(2 * p.target, tiles * parts)) : tiles);
+  const int64_t most = (int64_t)max_rows * group, all = rows * group;
+  int resident;  // workgroups that the card holds at once
+  if (most <= 32) {
+    p.columns = most <= 16 ? 16 : 32;
+    resident = 256 * (p.columns == 16 ? (head_dim == 128 ? 3 : 5) : (head_dim == 128 ? 2 : 3));
+    p.min_chunk = 128;
+  } else {
+    const int64_t n256 = (all + 255) / 256 * kv_heads, n128 = (all + 127) / 128 * kv_heads, rest = n128 % 512;
+    const bool fits = 20 * ((most + 255) / 256 * 2) <= 23 * ((most + 127) / 128);
+    const bool even = n256 >= 512 || (n256 < 256 ? capacity >= 4096
+                                                 : 20 * ((n256 + 255) / 256) <= 23 * (n128 / 512) + (rest > 256 ? 23 : rest ? 13 : 0));
+    p.columns = fits && even ? 256 : 128;
+    resident = p.columns == 256 ? 256 : 512;
+    p.min_chunk = 512;
+  }
+  p.target = std::max(1, resident / kv_heads);
+  const int64_t tiles = std::min<int64_t>(all / p.columns + sequences, all);
+  // Where the rows by themselves make enough tiles, or one workgroup reads so few tokens, none is cut.
+  p.split = capacity > p.min_chunk && all / p.columns < p.target;
+  p.items = (int)std::max<int64_t>(1, p.split ? std::max<int64_t>(tiles, p.target) : tiles);
   return p;
 }
 

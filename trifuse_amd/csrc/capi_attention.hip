@@ -75,10 +75,10 @@ int group_of(int32_t heads, const KvBatchArgs& b) {
   return heads / b.kv_heads;
 }
 
-AttentionPlan plan_of(int64_t rows, int32_t heads, int32_t window, const KvBatchArgs& b) {
+AttentionPlan plan_of(int64_t rows, int32_t heads, int32_t window, int32_t head_dim, const KvBatchArgs& b) {
   int64_t capacity = (int64_t)b.table_width << b.page_shift;
   if (window > 0) capacity = std::min<int64_t>(capacity, (int64_t)window + b.max_rows);
-  return attention_plan(rows, group_of(heads, b), b.kv_heads, b.sequences, b.max_rows, capacity);
+  return attention_plan(rows, group_of(heads, b), b.kv_heads, head_dim, b.sequences, b.max_rows, capacity);
 }
 
 struct AttentionWs {
@@ -92,8 +92,8 @@ AttentionWs carve_attention(const AttentionPlan& p, int kv_heads, int head_dim, 
   AttentionWs w{};
   if (!p.split) return w;
   Carver c(base);
-  // Tiles are cut only where they are fewer than the target, into fewer parts than twice that.
-  const size_t slots = (size_t)std::min(p.items, 2 * p.target) * (size_t)kv_heads * (size_t)p.columns;
+  // Tiles are cut only where they are fewer than the target, into at most that many parts.
+  const size_t slots = (size_t)p.target * (size_t)kv_heads * (size_t)p.columns;
   w.out = c.take<float>(slots * (size_t)head_dim);
   w.ml = c.take<float2>(slots);
   w.cut = c.take<int4>((size_t)p.target + 1);
@@ -200,7 +200,7 @@ size_t tfm_cache_attention_workspace_bytes(int64_t rows, int32_t heads, int32_t 
     CacheSpans at{};
     const KvBatchArgs b = need_batch(cache, batch, rows, &at);
     if (rows == 0 || b.sequences == 0 || b.max_rows == 0) return;
-    bytes = carve_attention(plan_of(rows, heads, window, b), b.kv_heads, cache->head_dim, nullptr).bytes;
+    bytes = carve_attention(plan_of(rows, heads, window, cache->head_dim, b), b.kv_heads, cache->head_dim, nullptr).bytes;
   });
   return bytes;  // 0 for arguments that the call refuses
 }
@@ -222,7 +222,7 @@ int tfm_cache_attention(const void* q, int64_t row_stride, int64_t head_stride, 
     const Span in = rows_span(q, rows, heads, cache->head_dim, row_stride, head_stride, "q");
     need_ptr(out, "out");
     if (reinterpret_cast<uintptr_t>(out) & 7) fail(TFM_E_INVALID, "out must be 8-byte aligned");
-    const AttentionPlan plan = plan_of(rows, heads, window, a.b);
+    const AttentionPlan plan = plan_of(rows, heads, window, cache->head_dim, a.b);
     if ((int64_t)plan.items * a.b.kv_heads >= (1 << 24)) fail(TFM_E_UNSUPPORTED, "more than 2^24 tiles of (row, head) are not built");
     const AttentionWs ws = carve_attention(plan, a.b.kv_heads, cache->head_dim, workspace);
     if (ws.bytes) need_ws(workspace, workspace_bytes, ws.bytes);
@@ -240,7 +240,6 @@ int tfm_cache_attention(const void* q, int64_t row_stride, int64_t head_stride, 
     a.window = window;
     a.min_chunk = plan.min_chunk;
     a.target = plan.target;
-    a.items = plan.items;
     a.part_out = ws.out;
     a.part_ml = ws.ml;
     a.cut = ws.cut;

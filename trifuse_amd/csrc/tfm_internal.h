@@ -425,20 +425,20 @@ struct AttentionArgs {
   float scale;        // times log2(e)
   bool causal;
   int window;         // 0: none
-  int min_chunk;      // least tokens of a split
-  int target;         // work items a key head that the splits aim at
-  int items;          // work items a key head in the grid
-  float* part_out;    // [items * kv_heads, columns, head_dim], null: no splits
-  float2* part_ml;    // [items * kv_heads, columns]: maximum and sum
+  int min_chunk;      // least tokens of a part
+  int target;         // workgroups a key head that the card holds at once
+  float* part_out;    // [target * kv_heads, columns, head_dim], null: no tile is cut
+  float2* part_ml;    // [target * kv_heads, columns]: maximum and sum
   int4* cut;          // [1 + target]: how many tiles are cut, and what each one is
   int* cut_entry;     // [target]: its first item
 };
 // How a call is cut into workgroups: `columns` (row, head) pairs of a key head each, and along the tokens.
 struct AttentionPlan {
-  int columns, min_chunk, target, items;
+  int columns, min_chunk, target, items;  // items: of the grid, a key head
   bool split;
 };
-AttentionPlan attention_plan(int64_t rows, int group, int kv_heads, int sequences, int max_rows, int64_t capacity);
+AttentionPlan attention_plan(int64_t rows, int group, int kv_heads, int head_dim, int sequences, int max_rows,
+                             int64_t capacity);
 void launch_cache_attention(bool f16, int head_dim, const AttentionPlan& plan, const AttentionArgs& a, hipStream_t s);
 
 }  // namespace tfm
