@@ -70,13 +70,13 @@ def attend64(q, cache, table, lengths, starts, scale, causal, window):
                 x = v[sees]
                 out[start + i, h] = w @ x
                 # fp32 sums of a score (D products, of codes plus 128, and the exponent's arithmetic) as a relative error of
-                # its weight, twice for the quotient; half a step of a half for each weight; weights
-                # below 2^-14 of the first to half their smallest step, 127 codes of the largest scale each; the
-                # output's own rounding.
+                # its weight, twice for the quotient; half a step of a half for each weight, in both sums; weights
+                # below 2^-14 of the first to half their smallest step, 2^-25: 127 codes of the largest scale in one
+                # sum, up to 16 times its scale's in the other; the output's own rounding.
                 lifted = (k[sees].abs() + 128 * sk[at, g][sees][:, None])
                 most = float((lifted @ row.abs()).max()) * abs(scale)
                 score = (dim + 16) * 2.0 ** -24 * (most + 8)
-                bound[start + i, h] = (w @ x.abs()) * (2 * score + 2.0 ** -11 + 2.0 ** -20) \
+                bound[start + i, h] = (w @ x.abs()) * (2 * score + 2.0 ** -11 + 2.0 ** -20 + int(sees.sum()) * 2.0 ** -21) \
                     + int(sees.sum()) * 2.0 ** -25 * 127 * float(sv[at, g][sees].max()) + half_step(q.dtype) * out[start + i, h].abs()
     return out, bound
 

@@ -10,10 +10,10 @@
 // products as they are, as halves that hold them exactly (keys plus 128, which the sum of q
 // takes out of a score again), q of bf16 exactly after a power of two for its row (28
 // binades; what is smaller loses bits below 2^-25 of the largest), and w to 2^-12 of itself,
-// in the first sum alone. m is a maximum that is taken again only when a weight has grown past
+// the same in both sums, so that a row that looks at few tokens loses less. m is a maximum that is taken again only when a weight has grown past
 // 2^15 (a half's relative precision is the same there), so most tiles look for none and
-// rescale nothing: what is left a score is a multiply-add, an exponential, an addition and
-// half a conversion of two.
+// rescale nothing: what is left a score is a multiply-add, an exponential, and half a
+// conversion and half a sum of two.
 //
 // "Columns" are the (row, head) pairs of one key head: they share its codes. Scores are
 // taken transposed, keys along the rows of a product and columns along its lanes: a lane
@@ -39,6 +39,9 @@ namespace {
 
 constexpr float kLow = -3.402823466e38f;  // below every score; finite, so that differences are
 constexpr float kMost = 32768.0f;         // sum of a lane's weights of a page from which the maximum is taken again
+// Weights below 2^-14 are subnormal halves, each off by up to 2^-25. In the sum of w / b that is
+// 2^-25 / b: pages whose 1 / b is over so many times the sum so far have theirs summed in fp32.
+constexpr float kLeast = 16.0f;
 
 __device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
 
@@ -332,7 +335,7 @@ __device__ __forceinline__ void few_weigh(const uint32_t (&x)[8][W], const f16x8
 
 // NC * 16 columns a workgroup of four waves, which take the part's tiles of 32 tokens in turn.
 template <bool F16, int D, int NC>
-__global__ __launch_bounds__(256, NC == 1 ? 3 : 2) void attention_few_kernel(AttentionArgs a) {
+__global__ __launch_bounds__(256, (D == 64 ? 5 : 4) - NC) void attention_few_kernel(AttentionArgs a) {
   constexpr int COLS = 16 * NC, NK = D / 32, NV = D / 16, PAD = D + 4;
   __shared__ float joined[4][16][PAD];
   __shared__ float stat_m[4][COLS], stat_l[4][COLS];
@@ -413,12 +416,13 @@ __global__ __launch_bounds__(256, NC == 1 ? 3 : 2) void attention_few_kernel(Att
   all_lo = __builtin_amdgcn_readfirstlane(all_lo);
   all_hi = __builtin_amdgcn_readfirstlane(all_hi);
 
-  float m[NC], l[NC];
+  float m[NC], l[NC], seen[NC];  // seen: at most what all lanes of the column have in l
   f32x4_t o[NC][NV];
 #pragma unroll
   for (int c = 0; c < NC; ++c) {
     m[c] = kLow;
     l[c] = 0.0f;
+    seen[c] = 0.0f;
 #pragma unroll
     for (int n = 0; n < NV; ++n) o[c][n] = f32x4_t{0, 0, 0, 0};
   }
@@ -442,49 +446,58 @@ __global__ __launch_bounds__(256, NC == 1 ? 3 : 2) void attention_few_kernel(Att
       }
     }
     if (more) few_load_keys<D>(a, kv_head, token + 128, next.k, t);
-    const float lv = __builtin_amdgcn_logf(scale.y), inverse = __builtin_amdgcn_rcpf(scale.y);
+    const float lv = __builtin_amdgcn_logf(scale.y), inverse_v = __builtin_amdgcn_rcpf(scale.y);
     const bool there = is_page(a.b, page.v), whole = token >= all_lo && token + 32 <= all_hi && !__any(!there);
     f16x8_t w[NC];
 #pragma unroll
     for (int c = 0; c < NC; ++c) {
-      float unit_k = not_zero(unit[c] * scale.x), shift = __builtin_fmaf(-bias[c], unit_k, lv);
+      float unit_k = not_zero(unit[c] * scale.x), shift = __builtin_fmaf(-bias[c], unit_k, lv), inverse = inverse_v;
       if (!whole) {
         asm volatile("");  // a branch, not selects
         const int lo = col[c].lo - token - 8 * g, hi = there ? col[c].hi - token - 8 * g : 0;
         if (max(lo, 0) >= min(hi, 8)) {  // nothing of the page: nor of its scales, whatever they are
           unit_k = 1.0f;
           shift = 0.0f;
+          inverse = 0.0f;
         }
 #pragma unroll
         for (int e = 0; e < 8; ++e) z[c][e / 4][e % 4] = e >= lo && e < hi ? z[c][e / 4][e % 4] : -__builtin_inff();
       }
       auto score = [&](int e, float low) { return __builtin_fmaf(z[c][e / 4][e % 4], unit_k, low); };
       auto weigh = [&] {
-        float sum = 0.0f;  // of fp32 weights: beside large value scales a small page's weights leave a half's range
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          const float p = exp2_fast(score(e, shift - m[c]));
-          sum += p;
-          w[c][e] = (_Float16)p;
-        }
-        return sum;
+        for (int e = 0; e < 8; ++e) w[c][e] = (_Float16)exp2_fast(score(e, shift - m[c]));
+        return add_halves(w[c], 0.0f);
       };
       float sum = weigh();
-      if (__any(sum > kMost)) {
-        float top = m[c];
+      if (__any(sum > kMost || inverse > kLeast * seen[c])) {
+        auto together = [&] {
+          const float t = __builtin_fmaf(sum, inverse, l[c]);
+          const float two = t + __shfl_xor(t, 16, kWave);
+          return two + __shfl_xor(two, 32, kWave);
+        };
+        if (__any(sum > kMost)) {
+          float top = m[c];
 #pragma unroll
-        for (int e = 0; e < 8; ++e) top = fmaxf(top, score(e, shift));
-        top = fmaxf(top, __shfl_xor(top, 16, kWave));
-        top = fmaxf(top, __shfl_xor(top, 32, kWave));
-        const float less = exp2_fast(m[c] - top);
-        m[c] = top;
-        l[c] *= less;
+          for (int e = 0; e < 8; ++e) top = fmaxf(top, score(e, shift));
+          top = fmaxf(top, __shfl_xor(top, 16, kWave));
+          top = fmaxf(top, __shfl_xor(top, 32, kWave));
+          const float less = exp2_fast(m[c] - top);
+          m[c] = top;
+          l[c] *= less;
 #pragma unroll
-        for (int n = 0; n < NV; ++n) o[c][n] *= less;
-        sum = weigh();
+          for (int n = 0; n < NV; ++n) o[c][n] *= less;
+          sum = weigh();
+        }
+        seen[c] = together();
+        if (__any(inverse > kLeast * seen[c])) {  // the sum in fp32, whatever the halves lose
+          sum = 0.0f;
+#pragma unroll
+          for (int e = 0; e < 8; ++e) sum += exp2_fast(score(e, shift - m[c]));
+          seen[c] = together();
+        }
       }
-      // A page that a column sees nothing of adds nothing, whatever its scale.
-      l[c] = sum == 0.0f ? l[c] : __builtin_fmaf(sum, inverse, l[c]);
+      l[c] = __builtin_fmaf(sum, inverse, l[c]);
     }
     uint32_t x[8][D / 64];
 #pragma unroll
@@ -735,7 +748,7 @@ __global__ __launch_bounds__(64 * WAVES, 2) void attention_tile_kernel(Attention
   // The key row that this lane's row of a product stands for: lanes of half g then hold tokens 16 g .. in order.
   const int key_row = 16 * (r >> 2 & 1) + 4 * (r >> 3) + (r & 3);
 
-  float m = kLow, l = 0.0f;
+  float m = kLow, l = 0.0f, seen = 0.0f;  // seen: at most what both lanes of the column have in l
   f32x16_t o[NV];
 #pragma unroll
   for (int n = 0; n < NV; ++n) o[n] = zeros16();
@@ -804,7 +817,7 @@ __global__ __launch_bounds__(64 * WAVES, 2) void attention_tile_kernel(Attention
       for (int j = 0; j < 4; ++j) fetch(j);
       f32x16_t z[2] = {zeros16(), zeros16()};
       f16x8_t w[2][2];
-      float unit_k[2], shift[2], sum[2];
+      float unit_k[2], shift[2], inverse[2], sum[2];
       auto scores = [&](int i, int k) {
         const int j = i * NK + k;
         z[i] = __builtin_amdgcn_mfma_f32_32x32x16_f16(ring[j % 4], q[k], z[i], 0, 0, 0);
@@ -815,19 +828,22 @@ __global__ __launch_bounds__(64 * WAVES, 2) void attention_tile_kernel(Attention
         o[v % NV] = __builtin_amdgcn_mfma_f32_32x32x16_f16(ring[j % 4], w[i][v / NV], o[v % NV], 0, 0, 0);
         fetch(j + 4);
       };
+      auto weight = [&](int i, int e) { return exp2_fast(__builtin_fmaf(z[i][e], unit_k[i], shift[i] - m)); };
       auto weigh = [&](int i, int from_e, int to_e) {
-        const float low = shift[i] - m;
+        const f16x2_t one = {(_Float16)1.0f, (_Float16)1.0f};
 #pragma unroll
-        for (int e = from_e; e < to_e; ++e) {
-          const float p = exp2_fast(__builtin_fmaf(z[i][e], unit_k[i], low));
-          sum[i] = e ? sum[i] + p : p;  // fp32 weights: beside large value scales a small page's leave a half's range
-          w[i][e / 8][e % 8] = (_Float16)p;
+        for (int e = from_e; e < to_e; e += 2) {
+          const f16x2_t p = {(_Float16)weight(i, e), (_Float16)weight(i, e + 1)};
+          w[i][e / 8][e % 8] = p[0];
+          w[i][e / 8][e % 8 + 1] = p[1];
+          sum[i] = __builtin_amdgcn_fdot2(p, one, e ? sum[i] : 0.0f, false);
         }
       };
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
         unit_k[i] = not_zero(unit * sc[i].x);
         shift[i] = __builtin_fmaf(-bias, unit_k[i], sc[i].y);
+        inverse[i] = sc[i].z;
       }
       const bool partly = base < all_lo || base + 64 > all_hi || __any(sc[0].w * sc[1].w == 0.0f);
       auto hide = [&](int i) {
@@ -837,27 +853,40 @@ __global__ __launch_bounds__(64 * WAVES, 2) void attention_tile_kernel(Attention
         if (max(lo, 0) >= min(hi, 16)) {  // nothing of the page: nor of its scales, whatever they are
           unit_k[i] = 1.0f;
           shift[i] = 0.0f;
+          inverse[i] = 0.0f;
         }
 #pragma unroll
         for (int e = 0; e < 16; ++e) z[i][e] = e >= lo && e < hi ? z[i][e] : -__builtin_inff();
       };
       auto settle = [&](int i) {
-        if (__any(sum[i] > kMost)) {
-          float top = m;
+        if (__any(sum[i] > kMost || inverse[i] > kLeast * seen)) {
+          auto together = [&] {
+            const float t = __builtin_fmaf(sum[i], inverse[i], l);
+            return t + __shfl_xor(t, 32, kWave);
+          };
+          if (__any(sum[i] > kMost)) {
+            float top = m;
 #pragma unroll
-          for (int e = 0; e < 16; ++e) top = fmaxf(top, __builtin_fmaf(z[i][e], unit_k[i], shift[i]));
-          top = fmaxf(top, __shfl_xor(top, 32, kWave));
-          const float less = exp2_fast(m - top);
-          m = top;
-          l *= less;
+            for (int e = 0; e < 16; ++e) top = fmaxf(top, __builtin_fmaf(z[i][e], unit_k[i], shift[i]));
+            top = fmaxf(top, __shfl_xor(top, 32, kWave));
+            const float less = exp2_fast(m - top);
+            m = top;
+            l *= less;
 #pragma unroll
-          for (int n = 0; n < NV; ++n)
+            for (int n = 0; n < NV; ++n)
 #pragma unroll
-            for (int e = 0; e < 16; ++e) o[n][e] *= less;
-          weigh(i, 0, 16);
+              for (int e = 0; e < 16; ++e) o[n][e] *= less;
+            weigh(i, 0, 16);
+          }
+          seen = together();
+          if (__any(inverse[i] > kLeast * seen)) {  // the sum in fp32, whatever the halves lose
+            sum[i] = 0.0f;
+#pragma unroll
+            for (int e = 0; e < 16; ++e) sum[i] += weight(i, e);
+            seen = together();
+          }
         }
-        // A page that a column sees nothing of adds nothing, whatever its scale.
-        l = sum[i] == 0.0f ? l : __builtin_fmaf(sum[i], sc[i].z, l);
+        l = __builtin_fmaf(sum[i], inverse[i], l);
       };
 #pragma unroll
       for (int k = 0; k < NK; ++k) {
@@ -1042,7 +1071,7 @@ AttentionPlan attention_plan(int64_t rows, int group, int kv_heads, int head_dim
   int resident;  // workgroups that the card holds at once
   if (most <= 32) {
     p.columns = most <= 16 ? 16 : 32;
-    resident = 256 * (p.columns == 16 ? (head_dim == 128 ? 3 : 5) : (head_dim == 128 ? 2 : 3));
+    resident = 256 * ((head_dim == 64 ? 5 : 4) - p.columns / 16);
     p.min_chunk = 128;
   } else {
     const int64_t n256 = (all + 255) / 256 * kv_heads, n128 = (all + 127) / 128 * kv_heads, rest = n128 % 512;
