@@ -470,25 +470,26 @@ __global__ __launch_bounds__(256, (D == 64 ? 5 : 4) - NC) void attention_few_ker
         return add_halves(w[c], 0.0f);
       };
       float sum = weigh();
-      if (__any(sum > kMost || inverse > kLeast * seen[c])) {
+      if (__any(sum > kMost)) {
+        float top = m[c];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) top = fmaxf(top, score(e, shift));
+        top = fmaxf(top, __shfl_xor(top, 16, kWave));
+        top = fmaxf(top, __shfl_xor(top, 32, kWave));
+        const float less = exp2_fast(m[c] - top);
+        m[c] = top;
+        l[c] *= less;
+        seen[c] *= less;
+#pragma unroll
+        for (int n = 0; n < NV; ++n) o[c][n] *= less;
+        sum = weigh();
+      }
+      if (__any(inverse > kLeast * seen[c])) {
         auto together = [&] {
           const float t = __builtin_fmaf(sum, inverse, l[c]);
           const float two = t + __shfl_xor(t, 16, kWave);
           return two + __shfl_xor(two, 32, kWave);
         };
-        if (__any(sum > kMost)) {
-          float top = m[c];
-#pragma unroll
-          for (int e = 0; e < 8; ++e) top = fmaxf(top, score(e, shift));
-          top = fmaxf(top, __shfl_xor(top, 16, kWave));
-          top = fmaxf(top, __shfl_xor(top, 32, kWave));
-          const float less = exp2_fast(m[c] - top);
-          m[c] = top;
-          l[c] *= less;
-#pragma unroll
-          for (int n = 0; n < NV; ++n) o[c][n] *= less;
-          sum = weigh();
-        }
         seen[c] = together();
         if (__any(inverse > kLeast * seen[c])) {  // the sum in fp32, whatever the halves lose
           sum = 0.0f;
@@ -859,25 +860,26 @@ __global__ __launch_bounds__(64 * WAVES, 2) void attention_tile_kernel(Attention
         for (int e = 0; e < 16; ++e) z[i][e] = e >= lo && e < hi ? z[i][e] : -__builtin_inff();
       };
       auto settle = [&](int i) {
-        if (__any(sum[i] > kMost || inverse[i] > kLeast * seen)) {
+        if (__any(sum[i] > kMost)) {
+          float top = m;
+#pragma unroll
+          for (int e = 0; e < 16; ++e) top = fmaxf(top, __builtin_fmaf(z[i][e], unit_k[i], shift[i]));
+          top = fmaxf(top, __shfl_xor(top, 32, kWave));
+          const float less = exp2_fast(m - top);
+          m = top;
+          l *= less;
+          seen *= less;
+#pragma unroll
+          for (int n = 0; n < NV; ++n)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) o[n][e] *= less;
+          weigh(i, 0, 16);
+        }
+        if (__any(inverse[i] > kLeast * seen)) {
           auto together = [&] {
             const float t = __builtin_fmaf(sum[i], inverse[i], l);
             return t + __shfl_xor(t, 32, kWave);
           };
-          if (__any(sum[i] > kMost)) {
-            float top = m;
-#pragma unroll
-            for (int e = 0; e < 16; ++e) top = fmaxf(top, __builtin_fmaf(z[i][e], unit_k[i], shift[i]));
-            top = fmaxf(top, __shfl_xor(top, 32, kWave));
-            const float less = exp2_fast(m - top);
-            m = top;
-            l *= less;
-#pragma unroll
-            for (int n = 0; n < NV; ++n)
-#pragma unroll
-              for (int e = 0; e < 16; ++e) o[n][e] *= less;
-            weigh(i, 0, 16);
-          }
           seen = together();
           if (__any(inverse[i] > kLeast * seen)) {  // the sum in fp32, whatever the halves lose
             sum[i] = 0.0f;
