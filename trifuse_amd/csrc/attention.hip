@@ -335,7 +335,7 @@ __device__ __forceinline__ void few_weigh(const uint32_t (&x)[8][W], const f16x8
 
 // NC * 16 columns a workgroup of four waves, which take the part's tiles of 32 tokens in turn.
 template <bool F16, int D, int NC>
-__global__ __launch_bounds__(256, (D == 64 ? 5 : 4) - NC) void attention_few_kernel(AttentionArgs a) {
+__global__ __launch_bounds__(256, D == 64 ? 7 - 2 * NC : 4 - NC) void attention_few_kernel(AttentionArgs a) {
   constexpr int COLS = 16 * NC, NK = D / 32, NV = D / 16, PAD = D + 4;
   __shared__ float joined[4][16][PAD];
   __shared__ float stat_m[4][COLS], stat_l[4][COLS];
@@ -927,10 +927,14 @@ __global__ __launch_bounds__(64 * WAVES, 2) void attention_tile_kernel(Attention
   }
 
   l += __shfl_xor(l, 32, kWave);
-  if (!col.real) return;
+  // Found again: kept across the tiles it would take registers that those are short of.
+  int thread = threadIdx.x;
+  asm volatile("" : "+v"(thread));
+  const Column column = column_of(a, s, kv_head, it.tile * COLS + thread / 64 * 32 + thread % 32);
+  if (!column.real) return;
   if (it.parts == 1) {
     const float inverse = l == 0.0f ? 0.0f : kValueUnit / l;
-    uint16_t* out = a.out + ((int64_t)col.row * a.heads + col.head) * D;
+    uint16_t* out = a.out + ((int64_t)column.row * a.heads + column.head) * D;
 #pragma unroll
     for (int n = 0; n < NV; ++n)
 #pragma unroll
@@ -939,7 +943,7 @@ __global__ __launch_bounds__(64 * WAVES, 2) void attention_tile_kernel(Attention
         put_out4<F16>(out + 32 * n + 2 * e + 4 * g, v);
       }
   } else {
-    const int64_t slot = ((int64_t)(it.entry + it.part) * a.b.kv_heads + kv_head) * COLS + 32 * wave + r;
+    const int64_t slot = ((int64_t)(it.entry + it.part) * a.b.kv_heads + kv_head) * COLS + thread / 64 * 32 + thread % 32;
     float* out = a.part_out + slot * D;
 #pragma unroll
     for (int n = 0; n < NV; ++n)
@@ -1073,7 +1077,7 @@ AttentionPlan attention_plan(int64_t rows, int group, int kv_heads, int head_dim
   int resident;  // workgroups that the card holds at once
   if (most <= 32) {
     p.columns = most <= 16 ? 16 : 32;
-    resident = 256 * ((head_dim == 64 ? 5 : 4) - p.columns / 16);
+    resident = 256 * (head_dim == 64 ? 7 - p.columns / 8 : 4 - p.columns / 16);
     p.min_chunk = 128;
   } else {
     const int64_t n256 = (all + 255) / 256 * kv_heads, n128 = (all + 127) / 128 * kv_heads, rest = n128 % 512;

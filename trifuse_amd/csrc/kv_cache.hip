@@ -28,25 +28,23 @@ __device__ __forceinline__ uint2 pack_codes(const float* x, float inverse, bool 
 
 // An item is 16 channels of a token: two vectors of eight, which are the halves of
 // eight pairs where those are turned. NI items a thread cover a whole page.
+// One wave a page (NT = 64): four pages a workgroup.
 template <bool F16, int D, int NT, int NI>
-__global__ __launch_bounds__(NT) void cache_append_kernel(KvAppendArgs a, int slots) {
+__global__ __launch_bounds__(NT == 64 ? 256 : NT) void cache_append_kernel(KvAppendArgs a, int slots) {
   __shared__ uint32_t most[(NT + 63) / 64];
+  constexpr int PAGES = NT == 64 ? 4 : 1;
   const KvBatchArgs& g = a.b;
-  const int b = blockIdx.x / slots, head = blockIdx.y;
+  const int thread = threadIdx.x % NT, unit = blockIdx.x * PAGES + threadIdx.x / NT;
+  const int b = unit / slots, head = blockIdx.y;
+  if (b >= g.sequences) return;
   const bool values = blockIdx.z != 0;
   const KvSeq s = kv_seq(g, b);
   const int page_tokens = 1 << g.page_shift;
-  const int at = (max(s.first(), 0) >> g.page_shift) + blockIdx.x % slots;  // table entry
+  const int at = (max(s.first(), 0) >> g.page_shift) + unit % slots;  // table entry
   const int base = at << g.page_shift;
   const int begin = max(max(s.first(), 0), base), end = min(s.len, base + page_tokens);
   if (begin >= end) return;
-  const int page = kv_page(g, b, begin);
-  if (page < 0) return;
-  const int64_t place = (int64_t)page * g.kv_heads + head;
-  int8_t* codes = (values ? g.v : g.k) + (place << g.page_shift) * D;
-  float* scale = (values ? g.v_scales : g.k_scales) + place;
   const int held = begin - base;  // tokens of the page that stay
-  const float before = held > 0 ? *scale : 0.0f;
 
   const uint16_t* x = (values ? a.v + head * a.v_head : a.k + head * a.k_head);
   const int64_t row_stride = values ? a.v_row : a.k_row;
@@ -63,21 +61,36 @@ __global__ __launch_bounds__(NT) void cache_append_kernel(KvAppendArgs a, int sl
       d1 = d0 + 8;
     }
   };
+  // The tokens are on their way while the page is looked up.
+  Vec8 raw[NI][2];
+#pragma unroll
+  for (int i = 0; i < NI; ++i) {
+    const int item = thread + i * NT;
+    if (item < items) {
+      const uint16_t* row = x + (int64_t)(s.start + begin + item / per - s.first()) * row_stride;
+      int d0, d1;
+      channels(item % per, d0, d1);
+      raw[i][0] = load8<true>(row + d0, 8);
+      raw[i][1] = load8<true>(row + d1, 8);
+    }
+  }
+  const int page = kv_page(g, b, begin);
+  if (page < 0) return;
+  const int64_t place = (int64_t)page * g.kv_heads + head;
+  int8_t* codes = (values ? g.v : g.k) + (place << g.page_shift) * D;
+  float* scale = (values ? g.v_scales : g.k_scales) + place;
+  const float before = held > 0 ? *scale : 0.0f;
   float v[NI][16];
   uint32_t top = 0;
 #pragma unroll
   for (int i = 0; i < NI; ++i) {
-    const int item = threadIdx.x + i * NT;
+    const int item = thread + i * NT;
     if (item < items) {
       const int token = begin + item / per, c = item % per;
-      const uint16_t* row = x + (int64_t)(s.start + token - s.first()) * row_stride;
-      int d0, d1;
-      channels(c, d0, d1);
-      const Vec8 p = load8<true>(row + d0, 8), q = load8<true>(row + d1, 8);
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
-        v[i][j] = elem<F16>(p, j);
-        v[i][8 + j] = elem<F16>(q, j);
+        v[i][j] = elem<F16>(raw[i][0], j);
+        v[i][8 + j] = elem<F16>(raw[i][1], j);
       }
       if (c < turned) {
 #pragma unroll
@@ -97,7 +110,7 @@ __global__ __launch_bounds__(NT) void cache_append_kernel(KvAppendArgs a, int sl
 #pragma unroll
   for (int m = 1; m < 64; m <<= 1) top = max(top, (uint32_t)__shfl_xor((int)top, m, kWave));
   if (NT > 64) {
-    if ((threadIdx.x & 63) == 0) most[threadIdx.x >> 6] = top;
+    if ((thread & 63) == 0) most[thread >> 6] = top;
     __syncthreads();  // behind every thread's read of the old scale, too
 #pragma unroll
     for (int w = 0; w < (NT + 63) / 64; ++w) top = max(top, most[w]);
@@ -107,7 +120,7 @@ __global__ __launch_bounds__(NT) void cache_append_kernel(KvAppendArgs a, int sl
   const float inverse = 1.0f / now;
 #pragma unroll
   for (int i = 0; i < NI; ++i) {
-    const int item = threadIdx.x + i * NT;
+    const int item = thread + i * NT;
     if (item < items) {
       const int token = begin + item / per, c = item % per;
       int8_t* to = codes + (token - base) * D;
@@ -119,7 +132,7 @@ __global__ __launch_bounds__(NT) void cache_append_kernel(KvAppendArgs a, int sl
   }
   if (held > 0 && now > before) {
     const float ratio = before / now;
-    for (int i = threadIdx.x; i < held * (D / 16); i += NT) {
+    for (int i = thread; i < held * (D / 16); i += NT) {
       uint4* at16 = reinterpret_cast<uint4*>(codes) + i;
       const uint4 old = *at16;
       uint32_t w[4] = {old.x, old.y, old.z, old.w};
@@ -136,7 +149,7 @@ __global__ __launch_bounds__(NT) void cache_append_kernel(KvAppendArgs a, int sl
       *at16 = make_uint4(w[0], w[1], w[2], w[3]);
     }
   }
-  if (threadIdx.x == 0) *scale = now;
+  if (thread == 0) *scale = now;
 }
 
 template <typename T>
@@ -198,10 +211,12 @@ template <bool F16, int D>
 void append(const KvAppendArgs& a, hipStream_t s) {
   const int page = 1 << a.b.page_shift;
   const int slots = (a.b.max_rows + page - 2) / page + 1;  // pages that max_rows tokens can meet
-  const dim3 grid((uint32_t)a.b.sequences * slots, a.b.kv_heads, 2);
-  auto go = [&](auto* kernel, int threads) { tfm_launch(kernel, grid, dim3(threads), 0, s, a, slots); };
+  const uint32_t units = (uint32_t)a.b.sequences * slots;
+  auto go = [&](auto* kernel, int threads, int pages = 1) {
+    tfm_launch(kernel, dim3((units + pages - 1) / pages, a.b.kv_heads, 2), dim3(threads), 0, s, a, slots);
+  };
   switch (page * (D / 16)) {
-    case 64: go(cache_append_kernel<F16, D, 64, 1>, 64); break;
+    case 64: go(cache_append_kernel<F16, D, 64, 1>, 256, 4); break;
     case 128: go(cache_append_kernel<F16, D, 128, 1>, 128); break;
     case 256: go(cache_append_kernel<F16, D, 256, 1>, 256); break;
     case 512: go(cache_append_kernel<F16, D, 256, 2>, 256); break;

@@ -7,14 +7,14 @@ namespace tfm {
 
 constexpr double kTurnsPerRadian = 0.15915494309189533577;  // 1 / (2 pi)
 
-// scale * (cos, sin) of 2 pi * turns. The turn is reduced to an eighth of a circle in
-// 64 bits: a far position's angle has millions of turns, of which fp32 keeps nothing.
-// What is left, |a| <= pi / 4, takes the Taylor polynomials of degree 9 and 10 in fp32
-// (next terms below 2e-9).
+// scale * (cos, sin) of 2 pi * turns. Whole turns are taken off in 64 bits: a far position's
+// angle has millions of them, of which fp32 keeps nothing. What is left, at most half a turn,
+// is right to 2^-26 of one in fp32; less its quarters, |a| <= pi / 4, it takes the Taylor
+// polynomials of degree 9 and 10 (next terms below 2e-9).
 __device__ __forceinline__ float2 turn_cos_sin(double turns, float scale) {
-  const double part = turns - __builtin_rint(turns);  // [-1/2, 1/2]
-  const double quarter = __builtin_rint(4.0 * part);
-  const float a = (float)(part - 0.25 * quarter) * 6.283185307179586f;
+  const float part = (float)(turns - __builtin_rint(turns));  // [-1/2, 1/2]
+  const float quarter = __builtin_rintf(4.0f * part);
+  const float a = (part - 0.25f * quarter) * 6.283185307179586f;
   const int q = (int)quarter;  // -2 .. 2
   const float z = a * a;
   float s = 2.7557319e-6f;
