@@ -54,30 +54,28 @@ def attend64(q, cache, table, lengths, starts, scale, causal, window):
         for h in range(heads):
             g = h // group
             k, v = ck[at, g, off] * sk[at, g][:, None], cv[at, g, off] * sv[at, g][:, None]
-            for i in range(n):
-                p = length - n + i
-                t = torch.arange(length)
-                sees = there.clone()
-                if causal:
-                    sees &= t <= p
-                if window:
-                    sees &= t > p - window
-                if not sees.any():
-                    continue
-                row = q[start + i, h].double()
-                z = k[sees] @ row * scale
-                w = torch.softmax(z, 0)
-                x = v[sees]
-                out[start + i, h] = w @ x
-                # fp32 sums of a score (D products, of codes plus 128, and the exponent's arithmetic) as a relative error of
-                # its weight, twice for the quotient; half a step of a half for each weight, in both sums; weights
-                # below 2^-14 of the first to half their smallest step, 2^-25: 127 codes of the largest scale in one
-                # sum, up to 16 times its scale's in the other; the output's own rounding.
-                lifted = (k[sees].abs() + 128 * sk[at, g][sees][:, None])
-                most = float((lifted @ row.abs()).max()) * abs(scale)
-                score = (dim + 16) * 2.0 ** -24 * (most + 8)
-                bound[start + i, h] = (w @ x.abs()) * (2 * score + 2.0 ** -11 + 2.0 ** -20 + int(sees.sum()) * 2.0 ** -21) \
-                    + int(sees.sum()) * 2.0 ** -25 * 127 * float(sv[at, g][sees].max()) + half_step(q.dtype) * out[start + i, h].abs()
+            t, p = torch.arange(length), torch.arange(length - n, length)[:, None]
+            sees = there.expand(n, length)
+            if causal:
+                sees = sees & (t <= p)
+            if window:
+                sees = sees & (t > p - window)
+            some = sees.any(1)
+            if not some.any():
+                continue
+            sees, row, to = sees[some], q[start:start + n, h].double()[some], torch.arange(start, start + n)[some]
+            w = torch.softmax((row @ k.t() * scale).masked_fill(~sees, -math.inf), 1)
+            out[to, h] = w @ v
+            # fp32 sums of a score (D products, of codes plus 128, and the exponent's arithmetic) as a relative error of
+            # its weight, twice for the quotient; half a step of a half for each weight, in both sums; weights
+            # below 2^-14 of the first to half their smallest step, 2^-25: 127 codes of the largest scale in one
+            # sum, up to 16 times its scale's in the other; the output's own rounding.
+            lifted = k.abs() + 128 * sk[at, g][:, None]
+            most = (row.abs() @ lifted.t()).masked_fill(~sees, 0).amax(1) * abs(scale)
+            score, count = (dim + 16) * 2.0 ** -24 * (most + 8), sees.sum(1)
+            largest = sv[at, g].expand_as(sees).masked_fill(~sees, 0).amax(1)
+            bound[to, h] = (w @ v.abs()) * (2 * score + 2.0 ** -11 + 2.0 ** -20 + count * 2.0 ** -21)[:, None] \
+                + (count * 2.0 ** -25 * 127 * largest)[:, None] + half_step(q.dtype) * out[to, h].abs()
     return out, bound
 
 
@@ -97,7 +95,10 @@ def make(gpu, lengths, kv_heads, page, dim, seed, spare=3, value_scale=1.0):
     return layer.KVCache(*(t.to(gpu) for t in (*codes, *scales))), table
 
 
-def run(q, cache, table, lengths, starts, gpu, **kw):
+def run(q, cache, table, lengths, starts, gpu, width=0, **kw):
+    """width: tokens that the table has room for at least; with long tables other kernels take the same rows."""
+    if width > table.shape[1] * cache.k.shape[2]:
+        table = torch.nn.functional.pad(table, (0, -(-width // cache.k.shape[2]) - table.shape[1]), value=-1)
     most = max((b - a for a, b in zip(starts, starts[1:])), default=0)
     return layer.cache_attention(q, cache, table.to(gpu), torch.tensor(lengths, dtype=torch.int32, device=gpu),
                                  starts=torch.tensor(starts, dtype=torch.int32, device=gpu), max_rows=kw.pop("max_rows", most), **kw)
@@ -370,8 +371,12 @@ def test_attention_in_parts(gpu, heads, kv_heads, dim, rows, length, window):
     compare(got, *attend64(q, cache, table, lengths, starts_of(n), dim ** -0.5, True, window))
 
 
-@pytest.mark.parametrize("rows", [1, 40])
-def test_sharp_scores(gpu, rows):
+# Rows of a sequence with two heads a key head, and the table's room: 16 and 32 columns a workgroup, 64, 128 and 256.
+FORMS = [(1, 0), (9, 0), (40, 0), (40, 2000), (68, 5000)]
+
+
+@pytest.mark.parametrize("rows,width", FORMS)
+def test_sharp_scores(gpu, rows, width):
     """Scores tens of steps of the running maximum apart, rising and falling along the tokens; sign and size of the scale."""
     lengths = [700]
     cache, table = make(gpu, lengths, 2, 16, 64, seed=8)
@@ -381,13 +386,13 @@ def test_sharp_scores(gpu, rows):
     for scales in (cache.k_scales * 3, cache.k_scales * ramp, cache.k_scales * (3.02 - ramp)):
         c = cache._replace(k_scales=scales)
         for scale in (0.125, -0.125, 0.0, 1e-30):
-            got = run(q, c, table, lengths, [0, rows], gpu, scale=scale)
+            got = run(q, c, table, lengths, [0, rows], gpu, width, scale=scale)
             compare(got, *attend64(q, c, table, lengths, [0, rows], scale, True, 0))
 
 
-@pytest.mark.parametrize("rows", [1, 40])
+@pytest.mark.parametrize("rows,width", FORMS)
 @pytest.mark.parametrize("spread", [2.0 ** 20, 2.0 ** 60, 2.0 ** 90])
-def test_pages_of_very_different_values(gpu, rows, spread):
+def test_pages_of_very_different_values(gpu, rows, width, spread):
     """Zero pages and small ones beside large ones: each row is right to its own terms."""
     lengths = [200]
     cache, table = make(gpu, lengths, 1, 16, 64, seed=21)
@@ -398,13 +403,13 @@ def test_pages_of_very_different_values(gpu, rows, spread):
         v[order[:1]] = 0
         c = cache._replace(v_scales=vs, v=v)
         q = queries(rows, 2, 64, torch.bfloat16, gpu, seed=2)
-        got = run(q, c, table, lengths, [0, rows], gpu)
+        got = run(q, c, table, lengths, [0, rows], gpu, width)
         compare(got, *attend64(q, c, table, lengths, [0, rows], 0.125, True, 0))
 
 
 @pytest.mark.parametrize("dtype", DT)
-@pytest.mark.parametrize("rows", [1, 40])
-def test_queries_of_any_size(gpu, dtype, rows):
+@pytest.mark.parametrize("rows,width", FORMS)
+def test_queries_of_any_size(gpu, dtype, rows, width):
     """Halves as they are, bf16 from its smallest normals to 2^100: products stay exact."""
     lengths = [90]
     cache, table = make(gpu, lengths, 1, 32, 64, seed=30)
@@ -413,14 +418,14 @@ def test_queries_of_any_size(gpu, dtype, rows):
         scale = float(torch.tensor(0.125 / size, dtype=torch.float32))
         if not math.isfinite(scale * 1.5):
             continue
-        got = run(q, cache, table, lengths, [0, rows], gpu, scale=scale)
+        got = run(q, cache, table, lengths, [0, rows], gpu, width, scale=scale)
         compare(got, *attend64(q, cache, table, lengths, [0, rows], scale, True, 0))
 
 
-@pytest.mark.parametrize("rows", [1, 9, 40])
-def test_not_finite_where_nothing_is_seen(gpu, rows):
+@pytest.mark.parametrize("rows,width", FORMS)
+def test_not_finite_where_nothing_is_seen(gpu, rows, width):
     """NaN scales of pages that no row, or only later rows, see; unused pages and entries; NaN queries of one row."""
-    page, lengths = 16, [100, 50]
+    page, lengths = 16, [100, max(50, rows + 2)]
     cache, table = make(gpu, lengths, 2, page, 64, seed=40)
     starts, n = [0, rows, 2 * rows], 2 * rows
     q = queries(n, 4, 64, torch.bfloat16, gpu, seed=4)
@@ -429,44 +434,44 @@ def test_not_finite_where_nothing_is_seen(gpu, rows):
     ks[free], vs[free] = math.nan, math.inf
     c = cache._replace(k_scales=ks, v_scales=vs)
     want, bound = attend64(q, cache, table, lengths, starts, 0.125, True, 0)
-    compare(run(q, c, table, lengths, starts, gpu), want, bound)
+    compare(run(q, c, table, lengths, starts, gpu, width), want, bound)
     # A poisoned page reaches the rows that see it, and no other.
     bad = c._replace(v_scales=vs.clone(), k_scales=ks.clone())
     bad.v_scales[table[0, 6]] = math.nan  # tokens 96 ..
     bad.k_scales[table[1, 0]] = math.nan  # tokens 0 .. 15
-    got = run(q, bad, table, lengths, starts, gpu).cpu()
+    got = run(q, bad, table, lengths, starts, gpu, width).cpu()
     position = torch.arange(100 - rows, 100)
     first = got[:rows]
     assert bool(torch.isnan(first[position >= 96]).all())
     if (position < 96).any():
         compare(first[position < 96], want[:rows][position < 96], bound[:rows][position < 96])
     assert bool(torch.isnan(got[rows:]).all())
-    windowed = run(q, bad, table, lengths, starts, gpu, window=3)[rows:].cpu()  # rows past token 18 see nothing of page 0
+    windowed = run(q, bad, table, lengths, starts, gpu, width, window=3)[rows:].cpu()  # rows past token 18 see nothing of page 0
     w, bd = attend64(q, cache, table, lengths, starts, 0.125, True, 3)
-    far = torch.arange(50 - rows, 50) >= 18
+    far = torch.arange(lengths[1] - rows, lengths[1]) >= 18
     compare(windowed[far], w[rows:][far], bd[rows:][far])
     q2 = q.clone()
     q2[0, 1] = math.nan
-    got = run(q2, c, table, lengths, starts, gpu).cpu()
+    got = run(q2, c, table, lengths, starts, gpu, width).cpu()
     assert bool(torch.isnan(got[0, 1]).all())
     keep = torch.ones(n, 4, dtype=torch.bool)
     keep[0, 1] = False
     compare(got[keep], want[keep], bound[keep])
 
 
-@pytest.mark.parametrize("rows", [1, 40])
-def test_bad_pages_and_odd_batches(gpu, rows):
+@pytest.mark.parametrize("rows,width", FORMS)
+def test_bad_pages_and_odd_batches(gpu, rows, width):
     page, lengths = 16, [100, 100, 64]
     cache, table = make(gpu, lengths, 1, page, 64, seed=50)
     table[0, 2], table[1, 6], table[2, 0] = -1, 10 ** 9, cache.k.shape[0]
     q = queries(3 * rows, 2, 64, torch.float16, gpu, seed=5)
     starts = [0, rows, 2 * rows, 3 * rows]
-    compare(run(q, cache, table, lengths, starts, gpu), *attend64(q, cache, table, lengths, starts, 0.125, True, 0))
+    compare(run(q, cache, table, lengths, starts, gpu, width), *attend64(q, cache, table, lengths, starts, 0.125, True, 0))
     none = torch.full_like(table, -1)
-    assert not run(q, cache, none, lengths, starts, gpu).any()
+    assert not run(q, cache, none, lengths, starts, gpu, width).any()
     # Lengths past the table and below zero; starts that no batch has: nothing leaves the arrays.
-    run(q, cache, table, [10 ** 9, -4, 100], starts, gpu)
-    run(q, cache, table, lengths, [5, -3, 1 << 30, 2], gpu, max_rows=rows)
+    run(q, cache, table, [10 ** 9, -4, 100], starts, gpu, width)
+    run(q, cache, table, lengths, [5, -3, 1 << 30, 2], gpu, width, max_rows=rows)
     torch.cuda.synchronize()
 
 
