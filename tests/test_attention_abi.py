@@ -162,6 +162,8 @@ def test_read_rejects(kw, code, msg):
     (dict(window=3, causal=0), 1, "causal"),
     (dict(scale=math.nan), 1, "scale"),
     (dict(scale=math.inf), 1, "scale"),
+    (dict(scale=3e38), 1, "scale"),  # past fp32 in the exponent's base
+    (dict(c=cache(kv_heads=1), rows=(1 << 22) - 1, heads=1024, b=batch(max_rows=(1 << 22) - 1)), 2, "2^30"),
     (dict(q=None), 1, "q is null"),
     (dict(out=None), 1, "out is null"),
     (dict(out=P + 9 * STEP + 2), 1, "aligned"),

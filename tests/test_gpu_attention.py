@@ -407,6 +407,22 @@ def test_pages_of_very_different_values(gpu, rows, width, spread):
         compare(got, *attend64(q, c, table, lengths, [0, rows], 0.125, True, 0))
 
 
+@pytest.mark.parametrize("rows,width", FORMS)
+def test_scales_of_zero(gpu, rows, width):
+    """Pages that hold zeros by their scale (never written, say) take their part of the weight and add nothing; so do all."""
+    lengths = [200]
+    cache, table = make(gpu, lengths, 1, 16, 64, seed=22)
+    used = table[0].long().to(gpu)
+    q = queries(rows, 2, 64, torch.bfloat16, gpu, seed=2)
+    for zero_k, zero_v in ((used[::2], used[:0]), (used[:0], used[1::2]), (used[:4], used[:4]), (used[5:], used[5:]), (used, used)):
+        ks, vs = cache.k_scales.clone(), cache.v_scales.clone()
+        ks[zero_k], vs[zero_v] = 0, 0
+        c = cache._replace(k_scales=ks, v_scales=vs)
+        want, bound = attend64(q, c, table, lengths, [0, rows], 0.125, True, 0)
+        # a value scale below 2^-100 counts as that: 128 of it at most
+        compare(run(q, c, table, lengths, [0, rows], gpu, width), want, bound + 2.0 ** -93)
+
+
 @pytest.mark.parametrize("dtype", DT)
 @pytest.mark.parametrize("rows,width", FORMS)
 def test_queries_of_any_size(gpu, dtype, rows, width):

@@ -86,7 +86,7 @@ __device__ __forceinline__ int tokens_of(const AttentionArgs& a, const KvSeq& s)
 // tokens are all of them where the tiles fill the card by themselves, else such that there
 // are at most a.target items: the batch's tokens (of every tile) over a.target where that
 // comes out, else over a.target less one a tile, which always does (the sums' fp32 rounding is
-// below the allowance of 2^-18). `tiles_cut` is the batch's number of tiles where they are
+// below the allowance of 2^-18; a chunk of 2^30 is all of any sequence). `tiles_cut` is the batch's number of tiles where they are
 // cut, else 0.
 __device__ Item find_item(const AttentionArgs& a, int columns, int index, int& tiles_cut) {
   const int lane = threadIdx.x & 63;
@@ -111,7 +111,7 @@ __device__ Item find_item(const AttentionArgs& a, int columns, int index, int& t
     const float tiles = over_batch([](float t, int) { return t; });
     if (tiles < (float)a.target) {
       const float tokens = over_batch([](float t, int n) { return t * (float)n; }) * (1.0f + 0x1p-18f);
-      auto chunk_for = [&](float parts) { return max(a.min_chunk, 64 * ((int)fminf(tokens / (64.0f * parts), 0x1p23f) + 1)); };
+      auto chunk_for = [&](float parts) { return max(a.min_chunk, 64 * ((int)fminf(tokens / (64.0f * parts), 0x1p24f - 1.0f) + 1)); };
       chunk = chunk_for((float)a.target);
       const float items = over_batch([&](float t, int n) { return t * (float)max(1, (n + chunk - 1) / chunk); });
       if (items > (float)a.target) chunk = chunk_for((float)a.target - tiles);
@@ -224,7 +224,8 @@ __device__ __forceinline__ float unit_of(float scale, float inverse) {
   static_assert(kKeyUnit == 0x1p24f, "two factors of 2^12");
   return fabsf(scale) * (inverse * 0x1p12f) * 0x1p12f;
 }
-// A unit so small that no score counts, but not zero: a hidden score, -inf, stays that.
+// A unit so small that no score counts, but not zero: a hidden score, -inf, stays that. So for a
+// page's value scale, which needs a logarithm and an inverse: a page never written holds zeros.
 __device__ __forceinline__ float not_zero(float unit) { return unit < 0x1p-100f ? 0x1p-100f : unit; }
 
 // Sum of eight halves on top of `sum`.
@@ -452,7 +453,7 @@ __global__ __launch_bounds__(256, D == 64 ? 7 - 2 * NC : 4 - NC) void attention_
       }
     }
     if (more) few_load_keys<D>(a, kv_head, token + 128, next.k, t);
-    const float lv = __builtin_amdgcn_logf(scale.y), inverse_v = __builtin_amdgcn_rcpf(scale.y);
+    const float lv = __builtin_amdgcn_logf(not_zero(scale.y)), inverse_v = __builtin_amdgcn_rcpf(not_zero(scale.y));
     const bool there = is_page(a.b, page.v), whole = token >= all_lo && token + 32 <= all_hi && !__any(!there);
     f16x8_t w[NC];
 #pragma unroll
@@ -656,7 +657,8 @@ struct Stage {
   // float4 of the wave's 16 tokens: key scale, log2 of the value scale, its inverse, whether there is a page.
   __device__ static void store_scales(const Staged<D>& t, float4* to) {
     // The same from every lane: no branch among the matrix instructions.
-    to[wave()] = make_float4(t.ks, __builtin_amdgcn_logf(t.vs), __builtin_amdgcn_rcpf(t.vs), t.there ? 1.0f : 0.0f);
+    const float vs = not_zero(t.vs);
+    to[wave()] = make_float4(t.ks, __builtin_amdgcn_logf(vs), __builtin_amdgcn_rcpf(vs), t.there ? 1.0f : 0.0f);
   }
   __device__ static void store(const Staged<D>& t, f16x8_t* keys_to, f16x8_t* values_to, float4* scales) {
 #pragma unroll

@@ -72,7 +72,9 @@ KvBatchArgs need_batch(const tfm_kv_cache* c, const tfm_kv_batch* b, int64_t row
 int group_of(int32_t heads, const KvBatchArgs& b) {
   need_heads(heads);
   need(heads % b.kv_heads == 0, "heads must be a multiple of kv_heads");
-  return heads / b.kv_heads;
+  const int group = heads / b.kv_heads;
+  if ((int64_t)b.rows * group > (1 << 30)) fail(TFM_E_UNSUPPORTED, "rows * heads / kv_heads past 2^30 is not built");
+  return group;
 }
 
 AttentionPlan plan_of(int64_t rows, int32_t heads, int32_t window, int32_t head_dim, const KvBatchArgs& b) {
@@ -213,9 +215,10 @@ int tfm_cache_attention(const void* q, int64_t row_stride, int64_t head_stride, 
     need_storage(dtype);
     need(window >= 0, "window must not be negative");
     need(causal || window == 0, "a window needs causal");
-    need(scale - scale == 0.0f, "scale must be finite");
     CacheSpans at{};
     AttentionArgs a{};
+    a.scale = (float)(scale * kLog2e);
+    need(a.scale - a.scale == 0.0f, "scale must be finite, times log2(e) too");
     a.b = need_batch(cache, batch, rows, &at);
     a.group = group_of(heads, a.b);
     if (rows == 0 || batch->sequences == 0 || batch->max_rows == 0) return;
@@ -235,7 +238,6 @@ int tfm_cache_attention(const void* q, int64_t row_stride, int64_t head_stride, 
     a.q_row = row_stride;
     a.q_head = head_stride;
     a.heads = heads;
-    a.scale = (float)(scale * kLog2e);
     a.causal = causal != 0;
     a.window = window;
     a.min_chunk = plan.min_chunk;
