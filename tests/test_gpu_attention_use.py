@@ -105,6 +105,34 @@ def test_pages_past_32_bits(gpu):
         compare(got, *attend64(q, small, local, lengths, [0, take, 2 * take], dim ** -0.5, True, 0))
 
 
+@pytest.mark.parametrize("dtype,sequences,rows,kv_heads,page,dim,pairs,interleaved", [
+    (BF16, 40, 350, 7, 16, 64, 32, False),    # four heads a workgroup
+    (F16, 40, 200, 7, 16, 64, 8, True),       # two
+    (F16, 25, 600, 5, 256, 128, 64, False),   # four
+    (BF16, 38, 520, 3, 64, 128, 24, True),    # two, of two items a thread
+    (BF16, 30, 100, 7, 32, 128, 0, False),    # two
+])
+def test_appends_of_many_heads(gpu, dtype, sequences, rows, kv_heads, page, dim, pairs, interleaved):
+    """Heads that share a workgroup get the bits that they get alone, on new pages and on pages that held tokens."""
+    g = torch.Generator().manual_seed(rows)
+    first = [(31 * i) % rows for i in range(sequences)]
+    second = [rows if i == 3 else (17 * i + 5) % (rows + 1) for i in range(sequences)]
+    lengths = [a + b for a, b in zip(first, second)]
+    cache, table = make(gpu, lengths, kv_heads, page, dim, seed=rows)
+    alone = [layer.KVCache(*(t[:, h:h + 1].contiguous() for t in cache)) for h in range(kv_heads)]
+    table, f = table.to(gpu), None
+    if pairs:
+        f, _ = layer.rotary_frequencies(pairs, device=gpu)
+    for step, (n, to) in enumerate(((first, first), (second, lengths))):
+        k, v = ((torch.randn((sum(n), kv_heads, dim), generator=g) * (1 + step)).to(dtype).to(gpu) for _ in "kv")
+        kw = dict(starts=i32(starts_of(n), gpu), max_rows=rows, frequencies=f, interleaved=interleaved)
+        layer.cache_append(k, v, cache, table, i32(to, gpu), **kw)
+        for h, one in enumerate(alone):
+            layer.cache_append(k[:, h:h + 1], v[:, h:h + 1], one, table, i32(to, gpu), **kw)
+            for all_heads, t in zip(cache, one):
+                assert torch.equal(all_heads[:, h:h + 1], t)
+
+
 def test_odd_rotary_widths(gpu):
     """Items with fewer than eight pairs or copied channels, in place and into wider rows, every shape of the ends."""
     g = torch.Generator().manual_seed(0)

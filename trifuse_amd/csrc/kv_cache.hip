@@ -244,10 +244,15 @@ void append(const KvAppendArgs& a, hipStream_t s) {
   const int page = 1 << a.b.page_shift;
   const int slots = (a.b.max_rows + page - 2) / page + 1;  // pages that max_rows tokens can meet
   const uint32_t units = (uint32_t)a.b.sequences * slots;
-  // Enough pages: four heads share their angles (16000 tokens of 16 heads of 128
-  // written and read back: 58 to 51 us).
-  if ((int64_t)units * a.b.kv_heads >= 2048)
+  // Enough waves: two or four heads share their angles. Tokens of 16 heads of 128, written, us with 1, 2 and 4: 4000
+  // in pages of 16 (16000 waves) 17.5, 16.9, 15.2; in pages of 256, two items a thread (8700) 20.9, 18.6, 24.3, of 64
+  // (8200) 17.5, 18.4, 17.2; 1200 in pages of 16 (8200) 10.2, 9.8, 12.1, of 64 (6100) 11.2, 11.9, 15.4.
+  const int items = page * D / 16, threads = items <= 256 ? items : items / 2;
+  const int64_t waves = (int64_t)units * a.b.kv_heads * 2 * (threads / 64);
+  if (waves >= 12288)
     append<F16, D, 4>(a, units, slots, s);
+  else if (waves > (items <= 256 ? 7168 : 8192))
+    append<F16, D, 2>(a, units, slots, s);
   else
     append<F16, D, 1>(a, units, slots, s);
 }
