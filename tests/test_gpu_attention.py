@@ -95,13 +95,17 @@ def make(gpu, lengths, kv_heads, page, dim, seed, spare=3, value_scale=1.0):
     return layer.KVCache(*(t.to(gpu) for t in (*codes, *scales))), table
 
 
-def run(q, cache, table, lengths, starts, gpu, width=0, **kw):
-    """width: tokens that the table has room for at least; with long tables other kernels take the same rows."""
+def run(q, cache, table, lengths, starts, gpu, width=0, spare=0, **kw):
+    """width: tokens that the table has room for at least, spare: rows (NaN) behind the last sequence's; with long tables or
+    many rows other kernels take the same sequences."""
     if width > table.shape[1] * cache.k.shape[2]:
         table = torch.nn.functional.pad(table, (0, -(-width // cache.k.shape[2]) - table.shape[1]), value=-1)
     most = max((b - a for a, b in zip(starts, starts[1:])), default=0)
-    return layer.cache_attention(q, cache, table.to(gpu), torch.tensor(lengths, dtype=torch.int32, device=gpu),
-                                 starts=torch.tensor(starts, dtype=torch.int32, device=gpu), max_rows=kw.pop("max_rows", most), **kw)
+    rows = q.shape[0]
+    q = torch.cat([q, q.new_full((spare,) + q.shape[1:], math.nan)]) if spare else q
+    out = layer.cache_attention(q, cache, table.to(gpu), torch.tensor(lengths, dtype=torch.int32, device=gpu),
+                                starts=torch.tensor(starts, dtype=torch.int32, device=gpu), max_rows=kw.pop("max_rows", most), **kw)
+    return out[:rows] if spare else out
 
 
 def queries(rows, heads, dim, dtype, gpu, seed, sigma=1.0):
@@ -371,14 +375,15 @@ def test_attention_in_parts(gpu, heads, kv_heads, dim, rows, length, window):
     compare(got, *attend64(q, cache, table, lengths, starts_of(n), dim ** -0.5, True, window))
 
 
-# Rows of a sequence with two heads a key head, and the table's room: 16 and 32 columns a workgroup, 64, 128 and 256.
-FORMS = [(1, 0), (9, 0), (40, 0), (40, 2000), (68, 5000)]
+# Rows of a sequence with two heads a key head, the table's room, rows behind the batch: one kernel of 16 columns a workgroup,
+# one of 32 (with few and many rows), and tiles of 64, 128 and 256.
+FORMS = [(1, 0, 0), (9, 0, 0), (40, 0, 0), (40, 0, 4500), (40, 500000, 0), (68, 500000, 0)]
 
 
-@pytest.mark.parametrize("rows,width", FORMS)
-def test_sharp_scores(gpu, rows, width):
+@pytest.mark.parametrize("rows,width,spare", FORMS)
+def test_sharp_scores(gpu, rows, width, spare):
     """Scores tens of steps of the running maximum apart, rising and falling along the tokens; sign and size of the scale."""
-    lengths = [700]
+    lengths = [390 if spare else 700]
     cache, table = make(gpu, lengths, 2, 16, 64, seed=8)
     ramp = torch.ones((cache.k_scales.shape[0], 1), device=gpu)
     ramp[table[0].long(), 0] = torch.linspace(0.02, 3.0, table.shape[1], device=gpu)
@@ -386,13 +391,13 @@ def test_sharp_scores(gpu, rows, width):
     for scales in (cache.k_scales * 3, cache.k_scales * ramp, cache.k_scales * (3.02 - ramp)):
         c = cache._replace(k_scales=scales)
         for scale in (0.125, -0.125, 0.0, 1e-30):
-            got = run(q, c, table, lengths, [0, rows], gpu, width, scale=scale)
+            got = run(q, c, table, lengths, [0, rows], gpu, width, spare, scale=scale)
             compare(got, *attend64(q, c, table, lengths, [0, rows], scale, True, 0))
 
 
-@pytest.mark.parametrize("rows,width", FORMS)
+@pytest.mark.parametrize("rows,width,spare", FORMS)
 @pytest.mark.parametrize("spread", [2.0 ** 20, 2.0 ** 60, 2.0 ** 90])
-def test_pages_of_very_different_values(gpu, rows, width, spread):
+def test_pages_of_very_different_values(gpu, rows, width, spare, spread):
     """Zero pages and small ones beside large ones: each row is right to its own terms."""
     lengths = [200]
     cache, table = make(gpu, lengths, 1, 16, 64, seed=21)
@@ -403,12 +408,12 @@ def test_pages_of_very_different_values(gpu, rows, width, spread):
         v[order[:1]] = 0
         c = cache._replace(v_scales=vs, v=v)
         q = queries(rows, 2, 64, torch.bfloat16, gpu, seed=2)
-        got = run(q, c, table, lengths, [0, rows], gpu, width)
+        got = run(q, c, table, lengths, [0, rows], gpu, width, spare)
         compare(got, *attend64(q, c, table, lengths, [0, rows], 0.125, True, 0))
 
 
-@pytest.mark.parametrize("rows,width", FORMS)
-def test_scales_of_zero(gpu, rows, width):
+@pytest.mark.parametrize("rows,width,spare", FORMS)
+def test_scales_of_zero(gpu, rows, width, spare):
     """Pages that hold zeros by their scale (never written, say) take their part of the weight and add nothing; so do all."""
     lengths = [200]
     cache, table = make(gpu, lengths, 1, 16, 64, seed=22)
@@ -420,12 +425,12 @@ def test_scales_of_zero(gpu, rows, width):
         c = cache._replace(k_scales=ks, v_scales=vs)
         want, bound = attend64(q, c, table, lengths, [0, rows], 0.125, True, 0)
         # a value scale below 2^-100 counts as that: 128 of it at most
-        compare(run(q, c, table, lengths, [0, rows], gpu, width), want, bound + 2.0 ** -93)
+        compare(run(q, c, table, lengths, [0, rows], gpu, width, spare), want, bound + 2.0 ** -93)
 
 
 @pytest.mark.parametrize("dtype", DT)
-@pytest.mark.parametrize("rows,width", FORMS)
-def test_queries_of_any_size(gpu, dtype, rows, width):
+@pytest.mark.parametrize("rows,width,spare", FORMS)
+def test_queries_of_any_size(gpu, dtype, rows, width, spare):
     """Halves as they are, bf16 from its smallest normals to 2^100: products stay exact."""
     lengths = [90]
     cache, table = make(gpu, lengths, 1, 32, 64, seed=30)
@@ -434,12 +439,12 @@ def test_queries_of_any_size(gpu, dtype, rows, width):
         scale = float(torch.tensor(0.125 / size, dtype=torch.float32))
         if not math.isfinite(scale * 1.5):
             continue
-        got = run(q, cache, table, lengths, [0, rows], gpu, width, scale=scale)
+        got = run(q, cache, table, lengths, [0, rows], gpu, width, spare, scale=scale)
         compare(got, *attend64(q, cache, table, lengths, [0, rows], scale, True, 0))
 
 
-@pytest.mark.parametrize("rows,width", FORMS)
-def test_not_finite_where_nothing_is_seen(gpu, rows, width):
+@pytest.mark.parametrize("rows,width,spare", FORMS)
+def test_not_finite_where_nothing_is_seen(gpu, rows, width, spare):
     """NaN scales of pages that no row, or only later rows, see; unused pages and entries; NaN queries of one row."""
     page, lengths = 16, [100, max(50, rows + 2)]
     cache, table = make(gpu, lengths, 2, page, 64, seed=40)
@@ -450,44 +455,44 @@ def test_not_finite_where_nothing_is_seen(gpu, rows, width):
     ks[free], vs[free] = math.nan, math.inf
     c = cache._replace(k_scales=ks, v_scales=vs)
     want, bound = attend64(q, cache, table, lengths, starts, 0.125, True, 0)
-    compare(run(q, c, table, lengths, starts, gpu, width), want, bound)
+    compare(run(q, c, table, lengths, starts, gpu, width, spare), want, bound)
     # A poisoned page reaches the rows that see it, and no other.
     bad = c._replace(v_scales=vs.clone(), k_scales=ks.clone())
     bad.v_scales[table[0, 6]] = math.nan  # tokens 96 ..
     bad.k_scales[table[1, 0]] = math.nan  # tokens 0 .. 15
-    got = run(q, bad, table, lengths, starts, gpu, width).cpu()
+    got = run(q, bad, table, lengths, starts, gpu, width, spare).cpu()
     position = torch.arange(100 - rows, 100)
     first = got[:rows]
     assert bool(torch.isnan(first[position >= 96]).all())
     if (position < 96).any():
         compare(first[position < 96], want[:rows][position < 96], bound[:rows][position < 96])
     assert bool(torch.isnan(got[rows:]).all())
-    windowed = run(q, bad, table, lengths, starts, gpu, width, window=3)[rows:].cpu()  # rows past token 18 see nothing of page 0
+    windowed = run(q, bad, table, lengths, starts, gpu, width, spare, window=3)[rows:].cpu()  # rows past token 18 see nothing of page 0
     w, bd = attend64(q, cache, table, lengths, starts, 0.125, True, 3)
     far = torch.arange(lengths[1] - rows, lengths[1]) >= 18
     compare(windowed[far], w[rows:][far], bd[rows:][far])
     q2 = q.clone()
     q2[0, 1] = math.nan
-    got = run(q2, c, table, lengths, starts, gpu, width).cpu()
+    got = run(q2, c, table, lengths, starts, gpu, width, spare).cpu()
     assert bool(torch.isnan(got[0, 1]).all())
     keep = torch.ones(n, 4, dtype=torch.bool)
     keep[0, 1] = False
     compare(got[keep], want[keep], bound[keep])
 
 
-@pytest.mark.parametrize("rows,width", FORMS)
-def test_bad_pages_and_odd_batches(gpu, rows, width):
+@pytest.mark.parametrize("rows,width,spare", FORMS)
+def test_bad_pages_and_odd_batches(gpu, rows, width, spare):
     page, lengths = 16, [100, 100, 64]
     cache, table = make(gpu, lengths, 1, page, 64, seed=50)
     table[0, 2], table[1, 6], table[2, 0] = -1, 10 ** 9, cache.k.shape[0]
     q = queries(3 * rows, 2, 64, torch.float16, gpu, seed=5)
     starts = [0, rows, 2 * rows, 3 * rows]
-    compare(run(q, cache, table, lengths, starts, gpu, width), *attend64(q, cache, table, lengths, starts, 0.125, True, 0))
+    compare(run(q, cache, table, lengths, starts, gpu, width, spare), *attend64(q, cache, table, lengths, starts, 0.125, True, 0))
     none = torch.full_like(table, -1)
-    assert not run(q, cache, none, lengths, starts, gpu, width).any()
+    assert not run(q, cache, none, lengths, starts, gpu, width, spare).any()
     # Lengths past the table and below zero; starts that no batch has: nothing leaves the arrays.
-    run(q, cache, table, [10 ** 9, -4, 100], starts, gpu, width)
-    run(q, cache, table, lengths, [5, -3, 1 << 30, 2], gpu, width, max_rows=rows)
+    run(q, cache, table, [10 ** 9, -4, 100], starts, gpu, width, spare)
+    run(q, cache, table, lengths, [5, -3, 1 << 30, 2], gpu, width, spare, max_rows=rows)
     torch.cuda.synchronize()
 
 

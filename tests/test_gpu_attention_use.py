@@ -22,14 +22,19 @@ def i32(values, gpu):
 # -- sizes that pick each kernel, and each way of sharing the work ---------------
 
 @pytest.mark.parametrize("dtype,heads,kv_heads,dim,page,rows,lengths,width,window", [
-    (BF16, 4, 2, 128, 64, [200, 131, 256], [2500, 131, 3001], 0, 0),       # 128 columns, in parts
-    (F16, 6, 2, 64, 16, [170, 43], [4500, 4200], 0, 0),                     # 256 columns, in parts
+    (BF16, 4, 2, 128, 64, [200, 131, 256], [2500, 131, 3001], 0, 0),       # 32 columns, in parts
+    (F16, 6, 2, 64, 16, [170, 43], [4500, 4200], 0, 0),
     (BF16, 2, 1, 128, 128, [250], [6000], 0, 1000),                         # of which the window leaves a few
-    (F16, 4, 4, 128, 32, [256, 255], [4900, 257], 0, 0),
-    (BF16, 32, 32, 64, 16, [700, 515, 1300, 513, 900, 200], [700, 600, 1300, 513, 950, 333], 0, 0),  # 256, whole
-    (F16, 24, 24, 128, 64, [1400, 700, 900], [1400, 700, 1000], 0, 129),
-    (F16, 2, 2, 64, 256, [1023], [1023], 0, 0),                             # 64 columns, each a half of the tokens
+    (F16, 2, 2, 64, 256, [1023], [1023], 0, 0),                             # 32 columns, whole
     (BF16, 3, 1, 128, 16, [5, 0, 90, 21], [1000, 16, 90, 900], 0, 65),
+    (F16, 12, 12, 128, 16, [380, 300], [380, 333], 0, 0),                   # 64 columns
+    (BF16, 24, 12, 64, 32, [130, 200, 60], [130, 390, 100], 0, 77),
+    (BF16, 4, 2, 128, 64, [150, 131, 140], [2500, 131, 3001], 100000, 0),   # 128 columns, in parts
+    (F16, 4, 4, 64, 16, [100, 43], [4500, 4200], 200000, 0),
+    (F16, 24, 24, 128, 64, [1400, 700, 900], [1400, 700, 1000], 0, 129),    # 128, whole
+    (F16, 6, 2, 64, 16, [170, 43], [4500, 4200], 200000, 0),                # 256, in parts
+    (BF16, 4, 4, 128, 32, [256, 255], [4900, 257], 50000, 0),
+    (BF16, 32, 32, 64, 16, [700, 515, 1300, 513, 900, 200], [700, 600, 1300, 513, 950, 333], 0, 0),  # 256, whole
 ])
 def test_tiles(gpu, dtype, heads, kv_heads, dim, page, rows, lengths, width, window):
     cache, table = make(gpu, lengths, kv_heads, page, dim, seed=sum(lengths))

@@ -25,7 +25,8 @@
 // Kernels. Few columns (decoding, drafts; up to 32): memory decides. Each wave takes
 // 32 tokens at a time straight from memory into registers: key codes as 16-byte pieces of
 // a row, value codes as D/16 bytes a lane of eight rows, transposed by byte permutes into
-// the product's operand. More columns: 256 a workgroup of eight waves, whose tiles of 128
+// the product's operand. So it is for more columns while all their workgroups are there at
+// once. Many: 256 a workgroup of eight waves, whose tiles of 128
 // tokens are converted to halves once on their way into LDS; 128 of four waves and tiles of
 // 64; or 64, where two waves share their columns and take a half of each tile.
 //
@@ -155,6 +156,14 @@ __device__ __forceinline__ void tell_join(const AttentionArgs& a, const Item& it
   if (tiles_cut && it.b >= 0 && it.part == 0)
     a.cut[1 + it.index] = make_int4(it.s.start, it.tile * columns, it.s.n * a.group, it.parts);
   if (tiles_cut && it.b >= 0 && it.part == 0) a.cut_entry[it.index] = it.entry;
+}
+
+// A sequence's last rows see the most tokens.
+__device__ __forceinline__ void longest_first(const AttentionArgs& a, int columns, Item& it) {
+  if (!a.causal) return;
+  const int tiles = tiles_of(a, it.s, columns);
+  it.entry += (tiles - 1 - 2 * it.tile) * it.parts;
+  it.tile = tiles - 1 - it.tile;
 }
 
 // A column of an item: its row and head, and the tokens [lo, hi) that it sees.
@@ -348,10 +357,11 @@ __global__ __launch_bounds__(256, D == 64 ? 7 - 2 * NC : 4 - NC) void attention_
   __shared__ float stat_m[4][COLS], stat_l[4][COLS];
   const int kv_head = blockIdx.x % a.b.kv_heads;
   int tiles_cut;
-  const Item it = find_item(a, COLS, blockIdx.x / a.b.kv_heads, tiles_cut);
+  Item it = find_item(a, COLS, blockIdx.x / a.b.kv_heads, tiles_cut);
   if (kv_head == 0) tell_join(a, it, COLS, tiles_cut);
   if (it.b < 0) return;
   const KvSeq& s = it.s;
+  longest_first(a, COLS, it);
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r = lane & 15, g = lane >> 4;
 
   // What the first tile needs is asked for before anything is waited for.
@@ -684,7 +694,7 @@ __device__ __forceinline__ f32x16_t zeros16() {
 // once.
 // PAIRS: two waves share 32 columns, and each takes one half of every 64 tokens: for prompts
 // whose columns are too few to fill the card otherwise, where the chain of tiles is what lasts
-// (512 rows of 16 heads 20.0 to 15.9 us).
+// (three of 200 rows and 16 heads 13.5 to 10.8 us).
 //
 // Bound: the matrix cores. 8192 rows of 16 heads of 128, causal, take 285 us (0.97 PFLOP/s);
 // the same kernel without exponentials, conversions and reads of LDS 217 (they cost 36, 17
@@ -704,11 +714,7 @@ __global__ __launch_bounds__(64 * WAVES, 2) void attention_tile_kernel(Attention
   if (kv_head == 0) tell_join(a, it, COLS, tiles_cut);
   if (it.b < 0) return;
   const KvSeq& s = it.s;
-  if (a.causal) {  // the longest first
-    const int tiles = tiles_of(a, s, COLS);
-    it.entry += (tiles - 1 - 2 * it.tile) * it.parts;
-    it.tile = tiles - 1 - it.tile;
-  }
+  longest_first(a, COLS, it);
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r = lane & 31, g = lane >> 5;
   const int half = PAIRS ? __builtin_amdgcn_readfirstlane(wave >> 1) : 0;  // the one that this wave takes
 
@@ -1111,6 +1117,23 @@ void launch_as(const AttentionPlan& p, const AttentionArgs& a, hipStream_t s) {
 
 }  // namespace
 
+// Whether the few kernel takes many columns sooner than the tile kernel. Its waves wait for nobody
+// and each takes its own tokens, 32 columns a workgroup, so a call lasts a quarter of the chain of
+// tiles while its workgroups are there at once or nearly; but each brings and converts its tokens
+// for 32 columns only, which is most of the work with heads of 128. Measured, us, tile and few:
+// - 16 heads of 128: a prompt of 512 rows 16.2 and 12.3, 900 27.8 and 17.3, 2000 48.9 and 45.4, 4000
+//   121 and 126; 300 rows behind 1500 tokens 28.4 and 25.4, behind 6000 41 and 44; 900 behind 900 38
+//   and 32, behind 2500 49 and 51; 8 of 100 rows 9.5 and 11.6, behind 900 31 and 24; 16 of 100 rows
+//   behind 900 40 and 44; 4 of 500 behind 200 36 and 33, behind 900 48 and 50.
+// - 24 heads of 64 over 8: 2000 rows 49 and 35, 4000 87 and 103; 4 of 500 20 and 22, behind 900 45 and
+//   41, behind 2500 84 and 75; 8 of 300 behind 900 43 and 47; 512 behind 2500 34 and 32, behind 8000 53
+//   and 62; 16 of 100 behind 200 16.5 and 19.1, behind 900 37 and 32.
+static bool few_suffice(int head_dim, int64_t n32, int64_t capacity, int64_t max_rows) {
+  if (n32 <= 512) return (n32 <= 256 || capacity >= 400) && n32 * capacity <= (head_dim == 64 ? 1200000 : 700000);
+  if (capacity < 600) return false;
+  return head_dim == 64 ? n32 <= 1536 : n32 <= 1024 && capacity <= 2 * max_rows;  // heads of 128: prompts
+}
+
 // How a call is cut. Measured on one card, us:
 // - few columns, least tokens of a part: 1 x 1407 tokens of 16 heads 9.8 with 128, 10.5 with 256,
 //   13.5 with 512 (one part 16.1).
@@ -1121,33 +1144,38 @@ void launch_as(const AttentionPlan& p, const AttentionArgs& a, hipStream_t s) {
 //   rows 45 against 63), or tiles are cut along many tokens (800 rows behind 30000 tokens, 32
 //   heads: 438 against 507; behind 500: 43 against 42).
 // - many columns, two waves to 32 of them (64 a workgroup): where 128 a workgroup would leave most
-//   compute units without one and their chain of tiles is short. 512 rows of 16 heads 20.0 to 15.9;
-//   behind 500 tokens 28.8 to 25.3, behind 2000 36.2 to 36.2 (8 key heads 31.2 to 34.4); 16 prompts
-//   of 40 rows 9.6 to 8.6, of 120 rows, 240 workgroups of 128 columns, 12.4 to 14.4.
+//   compute units without one and their chain of tiles is short. Three of 200 rows and 16 heads 13.5
+//   to 10.8, 8 of 60 rows behind 200 tokens, 4 key heads of 128, 16.0 to 13.0, 8 of 64 11.9 to 10.1;
+//   16 of 40 rows behind none 10.0 to 11.4 and 7.4 to 6.8; with 240 workgroups of 128, 12.4 to 14.4.
 // - many columns, least tokens of a part: 48 rows behind 4000 tokens 25 with 512, 36 with 1024;
 //   512 rows of a prompt 19.8 in one part, 22.5 in two.
+// - many columns in the few kernel, least tokens that are cut, and of a part: 300 rows behind 450
+//   tokens 21 in two parts, 14.9 in one; behind 1500 25.4 in parts of 512, 27.1 of 1024.
 AttentionPlan attention_plan(int64_t rows, int group, int kv_heads, int head_dim, int sequences, int max_rows,
                              int64_t capacity) {
   AttentionPlan p{};
   const int64_t most = (int64_t)max_rows * group, all = rows * group;
-  int resident;  // workgroups that the card holds at once
-  if (most <= 32) {
+  const int64_t n32 = (all + 31) / 32 * kv_heads, n128 = (all + 127) / 128 * kv_heads, n256 = (all + 255) / 256 * kv_heads;
+  int64_t whole;  // tokens from which on a sequence may be cut
+  int resident;   // workgroups that the card holds at once
+  if (most <= 32 || few_suffice(head_dim, n32, capacity, max_rows)) {
     p.columns = most <= 16 ? 16 : 32;
     resident = 256 * (head_dim == 64 ? 7 - p.columns / 8 : 4 - p.columns / 16);
-    p.min_chunk = 128;
+    p.min_chunk = most <= 32 ? 128 : 512;
+    whole = most <= 32 ? 128 : 1024;
   } else {
-    const int64_t n256 = (all + 255) / 256 * kv_heads, n128 = (all + 127) / 128 * kv_heads, rest = n128 % 512;
+    const int64_t rest = n128 % 512;
     const bool fits = 20 * ((most + 255) / 256 * 2) <= 23 * ((most + 127) / 128);
     const bool even = n256 >= 512 || (n256 < 256 ? capacity >= 4096
                                                  : 20 * ((n256 + 255) / 256) <= 23 * (n128 / 512) + (rest > 256 ? 23 : rest ? 13 : 0));
     p.columns = fits && even ? 256 : n128 <= 192 && capacity <= 1024 ? 64 : 128;
     resident = p.columns == 256 ? 256 : 512;
-    p.min_chunk = 512;
+    whole = p.min_chunk = 512;
   }
   p.target = std::max(1, resident / kv_heads);
   const int64_t tiles = std::min<int64_t>(all / p.columns + sequences, all);
   // Where the rows by themselves make enough tiles, or one workgroup reads so few tokens, none is cut.
-  p.split = capacity > p.min_chunk && all / p.columns < p.target;
+  p.split = capacity > whole && all / p.columns < p.target;
   p.items = (int)std::max<int64_t>(1, p.split ? std::max<int64_t>(tiles, p.target) : tiles);
   return p;
 }
