@@ -1032,7 +1032,7 @@ __device__ __forceinline__ float group_reduce(float v, float* part, F&& f) {
 constexpr int kJoinParts = 256;  // parts whose factors are held at once
 template <bool F16, int D, int EACH>
 __global__ __launch_bounds__(256) void attention_join_kernel(AttentionArgs a, int columns, int blocks) {
-  constexpr int GROUP = 256 / EACH, LANES = D / 4, WAYS = GROUP / LANES;
+  constexpr int GROUP = 256 / EACH, LANES = D / 4, WAYS = GROUP / LANES, AHEAD = 4;
   __shared__ float factors[EACH][kJoinParts];
   __shared__ float4 sums[256];
   __shared__ float part0[4], part1[4];
@@ -1046,6 +1046,11 @@ __global__ __launch_bounds__(256) void attention_join_kernel(AttentionArgs a, in
   const int at = blockIdx.x % blocks * EACH + of, column = info.y + at;
   const int parts = column < info.z ? info.w : 0;  // none where there is no column
   const int64_t slot = ((int64_t)entry * a.b.kv_heads + kv_head) * columns + at;
+  const float* sums_at = a.part_out + slot * D + d;
+  float4 ahead[AHEAD];  // asked for with the statistics
+#pragma unroll
+  for (int i = 0; i < AHEAD; ++i)
+    if (way + i * WAYS < parts) ahead[i] = *reinterpret_cast<const float4*>(sums_at + (way + i * WAYS) * step * D);
   float most = kLow;
   for (int p = t; p < parts; p += GROUP) most = fmaxf(most, a.part_ml[slot + p * step].x);
   most = group_reduce<GROUP>(most, part0, [](float x, float y) { return fmaxf(x, y); });
@@ -1060,15 +1065,20 @@ __global__ __launch_bounds__(256) void attention_join_kernel(AttentionArgs a, in
       total = __builtin_fmaf(ml.y, f, total);
     }
     __syncthreads();
-#pragma unroll 4
-    for (int p = way; p < n; p += WAYS) {
-      const float4 x = *reinterpret_cast<const float4*>(a.part_out + (slot + (p0 + p) * step) * D + d);
-      const float f = factors[of][p];
+    auto add = [&](const float4& x, float f) {
       v.x = __builtin_fmaf(x.x, f, v.x);
       v.y = __builtin_fmaf(x.y, f, v.y);
       v.z = __builtin_fmaf(x.z, f, v.z);
       v.w = __builtin_fmaf(x.w, f, v.w);
+    };
+    if (p0 == 0) {
+#pragma unroll
+      for (int i = 0; i < AHEAD; ++i)
+        if (way + i * WAYS < n) add(ahead[i], factors[of][way + i * WAYS]);
     }
+#pragma unroll 4
+    for (int p = way + (p0 == 0 ? AHEAD * WAYS : 0); p < n; p += WAYS)
+      add(*reinterpret_cast<const float4*>(sums_at + (p0 + p) * step * D), factors[of][p]);
     __syncthreads();
   }
   total = group_reduce<GROUP>(total, part1, [](float x, float y) { return x + y; });
