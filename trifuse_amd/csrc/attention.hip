@@ -1131,22 +1131,27 @@ void launch_as(const AttentionPlan& p, const AttentionArgs& a, hipStream_t s) {
 // and each takes its own tokens, 32 columns a workgroup, so a call lasts a quarter of the chain of
 // tiles while its workgroups are there at once or nearly; but each brings and converts its tokens
 // for 32 columns only, which is most of the work with heads of 128. Measured, us, tile and few:
-// - 16 heads of 128: a prompt of 512 rows 16.2 and 12.3, 900 27.8 and 17.3, 2000 48.9 and 45.4, 4000
-//   121 and 126; 300 rows behind 1500 tokens 28.4 and 25.4, behind 6000 41 and 44; 900 behind 900 38
-//   and 32, behind 2500 49 and 51; 8 of 100 rows 9.5 and 11.6, behind 900 31 and 24; 16 of 100 rows
-//   behind 900 40 and 44; 4 of 500 behind 200 36 and 33, behind 900 48 and 50.
-// - 24 heads of 64 over 8: 2000 rows 49 and 35, 4000 87 and 103; 4 of 500 20 and 22, behind 900 45 and
-//   41, behind 2500 84 and 75; 8 of 300 behind 900 43 and 47; 512 behind 2500 34 and 32, behind 8000 53
-//   and 62; 16 of 100 behind 200 16.5 and 19.1, behind 900 37 and 32.
-static bool few_suffice(int head_dim, int64_t n32, int64_t capacity, int64_t max_rows) {
-  if (n32 <= 512) return (n32 <= 256 || capacity >= 400) && n32 * capacity <= (head_dim == 64 ? 1200000 : 700000);
-  if (capacity < 600) return false;
-  return head_dim == 64 ? n32 <= 1536 : n32 <= 1024 && capacity <= 2 * max_rows;  // heads of 128: prompts
+// - 16 heads of 128: a prompt of 400 rows 16.2 and 12.3, 700 behind 100 tokens 21.7 and 16.6, behind
+//   1500 37.7 and 33.9, behind 3000 46.7 and 54.5; 8 of 60 rows behind 1000 30 and 19.5; 16 of 50
+//   behind 100 11.9 and 13.2, behind 1500 49 and 30.5; 8 of 150 behind 500 23.9 and 26.2, behind 1000
+//   44 and 34; 1300 behind 100 40.5 and 32.3, behind 1500 58.7 and 58.1; 4 of 1000 44 and 62.
+// - 24 heads of 64 over 8: 400 rows behind 500 18.5 and 12.7, behind 3000 32.0 and 32.4; 16 of 50
+//   behind 1000 32 and 19; 8 of 150 behind 100 11.7 and 14.6, behind 500 19.5 and 19.7, behind 3000 73
+//   and 56; 4 of 300 behind 1500 46 and 30; 1300 behind 1000 45 and 37; 3 of 1000 behind 500 45 and 49.
+static bool few_suffice(int head_dim, int64_t n32, int64_t capacity) {
+  if (n32 <= 512) return (n32 <= 256 || capacity >= 400) && n32 * capacity <= (head_dim == 64 ? 1200000 : 1000000);
+  if (head_dim == 64) return n32 <= 1536 && capacity >= 600;
+  return n32 <= 1024 && capacity > 1024 && n32 * capacity <= 1500000;
 }
 
 // How a call is cut. Measured on one card, us:
-// - few columns, least tokens of a part: 1 x 1407 tokens of 16 heads 9.8 with 128, 10.5 with 256,
-//   13.5 with 512 (one part 16.1).
+// - 32 columns at most, least tokens of a part: 1 x 1407 tokens of 16 heads 9.8 with 128, 10.5 with
+//   256, 13.5 with 512 (one part 16.1).
+// - The same, tokens from which on a sequence is cut, by the workgroups without (a launch and the join
+//   cost 3 to 5): 16 heads of 128, one token after 500 9.9 cut and 8.3 whole, after 800 9.8 and 10.9;
+//   16 sequences after 1100 19.3 and 15.4, after 2000 27 and 27; 32 after 3000 62 and 60; 24 heads of
+//   64 over 8, one after 800 9.8 and 8.5, after 1500 9.6 and 11.6; 64 after 2000 25.8 and 24.0; 300 rows
+//   behind 900 19.0 and 14.0, 512 behind 1500 25.8 and 22.3.
 // - many columns: four waves (two workgroups a compute unit) or eight (one, which brings and
 //   converts a tile for twice the columns, at 1.15 of the rate: 8192 rows of 16 heads 335 against
 //   289). Eight where a sequence's columns do not leave 1 / 1.15 of its tiles empty, and either
@@ -1157,10 +1162,11 @@ static bool few_suffice(int head_dim, int64_t n32, int64_t capacity, int64_t max
 //   compute units without one and their chain of tiles is short. Three of 200 rows and 16 heads 13.5
 //   to 10.8, 8 of 60 rows behind 200 tokens, 4 key heads of 128, 16.0 to 13.0, 8 of 64 11.9 to 10.1;
 //   16 of 40 rows behind none 10.0 to 11.4 and 7.4 to 6.8; with 240 workgroups of 128, 12.4 to 14.4.
-// - many columns, least tokens of a part: 48 rows behind 4000 tokens 25 with 512, 36 with 1024;
-//   512 rows of a prompt 19.8 in one part, 22.5 in two.
-// - many columns in the few kernel, least tokens that are cut, and of a part: 300 rows behind 450
-//   tokens 21 in two parts, 14.9 in one; behind 1500 25.4 in parts of 512, 27.1 of 1024.
+// - many columns, least tokens of a part: 48 rows behind 4000 tokens 25 with 512, 36 with 1024.
+// - more columns in the few kernel, least tokens of a part: 5 rows of 32 heads over 4 behind 1500 16.0
+//   with 512, 13.9 with 256; 48 rows of them behind 1500 16.6 and 19.9, behind 4000 23.1 and 23.8.
+// - tiles, tokens from which on they are cut: 24 heads of 64 over 8, 8 of 60 rows behind 500 17.4 cut and
+//   13.4 whole; 700 rows behind 100 19.5 and 17.1; of 128, 4 key heads, 16 of 50 behind 500 30 and 23.
 AttentionPlan attention_plan(int64_t rows, int group, int kv_heads, int head_dim, int sequences, int max_rows,
                              int64_t capacity) {
   AttentionPlan p{};
@@ -1168,11 +1174,12 @@ AttentionPlan attention_plan(int64_t rows, int group, int kv_heads, int head_dim
   const int64_t n32 = (all + 31) / 32 * kv_heads, n128 = (all + 127) / 128 * kv_heads, n256 = (all + 255) / 256 * kv_heads;
   int64_t whole;  // tokens from which on a sequence may be cut
   int resident;   // workgroups that the card holds at once
-  if (most <= 32 || few_suffice(head_dim, n32, capacity, max_rows)) {
+  if (most <= 32 || few_suffice(head_dim, n32, capacity)) {
     p.columns = most <= 16 ? 16 : 32;
     resident = 256 * (head_dim == 64 ? 7 - p.columns / 8 : 4 - p.columns / 16);
-    p.min_chunk = most <= 32 ? 128 : 512;
-    whole = most <= 32 ? 128 : 1024;
+    p.min_chunk = most <= 32 ? 128 : n32 * capacity <= 56000 ? 256 : 512;
+    const int64_t uncut = std::min<int64_t>(all / p.columns + sequences, sequences * ((most + p.columns - 1) / p.columns)) * kv_heads;
+    whole = head_dim == 64 ? 900 + 4 * uncut : 600 + 5 * uncut;
   } else {
     const int64_t rest = n128 % 512;
     const bool fits = 20 * ((most + 255) / 256 * 2) <= 23 * ((most + 127) / 128);
@@ -1180,7 +1187,8 @@ AttentionPlan attention_plan(int64_t rows, int group, int kv_heads, int head_dim
                                                  : 20 * ((n256 + 255) / 256) <= 23 * (n128 / 512) + (rest > 256 ? 23 : rest ? 13 : 0));
     p.columns = fits && even ? 256 : n128 <= 192 && capacity <= 1024 ? 64 : 128;
     resident = p.columns == 256 ? 256 : 512;
-    whole = p.min_chunk = 512;
+    p.min_chunk = 512;
+    whole = 1024;
   }
   p.target = std::max(1, resident / kv_heads);
   const int64_t tiles = std::min<int64_t>(all / p.columns + sequences, all);
