@@ -349,7 +349,8 @@ __device__ __forceinline__ void few_weigh(const uint32_t (&x)[8][W], const f16x8
 // before the end, where their sums meet in LDS. Registers instead of LDS, because each code is
 // used by one wave only; rows of an 8-bit product would be half the work, but the codes' bound is
 // memory: 64 sequences (2.1 GB of codes) in 320 us are 6.7 TB/s, and one of 1407 tokens 6.8 us,
-// of which a chain of loads (lengths, table, codes) is most.
+// of which a chain of loads (lengths, table, codes) is most. With more columns than fit one
+// workgroup the chain of tiles decides: 512 rows of 16 heads of 128, 256 workgroups, 12.3 us.
 template <bool F16, int D, int NC>
 __global__ __launch_bounds__(256, D == 64 ? 7 - 2 * NC : 4 - NC) void attention_few_kernel(AttentionArgs a) {
   constexpr int COLS = 16 * NC, NK = D / 32, NV = D / 16, PAD = D + 4;

@@ -224,6 +224,6 @@ def cache_attention(q: torch.Tensor, cache: KVCache, table: torch.Tensor, length
     lengths, starts and max_rows as in ``cache_append``, behind which it goes: row i of n of sequence b is at position
     lengths[b] - n + i, and sees tokens up to its own (causal) or all of its sequence, with window > 0 (causal) the
     last `window` of them. A row that sees none is zero; rows behind the last sequence are not written. scale: None
-    is head_dim ** -0.5. Pass max_rows with starts where it is known: it picks the kernel (up to 32 rows times query
-    heads a key head: the one that decodes)."""
+    is head_dim ** -0.5. Pass max_rows with starts where it is known: it picks the kernel, as the table's width does
+    (a table about as wide as the longest sequence is served best)."""
     return _enqueue("cache_attention", q, *cache, table, lengths, starts, max_rows, scale, causal, window, out)
