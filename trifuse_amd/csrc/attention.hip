@@ -75,12 +75,18 @@ struct Item {
   int index;  // of the tile in the batch
 };
 
+// The first token that a row at `position` sees. Rows stand before the first token too, and windows
+// are as long as an int: of a negative position nothing is taken off.
+__device__ __forceinline__ int lowest(const AttentionArgs& a, int position) {
+  return a.window ? max(0, max(position, 0) - a.window + 1) : 0;
+}
+
 // A sequence's tiles of columns, and tokens that some of its rows see.
 __device__ __forceinline__ int tiles_of(const AttentionArgs& a, const KvSeq& s, int columns) {
   return (s.n * a.group + columns - 1) / columns;
 }
 __device__ __forceinline__ int tokens_of(const AttentionArgs& a, const KvSeq& s) {
-  return max(s.len - (a.window ? max(0, s.first() - a.window + 1) : 0), 0);
+  return max(s.len - lowest(a, s.first()), 0);
 }
 
 // Item `index` of the batch. Every wave finds it by itself, a sequence a lane. A part's
@@ -179,7 +185,7 @@ __device__ __forceinline__ Column column_of(const AttentionArgs& a, const KvSeq&
   o.head = kv_head * a.group + c % a.group;
   // A column that is none has nothing written, and does not make a tile take the masked path.
   o.hi = a.causal && o.real ? min(s.len, position + 1) : s.len;
-  o.lo = a.window && o.real ? max(0, position - a.window + 1) : 0;
+  o.lo = o.real ? lowest(a, position) : 0;
   return o;
 }
 
@@ -190,7 +196,7 @@ __device__ __forceinline__ void part_of(const AttentionArgs& a, const KvSeq& s, 
   const int c1 = min(s.n * a.group, (it.tile + 1) * columns) - 1;
   const int first = s.first() + it.tile * columns / a.group, last = s.first() + c1 / a.group;
   const int hi = a.causal ? min(s.len, last + 1) : s.len;
-  const int lo = a.window ? max(0, first - a.window + 1) / step * step : 0;
+  const int lo = lowest(a, first) / step * step;
   const int each = ((max(hi - lo, 0) + it.parts - 1) / it.parts + step - 1) / step * step;
   from = min(lo + it.part * each, max(hi, 0));
   to = min(from + each, hi);
