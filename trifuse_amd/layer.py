@@ -19,7 +19,8 @@ the tfm_cache_* calls of include/trifuse_moe.h, which has the exact definitions)
 
 Tensors are torch tensors of one HIP device; work is enqueued on that device's
 current stream. There is no CPU fallback and no backward. Every sum, norm and
-softmax is held in fp32 (products in int32) and each output is rounded once.
+softmax statistic is held in fp32 (8-bit products in int32) and each output is
+rounded once; ``cache_attention`` multiplies with softmax weights as halves.
 """
 from __future__ import annotations
 
@@ -224,6 +225,7 @@ def cache_attention(q: torch.Tensor, cache: KVCache, table: torch.Tensor, length
     lengths, starts and max_rows as in ``cache_append``, behind which it goes: row i of n of sequence b is at position
     lengths[b] - n + i, and sees tokens up to its own (causal) or all of its sequence, with window > 0 (causal) the
     last `window` of them. A row that sees none is zero; rows behind the last sequence are not written. scale: None
-    is head_dim ** -0.5. Pass max_rows with starts where it is known: it picks the kernel, as the table's width does
+    is head_dim ** -0.5. Softmax weights are halves: 2^-11 of themselves, and a token more than 23 below a row's top
+    score (in nats) has none. Pass max_rows with starts where it is known: it picks the kernel, as the table's width does
     (a table about as wide as the longest sequence is served best)."""
     return _enqueue("cache_attention", q, *cache, table, lengths, starts, max_rows, scale, causal, window, out)
