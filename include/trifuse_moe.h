@@ -420,8 +420,8 @@ typedef struct tfm_kv_cache {
  * sequence are not read, and what they would write stays as it was. All arrays
  * are on the device and may change between replays of a captured call. A table
  * entry that is no page is allowed where no token lies (-1, say); where one
- * lies, that token is not written, reads as zero and is seen by no row. Lengths
- * past the table's tokens end there. */
+ * lies, that token is not written, reads as zero and is seen by no row. So is a
+ * token past the table's end; its row keeps its position. */
 typedef struct tfm_kv_batch {
   const int32_t* table;   /* [sequences, table_width]                      */
   const int32_t* lengths; /* [sequences]                                   */

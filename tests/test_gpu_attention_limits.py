@@ -1,15 +1,20 @@
-"""Attention over the 8-bit cache where its definition is easiest to lose: windows as long as an int, rows that
-look at many tokens a little."""
+"""Attention over the 8-bit cache, and appending to it, where the definition is easiest to lose: windows as long as an
+int, rows that look at many tokens a little, lengths past the table."""
 import math
 
 import pytest
 import torch
 
-from tests.test_gpu_attention import FORMS, attend64, compare, half_step, make, queries, run
+from tests.test_gpu_attention import FORMS, append_steps, attend64, compare, half_step, make, queries, run, same_cache, starts_of
+from trifuse_amd import layer
 
 pytestmark = pytest.mark.gpu
 
 BF16, F16 = torch.bfloat16, torch.float16
+
+
+def i32(values, gpu):
+    return torch.tensor(values, dtype=torch.int32, device=gpu)
 
 
 # -- windows -------------------------------------------------------------------------
@@ -89,3 +94,85 @@ def test_far_above_in_a_page_of_another_scale(gpu, rows, width, spare, spread):
         relative = 2.0 ** -10 + 7 * 2.0 ** -19 + 2.0 ** -17
         got = run(q, cache, table, [length], [0, rows], gpu, width, spare, causal=False, scale=scale)
         compare(got, want, want.abs() * (1.01 * relative + half_step(BF16)) + lost)
+
+
+# -- lengths past the table ------------------------------------------------------------
+
+def held_to(rows, lengths, room):
+    """[(rows, length)] of the same batch with the rows that have a place: row i of n is at position length - n + i."""
+    return [(max(0, min(n, room - (length - n))), min(length, room)) for n, length in zip(rows, lengths)]
+
+
+@pytest.mark.parametrize("page,kv_heads,dim,pairs", [(16, 2, 64, 0), (16, 5, 128, 64), (64, 1, 128, 0), (256, 2, 64, 16)])
+def test_rows_past_the_table_are_not_written(gpu, page, kv_heads, dim, pairs):
+    """A token behind the table's last place is nowhere: it is not written, and those before it stay."""
+    room = 3 * page
+    rows, lengths = [1, 30, 20, 5, 4, 7], [room + 1, room + 20, 1000 + room, 2 ** 31 - 1, 40, 2 ** 30 + 3]
+    cache, table = make(gpu, [room] * 6, kv_heads, page, dim, seed=93)
+    g = torch.Generator().manual_seed(93)
+    k, v = (torch.randn((sum(rows) + 2, kv_heads, dim), generator=g).to(BF16) * 3 for _ in "kv")
+    kw = dict(frequencies=layer.rotary_frequencies(pairs, device=gpu)[0]) if pairs else {}
+    other = layer.KVCache(*(t.clone() for t in cache))
+    want = [t.cpu().clone() for t in cache]
+    for _ in range(2):  # as replays of one step do
+        layer.cache_append(k.to(gpu), v.to(gpu), cache, table.to(gpu), i32(lengths, gpu), starts=i32(starts_of(rows), gpu),
+                           max_rows=30, **kw)
+    for b, (n, length) in enumerate(held_to(rows, lengths, room)):
+        start = starts_of(rows)[b]
+        mine = [t[start:start + n] for t in (k, v)]
+        for _ in range(2):
+            append_steps(want, *mine, table[b:b + 1], [length], [0, n])
+            if n:
+                layer.cache_append(*(t.to(gpu) for t in mine), other, table[b:b + 1].to(gpu), i32([length], gpu), **kw)
+    same_cache(cache, [t.cpu() for t in other])
+    if not pairs:
+        same_cache(cache, want)
+    back = layer.cache_read(cache, table.to(gpu), i32(lengths, gpu), 25, torch.float32)
+    for got, codes, scales in ((back[0], cache.k, cache.k_scales), (back[1], cache.v, cache.v_scales)):
+        values = (codes.float() * scales[:, :, None, None]).cpu()
+        got = got.cpu().view(6, 25, kv_heads, dim)
+        for b, length in enumerate(lengths):
+            for i in range(25):
+                t = length - 25 + i
+                assert torch.equal(got[b, i], values[table[b, t // page], :, t % page]) if t < room else not got[b, i].any()
+
+
+@pytest.mark.parametrize("causal,window", [(True, 0), (True, 33), (True, 2 ** 31 - 1), (False, 0)])
+@pytest.mark.parametrize("rows,width,spare", FORMS)
+def test_rows_past_the_table_stay_at_their_positions(gpu, rows, width, spare, causal, window):
+    """They see the tokens that there are, from where they stand."""
+    page, room = 16, 64 if spare else 160
+    lengths = [room + 1, room + rows // 2, room + 30, room + 1000]
+    cache, table = make(gpu, [room] * 4, 2, page, 64, seed=94)
+    q, starts = queries(4 * rows, 4, 64, F16, gpu, seed=94), [i * rows for i in range(5)]
+    longer = torch.nn.functional.pad(table, (0, -(-max(lengths) // page) - table.shape[1]), value=-1)
+    want, bound = attend64(q, cache, longer, lengths, starts, 0.125, causal, min(window, 10 ** 6))
+    compare(run(q, cache, table, lengths, starts, gpu, 0, spare, causal=causal, window=window), want, bound)
+    if width:  # the same with room for the tokens, but no pages: other kernels
+        compare(run(q, cache, table, lengths, starts, gpu, width, spare, causal=causal, window=window), want, bound)
+    far = [2 ** 31 - 1, 2 ** 30 + 7, 2 ** 31 - 20, 2 ** 30]
+    got = run(q, cache, table, far, starts, gpu, 0, spare, causal=causal, window=window)
+    if 0 < window < 2 ** 20:
+        assert not got.any()
+    else:  # all there are: the last position is 2^31 - 2, from where a window of 2^31 - 1 begins at token 0
+        want, bound = attend64(q, cache, longer, [room + 1000] * 4, starts, 0.125, causal, 0)
+        compare(got, want, bound)
+
+
+def test_append_leaves_what_is_not_its_own(gpu):
+    """Rows at negative positions, pages that are none, lengths past the table, rows behind the last sequence; starts that
+    no batch has."""
+    page, dim = 16, 64
+    cache, table = make(gpu, [40, 40, 40], 1, page, dim, seed=9)
+    table[1, 1] = -1
+    table[1, 2] = cache.k.shape[0]
+    lengths, rows = [3, 40, 1000], [10, 40, 20]
+    g = torch.Generator().manual_seed(97)
+    k, v = (torch.randn((75, 1, dim), generator=g).to(F16) for _ in "kv")
+    want = [t.cpu().clone() for t in cache]
+    layer.cache_append(k.to(gpu), v.to(gpu), cache, table.to(gpu), i32(lengths, gpu), starts=i32(starts_of(rows), gpu), max_rows=40)
+    append_steps(want, k, v, table[:2], lengths[:2], [0, 10, 50])
+    same_cache(cache, want)
+    layer.cache_append(k.to(gpu), v.to(gpu), cache, table.to(gpu), i32([-3, 40, 40], gpu), starts=i32([70, -5, 1 << 30, 3], gpu),
+                       max_rows=40)
+    torch.cuda.synchronize()

@@ -94,7 +94,7 @@ __device__ __forceinline__ int tiles_of(const AttentionArgs& a, const KvSeq& s, 
   return (s.n * a.group + columns - 1) / columns;
 }
 __device__ __forceinline__ int tokens_of(const AttentionArgs& a, const KvSeq& s) {
-  return max(s.len - lowest(a, s.first()), 0);
+  return max(s.len - lowest(a, s.first), 0);
 }
 
 // Item `index` of the batch. Every wave finds it by itself, a sequence a lane. A part's
@@ -106,7 +106,7 @@ __device__ __forceinline__ int tokens_of(const AttentionArgs& a, const KvSeq& s)
 __device__ Item find_item(const AttentionArgs& a, int columns, int index, int& tiles_cut) {
   const int lane = threadIdx.x & 63;
   auto mine = [&](int b) {
-    KvSeq s{0, 0, 0};
+    KvSeq s{0, 0, 0, 0};
     if (b < a.b.sequences) s = kv_seq(a.b, b);
     return s;
   };
@@ -145,7 +145,7 @@ __device__ Item find_item(const AttentionArgs& a, int columns, int index, int& t
       auto of = [&](int v) { return __builtin_amdgcn_readlane(v, l); };
       Item it;
       it.b = b0 + l;
-      it.s = KvSeq{of(s.start), of(s.n), of(s.len)};
+      it.s = KvSeq{of(s.start), of(s.n), of(s.first), of(s.len)};
       it.parts = of(parts);
       const int first = before + of(upto) - of(tiles) * it.parts, local = index - first;
       it.tile = local / it.parts;
@@ -188,7 +188,7 @@ struct Column {
 __device__ __forceinline__ Column column_of(const AttentionArgs& a, const KvSeq& s, int kv_head, int c) {
   Column o;
   o.real = c < s.n * a.group;
-  const int i = c / a.group, position = s.first() + i;
+  const int i = c / a.group, position = (int)((uint32_t)s.first + (uint32_t)i);  // past an int only where it is none
   o.row = s.start + i;
   o.head = kv_head * a.group + c % a.group;
   // A column that is none has nothing written, and does not make a tile take the masked path.
@@ -202,7 +202,7 @@ __device__ __forceinline__ Column column_of(const AttentionArgs& a, const KvSeq&
 __device__ __forceinline__ void part_of(const AttentionArgs& a, const KvSeq& s, const Item& it, int columns, int step,
                                         int& from, int& to) {
   const int c1 = min(s.n * a.group, (it.tile + 1) * columns) - 1;
-  const int first = s.first() + it.tile * columns / a.group, last = s.first() + c1 / a.group;
+  const int first = s.first + it.tile * columns / a.group, last = s.first + c1 / a.group;
   const int hi = a.causal ? min(s.len, last + 1) : s.len;
   const int lo = lowest(a, first) / step * step;
   const int each = ((max(hi - lo, 0) + it.parts - 1) / it.parts + step - 1) / step * step;

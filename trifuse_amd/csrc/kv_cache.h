@@ -14,8 +14,8 @@ typedef _Float16 f16x2_t __attribute__((ext_vector_type(2)));
 struct KvSeq {
   int start;  // its first row
   int n;      // its rows
-  int len;    // its tokens, those rows' own included
-  __device__ int first() const { return len - n; }  // position of its first row (negative: rows before the first token)
+  int first;  // position of its first row (negative: rows before the first token)
+  int len;    // its tokens, those rows' own included, that the table has room for: rows from there on have no place
 };
 
 __device__ __forceinline__ KvSeq kv_seq(const KvBatchArgs& a, int b) {
@@ -32,7 +32,9 @@ __device__ __forceinline__ KvSeq kv_seq(const KvBatchArgs& a, int b) {
   to = min(max(to, from), a.rows);
   s.start = from;
   s.n = min(to - from, a.max_rows);
-  s.len = min(max(a.lengths[b], 0), a.table_width << a.page_shift);
+  const int tokens = max(a.lengths[b], 0);
+  s.first = tokens - s.n;
+  s.len = min(tokens, a.table_width << a.page_shift);
   return s;
 }
 

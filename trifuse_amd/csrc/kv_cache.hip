@@ -40,10 +40,11 @@ __global__ __launch_bounds__(NT == 64 ? 256 : NT) void cache_append_kernel(KvApp
   if (b >= g.sequences) return;
   const bool values = blockIdx.z != 0;
   const KvSeq s = kv_seq(g, b);
+  if (s.first >= s.len) return;  // no row has a place
   const int page_tokens = 1 << g.page_shift;
-  const int at = (max(s.first(), 0) >> g.page_shift) + unit % slots;  // table entry
+  const int at = (max(s.first, 0) >> g.page_shift) + unit % slots;  // table entry
   const int base = at << g.page_shift;
-  const int begin = max(max(s.first(), 0), base), end = min(s.len, base + page_tokens);
+  const int begin = max(max(s.first, 0), base), end = min(s.len, base + page_tokens);
   if (begin >= end) return;
   const int held = begin - base;  // tokens of the page that stay
 
@@ -68,7 +69,7 @@ __global__ __launch_bounds__(NT == 64 ? 256 : NT) void cache_append_kernel(KvApp
     for (int i = 0; i < NI; ++i) {
       const int item = thread + i * NT;
       if (item < items) {
-        const uint16_t* row = x + (int64_t)(s.start + begin + item / per - s.first()) * row_stride + head * head_stride;
+        const uint16_t* row = x + (int64_t)(s.start + begin + item / per - s.first) * row_stride + head * head_stride;
         int d0, d1;
         channels(item % per, d0, d1);
         raw[i][0] = load8<true>(row + d0, 8);
@@ -194,7 +195,7 @@ __global__ __launch_bounds__(256) void cache_read_kernel(KvBatchArgs g, T* k, T*
   if (row >= (int64_t)g.rows) return;
   const int b = row / g.max_rows, c = i % per, head = i / per % g.kv_heads;
   const KvSeq s = kv_seq(g, b);
-  const int token = s.first() + (int)(row - s.start);
+  const int token = s.first + (int)(row - s.start);
   const int page = kv_page(g, b, token);
   const bool values = blockIdx.y != 0;
   T* to = (values ? v : k) + i * 16;

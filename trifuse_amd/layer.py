@@ -204,7 +204,7 @@ def cache_append(k: torch.Tensor, v: torch.Tensor, cache: KVCache, table: torch.
     one sequence; None: all rows), the last of its tokens; without starts every sequence has the same number.
     A page and head takes the larger of its scale and max|x| / 127 of its new tokens; codes that it
     held are rounded to a larger scale. An infinity or a NaN makes the page NaN. Pages are not shared between
-    sequences that write to them in one call."""
+    sequences that write to them in one call. A token past its table row's end is not written."""
     _enqueue("cache_append", k, v, *cache, table, lengths, starts, max_rows, frequencies, interleaved, rotary_scale)
 
 
