@@ -1,5 +1,5 @@
 """Attention over the 8-bit cache, and appending to it, where the definition is easiest to lose: windows as long as an
-int, rows that look at many tokens a little, lengths past the table."""
+int, rows that look at many tokens a little, lengths past the table, thousands of sequences."""
 import math
 
 import pytest
@@ -176,3 +176,53 @@ def test_append_leaves_what_is_not_its_own(gpu):
     layer.cache_append(k.to(gpu), v.to(gpu), cache, table.to(gpu), i32([-3, 40, 40], gpu), starts=i32([70, -5, 1 << 30, 3], gpu),
                        max_rows=40)
     torch.cuda.synchronize()
+
+
+# -- thousands of sequences ------------------------------------------------------------------
+
+@pytest.mark.parametrize("dtype,sequences,rows,heads,kv_heads,dim,even,width", [
+    (BF16, 3000, 1, 2, 2, 64, True, 0), (BF16, 3000, 1, 2, 2, 64, False, 0), (F16, 9000, 1, 4, 1, 64, False, 0), (F16, 9000, 1, 4, 1, 64, False, 4000),
+    (BF16, 3000, 2, 2, 1, 128, False, 4000), (F16, 1500, 5, 4, 1, 64, True, 0),  # 16 and 32 columns a workgroup
+    (BF16, 5000, 3, 16, 1, 128, False, 0), (BF16, 70, 130, 1, 1, 64, False, 0), (F16, 200, 40, 12, 1, 64, True, 0),
+    (BF16, 257, 9, 24, 4, 128, False, 0)])
+def test_thousands_of_sequences(gpu, dtype, sequences, rows, heads, kv_heads, dim, even, width):
+    """Each gets what it gets in a batch of its own: short ones of many lengths, some with neither rows nor tokens."""
+    g = torch.Generator().manual_seed(sequences)
+    n = [rows] * sequences if even else [0 if i % 7 == 3 else 1 + (5 * i) % rows for i in range(sequences)]
+    lengths = [0 if i % 11 == 5 else (13 * i) % 45 + m for i, m in enumerate(n)]
+    cache, table = make(gpu, [48] * 40, kv_heads, 16, dim, seed=sequences)
+    table = table[torch.randint(0, 40, (sequences,), generator=g)]
+    room = -(-max(lengths) // 16)  # the same pages again where a sequence is longer
+    table = table.repeat(1, -(-room // table.shape[1]))[:, :room].contiguous()
+    q, starts = queries(sum(n), heads, dim, dtype, gpu, seed=sequences), starts_of(n)
+    wide = torch.nn.functional.pad(table, (0, max(0, width // 16 - room)), value=-1).to(gpu)
+    out = torch.full((sum(n) + (0 if even else 3), heads, dim), 7.0, dtype=dtype, device=gpu)  # rows behind the last sequence
+    layer.cache_attention(torch.cat([q, q[:out.shape[0] - sum(n)]]), cache, wide, i32(lengths, gpu), out=out,
+                          **(dict() if even else dict(starts=i32(starts, gpu), max_rows=rows)))
+    assert bool((out[sum(n):] == 7.0).all())
+    some = sorted({0, 1, 63, 64, 65, sequences - 1, *torch.randint(0, sequences, (40,), generator=g).tolist()} & set(range(sequences)))
+    for b in some:
+        if n[b]:
+            mine = slice(starts[b], starts[b + 1])
+            compare(out[mine], *attend64(q[mine], cache, table[b:b + 1], [lengths[b]], [0, n[b]], dim ** -0.5, True, 0))
+    if rows * heads // kv_heads > 32:  # the rest may take another kernel in small batches
+        return
+    for b0 in range(0, sequences, 50):
+        b1 = min(b0 + 50, sequences)
+        mine = slice(starts[b0], starts[b1])
+        small = layer.cache_attention(q[mine], cache, table[b0:b1].to(gpu), i32(lengths[b0:b1], gpu),
+                                      starts=i32([s - starts[b0] for s in starts[b0:b1 + 1]], gpu), max_rows=rows)
+        assert torch.equal(out[mine], small)
+
+
+def test_starts_that_no_large_batch_has(gpu):
+    """Whatever starts say, nothing leaves the arrays and every workgroup ends."""
+    cache, table = make(gpu, [40], 2, 16, 64, seed=96)
+    q, g = queries(5000, 2, 64, BF16, gpu, seed=96), torch.Generator().manual_seed(96)
+    for n, group in ((5000, 1), (300, 1), (300, 17)):
+        rows = q[:, :1].expand(-1, 2 * group, -1)
+        for starts in (torch.randint(-(2 ** 31), 2 ** 31 - 1, (n + 1,), generator=g), torch.randint(-9, 5009, (n + 1,), generator=g),
+                       torch.arange(n, -1, -1), torch.full((n + 1,), 2 ** 31 - 1), torch.zeros(n + 1)):
+            layer.cache_attention(rows, cache, table.expand(n, -1).contiguous().to(gpu), i32([40] * n, gpu),
+                                  starts=starts.to(torch.int32).to(gpu), max_rows=7)
+            torch.cuda.synchronize()
