@@ -1,5 +1,6 @@
 """Attention over the 8-bit cache, and appending to it, where the definition is easiest to lose: windows as long as an
-int, rows that look at many tokens a little, lengths past the table, thousands of sequences."""
+int, rows that look at many tokens a little, lengths past the table, thousands of sequences, more parts than the joining
+kernel holds at once."""
 import math
 
 import pytest
@@ -226,3 +227,44 @@ def test_starts_that_no_large_batch_has(gpu):
             layer.cache_attention(rows, cache, table.expand(n, -1).contiguous().to(gpu), i32([40] * n, gpu),
                                   starts=starts.to(torch.int32).to(gpu), max_rows=7)
             torch.cuda.synchronize()
+
+
+# -- more parts than the joining kernel holds at once ---------------------------------------
+
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("rows,slope,others", [(1, 0.0, 0), (16, 0.0, 0), (1, 3.0, 0), (16, -3.0, 0), (8, 0.0, 79), (8, 3.0, 79)])
+def test_each_of_many_parts_counts(gpu, dtype, rows, slope, others):
+    """70000 tokens of one key head, in over 500 parts, alone and among short sequences (a column then has fewer threads in
+    the join). Channel c is zero but in its own 64th of the tokens, so that it is missing, or doubled, where those are."""
+    page, length, dim = 256, 70000, 64
+    cache, table = make(gpu, [length], 1, page, dim, seed=95)
+    at, t = table[0].long(), torch.arange(table.shape[1] * page)
+    # Scores 0, or rising or falling along the tokens by `slope` in all, a step every 276 of them.
+    k, v = torch.zeros((len(t), dim), dtype=torch.int8), torch.zeros((len(t), dim), dtype=torch.int8)
+    step = (t // 276).clamp_max(253) - 127
+    k[:, 0] = step.to(torch.int8) if slope else 0
+    mine = t * dim // length
+    inside = t < length
+    v[t[inside], mine[inside]] = (60 + mine[inside]).to(torch.int8)
+    cache.k[at, 0], cache.v[at, 0] = k.view(-1, page, dim).to(gpu), v.view(-1, page, dim).to(gpu)
+    cache.k_scales.fill_(0.5)
+    cache.v_scales.fill_(1.0)
+    q = torch.zeros((rows * (1 + others), 2, dim), dtype=dtype, device=gpu)
+    q[..., 0] = 1.0
+    scale = torch.tensor(slope / 127, dtype=torch.float32).item()
+    w = torch.softmax(step[:length].double() * 0.5 * scale, 0)
+    want = (w @ v[:length].double()).expand(rows, 2, dim)
+    # Half a step of a half for each weight, in both sums; an exponent below 16 with five roundings of 2^-21, times ln 2,
+    # in both; at most 1024 additions in fp32 in a row (a part's tokens, and the parts); the output's rounding.
+    bound = want.abs() * (2.0 ** -10 + 7 * 2.0 ** -21 + 2.0 ** -13 + half_step(dtype))
+    assert bool((want > 20 * bound).all())  # a channel that is missing, doubled or another's is seen
+    short = torch.full((others, table.shape[1]), -1, dtype=torch.int32)
+    short[:, 0] = table[0, 0]  # its first five tokens, which are alike
+    got = run(q, cache, torch.cat([table, short]), [length] + [5] * others, [i * rows for i in range(2 + others)], gpu,
+              causal=False, scale=scale)
+    compare(got[:rows], want, bound)
+    alike = v[0].double().expand(rows * others, 2, dim)
+    compare(got[rows:], alike, alike * (2.0 ** -10 + half_step(dtype)))
+    drop = torch.ones(length, dtype=torch.float64)
+    drop[256 * 128:257 * 128] = 0  # what the loss of one part alone would do
+    assert bool((((w * drop) @ v[:length].double() - want[0, 0]).abs() > 2 * bound[0, 0]).any())
