@@ -141,8 +141,9 @@ def rotary_frequencies(pairs: int, base: float = 10000.0, *, stretch: float = 1.
     * "base": base multiplied by stretch ** (pairs / (pairs - 1)), which keeps the fastest pair and slows the
       slowest to 1 / stretch; scale 1;
     * "bands": a pair that turns at least ``fast`` times over the trained ``context`` keeps its frequency, one
-      that turns at most ``slow`` times has it divided by stretch, between them the two are mixed in proportion to
-      the turns' place; scale 0.1 ln(stretch) + 1."""
+      that turns at most ``slow`` times has it divided by stretch, between them the two are mixed, linearly in the
+      turns; scale 0.1 ln(stretch) + 1. A model trained with another mixture (linear in the pair's number, say)
+      needs frequencies of its own."""
     if pairs < 1:
         raise ValueError("pairs must be positive")
     if not (base > 0 and stretch >= 1 and math.isfinite(base) and math.isfinite(stretch)):
