@@ -407,9 +407,9 @@ __device__ __forceinline__ void few_weigh(const uint32_t (&x)[8][W], const f16x8
 // wave has its next tile's codes on their way while it works, and no wave waits for another
 // before the end, where their sums meet in LDS. Registers instead of LDS, because each code is
 // used by one wave only; rows of an 8-bit product would be half the work, but the codes' bound is
-// memory: 64 sequences (2.1 GB of codes) in 320 us are 6.7 TB/s, and one of 1407 tokens 6.8 us,
+// memory: 64 sequences (1.79 GB of codes) in 320 us are 5.6 TB/s, and one of 1407 tokens 6.8 us,
 // of which a chain of loads (lengths, table, codes) is most. With more columns than fit one
-// workgroup the chain of tiles decides: 512 rows of 16 heads of 128, 256 workgroups, 12.3 us.
+// workgroup the chain of tiles decides: 512 rows of 16 heads of 128, 256 workgroups, 12.7 us.
 template <bool F16, int D, int NC>
 __global__ __launch_bounds__(256, D == 64 ? 7 - 2 * NC : 4 - NC) void attention_few_kernel(AttentionArgs a) {
   constexpr int COLS = 16 * NC, NK = D / 32, NV = D / 16, PAD = D + 4;
@@ -758,9 +758,9 @@ __device__ __forceinline__ f32x16_t zeros16() {
 // whose columns are too few to fill the card otherwise, where the chain of tiles is what lasts
 // (three of 200 rows and 16 heads 13.5 to 10.8 us).
 //
-// Bound: the matrix cores. 8192 rows of 16 heads of 128, causal, take 285 us (0.97 PFLOP/s);
-// the same kernel without exponentials, conversions and reads of LDS 217 (they cost 36, 17
-// and 17).
+// Bound: the matrix cores. 8192 rows of 16 heads of 128, causal, take 297 us (0.93 PFLOP/s; 290 to
+// 298 by the card). With weights as they are, not lifted, they took 285 to 293, of which
+// exponentials were 36, conversions 17 and reads of LDS 17.
 template <bool F16, int D, int WAVES, bool PAIRS>
 __global__ __launch_bounds__(64 * WAVES, 2) void attention_tile_kernel(AttentionArgs a) {
   static_assert(!PAIRS || WAVES == 4, "a pair's places in LDS are those of 64 tokens");
@@ -1194,7 +1194,8 @@ void launch_as(const AttentionPlan& p, const AttentionArgs& a, hipStream_t s) {
 // Whether the few kernel takes many columns sooner than the tile kernel. Its waves wait for nobody
 // and each takes its own tokens, 32 columns a workgroup, so a call lasts a quarter of the chain of
 // tiles while its workgroups are there at once or nearly; but each brings and converts its tokens
-// for 32 columns only, which is most of the work with heads of 128. Measured, us, tile and few:
+// for 32 columns only, which is most of the work with heads of 128. Measured, us, tile and few (as are
+// the figures below, before weights were lifted, which in prompts and chunks costs either 2 to 7 %):
 // - 16 heads of 128: a prompt of 400 rows 16.2 and 12.3, 700 behind 100 tokens 21.7 and 16.6, behind
 //   1500 37.7 and 33.9, behind 3000 46.7 and 54.5; 8 of 60 rows behind 1000 30 and 19.5; 16 of 50
 //   behind 100 11.9 and 13.2, behind 1500 49 and 30.5; 8 of 150 behind 500 23.9 and 26.2, behind 1000
