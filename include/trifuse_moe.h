@@ -457,15 +457,15 @@ int tfm_cache_read(const tfm_kv_cache* cache, const tfm_kv_batch* batch, int32_t
  * (else all of its sequence), and with window > 0 (causal only) j > position -
  * window. A row that sees none is zero. q [rows, heads, head_dim] with strides,
  * out [rows, heads, head_dim] dense. Products are of exact codes with halves (q
- * after a power of two for its row, softmax weights: those below 2^-22 of the
- * row's largest lose bits, those below 2^-33 are none), their sums, the
- * softmax's exponents and its statistics fp32, one rounding at the end. Scales are positive or zero (one
- * below 2^-100 counts as that), those of a head's pages up to 2^100 apart; rows *
- * heads / kv_heads is at most 2^30, and that over 16 and the sequences, times
- * kv_heads, below 2^24. Sequences are cut along their tokens in batches of up to
- * 4096 of them. The workspace (256-byte aligned, no status word) holds the parts of
- * sequences that several workgroups share, keeps nothing between calls, and may be
- * 0 bytes. */
+ * after a power of two for its row; softmax weights times their page's value
+ * scale, of which those below 2^-22 of the row's largest lose bits and those below
+ * 2^-33 are none), their sums, the softmax's exponents and its statistics fp32, one
+ * rounding at the end. Scales are positive or zero (one below 2^-100 counts as
+ * that), those of a head's pages up to 2^100 apart; rows * heads / kv_heads is at
+ * most 2^30, and that over 16 and the sequences, times kv_heads, below 2^24.
+ * Sequences are cut along their tokens in batches of up to 2048 of them. The
+ * workspace (256-byte aligned, no status word) holds the parts of sequences that
+ * several workgroups share, keeps nothing between calls, and may be 0 bytes. */
 size_t tfm_cache_attention_workspace_bytes(int64_t rows, int32_t heads, int32_t window,
                                            const tfm_kv_cache* cache, const tfm_kv_batch* batch);
 int tfm_cache_attention(const void* q, int64_t row_stride, int64_t head_stride, int64_t rows,

@@ -171,7 +171,8 @@ def test_append_leaves_what_is_not_its_own(gpu):
     g = torch.Generator().manual_seed(97)
     k, v = (torch.randn((75, 1, dim), generator=g).to(F16) for _ in "kv")
     want = [t.cpu().clone() for t in cache]
-    layer.cache_append(k.to(gpu), v.to(gpu), cache, table.to(gpu), i32(lengths, gpu), starts=i32(starts_of(rows), gpu), max_rows=40)
+    layer.cache_append(k.to(gpu), v.to(gpu), cache, table.to(gpu), i32(lengths, gpu), starts=i32(starts_of(rows), gpu),
+                       max_rows=40)
     append_steps(want, k, v, table[:2], lengths[:2], [0, 10, 50])
     same_cache(cache, want)
     layer.cache_append(k.to(gpu), v.to(gpu), cache, table.to(gpu), i32([-3, 40, 40], gpu), starts=i32([70, -5, 1 << 30, 3], gpu),
@@ -182,8 +183,9 @@ def test_append_leaves_what_is_not_its_own(gpu):
 # -- thousands of sequences ------------------------------------------------------------------
 
 @pytest.mark.parametrize("dtype,sequences,rows,heads,kv_heads,dim,even,width", [
-    (BF16, 3000, 1, 2, 2, 64, True, 0), (BF16, 3000, 1, 2, 2, 64, False, 0), (F16, 9000, 1, 4, 1, 64, False, 0), (F16, 9000, 1, 4, 1, 64, False, 4000),
-    (BF16, 3000, 2, 2, 1, 128, False, 4000), (F16, 1500, 5, 4, 1, 64, True, 0),  # 16 and 32 columns a workgroup
+    (BF16, 3000, 1, 2, 2, 64, True, 0), (BF16, 3000, 1, 2, 2, 64, False, 0), (F16, 9000, 1, 4, 1, 64, False, 0),
+    (F16, 9000, 1, 4, 1, 64, False, 4000), (BF16, 2000, 2, 2, 1, 128, False, 4000), (BF16, 2300, 2, 2, 1, 128, False, 4000),
+    (F16, 1500, 5, 4, 1, 64, True, 0),  # 16 and 32 columns a workgroup
     (BF16, 5000, 3, 16, 1, 128, False, 0), (BF16, 70, 130, 1, 1, 64, False, 0), (F16, 200, 40, 12, 1, 64, True, 0),
     (BF16, 257, 9, 24, 4, 128, False, 0)])
 def test_thousands_of_sequences(gpu, dtype, sequences, rows, heads, kv_heads, dim, even, width):

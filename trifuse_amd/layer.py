@@ -212,7 +212,8 @@ def cache_append(k: torch.Tensor, v: torch.Tensor, cache: KVCache, table: torch.
 def cache_read(cache: KVCache, table: torch.Tensor, lengths: torch.Tensor, rows: int,
                dtype: torch.dtype = torch.bfloat16) -> Tuple[torch.Tensor, torch.Tensor]:
     """(k, v) [sequences * rows, kv_heads, head_dim] in `dtype` (bf16, f16 or fp32): the last `rows` tokens of every
-    sequence as the values that their codes stand for, to be kept elsewhere. Tokens before the first are zero."""
+    sequence as the values that their codes stand for, to be kept elsewhere. Tokens before the first, and past the
+    table row's end, are zero."""
     return _enqueue("cache_read", cache.k, *cache[1:], table, lengths, rows, dtype)
 
 
