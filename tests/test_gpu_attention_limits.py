@@ -1,6 +1,6 @@
 """Attention over the 8-bit cache, and appending to it, where the definition is easiest to lose: windows as long as an
-int, rows that look at many tokens a little, lengths past the table, thousands of sequences, more parts than the joining
-kernel holds at once."""
+int, rows that look at many tokens a little, huge scores, lengths past the table, thousands of sequences, more parts
+than the joining kernel holds at once."""
 import math
 
 import pytest
@@ -95,6 +95,34 @@ def test_far_above_in_a_page_of_another_scale(gpu, rows, width, spare, spread):
         relative = 2.0 ** -10 + 7 * 2.0 ** -19 + 2.0 ** -17
         got = run(q, cache, table, [length], [0, rows], gpu, width, spare, causal=False, scale=scale)
         compare(got, want, want.abs() * (1.01 * relative + half_step(BF16)) + lost)
+
+
+# -- scores of any size ------------------------------------------------------------------------
+
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("rows,width,spare", FORMS)
+def test_the_largest_of_huge_scores_is_the_row(gpu, dtype, rows, width, spare):
+    """Scores so large that a step of fp32 is many binades of a weight: the token that stands above all others takes the row,
+    and nothing overflows."""
+    page, length, dim = 16, 390 if spare else 700, 64
+    cache, table = make(gpu, [length], 1, page, dim, seed=98)
+    cache.k_scales.fill_(1.0)
+    g = torch.Generator().manual_seed(98)
+    for top in (0, 37, length // 2, length - 1):
+        # Channel 0 alone makes the score: 127 for one token, at most 60 for the others; other channels only change sums.
+        cache.k[..., 0] = torch.randint(-127, 61, cache.k.shape[:3], generator=g).to(torch.int8).to(gpu)
+        at = table[0, top // page].item()
+        cache.k[at, 0, top % page, 0] = 127
+        q = torch.zeros((rows, 2, dim), dtype=dtype, device=gpu)
+        q[..., 0] = 1.0
+        q[..., 1:] = (torch.randn((rows, 2, dim - 1), generator=g) * 2.0 ** -8).to(dtype).to(gpu)
+        want = (cache.v[at, 0, top % page].cpu().double() * cache.v_scales[at, 0].cpu().double()).expand(rows, 2, dim)
+        for size in (2.0 ** 10, 2.0 ** 20, 2.0 ** 23, 2.0 ** 24, 2.0 ** 25, 2.0 ** 26, 2.0 ** 28, 2.0 ** 31, 2.0 ** 40, 2.0 ** 80):
+            # The others' sums: 63 channels of at most 4 x 2^-8 x 127, a standard deviation of 2^-8 x 40 x 8: below 20 of the 67
+            # between 127 and 60, so that they are over 300 below at the smallest size. The output is one value, code times
+            # scale: its weight is the same in both sums and falls out, which leaves an inverse, a division and a few products.
+            got = run(q, cache, table, [length], [0, rows], gpu, width, spare, causal=False, scale=size / 127)
+            compare(got, want, want.abs() * (half_step(dtype) + 2.0 ** -19))
 
 
 # -- lengths past the table ------------------------------------------------------------

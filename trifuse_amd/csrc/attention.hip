@@ -48,6 +48,11 @@ constexpr float kLow = -3.402823466e38f;  // below every score; finite, so that 
 // rows 291, 296 and 300.
 constexpr float kLift = 8.0f, kLiftUnit = 0x1p8f;
 constexpr float kMost = 0x1p100f;  // a lane's sum past this is infinite: a weight is past a half's range, and the maximum is taken again
+// Where a maximum is taken again, weights follow from the same rounded scores as it does, t - m and not
+// fma(.., shift - m): past 2^24 a score's step is binades of a weight, and what shift - m loses could
+// put one past a half once more. m is eight below in two steps of four, since one step of eight rounds
+// to 16 where fp32's step is that.
+__device__ __forceinline__ float below(float top) { return top - kLift / 2 - kLift / 2; }
 // Weights below 2^-22 are subnormal halves, each off by up to 2^-33. In the sum of w / b that is
 // 2^-33 / b: pages whose 1 / b is over so many times the sum so far have theirs summed in fp32.
 constexpr float kLeast = 16.0f;
@@ -541,26 +546,29 @@ __global__ __launch_bounds__(256, D == 64 ? 7 - 2 * NC : 4 - NC) void attention_
         for (int e = 0; e < 8; ++e) z[c][e / 4][e % 4] = e >= lo && e < hi ? z[c][e / 4][e % 4] : -__builtin_inff();
       }
       auto score = [&](int e, float low) { return __builtin_fmaf(z[c][e / 4][e % 4], unit_k, low); };
-      auto weigh = [&] {
+      auto weight = [&](int e) { return exp2_fast(score(e, shift - m[c])); };
+      auto held = [&](int e) { return exp2_fast(score(e, shift) - m[c]); };
+      auto weigh = [&](auto&& by) {
 #pragma unroll
-        for (int e = 0; e < 8; ++e) w[c][e] = (_Float16)exp2_fast(score(e, shift - m[c]));
+        for (int e = 0; e < 8; ++e) w[c][e] = (_Float16)by(e);
         return add_halves(w[c], 0.0f, 1.0f / kLiftUnit);
       };
-      float sum = weigh();
-      if (__any(sum > kMost)) {
+      float sum = weigh(weight);
+      const bool again = __any(sum > kMost);
+      if (again) {
         float top = kLow;
 #pragma unroll
         for (int e = 0; e < 8; ++e) top = fmaxf(top, score(e, shift));
         top = fmaxf(top, __shfl_xor(top, 16, kWave));
         top = fmaxf(top, __shfl_xor(top, 32, kWave));
-        top = fmaxf(m[c], top - kLift);
+        top = fmaxf(m[c], below(top));
         const float less = exp2_fast(m[c] - top);
         m[c] = top;
         l[c] *= less;
         seen[c] *= less;
 #pragma unroll
         for (int n = 0; n < NV; ++n) o[c][n] *= less;
-        sum = weigh();
+        sum = weigh(held);
       }
       if (__any(inverse > kLeast * seen[c])) {
         auto together = [&] {
@@ -571,8 +579,13 @@ __global__ __launch_bounds__(256, D == 64 ? 7 - 2 * NC : 4 - NC) void attention_
         seen[c] = together();
         if (__any(inverse > kLeast * seen[c])) {  // the sum in fp32, whatever the halves lose
           sum = 0.0f;
+          if (again) {
 #pragma unroll
-          for (int e = 0; e < 8; ++e) sum += exp2_fast(score(e, shift - m[c]));
+            for (int e = 0; e < 8; ++e) sum += held(e);
+          } else {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) sum += weight(e);
+          }
           sum *= 1.0f / kLiftUnit;
           seen[c] = together();
         }
@@ -923,16 +936,18 @@ __global__ __launch_bounds__(64 * WAVES, 2) void attention_tile_kernel(Attention
         fetch(j + 4);
       };
       auto weight = [&](int i, int e) { return exp2_fast(__builtin_fmaf(z[i][e], unit_k[i], shift[i] - m)); };
-      auto weigh = [&](int i, int from_e, int to_e) {
+      auto held = [&](int i, int e) { return exp2_fast(__builtin_fmaf(z[i][e], unit_k[i], shift[i]) - m); };
+      auto weigh_by = [&](int i, int from_e, int to_e, auto&& by) {
         const f16x2_t unit = {(_Float16)(1.0f / kLiftUnit), (_Float16)(1.0f / kLiftUnit)};
 #pragma unroll
         for (int e = from_e; e < to_e; e += 2) {
-          const f16x2_t p = {(_Float16)weight(i, e), (_Float16)weight(i, e + 1)};
+          const f16x2_t p = {(_Float16)by(i, e), (_Float16)by(i, e + 1)};
           w[i][e / 8][e % 8] = p[0];
           w[i][e / 8][e % 8 + 1] = p[1];
           sum[i] = __builtin_amdgcn_fdot2(p, unit, e ? sum[i] : 0.0f, false);
         }
       };
+      auto weigh = [&](int i, int from_e, int to_e) { weigh_by(i, from_e, to_e, weight); };
 #pragma unroll
       for (int i = 0; i < HALVES; ++i) {
         unit_k[i] = not_zero(unit * sc[i].x);
@@ -953,12 +968,13 @@ __global__ __launch_bounds__(64 * WAVES, 2) void attention_tile_kernel(Attention
         for (int e = 0; e < 16; ++e) z[i][e] = e >= lo && e < hi ? z[i][e] : -__builtin_inff();
       };
       auto settle = [&](int i) {
-        if (__any(sum[i] > kMost)) {
+        const bool again = __any(sum[i] > kMost);
+        if (again) {
           float top = kLow;
 #pragma unroll
           for (int e = 0; e < 16; ++e) top = fmaxf(top, __builtin_fmaf(z[i][e], unit_k[i], shift[i]));
           top = fmaxf(top, __shfl_xor(top, 32, kWave));
-          top = fmaxf(m, top - kLift);
+          top = fmaxf(m, below(top));
           const float less = exp2_fast(m - top);
           m = top;
           l *= less;
@@ -967,7 +983,7 @@ __global__ __launch_bounds__(64 * WAVES, 2) void attention_tile_kernel(Attention
           for (int n = 0; n < NV; ++n)
 #pragma unroll
             for (int e = 0; e < 16; ++e) o[n][e] *= less;
-          weigh(i, 0, 16);
+          weigh_by(i, 0, 16, held);
         }
         if (__any(inverse[i] > kLeast * seen)) {
           auto together = [&] {
@@ -977,8 +993,13 @@ __global__ __launch_bounds__(64 * WAVES, 2) void attention_tile_kernel(Attention
           seen = together();
           if (__any(inverse[i] > kLeast * seen)) {  // the sum in fp32, whatever the halves lose
             sum[i] = 0.0f;
+            if (again) {
 #pragma unroll
-            for (int e = 0; e < 16; ++e) sum[i] += weight(i, e);
+              for (int e = 0; e < 16; ++e) sum[i] += held(i, e);
+            } else {
+#pragma unroll
+              for (int e = 0; e < 16; ++e) sum[i] += weight(i, e);
+            }
             sum[i] *= 1.0f / kLiftUnit;
             seen = together();
           }
